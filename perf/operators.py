@@ -104,7 +104,7 @@ def _pack8(c):
 
 def _scale7(x, dim):
     a = x.abs().amax(dim, keepdim=True)
-    return torch.where(a > 0, a / 7, torch.ones_like(a))
+    return torch.where(a > 0, a / torch.full_like(a, 7), torch.ones_like(a))       # (by a plain 7 torch multiplies with 1/7)
 
 
 def _quant_dims(x):
