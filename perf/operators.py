@@ -227,10 +227,12 @@ def run(state):
     return {"attention": _plain_attention, "verify": _plain_verify, "append": _plain_append}[state["case"]["kind"]](state)
 
 
+_pkg = str(pathlib.Path(__file__).resolve().parents[1] / "k100lc-rt4_amd")
+
+
 def _run_own(st):
-    pkg = str(pathlib.Path(__file__).resolve().parents[1] / "k100lc-rt4_amd")
-    if pkg not in sys.path:
-        sys.path.insert(0, pkg)
+    if "rt4_amd" not in sys.modules and _pkg not in sys.path:
+        sys.path.insert(0, _pkg)
     import rt4_amd
     kind = st["case"]["kind"]
     if kind == "attention":
