@@ -292,6 +292,72 @@ int rt4_attention_prefill_cfg(float* out, const uint32_t* qq, const float* qsc, 
 int rt4_attention_launch_plan(int n_q, int n_heads, int ratio, int off, int n_tile, int kv_splits, int cus,
                               int* splits, int* one_launch, int* staged);
 
+/* ------------------------------------------- draft and verify steps ------ */
+/* One step of speculative decoding over B sequences, each with its own int4 cache of
+ * the layouts above (D = 256, G = 128, BG = 64), one cache after the other:
+ *   kc u32 [B][H][cap][32], ksc f32 [B][H][2][cap], vc u32 [B][H][cap/8][256],
+ *   vsc f32 [B][H][cap/64][256], stage f32 [B][H][64][256]   (H KV heads).
+ * Up to 64 new tokens per sequence form a tree, parent int32 [B][T]: node 0 is the root
+ * where parent is -1 (another value: the sequence is idle), node i > 0 hangs under node
+ * parent in [0, i); nodes whose chain does not end in the root are padding.  A chain is
+ * a tree, and so is one token: plain decoding.  A step quantizes the nodes' Q
+ * (rt4_attn_q_quant, row b*T + i) and K/V (rt4_kv_append_rows into a 64-key draft tile),
+ * attends (rt4_attention_tree), verifies the logits (rt4_verify_tree, which also advances
+ * the lengths) and appends the accepted rows (rt4_kv_append_rows).  Lengths, paths and
+ * counts stay on the device, so a step has no host synchronisation and can be captured.
+ * No counterparts in the reference, which decodes one sequence, compares argmaxes on the
+ * host and restores V tiles (src/model.cpp:1428-1460, :1838-1926). */
+
+/* Append of chosen rows: rows rows[b][0..n) of kf, vf f32 [B][T][H][256] (rows int32
+ * [B][T]; NULL: rows 0..n-1) become keys kv_len[b]-n .. kv_len[b]-1 of sequence b, n =
+ * count[b] clamped to [0, T] (NULL: T): kv_len holds the lengths once the rows are in.
+ * Codes, scales and stage as rt4_kv_append_k and rt4_kv_append_v write them for those
+ * rows, bit for bit.  kv_len NULL: every sequence starts at key 0, and stage may be NULL
+ * (a draft tile: kv_cap = 64).  A row index outside [0, T) appends zeros; a sequence whose
+ * keys would not lie in [0, kv_cap) is left as it is.  T <= kv_cap, kv_cap % 64 == 0 and at
+ * most 16777152; kf and vf must not overlap what is written. */
+int rt4_kv_append_rows(uint32_t* kc, float* ksc, uint32_t* vc, float* vsc, float* stage, const float* kf, const float* vf,
+                       const int32_t* kv_len, const int32_t* rows, const int32_t* count, int B, int T, int H, int kv_cap,
+                       void* stream);
+
+/* Attention of the trees' nodes, GQA (KV head = head / ratio): out f32 [n_heads][TP][256]
+ * row b*T + i = softmax(Q K^T) V over the keys before kv_len[b] of sequence b's cache and
+ * over node i and the nodes above it, whose K/V are keys 0..T-1 of the sequence's draft
+ * tile (kd, ksd, vd, vsd: a cache of 64 keys).  Scores, P and sums in fp32 (Q codes and
+ * scales as rt4_attn_q_quant writes them, qq u32 [n_heads][TP][32], TP >= B*T).  Rows of
+ * padding nodes and of idle sequences are zeros; rows from B*T on are left as they were.
+ * kv_len int32 [B] on the device, clamped to [0, kv_cap]; NULL: no cache (kc, ksc, vc, vsc
+ * are not read).  kv_max: the longest length to plan for (a longer one is still right).
+ * kv_splits: parts the keys are split into, 0 chooses (at most 64). */
+int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const uint32_t* kc, const float* ksc,
+                       const uint32_t* vc, const float* vsc, const int32_t* kv_len, const uint32_t* kd, const float* ksd,
+                       const uint32_t* vd, const float* vsd, const int32_t* parent, int B, int T, int TP, int n_heads,
+                       int ratio, int kv_cap, int kv_max, int kv_splits, void* stream);
+
+/* Verification: row b*T + i of logits (row stride ldl >= V floats) is the target's
+ * distribution after node i, p = softmax(logits / temp[b]); draft int32 [B][T] the nodes'
+ * tokens.  From the root, a node's children are tested in index order with the uniforms
+ * u f32 [B][T] in [0, 1):
+ *   draft_p NULL (tokens chosen outright): child i is accepted iff u[b][i] times the mass
+ *     not yet rejected is below p(draft[b][i]); a rejected token leaves p.
+ *   draft_p f32, row b*T + n (stride ldp) the distribution node n's children were drawn
+ *     from: accepted iff u[b][i] < r(x) / draft_p(x), r the residual, at first p and after
+ *     a rejection max(r - draft_p, 0) renormalized.  At most max_children children of a
+ *     node are tested, the rest are rejected.
+ * Where no child is accepted the last token is drawn from what is left: the smallest x
+ * whose cumulated residual exceeds u[b][0] times its total.  So the tokens are distributed
+ * as the target's own.  temp NULL: 1; temp[b] <= 0 (or NaN): greedy, a child is accepted
+ * iff it is the row's largest logit (lowest index among equals), and so is the last token.
+ * A NaN logit counts as -inf; a row of nothing but -inf ends the walk with token -1.
+ * A draft token outside [0, V) is rejected.
+ * Outputs: count[b] = n accepted nodes, the root included (0: idle); path int32 [B][T] their
+ * numbers; tokens int32 [B][T] the n new tokens (n-1 accepted drafts, then the last token);
+ * the rest of both is -1.  kv_len (optional): kv_len[b] += n, as rt4_kv_append_rows takes
+ * it.  Decisions are made in 64 bits.  T <= 64, V <= 4194304, B*T <= 65535. */
+int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_len, const float* logits, int64_t ldl,
+                    const int32_t* draft, const int32_t* parent, const float* u, const float* temp, const float* draft_p,
+                    int64_t ldp, int B, int T, int V, int max_children, void* stream);
+
 /* ----------------------------------------- W4A4 siblings (RT_ACT4 path) ---- */
 
 /* int4 activation quantizer.  Replaces k_quant_rows (src/kernels.h:36,

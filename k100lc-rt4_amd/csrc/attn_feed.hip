@@ -185,6 +185,92 @@ __global__ __launch_bounds__(256) void kv_append_v64_k(uint32_t* __restrict__ vc
     }
 }
 
+// Append of chosen rows to the caches of several sequences, at lengths known on the device
+// (rt4_kv_append_rows): sequence b's rows rows[b][0..n) (or 0..n) of kf, vf f32 [B][T][H][256]
+// become keys e-n..e-1, e = kv_len[b].  K codes as kv_append_k_k with G = 128, V codes, scales
+// and stage as kv_append_v64_k, bit for bit.  One launch: grid (vblocks + K workgroups, B), the
+// first vblocks = 4 H x tile slots workgroups a 64-key tile of 64 dims each, the others 8 K rows
+// of a head each.  A sequence whose keys would not lie in [0, kv_cap) is left as it is.
+__global__ __launch_bounds__(256) void kv_append_rows_k(uint32_t* __restrict__ kc, float* __restrict__ ksc,
+                                                        uint32_t* __restrict__ vc, float* __restrict__ vsc,
+                                                        float* __restrict__ stage, const float* __restrict__ kf,
+                                                        const float* __restrict__ vf, const int* __restrict__ kv_len,
+                                                        const int* __restrict__ rows, const int* __restrict__ count, int T, int H,
+                                                        int kv_cap, int vblocks) {
+    constexpr int D = 256, BG = 64;
+    __shared__ float red[4][64];
+    const int b = blockIdx.y;
+    const int n = count ? clampi(count[b], 0, T) : T;
+    const long long end = kv_len ? (long long)kv_len[b] : n;
+    if (n == 0 || end < n || end > kv_cap) return;
+    const int t0 = (int)end - n;
+    rows = rows ? rows + (size_t)b * T : nullptr;
+    // element 0 of the j-th appended row of src (H heads of D), null where rows names none
+    auto row = [&](const float* src, int j) {
+        const int r = rows ? rows[j] : j;
+        return r >= 0 && r < T ? src + ((size_t)b * T + r) * H * D : nullptr;
+    };
+    if ((int)blockIdx.x >= vblocks) {
+        const size_t i = (size_t)(blockIdx.x - vblocks) * 256 + threadIdx.x;
+        const int e8 = (int)(i & 31), th = (int)(i >> 5), h = th % H, j = th / H;
+        if (j >= n) return;                          // whole groups exit together
+        const float* xr = row(kf, j);
+        float v[8], amax = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            v[e] = xr ? xr[h * D + 8 * e8 + e] : 0.f;
+            amax = fmaxf(amax, fabsf(v[e]));
+        }
+        amax = run_max<16>(amax);
+        const float s = amax > 0.f ? amax / 7.f : 1.f;
+        const size_t key = ((size_t)b * H + h) * kv_cap + t0 + j;
+        kc[key * (D / 8) + e8] = codes8(v, s);
+        if (e8 % 16 == 0) ksc[(((size_t)b * H + h) * 2 + e8 / 16) * kv_cap + t0 + j] = s;
+        return;
+    }
+    const int lane = threadIdx.x & 63, p = threadIdx.x >> 6;
+    const int d = (blockIdx.x & 3) * 64 + lane, h = (blockIdx.x >> 2) % H, ti = (blockIdx.x >> 2) / H;
+    const int first = t0 / BG, last = (t0 + n - 1) / BG, tile = first + ti;
+    if (tile > last) return;
+    const size_t bh = (size_t)b * H + h;
+    float* st = stage ? stage + bh * BG * D + d : nullptr;
+    float v[16];
+    float amax = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const int key = tile * BG + 16 * p + e;
+        float x = 0.f;
+        if (key < t0) {
+            if (st) x = st[(size_t)(16 * p + e) * D];
+        } else if (key < t0 + n) {
+            const float* xr = row(vf, key - t0);
+            if (xr) x = xr[h * D + d];
+        }
+        v[e] = x;
+        amax = fmaxf(amax, fabsf(x));
+    }
+    red[p][lane] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(red[0][lane], red[1][lane]), fmaxf(red[2][lane], red[3][lane]));
+    const float s = amax > 0.f ? amax / 7.f : 1.f;
+    if (p == 0) vsc[(bh * (kv_cap / BG) + tile) * D + d] = s;
+    uint32_t* out = vc + (bh * (kv_cap / 8) + (size_t)tile * (BG / 8)) * D + d;
+#pragma unroll
+    for (int j = 0; j < 2; j++) out[(size_t)(2 * p + j) * D] = codes8(v + 8 * j, s);
+    if (ti != 0 || !st) return;
+    // the stage: the last tile's rows, beneath them those of the tile before it (a thread
+    // reads and writes the same slots, and only the first tile's workgroups read any)
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        int key = last * BG + 16 * p + e;
+        if (key >= t0 + n) key -= BG;
+        if (key >= t0) {
+            const float* xr = row(vf, key - t0);
+            st[(size_t)(16 * p + e) * D] = xr ? xr[h * D + d] : 0.f;
+        }
+    }
+}
+
 // -------------------------------------------------------------- launchers --
 
 hipError_t launch_attn_q_quant(uint32_t* qq, float* qs, const float* x, int T, int H, int D, int G, int TP,
@@ -236,6 +322,18 @@ hipError_t launch_kv_append_v(uint32_t* vc, float* vsc, float* stage, const floa
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kv_stage_v_k, dim3(H, (D + 63) / 64), dim3(64), 0, st, stage, vf, t0, T, H, D, BG);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_append_rows(uint32_t* kc, float* ksc, uint32_t* vc, float* vsc, float* stage, const float* kf,
+                                 const float* vf, const int* kv_len, const int* rows, const int* count, int B, int T, int H,
+                                 int kv_cap, hipStream_t st) {
+    // tiles that T rows can touch: from a tile's start, or from wherever a cache ends
+    const int slots = kv_len ? (T + 62) / 64 + 1 : (T + 63) / 64;
+    const int vblocks = 4 * H * slots;
+    const size_t kblocks = ((size_t)T * H * 32 + 255) / 256;
+    hipLaunchKernelGGL(kv_append_rows_k, dim3((unsigned)(vblocks + kblocks), B), dim3(256), 0, st, kc, ksc, vc, vsc, stage, kf, vf,
+                       kv_len, rows, count, T, H, kv_cap, vblocks);
     return hipGetLastError();
 }
 

@@ -35,7 +35,7 @@ hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 // the retired buffers of a slot add up to at most twice its final size.  Not
 // safe for concurrent calls from several threads (the reference's scratch has
 // the same property, src/k_gemv.hip:47-51).
-enum Slot { kSlotActQ = 0, kSlotActS = 1, kSlotGemmA = 2, kSlotGemmPart = 3, kSlotAttnPart = 4, kSlotGemvPart = 5, kSlotGemvCnt = 6, kSlotAttnCnt = 7, kSlotAttnKV = 8, kSlotGemmCnt = 9, kSlots = 10 };
+enum Slot { kSlotActQ = 0, kSlotActS = 1, kSlotGemmA = 2, kSlotGemmPart = 3, kSlotAttnPart = 4, kSlotGemvPart = 5, kSlotGemvCnt = 6, kSlotAttnCnt = 7, kSlotAttnKV = 8, kSlotGemmCnt = 9, kSlotVerify = 10, kSlots = 11 };
 constexpr int kMaxDev = 64;
 struct Buf {
     void* p = nullptr;
@@ -803,6 +803,69 @@ int rt4_attention_prefill(float* out, const uint32_t* qq, const float* qsc, cons
                           int n_tile, int n_heads, int ratio, int kv_cap, void* stream) {
     return rt4_attention_prefill_cfg(out, qq, qsc, kc, ksc, vc, vsc, n_q, n_kv, off, n_tile, n_heads, ratio, kv_cap,
                                      0, stream);
+}
+
+// ------------------------------------------------- draft and verify steps --
+
+int rt4_kv_append_rows(uint32_t* kc, float* ksc, uint32_t* vc, float* vsc, float* stage, const float* kf, const float* vf,
+                       const int32_t* kv_len, const int32_t* rows, const int32_t* count, int B, int T, int H, int kv_cap,
+                       void* stream) {
+    if (!kc || !ksc || !vc || !vsc || !kf || !vf) return fail(RT4_E_ARG, "rt4_kv_append_rows: null pointer");
+    if (kv_len && !stage) return fail(RT4_E_ARG, "rt4_kv_append_rows: appends at kv_len need the stage of the partial tiles");
+    if (B < 1 || B > 65535 || T < 1 || H < 1 || H > 65535 || kv_cap < 64 || kv_cap % 64 || kv_cap > kMaxKvCap || T > kv_cap ||
+        ((long long)T + 126) / 64 * 4 * H + ((long long)T * H + 7) / 8 > 0x7fffffffLL)
+        return fail(RT4_E_SHAPE, "rt4_kv_append_rows: B=%d T=%d H=%d kv_cap=%d (a multiple of 64, at least T, at most 16777152)", B,
+                    T, H, kv_cap);
+    if (!aligned(kc, 4) || !aligned(ksc, 4) || !aligned(vc, 4) || !aligned(vsc, 4) || !aligned(stage, 4) || !aligned(kf, 4) ||
+        !aligned(vf, 4) || !aligned(kv_len, 4) || !aligned(rows, 4) || !aligned(count, 4))
+        return fail(RT4_E_ARG, "rt4_kv_append_rows: misaligned pointer");
+    return hip_status(rt4::launch_kv_append_rows(kc, ksc, vc, vsc, stage, kf, vf, kv_len, rows, count, B, T, H, kv_cap,
+                                                 as_stream(stream)),
+                      "rt4_kv_append_rows launch");
+}
+
+int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const uint32_t* kc, const float* ksc, const uint32_t* vc,
+                       const float* vsc, const int32_t* kv_len, const uint32_t* kd, const float* ksd, const uint32_t* vd,
+                       const float* vsd, const int32_t* parent, int B, int T, int TP, int n_heads, int ratio, int kv_cap, int kv_max,
+                       int kv_splits, void* stream) {
+    if (!out || !qq || !qsc || !kd || !ksd || !vd || !vsd || !parent || (kv_len && (!kc || !ksc || !vc || !vsc)))
+        return fail(RT4_E_ARG, "rt4_attention_tree: null pointer");
+    if (B < 1 || B > 65535 || T < 1 || T > rt4::kTreeMaxT || (long long)TP < (long long)B * T || n_heads < 1 || n_heads > 65535 ||
+        ratio < 1 || n_heads % ratio)
+        return fail(RT4_E_SHAPE, "rt4_attention_tree: B=%d T=%d (1..64) TP=%d (at least B*T) n_heads=%d ratio=%d", B, T, TP, n_heads,
+                    ratio);
+    if (kv_len && (kv_cap < 64 || kv_cap % 64 || kv_cap > kMaxKvCap || kv_max < 0 || kv_max > kv_cap))
+        return fail(RT4_E_SHAPE, "rt4_attention_tree: kv_cap=%d (a multiple of 64, at most 16777152) kv_max=%d", kv_cap, kv_max);
+    if (kv_splits < 0 || kv_splits > 64) return fail(RT4_E_ARG, "rt4_attention_tree: kv_splits=%d (0..64)", kv_splits);
+    if (!aligned(qq, 16) || !aligned(kc, 16) || !aligned(vc, 16) || !aligned(kd, 16) || !aligned(vd, 16) || !aligned(out, 16) ||
+        !aligned(qsc, 4) || !aligned(ksc, 16) || !aligned(vsc, 16) || !aligned(ksd, 16) || !aligned(vsd, 16) || !aligned(parent, 4) ||
+        !aligned(kv_len, 4))
+        return fail(RT4_E_ARG, "rt4_attention_tree: misaligned pointer (out, qq, caches and draft tiles need 16 bytes)");
+    const rt4::AttnTree a = {out, qq, qsc, kc, ksc, vc, vsc, kv_len, kd, ksd, vd, vsd, parent, B, T, TP, n_heads, ratio, kv_cap};
+    return hip_status(rt4::launch_attn_tree(a, as_stream(stream)), "rt4_attention_tree launch");
+}
+
+int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_len, const float* logits, int64_t ldl,
+                    const int32_t* draft, const int32_t* parent, const float* u, const float* temp, const float* draft_p,
+                    int64_t ldp, int B, int T, int V, int max_children, void* stream) {
+    if (!tokens || !path || !count || !logits || !draft || !parent || !u) return fail(RT4_E_ARG, "rt4_verify_tree: null pointer");
+    if (B < 1 || T < 1 || T > rt4::kTreeMaxT || V < 1 || V > rt4::kVerifyMaxV || (long long)B * T > 65535 || ldl < V ||
+        (draft_p && (ldp < V || max_children < 1)))
+        return fail(RT4_E_SHAPE,
+                    "rt4_verify_tree: B=%d T=%d (1..64, B*T at most 65535) V=%d (at most 4194304) row strides %lld and %lld (at least "
+                    "V) max_children=%d (at least 1)",
+                    B, T, V, (long long)ldl, (long long)ldp, max_children);
+    if (!aligned(tokens, 4) || !aligned(path, 4) || !aligned(count, 4) || !aligned(kv_len, 4) || !aligned(logits, 4) ||
+        !aligned(draft, 4) || !aligned(parent, 4) || !aligned(u, 4) || !aligned(temp, 4) || !aligned(draft_p, 4))
+        return fail(RT4_E_ARG, "rt4_verify_tree: misaligned pointer");
+    const int most = T > 1 ? T - 1 : 1, levels = !draft_p ? 1 : max_children < most ? max_children : most;
+    hipStream_t st = as_stream(stream);
+    void* ws = nullptr;
+    int rc = lib_scratch(kSlotVerify, rt4::verify_ws_bytes(B, T, V, levels), &ws, st);
+    if (rc) return rc;
+    return hip_status(rt4::launch_verify_tree(tokens, path, count, kv_len, logits, (size_t)ldl, draft, parent, u, temp, draft_p,
+                                              (size_t)ldp, B, T, V, levels, ws, st),
+                      "rt4_verify_tree launch");
 }
 
 }  // extern "C"

@@ -138,4 +138,38 @@ hipError_t launch_fa_int4(float* out, const uint32_t* qq, const float* qsc, cons
                           int n_heads, int ratio, int kv_cap, int nsplit, float* part, int* cnt, void* kvx,
                           hipStream_t st);
 
+
+// ---- several sequences at once (attn_feed.hip, attn_tree.hip, verify.hip)
+hipError_t launch_kv_append_rows(uint32_t* kc, float* ksc, uint32_t* vc, float* vsc, float* stage, const float* kf,
+                                 const float* vf, const int* kv_len, const int* rows, const int* count, int B, int T, int H,
+                                 int kv_cap, hipStream_t st);
+
+// Arguments of the tree attention (rt4_attention_tree).
+constexpr int kTreeMaxT = 64;
+struct AttnTree {
+    float* out;
+    const uint32_t* qq;
+    const float* qsc;
+    const uint32_t* kc;
+    const float* ksc;
+    const uint32_t* vc;
+    const float* vsc;
+    const int* kv_len;
+    const uint32_t* kd;
+    const float* ksd;
+    const uint32_t* vd;
+    const float* vsd;
+    const int* parent;
+    int B, T, TP, n_heads, ratio, kv_cap;
+};
+hipError_t launch_attn_tree(const AttnTree& a, hipStream_t st);
+
+// Draft verification; `levels`: children tested per node where draft probabilities q are
+// given (else 1); ws: verify_ws_bytes of scratch.
+constexpr int kVerifyChunk = 4096, kVerifyMaxV = 1 << 22;
+size_t verify_ws_bytes(int B, int T, int V, int levels);
+hipError_t launch_verify_tree(int* tokens, int* path, int* count, int* kv_len, const float* logits, size_t ldl, const int* draft,
+                              const int* parent, const float* u, const float* temp, const float* q, size_t ldq, int B, int T, int V,
+                              int levels, void* ws, hipStream_t st);
+
 }  // namespace rt4

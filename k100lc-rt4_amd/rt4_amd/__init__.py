@@ -36,6 +36,7 @@ C_EXPORTS = (
     "rt4_gemm_w4a8", "rt4_gemm_w4a8_i8", "rt4_gemm_w4a8_groupsums",
     "rt4_attn_q_quant", "rt4_kv_append_k", "rt4_kv_append_v", "rt4_attention_prefill",
     "rt4_attention_prefill_cfg", "rt4_attention_launch_plan",
+    "rt4_kv_append_rows", "rt4_attention_tree", "rt4_verify_tree",
     "rt4_file_open", "rt4_file_close", "rt4_file_count", "rt4_file_find", "rt4_file_info", "rt4_file_data",
     "rt4_file_size", "rt4_file_upload", "rt4_file_upload_tensor",
 )
@@ -61,6 +62,7 @@ class RT4Error(RuntimeError):
 _lib = None
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_int64
 _SIGS = {
     "rt4_quant_act_a8": [_P, _P, _P, _P, _I, _I, _P],
     "rt4_quant_act_rowwise": [_P, _P, _P, _P, _I, _I, _I, _P],
@@ -90,6 +92,9 @@ _SIGS = {
     "rt4_attention_prefill": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
     "rt4_attention_prefill_cfg": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "rt4_attention_launch_plan": [_I, _I, _I, _I, _I, _I, _I, _P, _P, _P],
+    "rt4_kv_append_rows": [_P] * 10 + [_I] * 4 + [_P],
+    "rt4_attention_tree": [_P] * 13 + [_I] * 8 + [_P],
+    "rt4_verify_tree": [_P] * 5 + [_L] + [_P] * 5 + [_L] + [_I] * 4 + [_P],
 }
 
 
@@ -449,3 +454,122 @@ def attention_prefill(qq, qsc, kc, ksc, vc, vsc, n_kv: int, off: int, ratio: int
     _check(lib().rt4_attention_prefill_cfg(_ptr(out), _ptr(qq), _ptr(qsc), _ptr(kc), _ptr(ksc), _ptr(vc),
                                            _ptr(vsc), n_q, n_kv, off, n_tile, H, ratio, kv_cap, kv_splits, _stream()))
     return out
+
+
+# ------------------------------------------------ draft and verify steps ----
+def _dev():
+    torch = _torch()
+    return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else torch.cuda.current_device()
+
+
+def _arg(t, dtype, shape, dev, name):
+    """data_ptr of a tensor that the library reads as `dtype` [shape] on the current device (packed words: int32 or uint32)."""
+    if t.shape == shape and t.is_contiguous() and t.get_device() == dev and (t.dtype is dtype or _words(t.dtype, dtype)):
+        return t.data_ptr()
+    raise RT4Error(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on device {dev}, got "
+                   f"{t.dtype} {tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
+
+
+def _words(got, want):
+    torch = _torch()
+    return got is getattr(torch, "uint32", None) and want is torch.int32
+
+
+def kv_append_rows(kc, ksc, vc, vsc, stage, kf, vf, kv_len=None, rows=None, count=None):
+    """Append rows of kf, vf f32 [B, T, H, 256] to the caches of B sequences, in place: kc int32 [B, H, cap, 32], ksc f32
+    [B, H, 2, cap], vc int32 [B, H, cap/8, 256], vsc f32 [B, H, cap/64, 256], stage f32 [B, H, 64, 256].
+
+    rows int32 [B, T] (default 0, 1, ..) and count int32 [B] (default T) choose each sequence's rows; kv_len int32 [B] are
+    the lengths once they are in (default: they start at key 0, and stage may be None: a draft tile, cap 64).  See
+    rt4_kv_append_rows in include/rt4k.h."""
+    torch = _torch()
+    dev, f32, i32 = _dev(), torch.float32, torch.int32
+    if kf.dim() != 4 or kc.dim() != 4:
+        raise RT4Error("kv_append_rows: kf is [B, T, H, 256] and kc [B, H, cap, 32]")
+    B, T, H, _ = kf.shape
+    cap = kc.shape[2]
+    _check(lib().rt4_kv_append_rows(
+        _arg(kc, i32, (B, H, cap, 32), dev, "kc"), _arg(ksc, f32, (B, H, 2, cap), dev, "ksc"),
+        _arg(vc, i32, (B, H, cap // 8, HEAD_DIM), dev, "vc"), _arg(vsc, f32, (B, H, cap // KV_TILE, HEAD_DIM), dev, "vsc"),
+        None if stage is None else _arg(stage, f32, (B, H, KV_TILE, HEAD_DIM), dev, "stage"),
+        _arg(kf, f32, (B, T, H, HEAD_DIM), dev, "kf"), _arg(vf, f32, (B, T, H, HEAD_DIM), dev, "vf"),
+        None if kv_len is None else _arg(kv_len, i32, (B,), dev, "kv_len"),
+        None if rows is None else _arg(rows, i32, (B, T), dev, "rows"),
+        None if count is None else _arg(count, i32, (B,), dev, "count"), B, T, H, cap, _stream()))
+
+
+def attention_tree(qq, qsc, kc, ksc, vc, vsc, kv_len, kd, ksd, vd, vsd, parent, ratio: int, kv_max: int | None = None,
+                   out=None, kv_splits: int = 0):
+    """Attention of the nodes of B trees (parent int32 [B, T], T <= 64) over their caches and over themselves -> out f32
+    [n_heads, TP, 256], row b*T + i for node i of sequence b.
+
+    qq int32 [n_heads, TP, 32], qsc f32 [n_heads, 2, TP] from attn_q_quant; kc .. vsc the caches (see kv_append_rows) with
+    kv_len int32 [B] keys each (kv_len None: no cache); kd .. vsd the trees' own keys, caches of 64 keys.  kv_max: the
+    longest length to plan for (default: the caches' size).  A new `out` holds nothing in rows from B*T on."""
+    torch = _torch()
+    dev, f32, i32 = _dev(), torch.float32, torch.int32
+    if qq.dim() != 3 or parent.dim() != 2 or ratio < 1 or qq.shape[0] % ratio:
+        raise RT4Error(f"attention_tree: qq {tuple(qq.shape)} [n_heads, TP, 32], parent {tuple(parent.shape)} [B, T], ratio {ratio}")
+    QH, TP, _ = qq.shape
+    B, T = parent.shape
+    H = QH // ratio
+    if kv_len is None:
+        cache, cap, kv_max = (None, None, None, None, None), 0, 0
+    else:
+        if kc.dim() != 4:
+            raise RT4Error(f"attention_tree: kc {tuple(kc.shape)} is not [B, H, cap, 32]")
+        cap = kc.shape[2]
+        kv_max = cap if kv_max is None else kv_max
+        cache = (_arg(kc, i32, (B, H, cap, 32), dev, "kc"), _arg(ksc, f32, (B, H, 2, cap), dev, "ksc"),
+                 _arg(vc, i32, (B, H, cap // 8, HEAD_DIM), dev, "vc"),
+                 _arg(vsc, f32, (B, H, cap // KV_TILE, HEAD_DIM), dev, "vsc"), _arg(kv_len, i32, (B,), dev, "kv_len"))
+    if out is None:
+        out = torch.empty((QH, TP, HEAD_DIM), dtype=f32, device=qq.device)
+    _check(lib().rt4_attention_tree(
+        _arg(out, f32, (QH, TP, HEAD_DIM), dev, "out"), _arg(qq, i32, (QH, TP, 32), dev, "qq"),
+        _arg(qsc, f32, (QH, 2, TP), dev, "qsc"), *cache, _arg(kd, i32, (B, H, KV_TILE, 32), dev, "kd"),
+        _arg(ksd, f32, (B, H, 2, KV_TILE), dev, "ksd"), _arg(vd, i32, (B, H, 8, HEAD_DIM), dev, "vd"),
+        _arg(vsd, f32, (B, H, 1, HEAD_DIM), dev, "vsd"), _arg(parent, i32, (B, T), dev, "parent"), B, T, TP, QH, ratio, cap,
+        kv_max, kv_splits, _stream()))
+    return out
+
+
+def _rows(t, rows: int, V: int, dev, name):
+    """(data_ptr, row stride) of f32 rows [rows, V] whose rows are contiguous."""
+    torch = _torch()
+    if t.dim() == 2 and t.shape == (rows, V) and t.dtype is torch.float32 and t.get_device() == dev and (V == 1 or t.stride(1) == 1):
+        return t.data_ptr(), (t.stride(0) if rows > 1 else V)
+    raise RT4Error(f"{name}: expected f32 [{rows}, {V}] with contiguous rows on device {dev}, got {t.dtype} {tuple(t.shape)} "
+                   f"strides {t.stride()} on {t.device}")
+
+
+def verify_tree(logits, draft, parent, u, temp=None, draft_probs=None, max_children: int | None = None, kv_len=None,
+                tokens=None, path=None, count=None):
+    """Which nodes of B trees the target accepts, and the token that follows -> (tokens int32 [B, T], path int32 [B, T],
+    count int32 [B]): count accepted nodes (the root included), their numbers, and the new tokens; -1 behind them.
+
+    logits f32 [B*T, V] (rows may be strided), draft and parent int32 [B, T], u f32 [B, T] uniforms in [0, 1), temp f32 [B]
+    (default 1; <= 0: greedy).  draft_probs f32 [B*T, V]: row n the distribution node n's children were drawn from, at
+    most max_children of which are tested.  kv_len int32 [B] is advanced by count.  See rt4_verify_tree in include/rt4k.h."""
+    torch = _torch()
+    dev, f32, i32 = _dev(), torch.float32, torch.int32
+    if logits.dim() != 2 or parent.dim() != 2:
+        raise RT4Error(f"verify_tree: logits {tuple(logits.shape)} [B*T, V], parent {tuple(parent.shape)} [B, T]")
+    B, T = parent.shape
+    V = logits.shape[1]
+    if (draft_probs is None) != (max_children is None):
+        raise RT4Error("verify_tree: max_children goes with draft_probs")
+    lp, ldl = _rows(logits, B * T, V, dev, "logits")
+    qp, ldq = (None, 0) if draft_probs is None else _rows(draft_probs, B * T, V, dev, "draft_probs")
+    if tokens is None:
+        tokens = torch.empty((B, T), dtype=i32, device=logits.device)
+    if path is None:
+        path = torch.empty((B, T), dtype=i32, device=logits.device)
+    if count is None:
+        count = torch.empty((B,), dtype=i32, device=logits.device)
+    _check(lib().rt4_verify_tree(
+        _arg(tokens, i32, (B, T), dev, "tokens"), _arg(path, i32, (B, T), dev, "path"), _arg(count, i32, (B,), dev, "count"),
+        None if kv_len is None else _arg(kv_len, i32, (B,), dev, "kv_len"), lp, ldl, _arg(draft, i32, (B, T), dev, "draft"),
+        _arg(parent, i32, (B, T), dev, "parent"), _arg(u, f32, (B, T), dev, "u"),
+        None if temp is None else _arg(temp, f32, (B,), dev, "temp"), qp, ldq, B, T, V, max_children or 0, _stream()))
+    return tokens, path, count
