@@ -35,7 +35,7 @@ hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 // the retired buffers of a slot add up to at most twice its final size.  Not
 // safe for concurrent calls from several threads (the reference's scratch has
 // the same property, src/k_gemv.hip:47-51).
-enum Slot { kSlotActQ = 0, kSlotActS = 1, kSlotGemmA = 2, kSlotGemmPart = 3, kSlotAttnPart = 4, kSlotGemvPart = 5, kSlotGemvCnt = 6, kSlotAttnCnt = 7, kSlotAttnKV = 8, kSlotGemmCnt = 9, kSlotVerify = 10, kSlots = 11 };
+enum Slot { kSlotActQ = 0, kSlotActS = 1, kSlotGemmA = 2, kSlotGemmPart = 3, kSlotAttnPart = 4, kSlotGemvPart = 5, kSlotGemvCnt = 6, kSlotAttnCnt = 7, kSlotAttnKV = 8, kSlotGemmCnt = 9, kSlotVerify = 10, kSlotTreePart = 11, kSlots = 12 };
 constexpr int kMaxDev = 64;
 struct Buf {
     void* p = nullptr;
@@ -831,9 +831,9 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
     if (!out || !qq || !qsc || !kd || !ksd || !vd || !vsd || !parent || (kv_len && (!kc || !ksc || !vc || !vsc)))
         return fail(RT4_E_ARG, "rt4_attention_tree: null pointer");
     if (B < 1 || B > 65535 || T < 1 || T > rt4::kTreeMaxT || (long long)TP < (long long)B * T || n_heads < 1 || n_heads > 65535 ||
-        ratio < 1 || n_heads % ratio)
-        return fail(RT4_E_SHAPE, "rt4_attention_tree: B=%d T=%d (1..64) TP=%d (at least B*T) n_heads=%d ratio=%d", B, T, TP, n_heads,
-                    ratio);
+        ratio < 1 || n_heads % ratio || (long long)B * (n_heads / ratio) > 65535)
+        return fail(RT4_E_SHAPE, "rt4_attention_tree: B=%d T=%d (1..64) TP=%d (at least B*T) n_heads=%d ratio=%d (at most 65535 KV "
+                    "heads in all)", B, T, TP, n_heads, ratio);
     if (kv_len && (kv_cap < 64 || kv_cap % 64 || kv_cap > kMaxKvCap || kv_max < 0 || kv_max > kv_cap))
         return fail(RT4_E_SHAPE, "rt4_attention_tree: kv_cap=%d (a multiple of 64, at most 16777152) kv_max=%d", kv_cap, kv_max);
     if (kv_splits < 0 || kv_splits > 64) return fail(RT4_E_ARG, "rt4_attention_tree: kv_splits=%d (0..64)", kv_splits);
@@ -842,7 +842,16 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
         !aligned(kv_len, 4))
         return fail(RT4_E_ARG, "rt4_attention_tree: misaligned pointer (out, qq, caches and draft tiles need 16 bytes)");
     const rt4::AttnTree a = {out, qq, qsc, kc, ksc, vc, vsc, kv_len, kd, ksd, vd, vsd, parent, B, T, TP, n_heads, ratio, kv_cap};
-    return hip_status(rt4::launch_attn_tree(a, as_stream(stream)), "rt4_attention_tree launch");
+    int cus = 0, rc = device_cus(&cus);
+    if (rc) return rc;
+    hipStream_t st = as_stream(stream);
+    rt4::TreePlan plan = rt4::tree_plan(B, T, n_heads, ratio, kv_len ? kv_max : 0, kv_splits, cus);
+    // under capture, as many of the automatic splits as the workspace that is there holds
+    if (!kv_splits && plan.splits > 1 && capturing(st))
+        while (plan.splits > 1 && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan))) plan.splits--;
+    void* ws = nullptr;
+    if (plan.splits > 1 && (rc = lib_scratch(kSlotTreePart, rt4::tree_part_bytes(a, plan), &ws, st))) return rc;
+    return hip_status(rt4::launch_attn_tree(a, plan, ws, st), "rt4_attention_tree launch");
 }
 
 int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_len, const float* logits, int64_t ldl,

@@ -162,7 +162,15 @@ struct AttnTree {
     const int* parent;
     int B, T, TP, n_heads, ratio, kv_cap;
 };
-hipError_t launch_attn_tree(const AttnTree& a, hipStream_t st);
+// 16-row blocks per workgroup, workgroups per (sequence, KV head) and split, KV splits.
+struct TreePlan {
+    int blocks, groups, splits;
+};
+constexpr int kTreeMaxBlocks = 3, kTreeMaxSplits = 64;
+TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_splits, int cus);
+// Workspace of the splits' states (0 for one split).
+size_t tree_part_bytes(const AttnTree& a, const TreePlan& p);
+hipError_t launch_attn_tree(const AttnTree& a, const TreePlan& p, void* ws, hipStream_t st);
 
 // Draft verification; `levels`: children tested per node where draft probabilities q are
 // given (else 1); ws: verify_ws_bytes of scratch.
