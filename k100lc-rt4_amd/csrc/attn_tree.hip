@@ -46,8 +46,10 @@ __device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
 
 // Max over the four lanes that hold one query row's keys (lanes 16 and 32 apart).
 __device__ __forceinline__ float max_groups(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
 }
 
 // 16 int8 operand bytes (16 x code) of two code dwords.
@@ -76,17 +78,31 @@ __device__ __forceinline__ v8h codes_f16(uint32_t w) {
 }
 
 constexpr float kPBits = 7.f;            // P is held times 2^7: at most 2^15 with the lazy maximum
-constexpr float kLazy = 8.f;             // the running maximum moves when a tile exceeds it by 2^8
+constexpr float kLazy = 8.f;             // the running maximum moves when a score exceeds it by 2^8
+
+// Products x[4g + r] * y[c] of four 16x16 tiles in their accumulator layout on the matrix core
+// (registers 4b + r: tile b, x from lane 16b + 4g + r, y from lane 16b + c), each rounded once.
+__device__ __forceinline__ v16f outer16(float x_of_lane, float y) {
+    const v16f z = {};
+    return __builtin_amdgcn_mfma_f32_16x16x1f32(x_of_lane, y, z, 0, 0, 0);
+}
 
 // A workgroup owns 16 NB query rows of one (sequence, KV head) -- rows r * T + i, r the head in
-// the group, i the node -- and a range of the keys' 64-key tiles, the draft tile last; its four
-// waves take every fourth tile and keep their own softmax state, joined through LDS at the end.
+// the group, i the node -- and a range of the keys' 64-key tiles, the draft tile last, two tiles a
+// step.  Wave w makes S and P of its 32 keys of a step (each K dword is unpacked once), the P
+// fragments go through LDS in operand order, and wave w multiplies them with its 64 dims of V (each
+// V dword is unpacked once), so that no state has to be joined across waves but the row sums.  A
+// step's P x V runs beside the next step's scores; two workgroups share a CU.
 template <int NB>
-__global__ __launch_bounds__(256, 1) void attn_tree_k(const AttnTree A, const TreePlan P, float* __restrict__ opart,
+__global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const TreePlan P, float* __restrict__ opart,
                                                       float2* __restrict__ mlpart) {
     constexpr int RW = 16 * NB;
-    __shared__ __align__(16) float ol[4][16][HD];
-    __shared__ float ml[2][4][RW];
+    constexpr bool QL = NB > 2;                                // Q operands in LDS instead of registers
+    __shared__ __align__(16) v8h pf[NB][4][2][64];             // P: [32 keys][high, low part][lane]
+    __shared__ __align__(16) v4i qf[QL ? NB : 1][4][64];
+    __shared__ float mx[4][RW];
+    __shared__ u64 sees_l[RW];                                 // the draft keys a row sees (0: it is no node's)
+    __shared__ size_t row_l[RW];                               // its row of qq and out
     const int tid = threadIdx.x, lane = lane_id(), w = uniform(tid >> 6), c = lane & 15, g = lane >> 4;
     // the row groups of one unit (sequence, KV head, split) on one XCD: workgroups go round the 8
     const int rg = (int)(blockIdx.x / 8) % P.groups;
@@ -99,212 +115,281 @@ __global__ __launch_bounds__(256, 1) void attn_tree_k(const AttnTree A, const Tr
     const int nt = (len + BNK - 1) / BNK;                      // tile nt is the draft tile
     const int t0 = (int)((long long)(nt + 1) * split / P.splits), t1 = (int)((long long)(nt + 1) * (split + 1) / P.splits);
 
-    // Q operands: column c of block nb is row n
-    v4i qop[NB][4];
-    float qs0[NB], qs1[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; nb++) {
-        int n = rg * RW + nb * 16 + c;
-        n = n < R ? n : R - 1;
-        const size_t head = (size_t)vh * A.ratio + n / A.T, row = (size_t)b * A.T + n % A.T;
-        const uint32_t* qr = A.qq + (head * A.TP + row) * KDW + 4 * g;
-        const v4u d0 = *reinterpret_cast<const v4u*>(qr), d1 = *reinterpret_cast<const v4u*>(qr + 16);
-        qop[nb][0] = bytes16(d0.x, d0.y);
-        qop[nb][1] = bytes16(d0.z, d0.w);
-        qop[nb][2] = bytes16(d1.x, d1.y);
-        qop[nb][3] = bytes16(d1.z, d1.w);
-        qs0[nb] = A.qsc[(head * 2) * A.TP + row] * (L2E / 256.f);   // (both operands are 16 x code)
-        qs1[nb] = A.qsc[(head * 2 + 1) * A.TP + row] * (L2E / 256.f);
+    {
+        const u64 sees = tree_sees(A.parent + (size_t)b * A.T, A.T);
+        const int n = rg * RW + tid, r = n < R ? n / A.T : 0, i = n < R ? n % A.T : 0;
+        const u64 x = __shfl(sees, i);
+        if (tid < RW) {
+            sees_l[tid] = n < R ? x : 0;
+            row_l[tid] = ((size_t)vh * A.ratio + r) * A.TP + (size_t)b * A.T + i;
+        }
+        __syncthreads();
     }
 
-    v4f O[NB][16];
-    float m[NB], l[NB];
+    // Q operands (column c of block nb is row n) and this lane's column scales: lane 16 b + c has those
+    // of group b / 2, block 2 pr + b % 2
+    v4i qop[QL ? 1 : NB][4];
+    float qs[(NB + 1) / 2], m[NB], l[NB];
+#pragma unroll
+    for (int pr = 0; pr < (NB + 1) / 2; pr++) {
+        const int nb = 2 * pr + (g & 1);
+        const size_t row = row_l[(nb < NB ? nb : 0) * 16 + c], head = row / A.TP;
+        qs[pr] = A.qsc[row + (head + (g >> 1)) * A.TP] * (L2E / 256.f);       // (both operands are 16 x code)
+    }
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        m[nb] = -1e30f;
+        m[nb] = 0.f;
         l[nb] = 0.f;
+        if (QL && (nb & 3) != w) continue;
+        const uint32_t* qr = A.qq + row_l[nb * 16 + c] * KDW + 4 * g;
+        const v4u d0 = *reinterpret_cast<const v4u*>(qr), d1 = *reinterpret_cast<const v4u*>(qr + 16);
+        v4i (&q)[4] = qop[QL ? 0 : nb];
+        q[0] = bytes16(d0.x, d0.y);
+        q[1] = bytes16(d0.z, d0.w);
+        q[2] = bytes16(d1.x, d1.y);
+        q[3] = bytes16(d1.z, d1.w);
+        if (QL)
 #pragma unroll
-        for (int t = 0; t < 16; t++) O[nb][t] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < 4; k++) qf[nb][k][lane] = q[k];
     }
+    if (QL) __syncthreads();
 
-    v4u K[4][2], V[2][4];
-    v4f ks[4][2], vs[4];
-    auto load_k = [&](int t) __attribute__((always_inline)) {
-        const bool d = t == nt;
-        const size_t cap = d ? BNK : A.kv_cap, k0 = d ? 0 : (size_t)t * BNK;
-        const uint32_t* kb = (d ? A.kd : A.kc) + (seq * cap + k0) * KDW;
-        const float* sb = (d ? A.ksd : A.ksc) + (size_t)seq * 2 * cap + k0;
-        // operand row 4g + i of subtile 2h + p is key 32h + 8g + 4p + i: a lane's scores of subtiles
-        // 2h and 2h + 1 are then one V dword's eight keys
-        const uint32_t ko = (uint32_t)((8 * (c >> 2) + (c & 3)) * KDW + 4 * g);
+    v4f O[NB][4];
 #pragma unroll
-        for (int sub = 0; sub < 4; sub++) {
-            const int at = 32 * (sub >> 1) + 4 * (sub & 1);
-            K[sub][0] = *reinterpret_cast<const v4u*>(kb + ko + at * KDW);
-            K[sub][1] = *reinterpret_cast<const v4u*>(kb + ko + at * KDW + 16);
-            ks[sub][0] = *reinterpret_cast<const v4f*>(sb + 8 * g + at);
-            ks[sub][1] = *reinterpret_cast<const v4f*>(sb + cap + 8 * g + at);
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) O[nb][j] = v4f{0.f, 0.f, 0.f, 0.f};
+
+    const int hS = w & 1;                                      // half of the tile whose scores this wave makes
+    v4u K[2][2], V[4];
+    v4f vs[2];
+    float ks[2];
+    // Loads as a scalar base and 32-bit byte offsets that stay for the whole loop.
+    // K: operand row 4g + i of subtile p is key 8g + 4p + i, so a lane's scores are the eight keys of one
+    // V dword; lane 16 b + j supplies the scales of group b / 2, row j.
+    const uint32_t ko = (uint32_t)((8 * (c >> 2) + (c & 3)) * KDW + 4 * g) * 4;
+    const uint32_t so = (uint32_t)(8 * (c >> 2) + (c & 3)) * 4;
+    // V: dim tile j, column c is dim 64w + 4c + j
+    const uint32_t vo = (uint32_t)(g * HD + 4 * c) * 4, wo = (uint32_t)(16 * c);
+    auto load_k = [&](int tp) __attribute__((always_inline)) {
+        int t = tp + (w >> 1);
+        t = t < t1 ? t : t1 - 1;
+        const bool d = t == nt;
+        const size_t cap = d ? BNK : A.kv_cap, k0 = (d ? 0 : (size_t)t * BNK) + 32 * hS;
+        const char* kb = reinterpret_cast<const char*>((d ? A.kd : A.kc) + (seq * cap + k0) * KDW);
+        const char* sb = reinterpret_cast<const char*>((d ? A.ksd : A.ksc) + (size_t)seq * 2 * cap + k0);
+#pragma unroll
+        for (int p = 0; p < 2; p++)
+#pragma unroll
+            for (int G = 0; G < 2; G++) K[p][G] = *reinterpret_cast<const v4u*>(kb + ko + (4 * p * KDW + 16 * G) * 4);
+        const uint32_t sg = so + (g >> 1) * (uint32_t)cap * 4;
+#pragma unroll
+        for (int p = 0; p < 2; p++) ks[p] = *reinterpret_cast<const float*>(sb + sg + 16 * p);
+    };
+    auto load_v = [&](int tp) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            int t = tp + x;
+            t = t < t1 ? t : t1 - 1;                           // (past the range: P is zero)
+            const bool d = t == nt;
+            const size_t cap = d ? BNK : A.kv_cap, k0 = d ? 0 : (size_t)t * BNK;
+            const char* vb = reinterpret_cast<const char*>((d ? A.vd : A.vc) + (seq * (cap / 8) + k0 / 8) * HD + 64 * w);
+            const char* sb = reinterpret_cast<const char*>((d ? A.vsd : A.vsc) + (seq * (cap / BNK) + k0 / BNK) * HD + 64 * w);
+            V[2 * x] = *reinterpret_cast<const v4u*>(vb + vo);
+            V[2 * x + 1] = *reinterpret_cast<const v4u*>(vb + 4 * HD * 4 + vo);
+            vs[x] = *reinterpret_cast<const v4f*>(sb + wo);
         }
     };
-    auto load_v = [&](int t) __attribute__((always_inline)) {
-        const bool d = t == nt;
-        const size_t cap = d ? BNK : A.kv_cap, k0 = d ? 0 : (size_t)t * BNK;
-        const uint32_t* vb = (d ? A.vd : A.vc) + (seq * (cap / 8) + k0 / 8) * HD;
-        const float* sb = (d ? A.vsd : A.vsc) + (seq * (cap / BNK) + k0 / BNK) * HD;
-        // dim tile 4q + j, column c is dim 64q + 4c + j
+    float s[NB][8];
+    // S^T = K Q^T less the reference: lane (c, g) gets row c, keys 8g + 4p + i; publishes the rows' maxima
+    auto scores = [&](int tp) __attribute__((always_inline)) {
+        const int t = tp + (w >> 1);
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) V[h][q] = *reinterpret_cast<const v4u*>(vb + (4 * h + g) * HD + 64 * q + 4 * c);
-#pragma unroll
-        for (int q = 0; q < 4; q++) vs[q] = *reinterpret_cast<const v4f*>(sb + 64 * q + 4 * c);
-    };
-
-    int t = t0 + w;
-    if (t < t1) {
-        load_k(t);
-        load_v(t);
-    }
-    for (; t < t1; t += 4) {
-        // S^T = K Q^T: lane (c, g) gets row c, keys 32h + 8g + 4p + i
-        float s[NB][16];
-#pragma unroll
-        for (int sub = 0; sub < 4; sub++) {
-            const v4i a0 = bytes16(K[sub][0].x, K[sub][0].y), a1 = bytes16(K[sub][0].z, K[sub][0].w);
-            const v4i a2 = bytes16(K[sub][1].x, K[sub][1].y), a3 = bytes16(K[sub][1].z, K[sub][1].w);
+        for (int p = 0; p < 2; p++) {
+            const v4i a0 = bytes16(K[p][0].x, K[p][0].y), a1 = bytes16(K[p][0].z, K[p][0].w);
+            const v4i a2 = bytes16(K[p][1].x, K[p][1].y), a3 = bytes16(K[p][1].z, K[p][1].w);
+            v16f sc;
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
-                v4i x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-                x = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, qop[nb][0], x, 0, 0, 0);
-                y = __builtin_amdgcn_mfma_i32_16x16x64_i8(a2, qop[nb][2], y, 0, 0, 0);
-                x = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, qop[nb][1], x, 0, 0, 0);
-                y = __builtin_amdgcn_mfma_i32_16x16x64_i8(a3, qop[nb][3], y, 0, 0, 0);
+                if (NB > 2) __builtin_amdgcn_sched_barrier(0); // (or the compiler holds all blocks' operands at once and spills)
+                if (nb % 2 == 0) sc = outer16(ks[p], qs[nb / 2]);
+                const v4i z = {0, 0, 0, 0};
+                v4i x = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, QL ? qf[nb][0][lane] : qop[QL ? 0 : nb][0], z, 0, 0, 0);
+                v4i y = __builtin_amdgcn_mfma_i32_16x16x64_i8(a2, QL ? qf[nb][2][lane] : qop[QL ? 0 : nb][2], z, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, QL ? qf[nb][1][lane] : qop[QL ? 0 : nb][1], x, 0, 0, 0);
+                y = __builtin_amdgcn_mfma_i32_16x16x64_i8(a3, QL ? qf[nb][3][lane] : qop[QL ? 0 : nb][3], y, 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    s[nb][4 * sub + i] = fmaf((float)x[i] * ks[sub][0][i], qs0[nb], ((float)y[i] * ks[sub][1][i]) * qs1[nb]);
+                for (int i = 0; i < 4; i++) {
+                    float v = fmaf((float)x[i], sc[4 * (nb % 2) + i], fmaf((float)y[i], sc[8 + 4 * (nb % 2) + i], kPBits - m[nb]));
+                    asm volatile("" : "+v"(v));                // (computed here: sunk below the mask's branch, its operands of all
+                    s[nb][4 * p + i] = v;                      // blocks stay live and spill)
+                }
             }
         }
-        const int tn = t + 4;
-        const bool draft = t == nt;
-        if (tn < t1) load_k(tn);
-        if (draft || (t + 1) * BNK > len) {                    // a tile with keys that some row may not see
-            const u64 sees = draft ? tree_sees(A.parent + (size_t)b * A.T, A.T) : 0;
+        if (tp + 2 < t1) load_k(tp + 2);
+        if (t >= nt || (t + 1) * BNK > len || t >= t1) {       // keys that some row may not see
+            const u64 tail = t < nt && t < t1 ? (1ull << (len - t * BNK)) - 1 : 0;
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
-                int n = rg * RW + nb * 16 + c;
-                n = n < R ? n : R - 1;
-                u64 ok = __shfl(sees, n % A.T);
-                if (!draft) ok = (1ull << (len - t * BNK)) - 1;
-                ok >>= 8 * g;
+                u64 ok = t == nt && t < t1 ? sees_l[nb * 16 + c] : tail;
+                ok >>= 32 * hS + 8 * g;
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    if (!(ok >> (32 * (e >> 3) + (e & 7)) & 1)) s[nb][e] = -INFINITY;
+                for (int e = 0; e < 8; e++)
+                    if (!(ok >> e & 1)) s[nb][e] = -INFINITY;
             }
         }
-        v8h ph[NB][2], pl[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
             float mt = s[nb][0];
 #pragma unroll
-            for (int e = 1; e < 16; e++) mt = fmaxf(mt, s[nb][e]);
+            for (int e = 1; e < 8; e++) mt = fmaxf(mt, s[nb][e]);
             mt = max_groups(mt);
-            if (__any(mt > m[nb] + kLazy)) {
-                const float mn = fmaxf(m[nb], mt), alpha = __builtin_amdgcn_exp2f(m[nb] - mn);
-                m[nb] = mn;
-                l[nb] *= alpha;
-                float ar[4];
+            if (g == 0) mx[w][nb * 16 + c] = mt;
+        }
+    };
+    // Moves the references (all waves alike) where a score exceeds them by much, at first in any case
+    auto move = [&](bool first) __attribute__((always_inline)) {
+        float mt[NB];
+        bool any = first;
 #pragma unroll
-                for (int i = 0; i < 4; i++) ar[i] = __shfl(alpha, 4 * g + i);
+        for (int nb = 0; nb < NB; nb++) {
+            const int r = nb * 16 + c;
+            mt[nb] = fmaxf(fmaxf(mx[0][r], mx[1][r]), fmaxf(mx[2][r], mx[3][r])) - kPBits;
+            any |= mt[nb] > kLazy;
+        }
+        if (!__any(any)) return;
 #pragma unroll
-                for (int d = 0; d < 16; d++)
+        for (int nb = 0; nb < NB; nb++) {
+            // (a row that sees nothing yet keeps its reference: -inf would not come back)
+            if (NB > 2) __builtin_amdgcn_sched_barrier(0);
+            const float up = first ? (mt[nb] > -1e30f ? mt[nb] : 0.f) : fmaxf(mt[nb], 0.f);
+            m[nb] += up;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) O[nb][d][i] *= ar[i];
-            }
-            const float ref = kPBits - m[nb];
+            for (int e = 0; e < 8; e++) s[nb][e] -= up;
+            if (first) continue;
+            const float alpha = __builtin_amdgcn_exp2f(-up);
+            l[nb] *= alpha;
+            float ar[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) ar[i] = __shfl(alpha, 4 * g + i);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) O[nb][j][i] *= ar[i];
+        }
+    };
+    // P, and its fragments into LDS
+    auto weights = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            if (NB > 2) __builtin_amdgcn_sched_barrier(0);
+            v8h ph, pl;
             float sum = 0.f;
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const v2f p = {__builtin_amdgcn_exp2f(s[nb][8 * h + i] + ref), __builtin_amdgcn_exp2f(s[nb][8 * h + 4 + i] + ref)};
-                    sum += p[0] + p[1];
-                    const v2h hi = __builtin_convertvector(p, v2h);
-                    const v2f r = {p[0] - (float)hi[0], p[1] - (float)hi[1]};
-                    const v2h lo = __builtin_convertvector(r, v2h);
-                    ph[nb][h][2 * i] = hi[0];
-                    ph[nb][h][2 * i + 1] = hi[1];
-                    pl[nb][h][2 * i] = lo[0];
-                    pl[nb][h][2 * i + 1] = lo[1];
-                }
+            for (int i = 0; i < 4; i++) {
+                const v2f p = {__builtin_amdgcn_exp2f(s[nb][i]), __builtin_amdgcn_exp2f(s[nb][4 + i])};
+                sum += p[0] + p[1];
+                const v2h hi = __builtin_convertvector(p, v2h);
+                const v2f r = {p[0] - (float)hi[0], p[1] - (float)hi[1]};
+                const v2h lo = __builtin_convertvector(r, v2h);
+                ph[2 * i] = hi[0];
+                ph[2 * i + 1] = hi[1];
+                pl[2 * i] = lo[0];
+                pl[2 * i + 1] = lo[1];
+            }
             l[nb] += sum;
+            pf[nb][w][0][lane] = ph;
+            pf[nb][w][1][lane] = pl;
         }
-        // O += P V: rows 4g + i, dim 64q + 4c + j
+    };
+    // O += P V: rows 4g + i, dims 64w + 4c + j
+    auto product = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int d = 0; d < 16; d++) {
-            const v8h v0 = codes_f16(V[0][d >> 2][d & 3]), v1 = codes_f16(V[1][d >> 2][d & 3]);
+        for (int x = 0; x < 2; x++) {
+            v8h v[2][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v[0][j] = codes_f16(V[2 * x][j]);
+                v[1][j] = codes_f16(V[2 * x + 1][j]);
+            }
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
-                v4f a = {0.f, 0.f, 0.f, 0.f};
-                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[nb][0], v0, a, 0, 0, 0);
-                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[nb][0], v0, a, 0, 0, 0);
-                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[nb][1], v1, a, 0, 0, 0);
-                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[nb][1], v1, a, 0, 0, 0);
+                if (NB > 2) __builtin_amdgcn_sched_barrier(0);
+                const v8h p0 = pf[nb][2 * x][0][lane], p1 = pf[nb][2 * x][1][lane];
+                const v8h p2 = pf[nb][2 * x + 1][0][lane], p3 = pf[nb][2 * x + 1][1][lane];
 #pragma unroll
-                for (int i = 0; i < 4; i++) O[nb][d][i] = fmaf(a[i], vs[d >> 2][d & 3], O[nb][d][i]);
+                for (int j = 0; j < 4; j++) {
+                    v4f a = {0.f, 0.f, 0.f, 0.f};
+                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, v[0][j], a, 0, 0, 0);
+                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(p1, v[0][j], a, 0, 0, 0);
+                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(p2, v[1][j], a, 0, 0, 0);
+                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(p3, v[1][j], a, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        float o = fmaf(a[i], vs[x][j], O[nb][j][i]);
+                        if (x) asm volatile("" : "+v"(o));     // (nor are these, below the branch of the references)
+                        O[nb][j][i] = o;
+                    }
+                }
             }
         }
-        if (tn < t1) load_v(tn);
+    };
+
+    if (t0 < t1) {
+        load_k(t0);
+        load_v(t0);
+        scores(t0);
+        __syncthreads();
+        move(true);
+        weights();
+        __syncthreads();
+        for (int tp = t0 + 2; tp < t1; tp += 2) {
+            product();
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(tp);
+            scores(tp);
+            __syncthreads();                                   // the fragments are read, the maxima are there
+            move(false);
+            weights();
+            __syncthreads();
+        }
+        product();
     }
 
-    // join the waves
+    // row sums of the four waves; every wave holds the same references
+    __syncthreads();
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        float s = l[nb] + __shfl_xor(l[nb], 16);
-        s += __shfl_xor(s, 32);
-        if (g == 0) {
-            ml[0][w][nb * 16 + c] = m[nb];
-            ml[1][w][nb * 16 + c] = s;
-        }
+        float t = l[nb] + __shfl_xor(l[nb], 16);
+        t += __shfl_xor(t, 32);
+        if (g == 0) mx[w][nb * 16 + c] = t;
     }
-    const u64 sees = P.splits == 1 ? tree_sees(A.parent + (size_t)b * A.T, A.T) : 0;
-    const size_t prow = (size_t)unit * P.groups * RW + rg * RW;
+    __syncthreads();
+    const size_t prow = ((size_t)unit * P.groups + rg) * RW;
+    if (P.splits > 1) {
 #pragma unroll
-    for (int nb = 0; nb < NB; nb++) {
-        if (nb) __syncthreads();
-#pragma unroll
-        for (int q = 0; q < 4; q++)
+        for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                *reinterpret_cast<v4f*>(&ol[w][4 * g + i][64 * q + 4 * c]) =
-                    v4f{O[nb][4 * q][i], O[nb][4 * q + 1][i], O[nb][4 * q + 2][i], O[nb][4 * q + 3][i]};
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int r = 4 * k + w, n = rg * RW + nb * 16 + r;      // wave w joins row r, lane 4 dims
-            float M = ml[0][0][nb * 16 + r];
-            for (int x = 1; x < 4; x++) M = fmaxf(M, ml[0][x][nb * 16 + r]);
-            v4f o = {0.f, 0.f, 0.f, 0.f};
-            float ls = 0.f;
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const float f = __builtin_amdgcn_exp2f(ml[0][x][nb * 16 + r] - M);
-                ls = fmaf(ml[1][x][nb * 16 + r], f, ls);
-                const v4f v = *reinterpret_cast<const v4f*>(&ol[x][r][4 * lane]);
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[i] = fmaf(v[i], f, o[i]);
-            }
-            if (P.splits > 1) {
-                *reinterpret_cast<v4f*>(opart + (prow + nb * 16 + r) * HD + 4 * lane) = o;
-                if (lane == 0) mlpart[prow + nb * 16 + r] = make_float2(M, ls);
-            } else if (n < R) {
-                const int i = n % A.T;
-                const bool live = __shfl(sees, i) != 0;
-                const size_t head = (size_t)vh * A.ratio + n / A.T;
-                float* dst = A.out + (head * A.TP + (size_t)b * A.T + i) * HD + 4 * lane;
-                *reinterpret_cast<v4f*>(dst) = live ? v4f{o[0] / ls, o[1] / ls, o[2] / ls, o[3] / ls} : v4f{0.f, 0.f, 0.f, 0.f};
+                *reinterpret_cast<v4f*>(opart + (prow + nb * 16 + 4 * g + i) * HD + 64 * w + 4 * c) =
+                    v4f{O[nb][0][i], O[nb][1][i], O[nb][2][i], O[nb][3][i]};
+            if (w == 0 && g == 0) {
+                const int r = nb * 16 + c;
+                mlpart[prow + r] = make_float2(t0 < t1 ? m[nb] : -1e30f, mx[0][r] + mx[1][r] + mx[2][r] + mx[3][r]);
             }
         }
+        return;
     }
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = nb * 16 + 4 * g + i;
+            if (rg * RW + r >= R) continue;
+            const float ls = mx[0][r] + mx[1][r] + mx[2][r] + mx[3][r];
+            *reinterpret_cast<v4f*>(A.out + row_l[r] * HD + 64 * w + 4 * c) =
+                sees_l[r] ? v4f{O[nb][0][i] / ls, O[nb][1][i] / ls, O[nb][2][i] / ls, O[nb][3][i] / ls} : v4f{0.f, 0.f, 0.f, 0.f};
+        }
 }
 
 // Sums the splits' states: one wave per row, four dims a lane.
@@ -326,7 +411,7 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o);
     v4f o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
+#pragma unroll 4
     for (int s = 0; s < P.splits; s++) {
         const v4f v = *reinterpret_cast<const v4f*>(opart + (row + s * step) * HD + 4 * lane);
         const float fs = __shfl(f, s);
@@ -343,17 +428,17 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
 TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_splits, int cus) {
     const int R = T * ratio;
     TreePlan p = {1, 1, 1};
-    // rows per workgroup: 1400 cycles of unpacking a tile against about 2000 per block of 16 rows
+    // rows per workgroup: unpacking a tile costs about as much as two blocks of 16 rows
     long best = 0;
     for (int nb = 1; nb <= kTreeMaxBlocks; nb++) {
         const int rg = (R + 16 * nb - 1) / (16 * nb);
-        const long cost = (long)rg * (1400 + 2000 * nb);
+        const long cost = (long)rg * (2 + nb);
         if (nb == 1 || cost < best) best = cost, p.blocks = nb, p.groups = rg;
     }
     const long units = (long)B * (n_heads / ratio) * p.groups;
     const long tiles = kv_max / BNK + 2;
-    long s = kv_splits ? kv_splits : cus / units;
-    if (!kv_splits && s > (tiles + 3) / 4) s = (tiles + 3) / 4;      // a tile for every wave
+    long s = kv_splits ? kv_splits : 2 * cus / units;
+    if (!kv_splits && s > (tiles + 1) / 2) s = (tiles + 1) / 2;
     p.splits = s < 1 ? 1 : s > kTreeMaxSplits ? kTreeMaxSplits : (int)s;
     return p;
 }
@@ -373,7 +458,9 @@ hipError_t launch_attn_tree(const AttnTree& a, const TreePlan& p, void* ws, hipS
     switch (p.blocks) {
         case 1: hipLaunchKernelGGL(attn_tree_k<1>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
         case 2: hipLaunchKernelGGL(attn_tree_k<2>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
-        default: hipLaunchKernelGGL(attn_tree_k<3>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
+        case 3: hipLaunchKernelGGL(attn_tree_k<3>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
+        case 4: hipLaunchKernelGGL(attn_tree_k<4>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
+        default: hipLaunchKernelGGL(attn_tree_k<5>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
     }
     if (p.splits > 1)
         hipLaunchKernelGGL(attn_tree_join_k, dim3((a.T * a.ratio + 3) / 4, a.B * KVH), dim3(256), 0, st, a, p, opart, mlpart);
