@@ -57,13 +57,13 @@ __device__ __forceinline__ v4i bytes16(uint32_t a, uint32_t b) {
     return v4i{(int)even_x16(a), (int)odd_x16(a), (int)even_x16(b), (int)odd_x16(b)};
 }
 
-// The eight codes of a V dword as fp16, key pairs (0,4) (1,5) (2,6) (3,7): the nibble + 8 under
-// the exponent of 1024 is 1024 + u (or 1024 + 16 u one nibble up), from which a packed add (or
-// fma) takes the code exactly.
+// The eight codes of a V dword as fp16, key pairs (0,4) (1,5) (2,6) (3,7): a nibble with its sign
+// bit flipped is u = code + 8, and under the exponent of 1024 it reads 1024 + u (1024 + 16 u one
+// nibble up), from which a packed add (or fma) takes the code exactly.
 __device__ __forceinline__ v8h codes_f16(uint32_t w) {
-    const uint32_t x = w ^ 0x88888888u, y = x >> 8;
-    const uint32_t t[4] = {(x & 0x000F000Fu) | 0x64006400u, (x & 0x00F000F0u) | 0x64006400u, (y & 0x000F000Fu) | 0x64006400u,
-                           (y & 0x00F000F0u) | 0x64006400u};
+    const uint32_t y = w >> 8;
+    const uint32_t t[4] = {(w & 0x000F000Fu) ^ 0x64086408u, (w & 0x00F000F0u) ^ 0x64806480u, (y & 0x000F000Fu) ^ 0x64086408u,
+                           (y & 0x00F000F0u) ^ 0x64806480u};
     union {
         v2h p[4];
         v8h v;
@@ -75,6 +75,18 @@ __device__ __forceinline__ v8h codes_f16(uint32_t w) {
                          : a + v2h{(_Float16)-1032.f, (_Float16)-1032.f};
     }
     return r.v;
+}
+
+// p + n elements in bytes, held in scalar registers (or the compiler loads the pointers from the
+// kernel's arguments again at every use).
+template <class T>
+__device__ __forceinline__ const char* at(const T* p, size_t n) {
+    const char* r = reinterpret_cast<const char*>(sptr(p + n));
+    asm volatile("" : "+s"(r));
+    return r;
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const char* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, bytes, 0x00020000);     // 32-bit data format
 }
 
 constexpr float kPBits = 7.f;            // P is held times 2^7: at most 2^15 with the lazy maximum
@@ -115,33 +127,75 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
     const int nt = (len + BNK - 1) / BNK;                      // tile nt is the draft tile
     const int t0 = (int)((long long)(nt + 1) * split / P.splits), t1 = (int)((long long)(nt + 1) * (split + 1) / P.splits);
 
-    {
-        const u64 sees = tree_sees(A.parent + (size_t)b * A.T, A.T);
-        const int n = rg * RW + tid, r = n < R ? n / A.T : 0, i = n < R ? n % A.T : 0;
-        const u64 x = __shfl(sees, i);
-        if (tid < RW) {
-            sees_l[tid] = n < R ? x : 0;
-            row_l[tid] = ((size_t)vh * A.ratio + r) * A.TP + (size_t)b * A.T + i;
+    const int hS = w & 1;                                      // half of the tile whose scores this wave makes
+    v4u K[2][2], V[4];
+    v4f vs[2];
+    float ks[2];
+    // Buffer loads: a per-lane offset that stays for the whole loop and a scalar offset per tile (a KV
+    // head's cache is below 2^31 bytes), from the cache or the draft tile.
+    // K: operand row 4g + i of subtile p is key 8g + 4p + i, so a lane's scores are the eight keys of one
+    // V dword; lane 16 b + j supplies the scales of group b / 2, row j.  V: dim tile j, column c is dim
+    // 64w + 4c + j.
+    const char *kc = at(A.kc, (size_t)seq * A.kv_cap * KDW), *kd = at(A.kd, (size_t)seq * BNK * KDW);
+    const char *ksc = at(A.ksc, (size_t)seq * 2 * A.kv_cap), *ksd = at(A.ksd, (size_t)seq * 2 * BNK);
+    const char *vc = at(A.vc, (size_t)seq * (A.kv_cap / 8) * HD), *vd = at(A.vd, (size_t)seq * (BNK / 8) * HD);
+    const char *vsc = at(A.vsc, (size_t)seq * (A.kv_cap / BNK) * HD), *vsd = at(A.vsd, (size_t)seq * HD);
+    const int ko = ((8 * (c >> 2) + (c & 3)) * KDW + 4 * g) * 4 + 32 * hS * KDW * 4;
+    const int so = (8 * (c >> 2) + (c & 3) + 32 * hS) * 4;
+    const int vo = (g * HD + 4 * c + 64 * w) * 4, wo = (4 * c + 64 * w) * 4;
+    auto load_k = [&](int tp) __attribute__((always_inline)) {
+        int t = tp + (w >> 1);
+        t = t < t1 ? t : t1 - 1;
+        const bool d = t == nt;
+        const int cap = d ? BNK : A.kv_cap;
+        const auto rk = rsrc(d ? kd : kc, cap * KDW * 4), rs = rsrc(d ? ksd : ksc, 2 * cap * 4);
+        const int k0 = d ? 0 : t * BNK;
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+#pragma unroll
+            for (int G = 0; G < 2; G++)
+                K[p][G] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rk, ko + (4 * p * KDW + 16 * G) * 4, k0 * (KDW * 4), 0));
+            ks[p] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, so + 16 * p + (g >> 1) * cap * 4, k0 * 4, 0));
         }
-        __syncthreads();
+    };
+    auto load_v = [&](int tp, int x) __attribute__((always_inline)) {
+        int t = tp + x;
+        t = t < t1 ? t : t1 - 1;                               // (past the range: P is zero)
+        const bool d = t == nt;
+        const auto rv = rsrc(d ? vd : vc, (d ? BNK : A.kv_cap) / 8 * HD * 4);
+        const int t8 = d ? 0 : t * (BNK / 8 * HD * 4);
+        V[2 * x] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rv, vo, t8, 0));
+        V[2 * x + 1] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rv, vo, t8 + 4 * HD * 4, 0));
+    };
+    auto load_vs = [&](int tp, int x) __attribute__((always_inline)) {
+        int t = tp + x;
+        t = t < t1 ? t : t1 - 1;
+        const bool d = t == nt;
+        const auto rs = rsrc(d ? vsd : vsc, (d ? 1 : A.kv_cap / BNK) * HD * 4);
+        vs[x] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, wo, d ? 0 : t * (HD * 4), 0));
+    };
+    if (t0 < t1) {                                             // (in flight while the rows are set up)
+        load_k(t0);
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            load_v(t0, x);
+            load_vs(t0, x);
+        }
     }
-
     // Q operands (column c of block nb is row n) and this lane's column scales: lane 16 b + c has those
     // of group b / 2, block 2 pr + b % 2
+    auto row_of = [&](int n) __attribute__((always_inline)) {      // of qq and out
+        n = n < R ? n : 0;
+        return ((size_t)vh * A.ratio + n / A.T) * A.TP + (size_t)b * A.T + n % A.T;
+    };
     v4i qop[QL ? 1 : NB][4];
     float qs[(NB + 1) / 2], m[NB], l[NB];
-#pragma unroll
-    for (int pr = 0; pr < (NB + 1) / 2; pr++) {
-        const int nb = 2 * pr + (g & 1);
-        const size_t row = row_l[(nb < NB ? nb : 0) * 16 + c], head = row / A.TP;
-        qs[pr] = A.qsc[row + (head + (g >> 1)) * A.TP] * (L2E / 256.f);       // (both operands are 16 x code)
-    }
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
         m[nb] = 0.f;
         l[nb] = 0.f;
         if (QL && (nb & 3) != w) continue;
-        const uint32_t* qr = A.qq + row_l[nb * 16 + c] * KDW + 4 * g;
+        const uint32_t* qr = A.qq + row_of(rg * RW + nb * 16 + c) * KDW + 4 * g;
         const v4u d0 = *reinterpret_cast<const v4u*>(qr), d1 = *reinterpret_cast<const v4u*>(qr + 16);
         v4i (&q)[4] = qop[QL ? 0 : nb];
         q[0] = bytes16(d0.x, d0.y);
@@ -152,7 +206,22 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
 #pragma unroll
             for (int k = 0; k < 4; k++) qf[nb][k][lane] = q[k];
     }
-    if (QL) __syncthreads();
+#pragma unroll
+    for (int pr = 0; pr < (NB + 1) / 2; pr++) {
+        const int nb = 2 * pr + (g & 1), n = rg * RW + (nb < NB ? nb : 0) * 16 + c;
+        const size_t head = (size_t)vh * A.ratio + (n < R ? n : 0) / A.T;
+        qs[pr] = A.qsc[row_of(n) + (head + (g >> 1)) * A.TP] * (L2E / 256.f);     // (both operands are 16 x code)
+    }
+    {
+        const u64 sees = tree_sees(A.parent + (size_t)b * A.T, A.T);
+        const int n = rg * RW + tid;
+        const u64 x = __shfl(sees, (n < R ? n : 0) % A.T);
+        if (tid < RW) {
+            sees_l[tid] = n < R ? x : 0;
+            row_l[tid] = row_of(n);
+        }
+    }
+    __syncthreads();
 
     v4f O[NB][4];
 #pragma unroll
@@ -160,46 +229,6 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
 #pragma unroll
         for (int j = 0; j < 4; j++) O[nb][j] = v4f{0.f, 0.f, 0.f, 0.f};
 
-    const int hS = w & 1;                                      // half of the tile whose scores this wave makes
-    v4u K[2][2], V[4];
-    v4f vs[2];
-    float ks[2];
-    // Loads as a scalar base and 32-bit byte offsets that stay for the whole loop.
-    // K: operand row 4g + i of subtile p is key 8g + 4p + i, so a lane's scores are the eight keys of one
-    // V dword; lane 16 b + j supplies the scales of group b / 2, row j.
-    const uint32_t ko = (uint32_t)((8 * (c >> 2) + (c & 3)) * KDW + 4 * g) * 4;
-    const uint32_t so = (uint32_t)(8 * (c >> 2) + (c & 3)) * 4;
-    // V: dim tile j, column c is dim 64w + 4c + j
-    const uint32_t vo = (uint32_t)(g * HD + 4 * c) * 4, wo = (uint32_t)(16 * c);
-    auto load_k = [&](int tp) __attribute__((always_inline)) {
-        int t = tp + (w >> 1);
-        t = t < t1 ? t : t1 - 1;
-        const bool d = t == nt;
-        const size_t cap = d ? BNK : A.kv_cap, k0 = (d ? 0 : (size_t)t * BNK) + 32 * hS;
-        const char* kb = reinterpret_cast<const char*>((d ? A.kd : A.kc) + (seq * cap + k0) * KDW);
-        const char* sb = reinterpret_cast<const char*>((d ? A.ksd : A.ksc) + (size_t)seq * 2 * cap + k0);
-#pragma unroll
-        for (int p = 0; p < 2; p++)
-#pragma unroll
-            for (int G = 0; G < 2; G++) K[p][G] = *reinterpret_cast<const v4u*>(kb + ko + (4 * p * KDW + 16 * G) * 4);
-        const uint32_t sg = so + (g >> 1) * (uint32_t)cap * 4;
-#pragma unroll
-        for (int p = 0; p < 2; p++) ks[p] = *reinterpret_cast<const float*>(sb + sg + 16 * p);
-    };
-    auto load_v = [&](int tp) __attribute__((always_inline)) {
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            int t = tp + x;
-            t = t < t1 ? t : t1 - 1;                           // (past the range: P is zero)
-            const bool d = t == nt;
-            const size_t cap = d ? BNK : A.kv_cap, k0 = d ? 0 : (size_t)t * BNK;
-            const char* vb = reinterpret_cast<const char*>((d ? A.vd : A.vc) + (seq * (cap / 8) + k0 / 8) * HD + 64 * w);
-            const char* sb = reinterpret_cast<const char*>((d ? A.vsd : A.vsc) + (seq * (cap / BNK) + k0 / BNK) * HD + 64 * w);
-            V[2 * x] = *reinterpret_cast<const v4u*>(vb + vo);
-            V[2 * x + 1] = *reinterpret_cast<const v4u*>(vb + 4 * HD * 4 + vo);
-            vs[x] = *reinterpret_cast<const v4f*>(sb + wo);
-        }
-    };
     float s[NB][8];
     // S^T = K Q^T less the reference: lane (c, g) gets row c, keys 8g + 4p + i; publishes the rows' maxima
     auto scores = [&](int tp) __attribute__((always_inline)) {
@@ -226,7 +255,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
                 }
             }
         }
-        if (tp + 2 < t1) load_k(tp + 2);
+        load_k(tp + 2);
         if (t >= nt || (t + 1) * BNK > len || t >= t1) {       // keys that some row may not see
             const u64 tail = t < nt && t < t1 ? (1ull << (len - t * BNK)) - 1 : 0;
 #pragma unroll
@@ -303,7 +332,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
         }
     };
     // O += P V: rows 4g + i, dims 64w + 4c + j
-    auto product = [&]() __attribute__((always_inline)) {
+    auto product = [&](int tn) __attribute__((always_inline)) {    // (then loads step tn's V)
 #pragma unroll
         for (int x = 0; x < 2; x++) {
             v8h v[2][4];
@@ -312,6 +341,8 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
                 v[0][j] = codes_f16(V[2 * x][j]);
                 v[1][j] = codes_f16(V[2 * x + 1][j]);
             }
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(tn, x);
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
                 if (NB > 2) __builtin_amdgcn_sched_barrier(0);
@@ -332,28 +363,26 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
                     }
                 }
             }
+            load_vs(tn, x);
         }
     };
 
     if (t0 < t1) {
-        load_k(t0);
-        load_v(t0);
         scores(t0);
         __syncthreads();
         move(true);
         weights();
         __syncthreads();
         for (int tp = t0 + 2; tp < t1; tp += 2) {
-            product();
+            product(tp);
             __builtin_amdgcn_sched_barrier(0);
-            load_v(tp);
             scores(tp);
             __syncthreads();                                   // the fragments are read, the maxima are there
             move(false);
             weights();
             __syncthreads();
         }
-        product();
+        product(t1);
     }
 
     // row sums of the four waves; every wave holds the same references
@@ -371,8 +400,9 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
         for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                *reinterpret_cast<v4f*>(opart + (prow + nb * 16 + 4 * g + i) * HD + 64 * w + 4 * c) =
-                    v4f{O[nb][0][i], O[nb][1][i], O[nb][2][i], O[nb][3][i]};
+                if (rg * RW + nb * 16 + 4 * g + i < R)
+                    *reinterpret_cast<v4f*>(opart + (prow + nb * 16 + 4 * g + i) * HD + 64 * w + 4 * c) =
+                        v4f{O[nb][0][i], O[nb][1][i], O[nb][2][i], O[nb][3][i]};
             if (w == 0 && g == 0) {
                 const int r = nb * 16 + c;
                 mlpart[prow + r] = make_float2(t0 < t1 ? m[nb] : -1e30f, mx[0][r] + mx[1][r] + mx[2][r] + mx[3][r]);
@@ -392,17 +422,21 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
         }
 }
 
-// Sums the splits' states: one wave per row, four dims a lane.
+// Sums the splits' states: one workgroup per row, each wave a quarter of the splits (all of a
+// wave's loads in flight at once), four dims a lane.
 __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const TreePlan P, const float* __restrict__ opart,
                                                         const float2* __restrict__ mlpart) {
-    const int KVH = A.n_heads / A.ratio, R = A.T * A.ratio, lane = lane_id();
-    const int n = (int)blockIdx.x * 4 + uniform(threadIdx.x >> 6), seq = blockIdx.y, b = seq / KVH, vh = seq % KVH;
-    if (n >= R) return;
-    const int i = n % A.T;
-    const bool live = __shfl(tree_sees(A.parent + (size_t)b * A.T, A.T), i) != 0;
+    __shared__ __align__(16) v4f ol[4][64];
+    const int KVH = A.n_heads / A.ratio, lane = lane_id(), w = uniform(threadIdx.x >> 6);
+    const int n = blockIdx.x, seq = blockIdx.y, b = seq / KVH, vh = seq % KVH, i = n % A.T;
     const size_t step = (size_t)P.groups * 16 * P.blocks, row = (size_t)seq * P.splits * step + n;
     // lane s has split s's state
     const float2 x = lane < P.splits ? mlpart[row + lane * step] : make_float2(-1e30f, 0.f);
+    const bool live = __shfl(tree_sees(A.parent + (size_t)b * A.T, A.T), i) != 0;
+    const float* src = opart + (row + w * step) * HD + 4 * lane;
+    v4f v[kTreeMaxSplits / 4];
+#pragma unroll
+    for (int k = 0; k < kTreeMaxSplits / 4; k++) v[k] = w + 4 * k < P.splits ? *reinterpret_cast<const v4f*>(src + 4 * k * step * HD) : v4f{};
     float M = x.x;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
@@ -411,13 +445,18 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o);
     v4f o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < P.splits; s++) {
-        const v4f v = *reinterpret_cast<const v4f*>(opart + (row + s * step) * HD + 4 * lane);
-        const float fs = __shfl(f, s);
 #pragma unroll
-        for (int k = 0; k < 4; k++) o[k] = fmaf(v[k], fs, o[k]);
+    for (int k = 0; k < kTreeMaxSplits / 4; k++) {
+        if (w + 4 * k >= P.splits) break;
+        const float fs = __shfl(f, w + 4 * k);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = fmaf(v[k][e], fs, o[e]);
     }
+    ol[w][lane] = o;
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int k = 1; k < 4; k++) o += ol[k][lane];
     const size_t head = (size_t)vh * A.ratio + n / A.T;
     *reinterpret_cast<v4f*>(A.out + (head * A.TP + (size_t)b * A.T + i) * HD + 4 * lane) =
         live ? v4f{o[0] / ls, o[1] / ls, o[2] / ls, o[3] / ls} : v4f{0.f, 0.f, 0.f, 0.f};
@@ -460,10 +499,11 @@ hipError_t launch_attn_tree(const AttnTree& a, const TreePlan& p, void* ws, hipS
         case 2: hipLaunchKernelGGL(attn_tree_k<2>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
         case 3: hipLaunchKernelGGL(attn_tree_k<3>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
         case 4: hipLaunchKernelGGL(attn_tree_k<4>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
-        default: hipLaunchKernelGGL(attn_tree_k<5>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
+        case 5: hipLaunchKernelGGL(attn_tree_k<5>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
+        default: hipLaunchKernelGGL(attn_tree_k<6>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
     }
     if (p.splits > 1)
-        hipLaunchKernelGGL(attn_tree_join_k, dim3((a.T * a.ratio + 3) / 4, a.B * KVH), dim3(256), 0, st, a, p, opart, mlpart);
+        hipLaunchKernelGGL(attn_tree_join_k, dim3(a.T * a.ratio, a.B * KVH), dim3(256), 0, st, a, p, opart, mlpart);
     return hipGetLastError();
 }
 
