@@ -328,7 +328,7 @@ int rt4_kv_append_rows(uint32_t* kc, float* ksc, uint32_t* vc, float* vsc, float
  * padding nodes and of idle sequences are zeros; rows from B*T on are left as they were.
  * kv_len int32 [B] on the device, clamped to [0, kv_cap]; NULL: no cache (kc, ksc, vc, vsc
  * are not read).  kv_max: the longest length to plan for (a longer one is still right).
- * kv_splits: parts the keys are split into, 0 chooses (at most 64). */
+ * kv_splits: parts the keys are split into, 0 chooses (at most 128). */
 int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const uint32_t* kc, const float* ksc,
                        const uint32_t* vc, const float* vsc, const int32_t* kv_len, const uint32_t* kd, const float* ksd,
                        const uint32_t* vd, const float* vsd, const int32_t* parent, int B, int T, int TP, int n_heads,

@@ -52,6 +52,17 @@ __device__ __forceinline__ float max_groups(float v) {
     return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
 }
 
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ float wave_add(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
 // 16 int8 operand bytes (16 x code) of two code dwords.
 __device__ __forceinline__ v4i bytes16(uint32_t a, uint32_t b) {
     return v4i{(int)even_x16(a), (int)odd_x16(a), (int)even_x16(b), (int)odd_x16(b)};
@@ -238,15 +249,23 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
             const v4i a0 = bytes16(K[p][0].x, K[p][0].y), a1 = bytes16(K[p][0].z, K[p][0].w);
             const v4i a2 = bytes16(K[p][1].x, K[p][1].y), a3 = bytes16(K[p][1].z, K[p][1].w);
             v16f sc;
+            v4i qn[4];                                         // the next block's operands, read while this one's are in use
+            auto read_q = [&](int nb) __attribute__((always_inline)) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) qn[k] = QL ? qf[nb][k][lane] : qop[QL ? 0 : nb][k];
+            };
+            read_q(0);
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
+                const v4i q0 = qn[0], q1 = qn[1], q2 = qn[2], q3 = qn[3];
+                if (nb + 1 < NB) read_q(nb + 1);
                 if (NB > 2) __builtin_amdgcn_sched_barrier(0); // (or the compiler holds all blocks' operands at once and spills)
                 if (nb % 2 == 0) sc = outer16(ks[p], qs[nb / 2]);
                 const v4i z = {0, 0, 0, 0};
-                v4i x = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, QL ? qf[nb][0][lane] : qop[QL ? 0 : nb][0], z, 0, 0, 0);
-                v4i y = __builtin_amdgcn_mfma_i32_16x16x64_i8(a2, QL ? qf[nb][2][lane] : qop[QL ? 0 : nb][2], z, 0, 0, 0);
-                x = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, QL ? qf[nb][1][lane] : qop[QL ? 0 : nb][1], x, 0, 0, 0);
-                y = __builtin_amdgcn_mfma_i32_16x16x64_i8(a3, QL ? qf[nb][3][lane] : qop[QL ? 0 : nb][3], y, 0, 0, 0);
+                v4i x = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, q0, z, 0, 0, 0);
+                v4i y = __builtin_amdgcn_mfma_i32_16x16x64_i8(a2, q2, z, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, q1, x, 0, 0, 0);
+                y = __builtin_amdgcn_mfma_i32_16x16x64_i8(a3, q3, y, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     float v = fmaf((float)x[i], sc[4 * (nb % 2) + i], fmaf((float)y[i], sc[8 + 4 * (nb % 2) + i], kPBits - m[nb]));
@@ -332,7 +351,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
         }
     };
     // O += P V: rows 4g + i, dims 64w + 4c + j
-    auto product = [&](int tn) __attribute__((always_inline)) {    // (then loads step tn's V)
+    auto product = [&](int tn) __attribute__((always_inline)) {
 #pragma unroll
         for (int x = 0; x < 2; x++) {
             v8h v[2][4];
@@ -343,11 +362,17 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
             }
             __builtin_amdgcn_sched_barrier(0);
             load_v(tn, x);
+            v8h pn[4];                                         // likewise
+            auto read_p = [&](int nb) __attribute__((always_inline)) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) pn[k] = pf[nb][2 * x + k / 2][k % 2][lane];
+            };
+            read_p(0);
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
+                const v8h p0 = pn[0], p1 = pn[1], p2 = pn[2], p3 = pn[3];
+                if (nb + 1 < NB) read_p(nb + 1);
                 if (NB > 2) __builtin_amdgcn_sched_barrier(0);
-                const v8h p0 = pf[nb][2 * x][0][lane], p1 = pf[nb][2 * x][1][lane];
-                const v8h p2 = pf[nb][2 * x + 1][0][lane], p3 = pf[nb][2 * x + 1][1][lane];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     v4f a = {0.f, 0.f, 0.f, 0.f};
@@ -430,27 +455,33 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
     const int KVH = A.n_heads / A.ratio, lane = lane_id(), w = uniform(threadIdx.x >> 6);
     const int n = blockIdx.x, seq = blockIdx.y, b = seq / KVH, vh = seq % KVH, i = n % A.T;
     const size_t step = (size_t)P.groups * 16 * P.blocks, row = (size_t)seq * P.splits * step + n;
-    // lane s has split s's state
-    const float2 x = lane < P.splits ? mlpart[row + lane * step] : make_float2(-1e30f, 0.f);
+    // lane s has the states of splits s and s + 64
+    float2 x[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) x[k] = lane + 64 * k < P.splits ? mlpart[row + (lane + 64 * k) * step] : make_float2(-1e30f, 0.f);
     const bool live = __shfl(tree_sees(A.parent + (size_t)b * A.T, A.T), i) != 0;
     const float* src = opart + (row + w * step) * HD + 4 * lane;
-    v4f v[kTreeMaxSplits / 4];
+    v4f v[16];
+    auto read = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < kTreeMaxSplits / 4; k++) v[k] = w + 4 * k < P.splits ? *reinterpret_cast<const v4f*>(src + 4 * k * step * HD) : v4f{};
-    float M = x.x;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-    const float f = __builtin_amdgcn_exp2f(x.x - M);
-    float ls = x.y * f;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o);
+        for (int k = 0; k < 16; k++) v[k] = w + 64 * h + 4 * k < P.splits ? *reinterpret_cast<const v4f*>(src + (64 * h + 4 * k) * step * HD) : v4f{};
+    };
+    read(0);
+    const float M = wave_max(fmaxf(x[0].x, x[1].x));
+    const float f[2] = {__builtin_amdgcn_exp2f(x[0].x - M), __builtin_amdgcn_exp2f(x[1].x - M)};
+    const float ls = wave_add(x[0].y * f[0] + x[1].y * f[1]);
     v4f o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < kTreeMaxSplits / 4; k++) {
-        if (w + 4 * k >= P.splits) break;
-        const float fs = __shfl(f, w + 4 * k);
+    for (int h = 0; h < 2; h++) {
+        if (h && P.splits <= 64) break;
+        if (h) read(1);
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = fmaf(v[k][e], fs, o[e]);
+        for (int k = 0; k < 16; k++) {
+            if (w + 64 * h + 4 * k >= P.splits) break;
+            const float fs = __shfl(f[h], w + 4 * k);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = fmaf(v[k][e], fs, o[e]);
+        }
     }
     ol[w][lane] = o;
     __syncthreads();
@@ -464,21 +495,35 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
 
 }  // namespace
 
+// The rows per workgroup and the splits by a model of the time in us, fitted to sweeps of both over
+// 1 to 16 sequences of 1000 to 131001 keys and 1 to 64 nodes (off by 8% on average): a step of two
+// tiles takes 1.7, 2.1 or 2.9 (1 to 3 blocks) with one workgroup on a CU and 2.0, 3.05 or 4.2 with
+// two, all steps together at least the cache's bytes at 4.2 TB/s, the joining launch 3 and its states
+// (1 KB a row and split, written and read) 0.3 a MB.  A unit's row groups stay on one XCD (an eighth
+// of the CUs), so the XCD with the most units decides.  (4 to 6 blocks fit too: 276 to 283 us where 3
+// take 283, 64 nodes over 131001 keys, and 43 against 37, 16 nodes over 32000.  A join in the same
+// launch by the last workgroup of a row group took 14 us where both launches take 10: one node over
+// 1000 keys.)
 TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_splits, int cus) {
-    const int R = T * ratio;
+    constexpr double one[] = {1.7, 2.1, 2.9}, two[] = {2.0, 3.05, 4.2};
+    const int R = T * ratio, tiles = kv_max / BNK + 2;
+    const long seqs = (long)B * (n_heads / ratio), xcd = cus > 8 ? cus / 8 : 1;
+    const double read = seqs * (double)kv_max * (HD + 24) / 4.2e6;
     TreePlan p = {1, 1, 1};
-    // rows per workgroup: unpacking a tile costs about as much as two blocks of 16 rows
-    long best = 0;
+    double best = 0;
     for (int nb = 1; nb <= kTreeMaxBlocks; nb++) {
         const int rg = (R + 16 * nb - 1) / (16 * nb);
-        const long cost = (long)rg * (2 + nb);
-        if (nb == 1 || cost < best) best = cost, p.blocks = nb, p.groups = rg;
+        if (nb > 1 && rg == (R + 16 * nb - 17) / (16 * nb - 16)) continue;      // no fewer groups than with fewer blocks
+        for (int k = 0; k < 5; k++) {                          // one split, or k / 2 workgroups a CU
+            long s = k * xcd / 2 / rg * 8 / seqs;
+            s = s < (tiles + 1) / 2 ? s : (tiles + 1) / 2;
+            s = kv_splits ? kv_splits : s < 1 ? 1 : s < kTreeMaxSplits ? s : kTreeMaxSplits;
+            const long wgs = (seqs * s + 7) / 8 * rg, steps = ((tiles + s - 1) / s + 1) / 2;
+            const double run = steps * (wgs <= xcd ? one[nb - 1] : two[nb - 1] * fmax(1.0, wgs / (2.0 * xcd)));
+            const double cost = fmax(run, read) + (s == 1 ? 0 : 3 + 0.3e-3 * seqs * R * s);
+            if (best == 0 || cost < best) best = cost, p = TreePlan{nb, rg, (int)s};
+        }
     }
-    const long units = (long)B * (n_heads / ratio) * p.groups;
-    const long tiles = kv_max / BNK + 2;
-    long s = kv_splits ? kv_splits : 2 * cus / units;
-    if (!kv_splits && s > (tiles + 1) / 2) s = (tiles + 1) / 2;
-    p.splits = s < 1 ? 1 : s > kTreeMaxSplits ? kTreeMaxSplits : (int)s;
     return p;
 }
 
@@ -497,10 +542,7 @@ hipError_t launch_attn_tree(const AttnTree& a, const TreePlan& p, void* ws, hipS
     switch (p.blocks) {
         case 1: hipLaunchKernelGGL(attn_tree_k<1>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
         case 2: hipLaunchKernelGGL(attn_tree_k<2>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
-        case 3: hipLaunchKernelGGL(attn_tree_k<3>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
-        case 4: hipLaunchKernelGGL(attn_tree_k<4>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
-        case 5: hipLaunchKernelGGL(attn_tree_k<5>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
-        default: hipLaunchKernelGGL(attn_tree_k<6>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
+        default: hipLaunchKernelGGL(attn_tree_k<3>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
     }
     if (p.splits > 1)
         hipLaunchKernelGGL(attn_tree_join_k, dim3(a.T * a.ratio, a.B * KVH), dim3(256), 0, st, a, p, opart, mlpart);

@@ -836,7 +836,8 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
                     "heads in all)", B, T, TP, n_heads, ratio);
     if (kv_len && (kv_cap < 64 || kv_cap % 64 || kv_cap > kMaxKvCap || kv_max < 0 || kv_max > kv_cap))
         return fail(RT4_E_SHAPE, "rt4_attention_tree: kv_cap=%d (a multiple of 64, at most 16777152) kv_max=%d", kv_cap, kv_max);
-    if (kv_splits < 0 || kv_splits > 64) return fail(RT4_E_ARG, "rt4_attention_tree: kv_splits=%d (0..64)", kv_splits);
+    if (kv_splits < 0 || kv_splits > rt4::kTreeMaxSplits)
+        return fail(RT4_E_ARG, "rt4_attention_tree: kv_splits=%d (0..128)", kv_splits);
     if (!aligned(qq, 16) || !aligned(kc, 16) || !aligned(vc, 16) || !aligned(kd, 16) || !aligned(vd, 16) || !aligned(out, 16) ||
         !aligned(qsc, 4) || !aligned(ksc, 16) || !aligned(vsc, 16) || !aligned(ksd, 16) || !aligned(vsd, 16) || !aligned(parent, 4) ||
         !aligned(kv_len, 4))
@@ -847,8 +848,9 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
     hipStream_t st = as_stream(stream);
     rt4::TreePlan plan = rt4::tree_plan(B, T, n_heads, ratio, kv_len ? kv_max : 0, kv_splits, cus);
     // under capture, as many of the automatic splits as the workspace that is there holds
-    if (!kv_splits && plan.splits > 1 && capturing(st))
-        while (plan.splits > 1 && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan))) plan.splits--;
+    if (!kv_splits && plan.splits > 1 && capturing(st) && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan)))
+        do plan.splits--;
+        while (plan.splits > 1 && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan)));
     void* ws = nullptr;
     if (plan.splits > 1 && (rc = lib_scratch(kSlotTreePart, rt4::tree_part_bytes(a, plan), &ws, st))) return rc;
     return hip_status(rt4::launch_attn_tree(a, plan, ws, st), "rt4_attention_tree launch");

@@ -166,7 +166,7 @@ struct AttnTree {
 struct TreePlan {
     int blocks, groups, splits;
 };
-constexpr int kTreeMaxBlocks = 6, kTreeMaxSplits = 64;
+constexpr int kTreeMaxBlocks = 3, kTreeMaxSplits = 128;
 TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_splits, int cus);
 // Workspace of the splits' states (0 for one split).
 size_t tree_part_bytes(const AttnTree& a, const TreePlan& p);

@@ -198,7 +198,7 @@ def test_attention_refusals(rt4):
                                     TP, QH, ratio, cap, kv_max, splits, None)
     assert call(out=None) == 2 and call(kc=None) == 2
     assert call(out=ctypes.c_void_p(0x1004)) == 2 and "misaligned" in L.rt4_last_error().decode()
-    assert call(splits=-1) == 2 and call(splits=65) == 2
+    assert call(splits=-1) == 2 and call(splits=129) == 2
     for bad in (dict(B=0), dict(T=0), dict(T=65, TP=65), dict(TP=3), dict(B=2, TP=7), dict(QH=0), dict(ratio=0), dict(ratio=3),
                 dict(cap=0), dict(cap=96), dict(cap=1 << 24), dict(kv_max=129), dict(kv_max=-1)):
         assert call(**bad) == 1 and "rt4_attention_tree" in L.rt4_last_error().decode(), bad
@@ -417,7 +417,7 @@ def test_attention_lengths_beyond_the_plan(rt4, torch_gpu, orc):
     lens = [1400, 700]
     want, tol = tree_attention(qq, qs, kv, lens, draft, parent, 6)
     for kv_max in (0, 64, 1400):
-        for splits in (0, 2, 5, 64):
+        for splits in (0, 2, 5, 64, 65, 128):
             out = rt4.attention_tree(dev(qq), dev(qs), *map(dev, kv), dev(np.array(lens)), *map(dev, draft), dev(parent), ratio=6,
                                      kv_max=kv_max, kv_splits=splits)
             check_attention(out, want, tol)
