@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256) void kv_append_rows_k(uint32_t* __restrict__ k
                                                         float* __restrict__ stage, const float* __restrict__ kf,
                                                         const float* __restrict__ vf, const int* __restrict__ kv_len,
                                                         const int* __restrict__ rows, const int* __restrict__ count, int T, int H,
-                                                        int kv_cap, int vblocks) {
+                                                        int kv_cap, int vblocks, bool aligned) {
     constexpr int D = 256, BG = 64;
     __shared__ float red[4][64];
     const int b = blockIdx.y;
@@ -205,20 +205,23 @@ __global__ __launch_bounds__(256) void kv_append_rows_k(uint32_t* __restrict__ k
     if (n == 0 || end < n || end > kv_cap) return;
     const int t0 = (int)end - n;
     rows = rows ? rows + (size_t)b * T : nullptr;
-    // element 0 of the j-th appended row of src (H heads of D), null where rows names none
-    auto row = [&](const float* src, int j) {
-        const int r = rows ? rows[j] : j;
-        return r >= 0 && r < T ? src + ((size_t)b * T + r) * H * D : nullptr;
+    // the row that becomes key t0 + j, -1 where there is none
+    auto row = [&](int j) __attribute__((always_inline)) {
+        const bool in = j >= 0 && j < n;
+        const int r = rows ? rows[in ? j : 0] : j;
+        return in && r >= 0 && r < T ? r : -1;
     };
+    // Loads are unconditional, of row 0 where there is none: under a condition each waits for its own.
     if ((int)blockIdx.x >= vblocks) {
         const size_t i = (size_t)(blockIdx.x - vblocks) * 256 + threadIdx.x;
         const int e8 = (int)(i & 31), th = (int)(i >> 5), h = th % H, j = th / H;
         if (j >= n) return;                          // whole groups exit together
-        const float* xr = row(kf, j);
+        const int r = row(j);
         float v[8], amax = 0.f;
+        load8(kf + (((size_t)b * T + (r < 0 ? 0 : r)) * H + h) * D + 8 * e8, aligned, v);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            v[e] = xr ? xr[h * D + 8 * e8 + e] : 0.f;
+            v[e] = r < 0 ? 0.f : v[e];
             amax = fmaxf(amax, fabsf(v[e]));
         }
         amax = run_max<16>(amax);
@@ -228,26 +231,26 @@ __global__ __launch_bounds__(256) void kv_append_rows_k(uint32_t* __restrict__ k
         if (e8 % 16 == 0) ksc[(((size_t)b * H + h) * 2 + e8 / 16) * kv_cap + t0 + j] = s;
         return;
     }
-    const int lane = threadIdx.x & 63, p = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, p = uniform(threadIdx.x >> 6);
     const int d = (blockIdx.x & 3) * 64 + lane, h = (blockIdx.x >> 2) % H, ti = (blockIdx.x >> 2) / H;
     const int first = t0 / BG, last = (t0 + n - 1) / BG, tile = first + ti;
     if (tile > last) return;
     const size_t bh = (size_t)b * H + h;
     float* st = stage ? stage + bh * BG * D + d : nullptr;
+    const float* vr = vf + ((size_t)b * T * H + h) * D + d;      // row r: vr[r * H * D]
+    const int mine = row(tile * BG + lane - t0);                 // the row of the tile's key `lane`
     float v[16];
     float amax = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-        const int key = tile * BG + 16 * p + e;
-        float x = 0.f;
-        if (key < t0) {
-            if (st) x = st[(size_t)(16 * p + e) * D];
-        } else if (key < t0 + n) {
-            const float* xr = row(vf, key - t0);
-            if (xr) x = xr[h * D + d];
-        }
-        v[e] = x;
-        amax = fmaxf(amax, fabsf(x));
+        const int slot = 16 * p + e, r = __builtin_amdgcn_readlane(mine, slot);
+        v[e] = *(st && tile * BG + slot < t0 ? st + slot * D : vr + (size_t)(r < 0 ? 0 : r) * H * D);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const int slot = 16 * p + e;
+        if (!(st && tile * BG + slot < t0) && __builtin_amdgcn_readlane(mine, slot) < 0) v[e] = 0.f;
+        amax = fmaxf(amax, fabsf(v[e]));
     }
     red[p][lane] = amax;
     __syncthreads();
@@ -260,14 +263,26 @@ __global__ __launch_bounds__(256) void kv_append_rows_k(uint32_t* __restrict__ k
     if (ti != 0 || !st) return;
     // the stage: the last tile's rows, beneath them those of the tile before it (a thread
     // reads and writes the same slots, and only the first tile's workgroups read any)
+    if (last != first) {
+        int key = last * BG + lane;
+        key = key < t0 + n ? key : key - BG;
+        const int from = key >= t0 ? row(key - t0) : -2;         // -2: the slot keeps what it has
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int r = __builtin_amdgcn_readlane(from, 16 * p + e);
+            v[e] = vr[(size_t)(r < 0 ? 0 : r) * H * D];
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int r = __builtin_amdgcn_readlane(from, 16 * p + e);
+            if (r != -2) st[(16 * p + e) * D] = r < 0 ? 0.f : v[e];
+        }
+        return;
+    }
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-        int key = last * BG + 16 * p + e;
-        if (key >= t0 + n) key -= BG;
-        if (key >= t0) {
-            const float* xr = row(vf, key - t0);
-            st[(size_t)(16 * p + e) * D] = xr ? xr[h * D + d] : 0.f;
-        }
+        const int key = tile * BG + 16 * p + e;
+        if (key >= t0 && key < t0 + n) st[(16 * p + e) * D] = v[e];
     }
 }
 
@@ -333,7 +348,7 @@ hipError_t launch_kv_append_rows(uint32_t* kc, float* ksc, uint32_t* vc, float* 
     const int vblocks = 4 * H * slots;
     const size_t kblocks = ((size_t)T * H * 32 + 255) / 256;
     hipLaunchKernelGGL(kv_append_rows_k, dim3((unsigned)(vblocks + kblocks), B), dim3(256), 0, st, kc, ksc, vc, vsc, stage, kf, vf,
-                       kv_len, rows, count, T, H, kv_cap, vblocks);
+                       kv_len, rows, count, T, H, kv_cap, vblocks, ((uintptr_t)kf & 15) == 0);
     return hipGetLastError();
 }
 

@@ -52,17 +52,6 @@ __device__ __forceinline__ float max_groups(float v) {
     return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
-__device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
 // 16 int8 operand bytes (16 x code) of two code dwords.
 __device__ __forceinline__ v4i bytes16(uint32_t a, uint32_t b) {
     return v4i{(int)even_x16(a), (int)odd_x16(a), (int)even_x16(b), (int)odd_x16(b)};
@@ -469,7 +458,7 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
     read(0);
     const float M = wave_max(fmaxf(x[0].x, x[1].x));
     const float f[2] = {__builtin_amdgcn_exp2f(x[0].x - M), __builtin_amdgcn_exp2f(x[1].x - M)};
-    const float ls = wave_add(x[0].y * f[0] + x[1].y * f[1]);
+    const float ls = wave_sum(x[0].y * f[0] + x[1].y * f[1]);
     v4f o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int h = 0; h < 2; h++) {

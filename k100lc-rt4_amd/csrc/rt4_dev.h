@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <cstdint>
+#include <type_traits>
 
 namespace rt4 {
 
@@ -33,6 +34,82 @@ template <int W>
 __device__ __forceinline__ int run_sum(int v) {
 #pragma unroll
     for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// Reductions over all 64 lanes without the LDS crossbar: neighbours, quads, halves and rows of 16 by
+// DPP (quad_perm xor 1 and xor 2, then the mirrors, which pair what is already equal), the rest by
+// lane-half swaps.  A step is a few cycles; __shfl_xor's is a round trip of over a hundred.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_of(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+}
+template <int STEP>                      // the value of the lane that step pairs this one with
+__device__ __forceinline__ uint32_t pair_of(uint32_t v) {
+    if constexpr (STEP == 0) return dpp_of<0xB1>(v);
+    else if constexpr (STEP == 1) return dpp_of<0x4E>(v);
+    else if constexpr (STEP == 2) return dpp_of<0x141>(v);
+    else return dpp_of<0x140>(v);
+}
+template <int STEP, class T>
+__device__ __forceinline__ T pair_of(T v) {
+    static_assert(sizeof(T) == 4 || sizeof(T) == 8, "");
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, pair_of<STEP>(__builtin_bit_cast(uint32_t, v)));
+    } else {
+        const uint2 u = __builtin_bit_cast(uint2, v);
+        return __builtin_bit_cast(T, make_uint2(pair_of<STEP>(u.x), pair_of<STEP>(u.y)));
+    }
+}
+template <int WIDTH, class T, class F>   // f(own, other half's), WIDTH 16 or 32
+__device__ __forceinline__ T with_half(T v, F f) {
+    constexpr int N = sizeof(T) / 4;
+    uint32_t a[N], x[N], y[N];
+    __builtin_memcpy(a, &v, sizeof(T));
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const auto r = WIDTH == 16 ? __builtin_amdgcn_permlane16_swap(a[k], a[k], false, false)
+                                   : __builtin_amdgcn_permlane32_swap(a[k], a[k], false, false);
+        x[k] = r[0], y[k] = r[1];
+    }
+    T p, q;
+    __builtin_memcpy(&p, x, sizeof(T));
+    __builtin_memcpy(&q, y, sizeof(T));
+    return f(p, q);
+}
+template <class T, class F>
+__device__ __forceinline__ T wave_reduce(T v, F f) {
+    v = f(v, pair_of<0>(v));
+    v = f(v, pair_of<1>(v));
+    v = f(v, pair_of<2>(v));
+    v = f(v, pair_of<3>(v));
+    v = with_half<16>(v, f);
+    return with_half<32>(v, f);
+}
+__device__ __forceinline__ float wave_max(float v) {
+    return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ int wave_min(int v) {
+    return wave_reduce(v, [](int a, int b) { return a < b ? a : b; });
+}
+template <class T>
+__device__ __forceinline__ T wave_sum(T v) {
+    return wave_reduce(v, [](T a, T b) { return a + b; });
+}
+// Inclusive sums in lane order (row_shr 1, 2, 4, 8 within rows of 16, then the rows' last lanes).
+__device__ __forceinline__ double wave_scan(double v) {
+    auto add = [&](auto ctrl, auto mask) __attribute__((always_inline)) {
+        const uint2 u = __builtin_bit_cast(uint2, v);
+        const uint2 s = make_uint2((uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.x, decltype(ctrl)::value, decltype(mask)::value, 0xF, true),
+                                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.y, decltype(ctrl)::value, decltype(mask)::value, 0xF, true));
+        v += __builtin_bit_cast(double, s);
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
     return v;
 }
 

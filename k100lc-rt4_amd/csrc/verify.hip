@@ -64,29 +64,17 @@ __device__ __forceinline__ double weight(float l, float m, double it) {
     return l == m ? (m > -INFINITY ? 1.0 : 0.0) : x > -708.0 && l < m ? e : 0.0;
 }
 
-// (max, lowest index) of two.
-__device__ __forceinline__ void max_of(float& m, int& i, float m2, int i2) {
-    if (m2 > m || (m2 == m && i2 < i)) {
-        m = m2;
-        i = i2;
-    }
-}
-
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
 // The whole row's statistics from its chunks', by one wave, in a fixed order.
 __device__ __forceinline__ RowStat row_of_chunks(const RowStat* ch, int C, double it) {
     const int lane = threadIdx.x & 63;
-    RowStat r = {-INFINITY, INT_MAX, 0.0}, first = r;
+    RowStat first = {-INFINITY, INT_MAX, 0.0};
     if (lane < C) first = ch[lane];                          // (held: most rows have at most 64 chunks)
-    max_of(r.m, r.i, first.m, first.i);
-    for (int c = lane + 64; c < C; c += 64) max_of(r.m, r.i, ch[c].m, ch[c].i);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) max_of(r.m, r.i, __shfl_xor(r.m, o), __shfl_xor(r.i, o));
+    RowStat r = first;
+    for (int c = lane + 64; c < C; c += 64)
+        if (ch[c].m > r.m) r.m = ch[c].m, r.i = ch[c].i;     // (chunks in ascending order: the first of equals stays)
+    const float m = wave_max(r.m);
+    r.i = wave_min(r.m == m ? r.i : INT_MAX);
+    r.m = m;
     r.s = first.s * weight(first.m, r.m, it);
     for (int c = lane + 64; c < C; c += 64) r.s += ch[c].s * weight(ch[c].m, r.m, it);
     r.s = wave_sum(r.s);
@@ -96,6 +84,10 @@ __device__ __forceinline__ RowStat row_of_chunks(const RowStat* ch, int C, doubl
 __device__ __forceinline__ double inv_temp(const float* temp, int b) {
     const float t = temp ? temp[b] : 1.f;
     return t > 0.f ? 1.0 / (double)t : 0.0;                  // 0: greedy
+}
+
+__device__ __forceinline__ double lane_of(double v, int j) {     // (j the same in every lane)
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), j), __builtin_amdgcn_readlane(__double2loint(v), j));
 }
 
 // A wave's view of sequence b's tree: lane i is node i.
@@ -110,12 +102,11 @@ __device__ __forceinline__ Tree tree_of(const int* parent, int b, int T) {
     const bool root = i == 0 && t.par == -1, node = i > 0 && t.par >= 0 && t.par < i;
     int up = node ? t.par : i;
     u64 anc = 1ull << i;
-#pragma unroll
-    for (int s = 0; s < 6; s++) {        // pointer doubling: 2^6 covers the deepest chain
+    for (int s = 1; s < T; s <<= 1) {    // pointer doubling: the deepest chain has T - 1 links
         anc |= __shfl(anc, up);
         up = __shfl(up, up);
     }
-    const bool rooted = __shfl((int)root, 0);
+    const bool rooted = __builtin_amdgcn_readlane((int)root, 0);
     t.anc = (root || node) && rooted && (anc & 1) ? anc : 0;
     if (!t.anc) t.par = -2;
     return t;
@@ -166,8 +157,7 @@ __global__ __launch_bounds__(256) void verify_stats_k(const float* __restrict__ 
     const double it = inv_temp(temp, b);
 #pragma unroll
     for (int e = 0; e < PT; e++) m = fmaxf(m, v[e]);           // (drops NaN)
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    m = wave_max(m);
     if ((threadIdx.x & 63) == 0) sm[w] = m;
     __syncthreads();
     m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
@@ -178,11 +168,7 @@ __global__ __launch_bounds__(256) void verify_stats_k(const float* __restrict__ 
         if (v[e] == m && m > -INFINITY) mi = at + 256 * (e & ~3) + (e & 3);
         if (it > 0) s += weight(v[e], m, it);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const int x = __shfl_xor(mi, o);
-        mi = x < mi ? x : mi;
-    }
+    mi = wave_min(mi);
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) si[w] = mi, ss[w] = s;
     __syncthreads();
@@ -238,33 +224,52 @@ struct Draw {
     double a;                            // q: the residual is max(p - a q, 0)
     RowStat r;                           // of the row
     int rej[64];
+    double rejw[64];                     // their weights
 };
+
+// What one wave reads of sequence b's tree, lane i node i.
+struct Nodes {
+    Tree t;
+    int tok;
+    float lt;                            // its token's logit in its parent's row
+    double qc, u;                        // and probability there; its uniform
+};
+__device__ __forceinline__ Nodes read_nodes(const Verify& A, int b) {
+    const int i = threadIdx.x & 63;
+    Nodes n;
+    int tok = i < A.T ? A.draft[(size_t)b * A.T + i] : -1;
+    const float u = i < A.T ? A.u[(size_t)b * A.T + i] : 0.f;
+    n.t = tree_of(A.parent, b, A.T);
+    const bool kid = n.t.anc && i > 0, real = kid && tok >= 0 && tok < A.V;
+    const size_t prow = (size_t)b * A.T + (kid ? n.t.par : 0);
+    n.tok = kid ? tok : -1;
+    n.lt = real ? A.logits[prow * A.ldl + tok] : -INFINITY;
+    n.qc = real && A.q ? (double)A.q[prow * A.ldq + tok] : 0.0;
+    n.u = kid ? (double)u : 0.0;
+    return n;
+}
 
 // The path of sequence b, by one wave, lane i node i; rows: the statistics of its T rows.  Whether a
 // node is accepted, once reached, depends on its parent's row and its earlier siblings alone, so all
 // nodes are tested at once and the path is the set whose ancestors all passed.
-__device__ void walk(const Verify& A, int b, double it, const RowStat* rows, bool write, Draw* d) {
-    const int i = threadIdx.x & 63, T = A.T, V = A.V, R = A.B * T, C = A.C;
-    const Tree t = tree_of(A.parent, b, T);
+__device__ void walk(const Verify& A, int b, double it, const Nodes& nd, const RowStat* rows, bool write, Draw* d) {
+    const int i = threadIdx.x & 63, T = A.T, R = A.B * T, C = A.C;
+    const Tree t = nd.t;
     const bool kid = t.anc && i > 0;
-    const int tok = kid ? A.draft[(size_t)b * T + i] : -1;
-    const bool real = tok >= 0 && tok < V;
-    const int pn = kid ? t.par : 0;
-    const size_t prow = (size_t)b * T + pn;
-    const float lt = kid && real ? A.logits[prow * A.ldl + tok] : -INFINITY;
-    const double qc = kid && real && A.q ? (double)A.q[prow * A.ldq + tok] : 0.0;
-    const double ui = kid ? (double)A.u[(size_t)b * T + i] : 0.0;
+    const int tok = nd.tok, pn = kid ? t.par : 0;
+    const bool real = tok >= 0 && tok < A.V;
     const RowStat r = rows[pn];
-    const double pc = it > 0 && r.s > 0 ? weight(lt, r.m, it) / r.s : 0.0;
-    u64 sib = 0, same = 0;               // earlier siblings; those with this token
-    for (int j = 1; j < T; j++) {
-        const int pj = __shfl(t.par, j), tj = __shfl(tok, j);      // (by every lane)
-        const bool s = pj == t.par && j < i && kid;
-        sib |= (u64)s << j;
-        same |= (u64)(s && tj == tok) << j;
-    }
-    const bool first = !same;
+    const double wt = it > 0 ? weight(nd.lt, r.m, it) : 0.0, pc = r.s > 0 ? wt / r.s : 0.0;
+    u64 sib = 0;                         // earlier siblings
+    bool first = true;                   // none of them has this token
     double W = 1.0, a = 0.0;
+    for (int j = 1; j < T; j++) {
+        const int pj = __builtin_amdgcn_readlane(t.par, j), tj = __builtin_amdgcn_readlane(tok, j);
+        if (pj == t.par && j < i && kid) {
+            sib |= 1ull << j;
+            first = first && tj != tok;
+        }
+    }
     bool tested = kid;
     if (A.q) {
         const int rank = __popcll(sib);
@@ -280,13 +285,13 @@ __device__ void walk(const Verify& A, int b, double it, const RowStat* rows, boo
             }
         }
     } else {
+        const double mine = first ? pc : 0.0;
         for (int j = 1; j < T; j++) {
-            const double pj = __shfl(pc, j);
-            const bool fj = __shfl((int)first, j);
-            if (fj && (sib >> j & 1)) W -= pj;
+            const double pj = lane_of(mine, j);
+            if (sib >> j & 1) W -= pj;
         }
     }
-    bool yes = A.q ? ui * W * qc < pc - a * qc : first && ui * W < pc;
+    bool yes = A.q ? nd.u * W * nd.qc < pc - a * nd.qc : first && nd.u * W < pc;
     if (!(it > 0)) yes = tok == r.i;
     yes = yes && tested && real;
     const u64 yesm = __ballot(yes);
@@ -297,7 +302,11 @@ __device__ void walk(const Verify& A, int b, double it, const RowStat* rows, boo
     const int last = n ? 63 - __clzll(onm) : 0;
     const bool rejected = kid && t.par == last && n;
     const u64 rejm = __ballot(rejected && (A.q ? tested : real && first));
-    if (rejm >> i & 1) d->rej[__popcll(rejm & ((1ull << i) - 1))] = tok;
+    if (rejm >> i & 1) {
+        const int k = __popcll(rejm & ((1ull << i) - 1));
+        d->rej[k] = tok;
+        d->rejw[k] = wt;
+    }
     // the residual's a after its children: a of the last one tested plus that one's W
     if (A.q && rejm && i == 63 - __clzll(rejm)) d->a = a + W;
     if (i == 0) {
@@ -308,10 +317,10 @@ __device__ void walk(const Verify& A, int b, double it, const RowStat* rows, boo
         d->r = rows[last];
     }
     if (!write) return;
-    // -1 wherever no value belongs
-    if (i < T) {
-        if (i >= n) A.path[(size_t)b * T + i] = -1;
-        if (i >= n) A.tokens[(size_t)b * T + i] = -1;          // (the last token comes after the draw)
+    // -1 wherever no value belongs (the last token comes after the draw)
+    if (i < T && i >= n) {
+        A.path[(size_t)b * T + i] = -1;
+        A.tokens[(size_t)b * T + i] = -1;
     }
     if (on) A.path[(size_t)b * T + pos] = i;
     if (on && i > 0) A.tokens[(size_t)b * T + pos - 1] = tok;
@@ -321,82 +330,155 @@ __device__ void walk(const Verify& A, int b, double it, const RowStat* rows, boo
     }
 }
 
-// Residual weights of thread's E consecutive tokens from `at` on; their sum.
-template <int E>
+// Residual weights of a thread's E tokens at, at + STEP, ..; their sum.
+template <int E, int STEP>
 __device__ __forceinline__ double residuals(double (&w)[E], const Verify& A, const Draw& d, double it, int at) {
     const float* l = A.logits + (size_t)d.row * A.ldl;
     const float* q = A.q ? A.q + (size_t)d.row * A.ldq : nullptr;
     const double is = d.r.s > 0 ? 1.0 / d.r.s : 0.0;
-    double s = 0;
+    float lv[E], qv[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
-        const int i = at + e;
-        w[e] = 0.0;
-        if (i < A.V) {
-            w[e] = weight(l[i], d.r.m, it);
-            if (q) w[e] = fmax(w[e] * is - d.a * (double)q[i], 0.0);
-        }
+        const int i = at + e * STEP;
+        lv[e] = i < A.V ? l[i] : -INFINITY;
+        qv[e] = q && i < A.V ? q[i] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        w[e] = weight(lv[e], d.r.m, it);
+        if (q) w[e] = fmax(w[e] * is - d.a * (double)qv[e], 0.0);
     }
     for (int k = 0; k < d.nrej; k++) {
         const int i = d.rej[k] - at;
 #pragma unroll
         for (int e = 0; e < E; e++)
-            if (i == e) w[e] = 0.0;
+            if (i == e * STEP) w[e] = 0.0;
     }
+    double s = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) s += w[e];
     return s;
 }
 
-// Statistics of sequence b's rows into LDS, a wave per row.
-__device__ __forceinline__ void rows_to_lds(const Verify& A, int b, double it, RowStat* rows) {
+// Statistics of sequence b's rows into LDS, a wave per row, beside what the first wave reads of its
+// tree, and the walk.
+__device__ __forceinline__ void walk_sequence(const Verify& A, int b, double it, RowStat* rows, bool write, Draw* d) {
+    Nodes nd;
+    if (threadIdx.x < 64) nd = read_nodes(A, b);
     for (int n = threadIdx.x >> 6; n < A.T; n += blockDim.x >> 6) {
         const RowStat r = row_of_chunks(A.ch + ((size_t)b * A.T + n) * A.C, A.C, it);
         if ((threadIdx.x & 63) == 0) rows[n] = r;
     }
     __syncthreads();
+    if (threadIdx.x < 64) walk(A, b, it, nd, rows, write, d);
+    __syncthreads();
 }
 
 // With draft probabilities, the walk and the chunk sums of the residual: every workgroup of a
-// sequence walks for itself (a launch less), the first one writes.  grid (C, B), 256 threads.
-__global__ __launch_bounds__(256) void verify_residual_k(const Verify A) {
-    __shared__ double ss[4];
+// sequence walks for itself (a launch less), the first one writes.  grid (C, B), 512 threads.
+__global__ __launch_bounds__(512) void verify_residual_k(const Verify A) {
+    constexpr int E = CH / 512;
+    __shared__ double ss[8];
     __shared__ RowStat rows[64];
     __shared__ Draw d;
     const int b = blockIdx.y, c = blockIdx.x;
     const double it = inv_temp(A.temp, b);
-    rows_to_lds(A, b, it, rows);
-    if (threadIdx.x < 64) walk(A, b, it, rows, c == 0, &d);
-    __syncthreads();
+    walk_sequence(A, b, it, rows, c == 0, &d);
     if (c == 0 && threadIdx.x < sizeof(Draw) / 4) reinterpret_cast<int*>(A.draw + b)[threadIdx.x] = reinterpret_cast<const int*>(&d)[threadIdx.x];
     if (d.row < 0 || !(it > 0)) return;
-    double w[PT];
-    double s = residuals(w, A, d, it, c * CH + (int)threadIdx.x * PT);
-    s = wave_sum(s);
+    double w[E];
+    const double s = wave_sum(residuals<E, 512>(w, A, d, it, c * CH + (int)threadIdx.x));
     if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) A.sums[(size_t)b * A.C + c] = ss[0] + ss[1] + ss[2] + ss[3];
+    if (threadIdx.x == 0) {
+        double t = 0;
+        for (int k = 0; k < 8; k++) t += ss[k];
+        A.sums[(size_t)b * A.C + c] = t;
+    }
 }
 
-// The last token, after the walk where there are no draft probabilities.  grid B, 1024 threads.
-//
-// Without them a chunk's mass is the sum that verify_stats_k left, less the rejected tokens'.  Where
-// hardly anything is left that difference says little, and the chunks are summed anew.
-__global__ __launch_bounds__(1024) void verify_draw_k(const Verify A) {
-    constexpr int E = CH / 1024;
-    __shared__ RowStat rows[64];
-    __shared__ Draw d;
-    __shared__ double part[16], s_total, s_r;
-    __shared__ int s_chunk, s_wave, s_tok;
-    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const double it = inv_temp(A.temp, b);
-    if (!A.q) {
-        rows_to_lds(A, b, it, rows);
-        if (tid < 64) walk(A, b, it, rows, true, &d);
-    } else if (tid < (int)(sizeof(Draw) / 4)) {
-        reinterpret_cast<int*>(&d)[tid] = reinterpret_cast<const int*>(A.draw + b)[tid];
+// The first thread at which the masses' running sum (in thread order) exceeds r, or u times their total
+// where r is negative; where rounding leaves none, the last one with any; -1 where there is no mass.
+// Every thread gets it; r becomes what of it is left there.  kDrawThreads threads.
+constexpr int kDrawThreads = 512, kDrawWaves = kDrawThreads / 64;
+struct PickLds {
+    double part[kDrawWaves], left;
+    int at;
+};
+__device__ __forceinline__ int block_pick(double mine, double u, double& r, PickLds& L) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const double inc = wave_scan(mine);
+    if (lane == 63) L.part[w] = inc;
+    if (threadIdx.x == 0) L.at = -1;
+    __syncthreads();
+    double part[kDrawWaves], total = 0, base = 0;
+#pragma unroll
+    for (int k = 0; k < kDrawWaves; k++) {
+        part[k] = L.part[k];
+        if (k == w) base = total;
+        total += part[k];
+    }
+    if (r < 0) r = u * total;
+    double acc = 0;
+    int ws = -1, some = -1;                                    // the wave of the crossing; the last with mass
+#pragma unroll
+    for (int k = 0; k < kDrawWaves; k++) {
+        acc += part[k];
+        if (ws < 0 && acc > r) ws = k;
+        if (part[k] > 0) some = k;
+    }
+    if (ws < 0) ws = some;
+    if (w == ws) {
+        const u64 hit = __ballot(base + inc > r && mine > 0), any = __ballot(mine > 0);
+        if (lane == (hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll(any))) {
+            L.at = threadIdx.x;
+            L.left = r - (base + inc - mine);
+        }
     }
     __syncthreads();
+    r = L.left;
+    return L.at;
+}
+// Of a thread's E masses from `left` on: the first at which their sum exceeds it, else the last with any;
+// `left` becomes what of it is left there.
+template <int E>
+__device__ __forceinline__ int thread_pick(const double (&x)[E], double& left) {
+    int at = -1;
+    double acc = 0, before = 0;
+    bool done = false;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        if (!done && x[e] > 0) at = e, before = acc;
+        acc += x[e];
+        done = done || (acc > left && x[e] > 0);
+    }
+    left -= before;
+    return at;
+}
+
+// The last token, after the walk where there are no draft probabilities.  grid B, kDrawThreads threads: a
+// thread has CE chunks in a row (V <= 2^22), then TE tokens of the chunk that is picked.
+//
+// Without draft probabilities a chunk's mass is the sum that verify_stats_k left, less the rejected
+// tokens'.  Where hardly anything is left that difference says little, and the chunks are summed anew.
+__global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
+    constexpr int CE = kVerifyMaxV / CH / kDrawThreads, TE = CH / kDrawThreads;
+    __shared__ RowStat rows[64];
+    __shared__ Draw d;
+    __shared__ PickLds L;
+    __shared__ double s_sum[kDrawWaves], s_left;
+    __shared__ int s_chunk;
+    const int b = blockIdx.x, tid = threadIdx.x;
+    const double it = inv_temp(A.temp, b), u = (double)A.u[(size_t)b * A.T];
+    double mass[CE];
+#pragma unroll
+    for (int e = 0; e < CE; e++) mass[e] = A.q && CE * tid + e < A.C ? A.sums[(size_t)b * A.C + CE * tid + e] : 0.0;
+    if (!A.q) {
+        walk_sequence(A, b, it, rows, true, &d);
+    } else {
+        if (tid < (int)(sizeof(Draw) / 4)) reinterpret_cast<int*>(&d)[tid] = reinterpret_cast<const int*>(A.draw + b)[tid];
+        __syncthreads();
+    }
     if (d.row < 0) return;
     int* out = A.tokens + (size_t)b * A.T + d.n - 1;
     const int best = d.r.i < A.V ? d.r.i : -1;
@@ -404,123 +486,57 @@ __global__ __launch_bounds__(1024) void verify_draw_k(const Verify A) {
         if (tid == 0) *out = best;
         return;
     }
-    const RowStat* ch = A.ch + (size_t)d.row * A.C;
-    double* sums = A.sums + (size_t)b * A.C;
-    if (w == 0) {
-        if (tid == 0) s_chunk = -1, s_tok = best;              // (nothing left: the largest)
-        double total = 0, all = 0;
-        for (int c = lane; c < A.C; c += 64) {
-            double s = sums[c];
-            if (!A.q) {
-                s = ch[c].s * weight(ch[c].m, d.r.m, it);
-                all += s;
-                for (int k = 0; k < d.nrej; k++)
-                    if (d.rej[k] / CH == c) s -= weight(A.logits[(size_t)d.row * A.ldl + d.rej[k]], d.r.m, it);
-                s = fmax(s, 0.0);
-                sums[c] = s;
+    if (!A.q) {
+        double gone = 0;
+#pragma unroll
+        for (int e = 0; e < CE; e++) {
+            const int c = CE * tid + e;
+            if (c < A.C) {
+                const RowStat s = A.ch[(size_t)d.row * A.C + c];
+                mass[e] = s.s * weight(s.m, d.r.m, it);
             }
-            total += s;
+            for (int k = 0; k < d.nrej; k++)
+                if (d.rej[k] / CH == c) mass[e] -= d.rejw[k];
+            mass[e] = fmax(mass[e], 0.0);
         }
-        total = wave_sum(total);
-        all = wave_sum(all);
-        if (tid == 0) s_total = !A.q && total < 1e-6 * all ? -1.0 : total;
+        for (int k = 0; k < d.nrej; k++) gone += d.rejw[k];
+        if (d.r.s - gone < 1e-6 * d.r.s) {
+            for (int c = 0; c < A.C; c++) {
+                double x[TE];
+                const double s = wave_sum(residuals<TE, 1>(x, A, d, it, c * CH + tid * TE));
+                if ((tid & 63) == 0) s_sum[tid >> 6] = s;
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < CE; e++)
+                    if (CE * tid + e == c) {
+                        mass[e] = 0;
+                        for (int k = 0; k < kDrawWaves; k++) mass[e] += s_sum[k];
+                    }
+                __syncthreads();
+            }
+        }
+    }
+    double mine = 0, r = -1.0;
+#pragma unroll
+    for (int e = 0; e < CE; e++) mine += mass[e];
+    const int owner = block_pick(mine, u, r, L);
+    if (owner < 0) {                                           // nothing left: the largest
+        if (tid == 0) *out = best;
+        return;
+    }
+    if (tid == owner) {
+        s_chunk = CE * tid + thread_pick(mass, r);
+        s_left = fmax(r, 0.0);
     }
     __syncthreads();
-    if (s_total < 0) {
-        for (int c = 0; c < A.C; c++) {
-            double x[E];
-            const double s = wave_sum(residuals(x, A, d, it, c * CH + tid * E));
-            if (lane == 0) part[w] = s;
-            __syncthreads();
-            if (tid == 0) {
-                double t = 0;
-                for (int k = 0; k < 16; k++) t += part[k];
-                sums[c] = t;
-            }
-            __syncthreads();
-        }
+    const int at = s_chunk * CH + tid * TE;
+    double x[TE], left = s_left;
+    const int th = block_pick(residuals<TE, 1>(x, A, d, it, at), u, left, L);
+    if (th < 0) {                                              // (a chunk whose mass was rounding alone)
+        if (tid == 0) *out = best;
+    } else if (tid == th) {
+        *out = at + thread_pick(x, left);
     }
-    if (w == 0) {
-        // the first chunk whose cumulated sum exceeds u times the total; lane order is chunk order
-        double total = 0;
-        for (int c = lane; c < A.C; c += 64) total += sums[c];
-        total = wave_sum(total);
-        const double want = (double)A.u[(size_t)b * A.T] * total;
-        double acc = 0;
-        int pick = -1, some = -1;
-        double before = 0, sbefore = 0;
-        for (int c0 = 0; c0 < A.C && pick < 0; c0 += 64) {
-            const double s = c0 + lane < A.C ? sums[c0 + lane] : 0.0;
-            double x = s;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double y = __shfl_up(x, o);
-                if (lane >= o) x += y;
-            }
-            const u64 hit = __ballot(acc + x > want && s > 0), any = __ballot(s > 0);
-            if (any) {
-                some = 63 - __clzll(any);
-                sbefore = acc + __shfl(x - s, some);
-                some += c0;
-            }
-            if (hit) {
-                pick = __ffsll((unsigned long long)hit) - 1;
-                before = acc + __shfl(x - s, pick);
-                pick += c0;
-            }
-            acc += __shfl(x, 63);
-        }
-        if (pick < 0) pick = some, before = sbefore;           // (rounding left none: the last one with mass)
-        if (lane == 0) {
-            s_chunk = pick;
-            s_r = want - before;
-        }
-    }
-    __syncthreads();
-    const int c = s_chunk;
-    if (c >= 0) {
-        double x[E];
-        const double mine = residuals(x, A, d, it, c * CH + tid * E);
-        double inc = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double y = __shfl_up(inc, o);
-            if (lane >= o) inc += y;
-        }
-        if (lane == 63) part[w] = inc;
-        if (tid == 0) s_wave = -1;
-        __syncthreads();
-        double base = 0;
-        for (int k = 0; k < w; k++) base += part[k];
-        const double r = s_r;
-        // the wave, then the lane, then the token in which the sum first exceeds r; the last token with
-        // weight where none does
-        const u64 hit = __ballot(base + inc > r && mine > 0), any = __ballot(mine > 0);
-        if (lane == 0 && hit) atomicMin(reinterpret_cast<unsigned*>(&s_wave), (unsigned)w);
-        __syncthreads();
-        int ws = s_wave;
-        if (ws < 0) {                                          // none: the last wave with any
-            __syncthreads();
-            if (lane == 0 && any) atomicMax(&s_wave, w);
-            __syncthreads();
-            ws = s_wave;
-        }
-        if (w == ws) {
-            const int ln = hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll(any);
-            if (lane == ln) {
-                double acc = base + inc - mine;
-                int at = -1;
-                for (int e = 0; e < E; e++) {
-                    if (x[e] > 0) at = e;
-                    acc += x[e];
-                    if (acc > r && x[e] > 0) break;
-                }
-                s_tok = c * CH + tid * E + at;
-            }
-        }
-        __syncthreads();
-    }
-    if (tid == 0) *out = s_tok;
 }
 
 size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
@@ -550,8 +566,8 @@ hipError_t launch_verify_tree(int* tokens, int* path, int* count, int* kv_len, c
         hipLaunchKernelGGL(verify_stats_k<false>, dim3(C, R), dim3(256), 0, st, logits, ldl, parent, temp, T, V, ch);
     for (int k = 1; k < levels; k++)
         hipLaunchKernelGGL(verify_mass_k, dim3(C, R), dim3(256), 0, st, logits, ldl, q, ldq, parent, temp, T, V, k, ch, av, part);
-    if (q) hipLaunchKernelGGL(verify_residual_k, dim3(C, B), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(verify_draw_k, dim3(B), dim3(1024), 0, st, a);
+    if (q) hipLaunchKernelGGL(verify_residual_k, dim3(C, B), dim3(512), 0, st, a);
+    hipLaunchKernelGGL(verify_draw_k, dim3(B), dim3(kDrawThreads), 0, st, a);
     return hipGetLastError();
 }
 
