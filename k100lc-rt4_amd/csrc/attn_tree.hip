@@ -89,6 +89,54 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const char* p, int bytes)
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, bytes, 0x00020000);     // 32-bit data format
 }
 
+// How the key tiles of the sequences (the cache's, then the draft tile) are shared out, lengths being
+// known here only.  A unit is a run of tiles of one sequence, for each KV head and row group a
+// workgroup: `fixed` units a sequence, or runs of equal length over all of them, such that there
+// are at most units + B of them, no sequence has more than kTreeMaxSplits and none is shorter than a
+// step.  So a batch's longest sequence takes no longer than its share.
+struct Run {
+    int b, split, splits, first, tiles;  // sequence, which of its units, their number, the first's, its tiles
+};
+// Unit x (by_unit), b -1 past the last one, or sequence x.  By a whole wave; every lane gets it.
+template <bool BY_UNIT>
+__device__ __forceinline__ Run run_of(const AttnTree& A, const TreePlan& P, int x) {
+    const int lane = lane_id();
+    auto tiles_of = [&](int b) __attribute__((always_inline)) {
+        if (b >= A.B) return 0;
+        const int len = A.kv_len ? A.kv_len[b] : 0;
+        return ((len < 0 ? 0 : len > A.kv_cap ? A.kv_cap : len) + BNK - 1) / BNK + 1;
+    };
+    const int held = tiles_of(lane);
+    int q = 0;
+    if (!P.fixed) {
+        int total = wave_sum(held), most = wave_max(held);
+        for (int b0 = 64; b0 < A.B; b0 += 64) {
+            const int t = tiles_of(b0 + lane);
+            total += wave_sum(t);
+            most = max(most, wave_max(t));
+        }
+        q = max(max(2, (total + P.units - 1) / P.units), (most + kTreeMaxSplits - 1) / kTreeMaxSplits);
+    }
+    Run r = {-1, 0, 0, 0, 0};
+    int before = 0;
+    for (int b0 = 0; b0 < A.B; b0 += 64) {
+        const int t = b0 ? tiles_of(b0 + lane) : held, n = P.fixed ? min(P.fixed, t) : (t + q - 1) / q;
+        const int end = before + wave_scan(n);
+        const u64 hit = __ballot(BY_UNIT ? x >= end - n && x < end : b0 + lane == x);
+        if (hit) {
+            const int k = __ffsll((unsigned long long)hit) - 1;
+            r.b = b0 + k;
+            r.splits = __builtin_amdgcn_readlane(n, k);
+            r.first = __builtin_amdgcn_readlane(end, k) - r.splits;
+            r.split = x - r.first;
+            r.tiles = __builtin_amdgcn_readlane(t, k);
+            return r;
+        }
+        before = __builtin_amdgcn_readlane(end, 63);
+    }
+    return r;
+}
+
 constexpr float kPBits = 7.f;            // P is held times 2^7: at most 2^15 with the lazy maximum
 constexpr float kLazy = 8.f;             // the running maximum moves when a score exceeds it by 2^8
 
@@ -120,12 +168,14 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
     const int rg = (int)(blockIdx.x / 8) % P.groups;
     const int unit = (int)(blockIdx.x / (8 * P.groups)) * 8 + (int)(blockIdx.x % 8);
     const int KVH = A.n_heads / A.ratio, R = A.T * A.ratio;
-    if (unit >= A.B * KVH * P.splits) return;
-    const int split = unit % P.splits, seq = unit / P.splits, b = seq / KVH, vh = seq % KVH;
+    const Run run = run_of<true>(A, P, unit / KVH);
+    if (run.b < 0) return;
+    const int b = run.b, vh = unit % KVH;
+    const size_t seq = (size_t)b * KVH + vh;
     int len = A.kv_len ? A.kv_len[b] : 0;
     len = uniform(len < 0 ? 0 : len > A.kv_cap ? A.kv_cap : len);
-    const int nt = (len + BNK - 1) / BNK;                      // tile nt is the draft tile
-    const int t0 = (int)((long long)(nt + 1) * split / P.splits), t1 = (int)((long long)(nt + 1) * (split + 1) / P.splits);
+    const int nt = run.tiles - 1;                              // tile nt is the draft tile
+    const int t0 = (int)((long long)run.tiles * run.split / run.splits), t1 = (int)((long long)run.tiles * (run.split + 1) / run.splits);
 
     const int hS = w & 1;                                      // half of the tile whose scores this wave makes
     v4u K[2][2], V[4];
@@ -136,10 +186,10 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
     // K: operand row 4g + i of subtile p is key 8g + 4p + i, so a lane's scores are the eight keys of one
     // V dword; lane 16 b + j supplies the scales of group b / 2, row j.  V: dim tile j, column c is dim
     // 64w + 4c + j.
-    const char *kc = at(A.kc, (size_t)seq * A.kv_cap * KDW), *kd = at(A.kd, (size_t)seq * BNK * KDW);
-    const char *ksc = at(A.ksc, (size_t)seq * 2 * A.kv_cap), *ksd = at(A.ksd, (size_t)seq * 2 * BNK);
-    const char *vc = at(A.vc, (size_t)seq * (A.kv_cap / 8) * HD), *vd = at(A.vd, (size_t)seq * (BNK / 8) * HD);
-    const char *vsc = at(A.vsc, (size_t)seq * (A.kv_cap / BNK) * HD), *vsd = at(A.vsd, (size_t)seq * HD);
+    const char *kc = at(A.kc, seq * A.kv_cap * KDW), *kd = at(A.kd, seq * BNK * KDW);
+    const char *ksc = at(A.ksc, seq * 2 * A.kv_cap), *ksd = at(A.ksd, seq * 2 * BNK);
+    const char *vc = at(A.vc, seq * (A.kv_cap / 8) * HD), *vd = at(A.vd, seq * (BNK / 8) * HD);
+    const char *vsc = at(A.vsc, seq * (A.kv_cap / BNK) * HD), *vsd = at(A.vsd, seq * HD);
     const int ko = ((8 * (c >> 2) + (c & 3)) * KDW + 4 * g) * 4 + 32 * hS * KDW * 4;
     const int so = (8 * (c >> 2) + (c & 3) + 32 * hS) * 4;
     const int vo = (g * HD + 4 * c + 64 * w) * 4, wo = (4 * c + 64 * w) * 4;
@@ -409,7 +459,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
     }
     __syncthreads();
     const size_t prow = ((size_t)unit * P.groups + rg) * RW;
-    if (P.splits > 1) {
+    if (P.fixed != 1) {                                        // attn_tree_join_k sums the splits
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
@@ -443,17 +493,19 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
     __shared__ __align__(16) v4f ol[4][64];
     const int KVH = A.n_heads / A.ratio, lane = lane_id(), w = uniform(threadIdx.x >> 6);
     const int n = blockIdx.x, seq = blockIdx.y, b = seq / KVH, vh = seq % KVH, i = n % A.T;
-    const size_t step = (size_t)P.groups * 16 * P.blocks, row = (size_t)seq * P.splits * step + n;
+    const Run run = run_of<false>(A, P, b);
+    const size_t step = (size_t)KVH * P.groups * 16 * P.blocks, row = (size_t)run.first * step + (size_t)vh * P.groups * 16 * P.blocks + n;
+    const int splits = run.splits;
     // lane s has the states of splits s and s + 64
     float2 x[2];
 #pragma unroll
-    for (int k = 0; k < 2; k++) x[k] = lane + 64 * k < P.splits ? mlpart[row + (lane + 64 * k) * step] : make_float2(-1e30f, 0.f);
+    for (int k = 0; k < 2; k++) x[k] = lane + 64 * k < splits ? mlpart[row + (lane + 64 * k) * step] : make_float2(-1e30f, 0.f);
     const bool live = __shfl(tree_sees(A.parent + (size_t)b * A.T, A.T), i) != 0;
     const float* src = opart + (row + w * step) * HD + 4 * lane;
     v4f v[16];
     auto read = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
-        for (int k = 0; k < 16; k++) v[k] = w + 64 * h + 4 * k < P.splits ? *reinterpret_cast<const v4f*>(src + (64 * h + 4 * k) * step * HD) : v4f{};
+        for (int k = 0; k < 16; k++) v[k] = w + 64 * h + 4 * k < splits ? *reinterpret_cast<const v4f*>(src + (64 * h + 4 * k) * step * HD) : v4f{};
     };
     read(0);
     const float M = wave_max(fmaxf(x[0].x, x[1].x));
@@ -462,11 +514,11 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
     v4f o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        if (h && P.splits <= 64) break;
+        if (h && splits <= 64) break;
         if (h) read(1);
 #pragma unroll
         for (int k = 0; k < 16; k++) {
-            if (w + 64 * h + 4 * k >= P.splits) break;
+            if (w + 64 * h + 4 * k >= splits) break;
             const float fs = __shfl(f[h], w + 4 * k);
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] = fmaf(v[k][e], fs, o[e]);
@@ -484,47 +536,51 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
 
 }  // namespace
 
-// The rows per workgroup and the splits by a model of the time in us, fitted to sweeps of both over
+// The rows per workgroup and the units by a model of the time in us, fitted to sweeps of both over
 // 1 to 16 sequences of 1000 to 131001 keys and 1 to 64 nodes (off by 8% on average): a step of two
 // tiles takes 1.7, 2.1 or 2.9 (1 to 3 blocks) with one workgroup on a CU and 2.0, 3.05 or 4.2 with
 // two, all steps together at least the cache's bytes at 4.2 TB/s, the joining launch 3 and its states
-// (1 KB a row and split, written and read) 0.3 a MB.  A unit's row groups stay on one XCD (an eighth
+// (1 KB a row and unit, written and read) 0.3 a MB.  A unit's row groups stay on one XCD (an eighth
 // of the CUs), so the XCD with the most units decides.  (4 to 6 blocks fit too: 276 to 283 us where 3
 // take 283, 64 nodes over 131001 keys, and 43 against 37, 16 nodes over 32000.  A join in the same
 // launch by the last workgroup of a row group took 14 us where both launches take 10: one node over
 // 1000 keys.)
 TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_splits, int cus) {
     constexpr double one[] = {1.7, 2.1, 2.9}, two[] = {2.0, 3.05, 4.2};
-    const int R = T * ratio, tiles = kv_max / BNK + 2;
-    const long seqs = (long)B * (n_heads / ratio), xcd = cus > 8 ? cus / 8 : 1;
-    const double read = seqs * (double)kv_max * (HD + 24) / 4.2e6;
-    TreePlan p = {1, 1, 1};
+    const int R = T * ratio;
+    const long KVH = n_heads / ratio, tiles = (long)B * (kv_max / BNK + 2), xcd = cus > 8 ? cus / 8 : 1;
+    const double read = KVH * B * (double)kv_max * (HD + 24) / 4.2e6;
+    TreePlan p = {1, 1, 0, 0};
     double best = 0;
     for (int nb = 1; nb <= kTreeMaxBlocks; nb++) {
         const int rg = (R + 16 * nb - 1) / (16 * nb);
         if (nb > 1 && rg == (R + 16 * nb - 17) / (16 * nb - 16)) continue;      // no fewer groups than with fewer blocks
-        for (int k = 0; k < 5; k++) {                          // one split, or k / 2 workgroups a CU
-            long s = k * xcd / 2 / rg * 8 / seqs;
-            s = s < (tiles + 1) / 2 ? s : (tiles + 1) / 2;
-            s = kv_splits ? kv_splits : s < 1 ? 1 : s < kTreeMaxSplits ? s : kTreeMaxSplits;
-            const long wgs = (seqs * s + 7) / 8 * rg, steps = ((tiles + s - 1) / s + 1) / 2;
+        for (int k = 0; k < 5; k++) {                          // a unit a sequence, or k / 2 workgroups a CU
+            if (kv_splits && k != (kv_splits > 1)) continue;
+            // (of several sequences each may have a unit more than its share)
+            long units = kv_splits ? (long)B * kv_splits : k ? k * xcd / 2 / rg * 8 / KVH - (B > 1 ? B : 0) : B;
+            units = units < B ? B : kv_splits || units < (tiles + 1) / 2 ? units : (tiles + 1) / 2;
+            const long wgs = (units * KVH + 7) / 8 * rg, steps = ((tiles + units - 1) / units + 1) / 2;
             const double run = steps * (wgs <= xcd ? one[nb - 1] : two[nb - 1] * fmax(1.0, wgs / (2.0 * xcd)));
-            const double cost = fmax(run, read) + (s == 1 ? 0 : 3 + 0.3e-3 * seqs * R * s);
-            if (best == 0 || cost < best) best = cost, p = TreePlan{nb, rg, (int)s};
+            const double cost = fmax(run, read) + (k == 0 ? 0 : 3 + 0.3e-3 * KVH * R * units);
+            if (best == 0 || cost < best) best = cost, p = TreePlan{nb, rg, (int)units, kv_splits ? kv_splits : k == 0};
         }
     }
     return p;
 }
 
+// Units that a launch may have.
+static size_t max_units(const AttnTree& a, const TreePlan& p) { return p.fixed ? (size_t)a.B * p.fixed : (size_t)p.units + a.B; }
+
 size_t tree_part_bytes(const AttnTree& a, const TreePlan& p) {
-    if (p.splits == 1) return 0;
-    const size_t rows = (size_t)a.B * (a.n_heads / a.ratio) * p.splits * p.groups * 16 * p.blocks;
+    if (p.fixed == 1) return 0;
+    const size_t rows = max_units(a, p) * (a.n_heads / a.ratio) * p.groups * 16 * p.blocks;
     return rows * (HD * sizeof(float) + sizeof(float2));
 }
 
 hipError_t launch_attn_tree(const AttnTree& a, const TreePlan& p, void* ws, hipStream_t st) {
     const int KVH = a.n_heads / a.ratio;
-    const size_t units = (size_t)a.B * KVH * p.splits, rows = units * p.groups * 16 * p.blocks;
+    const size_t units = max_units(a, p) * KVH, rows = units * p.groups * 16 * p.blocks;
     float* opart = static_cast<float*>(ws);
     float2* mlpart = reinterpret_cast<float2*>(opart + rows * HD);
     const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.groups));
@@ -533,7 +589,7 @@ hipError_t launch_attn_tree(const AttnTree& a, const TreePlan& p, void* ws, hipS
         case 2: hipLaunchKernelGGL(attn_tree_k<2>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
         default: hipLaunchKernelGGL(attn_tree_k<3>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
     }
-    if (p.splits > 1)
+    if (p.fixed != 1)
         hipLaunchKernelGGL(attn_tree_join_k, dim3(a.T * a.ratio, a.B * KVH), dim3(256), 0, st, a, p, opart, mlpart);
     return hipGetLastError();
 }

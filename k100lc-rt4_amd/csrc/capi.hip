@@ -847,12 +847,13 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
     if (rc) return rc;
     hipStream_t st = as_stream(stream);
     rt4::TreePlan plan = rt4::tree_plan(B, T, n_heads, ratio, kv_len ? kv_max : 0, kv_splits, cus);
-    // under capture, as many of the automatic splits as the workspace that is there holds
-    if (!kv_splits && plan.splits > 1 && capturing(st) && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan)))
-        do plan.splits--;
-        while (plan.splits > 1 && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan)));
+    // under capture, as many units as the workspace that is there holds, at worst one a sequence
+    if (!kv_splits && plan.fixed != 1 && capturing(st) && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan))) {
+        while (plan.units > B && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan))) plan.units = plan.units > 2 * B ? plan.units / 2 : B;
+        if (!scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan))) plan.fixed = 1;
+    }
     void* ws = nullptr;
-    if (plan.splits > 1 && (rc = lib_scratch(kSlotTreePart, rt4::tree_part_bytes(a, plan), &ws, st))) return rc;
+    if (plan.fixed != 1 && (rc = lib_scratch(kSlotTreePart, rt4::tree_part_bytes(a, plan), &ws, st))) return rc;
     return hip_status(rt4::launch_attn_tree(a, plan, ws, st), "rt4_attention_tree launch");
 }
 

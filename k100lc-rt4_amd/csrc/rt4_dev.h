@@ -3,7 +3,6 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <cstdint>
-#include <type_traits>
 
 namespace rt4 {
 
@@ -89,6 +88,9 @@ __device__ __forceinline__ T wave_reduce(T v, F f) {
 __device__ __forceinline__ float wave_max(float v) {
     return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
+__device__ __forceinline__ int wave_max(int v) {
+    return wave_reduce(v, [](int a, int b) { return a > b ? a : b; });
+}
 __device__ __forceinline__ int wave_min(int v) {
     return wave_reduce(v, [](int a, int b) { return a < b ? a : b; });
 }
@@ -97,20 +99,25 @@ __device__ __forceinline__ T wave_sum(T v) {
     return wave_reduce(v, [](T a, T b) { return a + b; });
 }
 // Inclusive sums in lane order (row_shr 1, 2, 4, 8 within rows of 16, then the rows' last lanes).
-__device__ __forceinline__ double wave_scan(double v) {
-    auto add = [&](auto ctrl, auto mask) __attribute__((always_inline)) {
-        const uint2 u = __builtin_bit_cast(uint2, v);
-        const uint2 s = make_uint2((uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.x, decltype(ctrl)::value, decltype(mask)::value, 0xF, true),
-                                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.y, decltype(ctrl)::value, decltype(mask)::value, 0xF, true));
-        v += __builtin_bit_cast(double, s);
-    };
-    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});
-    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
-    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
-    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
-    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
-    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
-    return v;
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T scan_step(T v) {
+    constexpr int N = sizeof(T) / 4;
+    uint32_t a[N];
+    __builtin_memcpy(a, &v, sizeof(T));
+#pragma unroll
+    for (int k = 0; k < N; k++) a[k] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a[k], CTRL, ROWS, 0xF, true);
+    T s;
+    __builtin_memcpy(&s, a, sizeof(T));
+    return v + s;
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v = scan_step<0x111, 0xF>(v);
+    v = scan_step<0x112, 0xF>(v);
+    v = scan_step<0x114, 0xF>(v);
+    v = scan_step<0x118, 0xF>(v);
+    v = scan_step<0x142, 0xA>(v);
+    return scan_step<0x143, 0xC>(v);
 }
 
 // int4 -> int8 unpack used by every MFMA kernel here.  An RT4 dword holds

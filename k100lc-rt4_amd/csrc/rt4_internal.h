@@ -162,13 +162,14 @@ struct AttnTree {
     const int* parent;
     int B, T, TP, n_heads, ratio, kv_cap;
 };
-// 16-row blocks per workgroup, workgroups per (sequence, KV head) and split, KV splits.
+// 16-row blocks per workgroup, workgroups per unit (a run of keys of a sequence) and KV head, units
+// of all sequences (at most that many and B more), or `fixed` units of each.
 struct TreePlan {
-    int blocks, groups, splits;
+    int blocks, groups, units, fixed;
 };
 constexpr int kTreeMaxBlocks = 3, kTreeMaxSplits = 128;
 TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_splits, int cus);
-// Workspace of the splits' states (0 for one split).
+// Workspace of the units' states (0 where a sequence is one unit).
 size_t tree_part_bytes(const AttnTree& a, const TreePlan& p);
 hipError_t launch_attn_tree(const AttnTree& a, const TreePlan& p, void* ws, hipStream_t st);
 
