@@ -106,6 +106,11 @@ __device__ __forceinline__ Run run_of(const AttnTree& A, const TreePlan& P, int 
         const int len = A.kv_len ? A.kv_len[b] : 0;
         return ((len < 0 ? 0 : len > A.kv_cap ? A.kv_cap : len) + BNK - 1) / BNK + 1;
     };
+    if (A.B == 1) {                                            // (the same without the reductions)
+        const int t = uniform(tiles_of(0)), q = max(max(2, (t + P.units - 1) / P.units), (t + kTreeMaxSplits - 1) / kTreeMaxSplits);
+        const int n = P.fixed ? min(P.fixed, t) : (t + q - 1) / q;
+        return Run{!BY_UNIT || x < n ? 0 : -1, x, n, 0, t};
+    }
     const int held = tiles_of(lane);
     int q = 0;
     if (!P.fixed) {
@@ -377,7 +382,10 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
                 const v2f p = {__builtin_amdgcn_exp2f(s[nb][i]), __builtin_amdgcn_exp2f(s[nb][4 + i])};
                 sum += p[0] + p[1];
                 const v2h hi = __builtin_convertvector(p, v2h);
-                const v2f r = {p[0] - (float)hi[0], p[1] - (float)hi[1]};
+                const uint32_t hb = __builtin_bit_cast(uint32_t, hi);
+                v2f r;                                         // p - hi, the conversion back within the instruction
+                asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r[0]) : "v"(hb), "v"(p[0]));
+                asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r[1]) : "v"(hb), "v"(p[1]));
                 const v2h lo = __builtin_convertvector(r, v2h);
                 ph[2 * i] = hi[0];
                 ph[2 * i + 1] = hi[1];
