@@ -848,7 +848,7 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
     hipStream_t st = as_stream(stream);
     rt4::TreePlan plan = rt4::tree_plan(B, T, n_heads, ratio, kv_len ? kv_max : 0, kv_splits, cus);
     // under capture, as many units as the workspace that is there holds, at worst one a sequence
-    if (!kv_splits && plan.fixed != 1 && capturing(st) && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan))) {
+    if (!kv_splits && plan.fixed != 1 && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan)) && capturing(st)) {
         while (plan.units > B && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan))) plan.units = plan.units > 2 * B ? plan.units / 2 : B;
         if (!scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan))) plan.fixed = 1;
     }

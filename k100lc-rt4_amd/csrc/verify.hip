@@ -234,6 +234,20 @@ struct Nodes {
     float lt;                            // its token's logit in its parent's row
     double qc, u;                        // and probability there; its uniform
 };
+// Earlier siblings of lane i's node (nodes are in index order), and whether none of them has its token.
+__device__ __forceinline__ u64 siblings(const Tree& t, int tok, int T, bool& first) {
+    const int i = threadIdx.x & 63;
+    u64 sib = 0;
+    first = true;
+    for (int j = 1; j < T; j++) {
+        const int pj = __builtin_amdgcn_readlane(t.par, j), tj = __builtin_amdgcn_readlane(tok, j);
+        if (pj == t.par && j < i && i > 0 && t.anc) {
+            sib |= 1ull << j;
+            first = first && tj != tok;
+        }
+    }
+    return sib;
+}
 __device__ __forceinline__ Nodes read_nodes(const Verify& A, int b) {
     const int i = threadIdx.x & 63;
     Nodes n;
@@ -252,38 +266,23 @@ __device__ __forceinline__ Nodes read_nodes(const Verify& A, int b) {
 // The path of sequence b, by one wave, lane i node i; rows: the statistics of its T rows.  Whether a
 // node is accepted, once reached, depends on its parent's row and its earlier siblings alone, so all
 // nodes are tested at once and the path is the set whose ancestors all passed.
-__device__ void walk(const Verify& A, int b, double it, const Nodes& nd, const RowStat* rows, bool write, Draw* d) {
-    const int i = threadIdx.x & 63, T = A.T, R = A.B * T, C = A.C;
+__device__ void walk(const Verify& A, int b, double it, const Nodes& nd, const RowStat* rows, const double* mass, bool write, Draw* d) {
+    const int i = threadIdx.x & 63, T = A.T, R = A.B * T;
     const Tree t = nd.t;
     const bool kid = t.anc && i > 0;
     const int tok = nd.tok, pn = kid ? t.par : 0;
+    const size_t prow = (size_t)b * T + pn;
     const bool real = tok >= 0 && tok < A.V;
     const RowStat r = rows[pn];
     const double wt = it > 0 ? weight(nd.lt, r.m, it) : 0.0, pc = r.s > 0 ? wt / r.s : 0.0;
-    u64 sib = 0;                         // earlier siblings
-    bool first = true;                   // none of them has this token
+    bool first;
+    const u64 sib = siblings(t, tok, T, first);
     double W = 1.0, a = 0.0;
-    for (int j = 1; j < T; j++) {
-        const int pj = __builtin_amdgcn_readlane(t.par, j), tj = __builtin_amdgcn_readlane(tok, j);
-        if (pj == t.par && j < i && kid) {
-            sib |= 1ull << j;
-            first = first && tj != tok;
-        }
-    }
     bool tested = kid;
     if (A.q) {
         const int rank = __popcll(sib);
         tested = kid && rank < A.levels;
-        for (int k = 1; k < A.levels; k++) {                 // (wave-uniform loops: part is summed by the whole wave)
-            for (int n = 0; n < T; n++) {
-                const size_t pr = (size_t)b * T + n;
-                if (__popcll(__ballot(kid && t.par == n)) <= k || !(it > 0)) continue;
-                double w = 0;
-                for (int c = i; c < C; c += 64) w += A.part[((size_t)k * R + pr) * C + c];
-                w = wave_sum(w);
-                if (kid && t.par == n && rank == k) W = w, a = A.av[(size_t)k * R + pr];
-            }
-        }
+        if (tested && rank > 0) W = mass[i], a = A.av[(size_t)rank * R + prow];
     } else {
         const double mine = first ? pc : 0.0;
         for (int j = 1; j < T; j++) {
@@ -361,16 +360,31 @@ __device__ __forceinline__ double residuals(double (&w)[E], const Verify& A, con
 }
 
 // Statistics of sequence b's rows into LDS, a wave per row, beside what the first wave reads of its
-// tree, and the walk.
-__device__ __forceinline__ void walk_sequence(const Verify& A, int b, double it, RowStat* rows, bool write, Draw* d) {
+// tree, and the walk.  mass [64]: the residual's sum that a later sibling is tested against.
+__device__ __forceinline__ void walk_sequence(const Verify& A, int b, double it, RowStat* rows, double* mass, bool write, Draw* d) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
     Nodes nd;
-    if (threadIdx.x < 64) nd = read_nodes(A, b);
-    for (int n = threadIdx.x >> 6; n < A.T; n += blockDim.x >> 6) {
+    if (w == 0) nd = read_nodes(A, b);
+    for (int n = w; n < A.T; n += waves) {
         const RowStat r = row_of_chunks(A.ch + ((size_t)b * A.T + n) * A.C, A.C, it);
-        if ((threadIdx.x & 63) == 0) rows[n] = r;
+        if (lane == 0) rows[n] = r;
+    }
+    if (A.q && A.levels > 1 && it > 0) {
+        bool first;
+        const Tree t = tree_of(A.parent, b, A.T);
+        const int rank = __popcll(siblings(t, 0, A.T, first));
+        for (int i = 1 + w; i < A.T; i += waves) {
+            const int k = __builtin_amdgcn_readlane(rank, i), pn = __builtin_amdgcn_readlane(t.par, i);
+            if (k < 1 || k >= A.levels) continue;
+            const double* src = A.part + ((size_t)k * A.B * A.T + (size_t)b * A.T + pn) * A.C;
+            double s = 0;
+            for (int c = lane; c < A.C; c += 64) s += src[c];
+            s = wave_sum(s);
+            if (lane == 0) mass[i] = s;
+        }
     }
     __syncthreads();
-    if (threadIdx.x < 64) walk(A, b, it, nd, rows, write, d);
+    if (w == 0) walk(A, b, it, nd, rows, mass, write, d);
     __syncthreads();
 }
 
@@ -380,10 +394,11 @@ __global__ __launch_bounds__(512) void verify_residual_k(const Verify A) {
     constexpr int E = CH / 512;
     __shared__ double ss[8];
     __shared__ RowStat rows[64];
+    __shared__ double mass[64];
     __shared__ Draw d;
     const int b = blockIdx.y, c = blockIdx.x;
     const double it = inv_temp(A.temp, b);
-    walk_sequence(A, b, it, rows, c == 0, &d);
+    walk_sequence(A, b, it, rows, mass, c == 0, &d);
     if (c == 0 && threadIdx.x < sizeof(Draw) / 4) reinterpret_cast<int*>(A.draw + b)[threadIdx.x] = reinterpret_cast<const int*>(&d)[threadIdx.x];
     if (d.row < 0 || !(it > 0)) return;
     double w[E];
@@ -474,7 +489,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
 #pragma unroll
     for (int e = 0; e < CE; e++) mass[e] = A.q && CE * tid + e < A.C ? A.sums[(size_t)b * A.C + CE * tid + e] : 0.0;
     if (!A.q) {
-        walk_sequence(A, b, it, rows, true, &d);
+        walk_sequence(A, b, it, rows, nullptr, true, &d);
     } else {
         if (tid < (int)(sizeof(Draw) / 4)) reinterpret_cast<int*>(&d)[tid] = reinterpret_cast<const int*>(A.draw + b)[tid];
         __syncthreads();
