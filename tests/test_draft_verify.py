@@ -666,3 +666,170 @@ def test_python_refusals_on_the_device(rt4, torch_gpu):
                  ((*q, *kv(128), i(1).long(), *kv(), i(1, 4)), dict(ratio=2))):
         with pytest.raises(rt4.RT4Error):
             rt4.attention_tree(*a, **k)
+
+
+@pytest.mark.gpu
+def test_many_sequences(rt4, torch_gpu, orc):
+    """More sequences than a wave has lanes, of all lengths: the shares of the keys, the joins and the walks."""
+    rng = np.random.default_rng(21)
+    B, T, H, ratio, cap = 150, 2, 1, 2, 192
+    qq, qs, kv, draft = attention_case(orc, rng, B, T, H, ratio, cap, 2)
+    lens = rng.integers(-1, cap + 2, B)
+    parent = np.tile([[-1, 0]], (B, 1))
+    parent[rng.integers(0, B, 20), 0] = -2
+    spoil_unseen(kv, draft, lens, T)
+    want, tol = tree_attention(qq, qs, kv, lens, draft, parent, ratio)
+    for splits in (0, 1, 2, 100):
+        print(f"case many sequences, kv_splits={splits}", flush=True)
+        out = rt4.attention_tree(dev(qq), dev(qs), *map(dev, kv), dev(lens), *map(dev, draft), dev(parent), ratio=ratio, kv_splits=splits)
+        check_attention(out, want, tol)
+    for probs in (False, True):
+        logits, tok, par, u, q = verify_case(rng, B, 5, 500, 2, probs)
+        check_verify(rt4, logits, tok, par, u, [(1.0, 0.0)[b % 2] for b in range(B)], q, 2 if probs else None, kv_len=list(range(B)))
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(rt4, torch_gpu, orc):
+    """The longest cache there may be, 2^24 - 64 keys, for two sequences: byte offsets pass 2^31 within one and 2^32 over both."""
+    torch = torch_gpu
+    print("case longest cache", flush=True)
+    cap, B, H, ratio, T = (1 << 24) - 64, 2, 1, 2, 2
+    g = torch.Generator(device="cuda").manual_seed(7)
+    ri = lambda *s: torch.randint(-2**31, 2**31 - 1, s, dtype=torch.int32, device="cuda", generator=g)  # noqa: E731
+    kv = [ri(B, H, cap, 32), torch.rand((B, H, 2, cap), device="cuda", generator=g), ri(B, H, cap // 8, D),
+          torch.rand((B, H, cap // BG, D), device="cuda", generator=g)]
+    rng = np.random.default_rng(7)
+    lens = [cap - 70, cap - 3]
+    # the last keys, through the append (within a tile, and to the cache's very end)
+    kf, vf = (rng.standard_normal((B, 3, H, D)).astype(np.float32) for _ in range(2))
+    stage = rng.standard_normal((B, H, BG, D)).astype(np.float32)
+    tail = [host(x) for x in (kv[0][:, :, -128:], kv[1][:, :, :, -128:], kv[2][:, :, -16:], kv[3][:, :, -2:])]
+    tail = [np.ascontiguousarray(x).view(np.uint32) if x.dtype == np.int32 else np.ascontiguousarray(x) for x in tail]
+    st = dev(stage)
+    rt4.kv_append_rows(*kv, st, dev(kf), dev(vf), kv_len=dev(np.array(lens) + 3))
+    lens = [n + 3 for n in lens]
+    append_expected(orc, tail, stage, kf, vf, np.array([128 - 70, 128 - 3]), np.tile(np.arange(3), (B, 1)), np.array([3, 3]))
+    for g_, w in zip((kv[0][:, :, -128:], kv[1][:, :, :, -128:], kv[2][:, :, -16:], kv[3][:, :, -2:], st), (*tail, stage)):
+        assert np.array_equal(np.ascontiguousarray(host(g_)).view(np.uint32), w.view(np.uint32))
+    # attention over all of it, against 64-bit sums by pieces
+    qq, qs, _, draft = attention_case(orc, rng, B, T, H, ratio, BG, 0.2)
+    parent = np.array([[-1, 0], [-1, 0]])
+    out = rt4.attention_tree(dev(qq), dev(qs), *kv, dev(np.array(lens)), *map(dev, draft), dev(parent), ratio=ratio)
+    nib = lambda w: torch.stack([(w << (28 - 4 * e)) >> 28 for e in range(8)], -1)  # noqa: E731
+    for b in range(B):
+        Kd, Vd = cache_values(*(x[b, 0] for x in draft))
+        for r in range(ratio):
+            for i in range(T):
+                q = nibbles(qq[r, b * T + i]).reshape(D) * np.repeat(qs[r, :, b * T + i].astype(np.float64), G)
+                s_d = Kd[:i + 1] @ q
+                qd = torch.tensor(q, device="cuda")
+                parts, top, step = [], s_d.max(), 1 << 21
+                for k0 in range(0, lens[b], step):
+                    k1 = min(k0 + step, lens[b])
+                    kk = nib(kv[0][b, 0, k0:k1]).reshape(k1 - k0, D).double()
+                    s = (kk[:, :G] @ qd[:G]) * kv[1][b, 0, 0, k0:k1].double() + (kk[:, G:] @ qd[G:]) * kv[1][b, 0, 1, k0:k1].double()
+                    del kk
+                    m = float(s.max())
+                    p = (s - m).exp()
+                    t0, t1 = k0 // BG, (k1 + BG - 1) // BG
+                    pt = torch.zeros((t1 - t0) * BG, dtype=torch.float64, device="cuda")
+                    pt[:k1 - k0] = p
+                    v = nib(kv[2][b, 0, t0 * 8:t1 * 8]).transpose(1, 2).reshape(-1, BG, D).float()
+                    o = (torch.bmm(pt.view(-1, 1, BG).float(), v)[:, 0].double() * kv[3][b, 0, t0:t1].double()).sum(0)
+                    parts.append((m, float(p.sum()), host(o)))
+                    top = max(top, m)
+                pd = np.exp(s_d - top)
+                l = pd.sum() + sum(ls * np.exp(m - top) for m, ls, _ in parts)
+                o = pd @ Vd[:i + 1] + sum(o * np.exp(m - top) for m, _, o in parts)
+                got = host(out)[r, b * T + i].astype(np.float64)
+                # as in tree_attention with |V| <= 8, S <= 2 x 16 x 16 x 0.2 x .. below 64, and the pieces' own fp32 products
+                bound = 8 * ((8 * 64 + 168 + 128) * 2.0**-24 + 2.0**-22 + lens[b] * 2.0**-32)
+                assert np.abs(got - o / l).max() <= bound, (np.abs(got - o / l).max(), bound)
+
+
+CAPTURE = r"""
+import sys
+sys.path[:0] = [{root!r}, {pkg!r}]
+import torch
+import rt4_amd
+torch.cuda.set_device(0)
+g = torch.Generator(device="cuda").manual_seed(3)
+f = lambda *s: torch.randn(s, device="cuda", generator=g)
+i = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+B, T, H, ratio, cap, V = 2, 4, 2, 3, 4096, 30000
+kv = (i(B, H, cap, 32), torch.ones((B, H, 2, cap), device="cuda"), i(B, H, cap // 8, 256), torch.ones((B, H, cap // 64, 256), device="cuda"))
+dr = (i(B, H, 64, 32), torch.ones((B, H, 2, 64), device="cuda"), i(B, H, 8, 256), torch.ones((B, H, 1, 256), device="cuda"))
+stage = torch.zeros((B, H, 64, 256), device="cuda")
+kv_len = torch.tensor([4000, 77], dtype=torch.int32, device="cuda")
+for k in range(0, 4096, 512):
+    n = torch.full((B,), k + 512, dtype=torch.int32, device="cuda")
+    rt4_amd.kv_append_rows(*kv, stage, f(B, 512, H, 256), f(B, 512, H, 256), kv_len=n)
+kf, vf = f(B, T, H, 256), f(B, T, H, 256)
+qq, qs = rt4_amd.attn_q_quant(f(B * T, H * ratio, 256) / 8, B * T)
+parent = torch.tensor([[-1, 0, 0, 1], [-1, 0, 1, 2]], dtype=torch.int32, device="cuda")
+logits, u = f(B * T, V), torch.rand((B, T), device="cuda", generator=g)
+draft = logits.view(B, T, V)[:, :1].topk(T, -1).indices[:, 0].int().contiguous()
+out = torch.empty((H * ratio, B * T, 256), device="cuda")
+outs = (i(B, T), i(B, T), i(B))
+
+def attention(o=None):
+    rt4_amd.kv_append_rows(*dr, None, kf, vf)
+    return rt4_amd.attention_tree(qq, qs, *kv, kv_len, *dr, parent, ratio=ratio, out=o)
+
+def verify(o=(None, None, None)):
+    return rt4_amd.verify_tree(logits, draft, parent, u, tokens=o[0], path=o[1], count=o[2])
+
+def capture(fn):
+    gr, err = torch.cuda.CUDAGraph(), None
+    with torch.cuda.graph(gr):
+        try:
+            fn()
+        except rt4_amd.RT4Error as e:
+            err = str(e)
+    return gr, err
+
+torch.cuda.synchronize()
+ga, err = capture(lambda: attention(out))
+print("attention, first call:", err, flush=True)
+assert err is None                                        # one unit a sequence needs no workspace
+_, err = capture(lambda: verify(outs))
+print("verification, first call:", err, flush=True)
+assert err is not None and "captur" in err
+want, wv = attention().clone(), [x.clone() for x in verify()]
+gv, err = capture(lambda: verify(outs))
+assert err is None, err
+gb, err = capture(lambda: attention(out))
+assert err is None, err
+for rep in range(3):
+    for gr in (ga, gb):
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        gr.replay()
+        torch.cuda.synchronize()
+        rel = float((out - want).norm() / want.norm())
+        assert rel < 2 * 168 * 2.0**-24 and (gr is ga or torch.equal(out, want)), rel        # (sums in another order)
+    for x in outs:
+        x.fill_(9)
+    attention()                                           # the program's own work between the replays
+    gv.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, wv))
+rt4_amd.release_scratch()
+again = attention()
+assert torch.equal(again, want) and all(torch.equal(a, b) for a, b in zip(verify(), wv))
+print("CAPTURE-OK", flush=True)
+"""
+
+
+@pytest.mark.gpu
+def test_capture_before_any_eager_call():
+    """In a fresh process nothing is allocated under capture: the attention takes one unit a sequence, the verification refuses."""
+    import subprocess
+    import sys
+
+    from conftest import PKG_DIR, ROOT
+    print("case capture in a fresh process", flush=True)
+    r = subprocess.run([sys.executable, "-u", "-c", CAPTURE.format(root=str(ROOT), pkg=str(PKG_DIR))], capture_output=True, text=True,
+                       timeout=300)
+    print(r.stdout[-3000:], r.stderr[-3000:])
+    assert r.returncode == 0 and "CAPTURE-OK" in r.stdout
