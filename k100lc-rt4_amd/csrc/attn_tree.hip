@@ -44,12 +44,22 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
 
+// Maxima by the instruction itself: fmaxf first quiets operands that it cannot see made (a third of
+// the scores' maximum was that).
+__device__ __forceinline__ float max2(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 // Max over the four lanes that hold one query row's keys (lanes 16 and 32 apart).
 __device__ __forceinline__ float max_groups(float v) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
+    v = with_half<16>(v, max2);
+    return with_half<32>(v, max2);
 }
 
 // 16 int8 operand bytes (16 x code) of two code dwords.
@@ -332,10 +342,8 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
         }
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
-            float mt = s[nb][0];
-#pragma unroll
-            for (int e = 1; e < 8; e++) mt = fmaxf(mt, s[nb][e]);
-            mt = max_groups(mt);
+            float mt = max3(max3(s[nb][0], s[nb][1], s[nb][2]), s[nb][3], s[nb][4]);
+            mt = max_groups(max3(max2(mt, s[nb][5]), s[nb][6], s[nb][7]));
             if (g == 0) mx[w][nb * 16 + c] = mt;
         }
     };
@@ -346,7 +354,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
             const int r = nb * 16 + c;
-            mt[nb] = fmaxf(fmaxf(mx[0][r], mx[1][r]), fmaxf(mx[2][r], mx[3][r])) - kPBits;
+            mt[nb] = max3(max2(mx[0][r], mx[1][r]), mx[2][r], mx[3][r]) - kPBits;
             any |= mt[nb] > kLazy;
         }
         if (!__any(any)) return;
