@@ -345,9 +345,11 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
  *     a rejection max(r - draft_p, 0) renormalized.  At most max_children children of a
  *     node are tested, the rest are rejected.
  * Where no child is accepted the last token is drawn from what is left: the smallest x
- * whose cumulated residual exceeds u[b][0] times its total.  So the tokens are distributed
- * as the target's own.  temp NULL: 1; temp[b] <= 0 (or NaN): greedy, a child is accepted
- * iff it is the row's largest logit (lowest index among equals), and so is the last token.
+ * whose cumulated residual exceeds u[b][0] times its total (the row's largest logit where
+ * nothing is left, which only distributions that do not sum to 1 come to).  So the tokens
+ * are distributed as the target's own.  temp NULL: 1; temp[b] <= 0 (or NaN): greedy, a child
+ * is accepted iff it is the row's largest logit (lowest index among equals), and so is the
+ * last token; temp[b] infinite: every logit that is not -inf weighs the same.
  * A NaN logit counts as -inf; a row of nothing but -inf ends the walk with token -1.
  * A draft token outside [0, V) is rejected.
  * Outputs: count[b] = n accepted nodes, the root included (0: idle); path int32 [B][T] their

@@ -83,7 +83,7 @@ __device__ __forceinline__ RowStat row_of_chunks(const RowStat* ch, int C, doubl
 
 __device__ __forceinline__ double inv_temp(const float* temp, int b) {
     const float t = temp ? temp[b] : 1.f;
-    return t > 0.f ? 1.0 / (double)t : 0.0;                  // 0: greedy
+    return t > 0.f ? 1.0 / (double)t : -1.0;                 // -1: greedy (0: an infinite temperature)
 }
 
 __device__ __forceinline__ double lane_of(double v, int j) {     // (j the same in every lane)
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(256) void verify_stats_k(const float* __restrict__ 
 #pragma unroll
     for (int e = PT - 1; e >= 0; e--) {
         if (v[e] == m && m > -INFINITY) mi = at + 256 * (e & ~3) + (e & 3);
-        if (it > 0) s += weight(v[e], m, it);
+        if (it >= 0) s += weight(v[e], m, it);
     }
     mi = wave_min(mi);
     s = wave_sum(s);
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256) void verify_mass_k(const float* __restrict__ l
     const Tree t = tree_of(parent, b, T);
     if (__popcll(__ballot(t.par == row % T)) <= level) return;
     const double it = inv_temp(temp, b);
-    if (!(it > 0)) return;
+    if (!(it >= 0)) return;
     float l[PT], pq[PT];
 #pragma unroll
     for (int e = 0; e < PT; e++) {
@@ -274,7 +274,7 @@ __device__ void walk(const Verify& A, int b, double it, const Nodes& nd, const R
     const size_t prow = (size_t)b * T + pn;
     const bool real = tok >= 0 && tok < A.V;
     const RowStat r = rows[pn];
-    const double wt = it > 0 ? weight(nd.lt, r.m, it) : 0.0, pc = r.s > 0 ? wt / r.s : 0.0;
+    const double wt = it >= 0 ? weight(nd.lt, r.m, it) : 0.0, pc = r.s > 0 ? wt / r.s : 0.0;
     bool first;
     const u64 sib = siblings(t, tok, T, first);
     double W = 1.0, a = 0.0;
@@ -291,7 +291,7 @@ __device__ void walk(const Verify& A, int b, double it, const Nodes& nd, const R
         }
     }
     bool yes = A.q ? nd.u * W * nd.qc < pc - a * nd.qc : first && nd.u * W < pc;
-    if (!(it > 0)) yes = tok == r.i;
+    if (!(it >= 0)) yes = tok == r.i;
     yes = yes && tested && real;
     const u64 yesm = __ballot(yes);
     const u64 okm = __ballot(yes && !(sib & yesm));
@@ -369,7 +369,7 @@ __device__ __forceinline__ void walk_sequence(const Verify& A, int b, double it,
         const RowStat r = row_of_chunks(A.ch + ((size_t)b * A.T + n) * A.C, A.C, it);
         if (lane == 0) rows[n] = r;
     }
-    if (A.q && A.levels > 1 && it > 0) {
+    if (A.q && A.levels > 1 && it >= 0) {
         bool first;
         const Tree t = tree_of(A.parent, b, A.T);
         const int rank = __popcll(siblings(t, 0, A.T, first));
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(512) void verify_residual_k(const Verify A) {
     const double it = inv_temp(A.temp, b);
     walk_sequence(A, b, it, rows, mass, c == 0, &d);
     if (c == 0 && threadIdx.x < sizeof(Draw) / 4) reinterpret_cast<int*>(A.draw + b)[threadIdx.x] = reinterpret_cast<const int*>(&d)[threadIdx.x];
-    if (d.row < 0 || !(it > 0)) return;
+    if (d.row < 0 || !(it >= 0)) return;
     double w[E];
     const double s = wave_sum(residuals<E, 512>(w, A, d, it, c * CH + (int)threadIdx.x));
     if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = s;
@@ -475,7 +475,8 @@ __device__ __forceinline__ int thread_pick(const double (&x)[E], double& left) {
 // thread has CE chunks in a row (V <= 2^22), then TE tokens of the chunk that is picked.
 //
 // Without draft probabilities a chunk's mass is the sum that verify_stats_k left, less the rejected
-// tokens'.  Where hardly anything is left that difference says little, and the chunks are summed anew.
+// tokens'.  Where hardly anything is left that difference says little, and the chunks are summed anew; so
+// they are where the chunk that is picked turns out to hold rejected tokens alone.
 __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
     constexpr int CE = kVerifyMaxV / CH / kDrawThreads, TE = CH / kDrawThreads;
     __shared__ RowStat rows[64];
@@ -497,10 +498,11 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
     if (d.row < 0) return;
     int* out = A.tokens + (size_t)b * A.T + d.n - 1;
     const int best = d.r.i < A.V ? d.r.i : -1;
-    if (!(it > 0) || best < 0) {                               // greedy, or a row with nothing in it
+    if (!(it >= 0) || best < 0) {                              // greedy, or a row with nothing in it
         if (tid == 0) *out = best;
         return;
     }
+    bool anew = A.q;
     if (!A.q) {
         double gone = 0;
 #pragma unroll
@@ -515,7 +517,10 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
             mass[e] = fmax(mass[e], 0.0);
         }
         for (int k = 0; k < d.nrej; k++) gone += d.rejw[k];
-        if (d.r.s - gone < 1e-6 * d.r.s) {
+        anew = d.r.s - gone < 1e-6 * d.r.s;
+    }
+    for (;; anew = true) {
+        if (!A.q && anew) {
             for (int c = 0; c < A.C; c++) {
                 double x[TE];
                 const double s = wave_sum(residuals<TE, 1>(x, A, d, it, c * CH + tid * TE));
@@ -530,27 +535,24 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
                 __syncthreads();
             }
         }
-    }
-    double mine = 0, r = -1.0;
+        double mine = 0, r = -1.0;
 #pragma unroll
-    for (int e = 0; e < CE; e++) mine += mass[e];
-    const int owner = block_pick(mine, u, r, L);
-    if (owner < 0) {                                           // nothing left: the largest
-        if (tid == 0) *out = best;
-        return;
-    }
-    if (tid == owner) {
-        s_chunk = CE * tid + thread_pick(mass, r);
-        s_left = fmax(r, 0.0);
-    }
-    __syncthreads();
-    const int at = s_chunk * CH + tid * TE;
-    double x[TE], left = s_left;
-    const int th = block_pick(residuals<TE, 1>(x, A, d, it, at), u, left, L);
-    if (th < 0) {                                              // (a chunk whose mass was rounding alone)
-        if (tid == 0) *out = best;
-    } else if (tid == th) {
-        *out = at + thread_pick(x, left);
+        for (int e = 0; e < CE; e++) mine += mass[e];
+        const int owner = block_pick(mine, u, r, L);
+        if (owner < 0) {                                       // nothing left: the largest
+            if (tid == 0) *out = best;
+            return;
+        }
+        if (tid == owner) {
+            s_chunk = CE * tid + thread_pick(mass, r);
+            s_left = fmax(r, 0.0);
+        }
+        __syncthreads();
+        const int at = s_chunk * CH + tid * TE;
+        double x[TE], left = s_left;
+        const int th = block_pick(residuals<TE, 1>(x, A, d, it, at), u, left, L);
+        if (th == tid) *out = at + thread_pick(x, left);
+        if (th >= 0 || anew) return;                           // (else a chunk whose mass was rounding alone)
     }
 }
 

@@ -833,3 +833,47 @@ def test_capture_before_any_eager_call():
                        timeout=300)
     print(r.stdout[-3000:], r.stderr[-3000:])
     assert r.returncode == 0 and "CAPTURE-OK" in r.stdout
+
+
+@pytest.mark.gpu
+def test_verify_rejected_mass_leaves_nothing(rt4, torch_gpu):
+    """A run of the vocabulary whose only tokens were rejected has no mass: u = 0 draws the first token with any behind it."""
+    print("case rejected mass", flush=True)
+    rng = np.random.default_rng(11)
+    B, T, V = 64, 3, 9000
+    logits = np.full((B * T, V), -np.inf, np.float32)
+    first = logits[::T]
+    first[:, 3], first[:, 5], first[:, 8000] = 0.0, -rng.random(B) - 0.1, -rng.random(B)
+    draft, parent = np.tile([0, 3, 5], (B, 1)), np.tile([-1, 0, 0], (B, 1))
+    u = np.tile(np.array([0.0, 1 - 2.0**-23, 1 - 2.0**-23], np.float32), (B, 1))
+    want = verify(logits, draft, parent, u, np.ones(B))
+    assert (want[0][:, 0] == 8000).all() and (want[2] == 1).all()
+    got = rt4.verify_tree(dev(logits), dev(draft), dev(parent), dev(u))
+    for g, w in zip(got, want):
+        assert np.array_equal(host(g), w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_infinite_temperature(rt4, torch_gpu, probs):
+    """At an infinite temperature every token whose logit is not -inf weighs the same."""
+    print(f"case infinite temperature probs={probs}", flush=True)
+    rng = np.random.default_rng(12)
+    B, T, V = 8, 4, 6000
+    logits = rng.standard_normal((B * T, V)).astype(np.float32)
+    parent = np.tile([-1, 0, 0, 1], (B, 1))
+    draft = rng.integers(0, V, (B, T))
+    # uniforms between the multiples of 1 / V, so that no sum's rounding decides
+    u = ((rng.integers(0, V, (B, T)) + 0.5) / V).astype(np.float32)
+    u[::2, 1:] = 0.25 / V
+    q = None
+    if probs:
+        q = rng.random((B * T, V)).astype(np.float32)
+        q /= q.sum(1, keepdims=True)
+        q[np.arange(B) * T, draft[:, 1]] = 0.5
+    temp = np.full(B, np.inf, np.float32)
+    want = verify(logits, draft, parent, u, temp, q, 2 if probs else None)
+    got = rt4.verify_tree(dev(logits), dev(draft), dev(parent), dev(u), temp=dev(temp), draft_probs=None if q is None else dev(q),
+                          max_children=2 if probs else None)
+    for g, w in zip(got, want):
+        assert np.array_equal(host(g), w)
