@@ -95,10 +95,10 @@ struct Tree {
     int par;
     u64 anc;                             // the node and those above it; 0: not in the tree
 };
-__device__ __forceinline__ Tree tree_of(const int* parent, int b, int T) {
+__device__ __forceinline__ Tree tree_of(int par, int T) {      // (par: node i's parent, -2 past the last node)
     const int i = threadIdx.x & 63;
     Tree t;
-    t.par = i < T ? parent[(size_t)b * T + i] : -2;
+    t.par = par;
     const bool root = i == 0 && t.par == -1, node = i > 0 && t.par >= 0 && t.par < i;
     int up = node ? t.par : i;
     u64 anc = 1ull << i;
@@ -186,8 +186,8 @@ __global__ __launch_bounds__(256) void verify_mass_k(const float* __restrict__ l
                                                      double* __restrict__ av, double* __restrict__ part) {
     __shared__ double ss[4];
     const int row = blockIdx.y, b = row / T, c = blockIdx.x, C = gridDim.x, R = gridDim.y;
-    const Tree t = tree_of(parent, b, T);
-    if (__popcll(__ballot(t.par == row % T)) <= level) return;
+    const int i = threadIdx.x & 63, n = row % T;               // (children of padding are counted too, to no harm)
+    if (__popcll(__ballot(i > n && i < T && parent[(size_t)b * T + i] == n)) <= level) return;
     const double it = inv_temp(temp, b);
     if (!(it >= 0)) return;
     float l[PT], pq[PT];
@@ -234,31 +234,31 @@ struct Nodes {
     float lt;                            // its token's logit in its parent's row
     double qc, u;                        // and probability there; its uniform
 };
-// Earlier siblings of lane i's node (nodes are in index order), and whether none of them has its token.
-__device__ __forceinline__ u64 siblings(const Tree& t, int tok, int T, bool& first) {
+// Earlier siblings of lane i's node (nodes are in index order), by one wave; kids [64] in LDS, the wave's own.
+__device__ __forceinline__ u64 siblings(const Tree& t, u64* kids) {
     const int i = threadIdx.x & 63;
-    u64 sib = 0;
-    first = true;
-    for (int j = 1; j < T; j++) {
-        const int pj = __builtin_amdgcn_readlane(t.par, j), tj = __builtin_amdgcn_readlane(tok, j);
-        if (pj == t.par && j < i && i > 0 && t.anc) {
-            sib |= 1ull << j;
-            first = first && tj != tok;
-        }
-    }
-    return sib;
+    const bool kid = t.anc && i > 0;
+    kids[i] = 0;
+    __builtin_amdgcn_wave_barrier();
+    if (kid) atomicOr(kids + t.par, 1ull << i);
+    __builtin_amdgcn_wave_barrier();
+    return kid ? kids[t.par] & ((1ull << i) - 1) : 0;
 }
 __device__ __forceinline__ Nodes read_nodes(const Verify& A, int b) {
     const int i = threadIdx.x & 63;
     Nodes n;
     int tok = i < A.T ? A.draft[(size_t)b * A.T + i] : -1;
     const float u = i < A.T ? A.u[(size_t)b * A.T + i] : 0.f;
-    n.t = tree_of(A.parent, b, A.T);
-    const bool kid = n.t.anc && i > 0, real = kid && tok >= 0 && tok < A.V;
-    const size_t prow = (size_t)b * A.T + (kid ? n.t.par : 0);
+    const int par = i < A.T ? A.parent[(size_t)b * A.T + i] : -2;
+    // (what a node names is read while the tree is made out: padding reads too)
+    const bool named = i > 0 && par >= 0 && par < i && tok >= 0 && tok < A.V;
+    const size_t prow = (size_t)b * A.T + (named ? par : 0);
+    const float lt = A.logits[prow * A.ldl + (named ? tok : 0)], qc = A.q ? A.q[prow * A.ldq + (named ? tok : 0)] : 0.f;
+    n.t = tree_of(par, A.T);
+    const bool kid = n.t.anc && i > 0, real = kid && named;
     n.tok = kid ? tok : -1;
-    n.lt = real ? A.logits[prow * A.ldl + tok] : -INFINITY;
-    n.qc = real && A.q ? (double)A.q[prow * A.ldq + tok] : 0.0;
+    n.lt = real ? lt : -INFINITY;
+    n.qc = real ? (double)qc : 0.0;
     n.u = kid ? (double)u : 0.0;
     return n;
 }
@@ -266,7 +266,7 @@ __device__ __forceinline__ Nodes read_nodes(const Verify& A, int b) {
 // The path of sequence b, by one wave, lane i node i; rows: the statistics of its T rows.  Whether a
 // node is accepted, once reached, depends on its parent's row and its earlier siblings alone, so all
 // nodes are tested at once and the path is the set whose ancestors all passed.
-__device__ void walk(const Verify& A, int b, double it, const Nodes& nd, const RowStat* rows, const double* mass, bool write, Draw* d) {
+__device__ void walk(const Verify& A, int b, double it, const Nodes& nd, const RowStat* rows, const double* mass, u64* kids, bool write, Draw* d) {
     const int i = threadIdx.x & 63, T = A.T, R = A.B * T;
     const Tree t = nd.t;
     const bool kid = t.anc && i > 0;
@@ -275,19 +275,22 @@ __device__ void walk(const Verify& A, int b, double it, const Nodes& nd, const R
     const bool real = tok >= 0 && tok < A.V;
     const RowStat r = rows[pn];
     const double wt = it >= 0 ? weight(nd.lt, r.m, it) : 0.0, pc = r.s > 0 ? wt / r.s : 0.0;
-    bool first;
-    const u64 sib = siblings(t, tok, T, first);
+    const u64 sib = siblings(t, kids);
     double W = 1.0, a = 0.0;
-    bool tested = kid;
+    bool tested = kid, first = true;                           // first: no earlier sibling has its token
     if (A.q) {
         const int rank = __popcll(sib);
         tested = kid && rank < A.levels;
         if (tested && rank > 0) W = mass[i], a = A.av[(size_t)rank * R + prow];
     } else {
-        const double mine = first ? pc : 0.0;
-        for (int j = 1; j < T; j++) {
-            const double pj = lane_of(mine, j);
-            if (sib >> j & 1) W -= pj;
+        // the k-th earlier siblings of all nodes at once; that one has been compared with its own k by then
+        for (u64 rest = sib; __any(rest != 0); rest &= rest - 1) {
+            const int j = rest ? __ffsll((unsigned long long)rest) - 1 : i, tj = __shfl(tok, j);
+            const double pj = __shfl(first ? pc : 0.0, j);
+            if (rest) {
+                W -= pj;
+                first = first && tj != tok;
+            }
         }
     }
     bool yes = A.q ? nd.u * W * nd.qc < pc - a * nd.qc : first && nd.u * W < pc;
@@ -362,7 +365,8 @@ __device__ __forceinline__ double residuals(double (&w)[E], const Verify& A, con
 // Statistics of sequence b's rows into LDS, a wave per row, beside what the first wave reads of its
 // tree, and the walk.  mass [64]: the residual's sum that a later sibling is tested against.
 __device__ __forceinline__ void walk_sequence(const Verify& A, int b, double it, RowStat* rows, double* mass, bool write, Draw* d) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    __shared__ u64 kids[64];
+    const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), waves = blockDim.x >> 6;
     Nodes nd;
     if (w == 0) nd = read_nodes(A, b);
     for (int n = w; n < A.T; n += waves) {
@@ -370,12 +374,11 @@ __device__ __forceinline__ void walk_sequence(const Verify& A, int b, double it,
         if (lane == 0) rows[n] = r;
     }
     if (A.q && A.levels > 1 && it >= 0) {
-        bool first;
-        const Tree t = tree_of(A.parent, b, A.T);
-        const int rank = __popcll(siblings(t, 0, A.T, first));
-        for (int i = 1 + w; i < A.T; i += waves) {
-            const int k = __builtin_amdgcn_readlane(rank, i), pn = __builtin_amdgcn_readlane(t.par, i);
-            if (k < 1 || k >= A.levels) continue;
+        const int par = lane < A.T ? A.parent[(size_t)b * A.T + lane] : -2;
+        for (int i = 1 + w; i < A.T; i += waves) {             // (of padding too: nothing reads that)
+            const int pn = __builtin_amdgcn_readlane(par, i);
+            const int k = __popcll(__ballot(lane > pn && lane < i && par == pn));
+            if (pn < 0 || pn >= i || k < 1 || k >= A.levels) continue;
             const double* src = A.part + ((size_t)k * A.B * A.T + (size_t)b * A.T + pn) * A.C;
             double s = 0;
             for (int c = lane; c < A.C; c += 64) s += src[c];
@@ -384,15 +387,15 @@ __device__ __forceinline__ void walk_sequence(const Verify& A, int b, double it,
         }
     }
     __syncthreads();
-    if (w == 0) walk(A, b, it, nd, rows, mass, write, d);
+    if (w == 0) walk(A, b, it, nd, rows, mass, kids, write, d);
     __syncthreads();
 }
 
 // With draft probabilities, the walk and the chunk sums of the residual: every workgroup of a
 // sequence walks for itself (a launch less), the first one writes.  grid (C, B), 512 threads.
-__global__ __launch_bounds__(512) void verify_residual_k(const Verify A) {
-    constexpr int E = CH / 512;
-    __shared__ double ss[8];
+__global__ __launch_bounds__(1024) void verify_residual_k(const Verify A) {
+    constexpr int E = CH / 1024;
+    __shared__ double ss[16];
     __shared__ RowStat rows[64];
     __shared__ double mass[64];
     __shared__ Draw d;
@@ -402,12 +405,12 @@ __global__ __launch_bounds__(512) void verify_residual_k(const Verify A) {
     if (c == 0 && threadIdx.x < sizeof(Draw) / 4) reinterpret_cast<int*>(A.draw + b)[threadIdx.x] = reinterpret_cast<const int*>(&d)[threadIdx.x];
     if (d.row < 0 || !(it >= 0)) return;
     double w[E];
-    const double s = wave_sum(residuals<E, 512>(w, A, d, it, c * CH + (int)threadIdx.x));
+    const double s = wave_sum(residuals<E, 1024>(w, A, d, it, c * CH + (int)threadIdx.x));
     if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
         double t = 0;
-        for (int k = 0; k < 8; k++) t += ss[k];
+        for (int k = 0; k < 16; k++) t += ss[k];
         A.sums[(size_t)b * A.C + c] = t;
     }
 }
@@ -415,35 +418,24 @@ __global__ __launch_bounds__(512) void verify_residual_k(const Verify A) {
 // The first thread at which the masses' running sum (in thread order) exceeds r, or u times their total
 // where r is negative; where rounding leaves none, the last one with any; -1 where there is no mass.
 // Every thread gets it; r becomes what of it is left there.  kDrawThreads threads.
-constexpr int kDrawThreads = 512, kDrawWaves = kDrawThreads / 64;
+constexpr int kDrawThreads = 1024, kDrawWaves = kDrawThreads / 64;
 struct PickLds {
     double part[kDrawWaves], left;
     int at;
 };
 __device__ __forceinline__ int block_pick(double mine, double u, double& r, PickLds& L) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
     const double inc = wave_scan(mine);
     if (lane == 63) L.part[w] = inc;
     if (threadIdx.x == 0) L.at = -1;
     __syncthreads();
-    double part[kDrawWaves], total = 0, base = 0;
-#pragma unroll
-    for (int k = 0; k < kDrawWaves; k++) {
-        part[k] = L.part[k];
-        if (k == w) base = total;
-        total += part[k];
-    }
-    if (r < 0) r = u * total;
-    double acc = 0;
-    int ws = -1, some = -1;                                    // the wave of the crossing; the last with mass
-#pragma unroll
-    for (int k = 0; k < kDrawWaves; k++) {
-        acc += part[k];
-        if (ws < 0 && acc > r) ws = k;
-        if (part[k] > 0) some = k;
-    }
-    if (ws < 0) ws = some;
+    // lane k has wave k's (sums over them one after the other, in every wave, took 1 us more)
+    const double part = lane < kDrawWaves ? L.part[lane] : 0.0, upto = wave_scan(part);
+    if (r < 0) r = u * lane_of(upto, 63);
+    const u64 over = __ballot(upto > r && part > 0), some = __ballot(part > 0);
+    const int ws = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll(some);    // -1: none
     if (w == ws) {
+        const double base = ws ? lane_of(upto, ws - 1) : 0.0;
         const u64 hit = __ballot(base + inc > r && mine > 0), any = __ballot(mine > 0);
         if (lane == (hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll(any))) {
             L.at = threadIdx.x;
@@ -583,7 +575,7 @@ hipError_t launch_verify_tree(int* tokens, int* path, int* count, int* kv_len, c
         hipLaunchKernelGGL(verify_stats_k<false>, dim3(C, R), dim3(256), 0, st, logits, ldl, parent, temp, T, V, ch);
     for (int k = 1; k < levels; k++)
         hipLaunchKernelGGL(verify_mass_k, dim3(C, R), dim3(256), 0, st, logits, ldl, q, ldq, parent, temp, T, V, k, ch, av, part);
-    if (q) hipLaunchKernelGGL(verify_residual_k, dim3(C, B), dim3(512), 0, st, a);
+    if (q) hipLaunchKernelGGL(verify_residual_k, dim3(C, B), dim3(1024), 0, st, a);
     hipLaunchKernelGGL(verify_draw_k, dim3(B), dim3(kDrawThreads), 0, st, a);
     return hipGetLastError();
 }
