@@ -127,9 +127,34 @@ struct Verify {                          // the arguments of rt4_verify_tree and
     int B, T, V, C, levels;
 };
 
+// A thread's elements of chunk c of a row, element e of thread i at 1024 (e / 4) + 4 i + e % 4, `rest` past
+// the row's end.  Rows need not start at a multiple of 16 bytes (loads of 16 bytes need 4 here).
+__device__ __forceinline__ void load_chunk(float (&v)[PT], const float* row, int c, int V, float rest) {
+    struct __attribute__((packed, aligned(4))) Quad {
+        float f[4];
+    };
+    const int at = c * CH + 4 * (int)threadIdx.x;
+    if ((c + 1) * CH <= V) {
+#pragma unroll
+        for (int e = 0; e < PT; e += 4) {
+            const Quad q = *reinterpret_cast<const Quad*>(row + at + 256 * e);
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[e + k] = q.f[k];
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < PT; e++) {                             // (unconditional loads: under a condition each waits)
+        const int i = at + 256 * (e & ~3) + (e & 3);
+        v[e] = row[i < V ? i : V - 1];
+    }
+#pragma unroll
+    for (int e = 0; e < PT; e++)
+        if (at + 256 * (e & ~3) + (e & 3) >= V) v[e] = rest;
+}
+
 // Statistics of a chunk of a row: one read of the logits, held in registers between the maximum and
 // the sum.  grid (C, B * T), 256 threads.  Rows of nodes that hang under nothing are not read.
-template <bool ALIGNED>
 __global__ __launch_bounds__(256) void verify_stats_k(const float* __restrict__ logits, size_t ldl, const int* __restrict__ parent,
                                                       const float* __restrict__ temp, int T, int V, RowStat* __restrict__ ch) {
     __shared__ float sm[4];
@@ -138,22 +163,9 @@ __global__ __launch_bounds__(256) void verify_stats_k(const float* __restrict__ 
     const int row = blockIdx.y, b = row / T, c = blockIdx.x, w = threadIdx.x >> 6;
     if (parent[(size_t)b * T] != -1 || (row % T && parent[row] < 0)) return;
     const float* l = logits + (size_t)row * ldl;
-    // element e of thread i: 1024 (e / 4) + 4 i + e % 4
     float v[PT], m = -INFINITY;
     const int at = c * CH + 4 * (int)threadIdx.x;
-    if (ALIGNED && (c + 1) * CH <= V) {
-#pragma unroll
-        for (int e = 0; e < PT; e += 4) {
-            const float4 q = *reinterpret_cast<const float4*>(l + at + 256 * e);
-            v[e] = q.x, v[e + 1] = q.y, v[e + 2] = q.z, v[e + 3] = q.w;
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < PT; e++) {
-            const int i = at + 256 * (e & ~3) + (e & 3);
-            v[e] = i < V ? l[i] : -INFINITY;
-        }
-    }
+    load_chunk(v, l, c, V, -INFINITY);
     const double it = inv_temp(temp, b);
 #pragma unroll
     for (int e = 0; e < PT; e++) m = fmaxf(m, v[e]);           // (drops NaN)
@@ -191,12 +203,8 @@ __global__ __launch_bounds__(256) void verify_mass_k(const float* __restrict__ l
     const double it = inv_temp(temp, b);
     if (!(it >= 0)) return;
     float l[PT], pq[PT];
-#pragma unroll
-    for (int e = 0; e < PT; e++) {
-        const int i = c * CH + e * 256 + threadIdx.x;
-        l[e] = i < V ? logits[(size_t)row * ldl + i] : -INFINITY;
-        pq[e] = i < V ? q[(size_t)row * ldq + i] : 0.f;
-    }
+    load_chunk(l, logits + (size_t)row * ldl, c, V, -INFINITY);
+    load_chunk(pq, q + (size_t)row * ldq, c, V, 0.f);
     double a = 1.0;
     if (level > 1) {
         const double* prev = part + ((size_t)(level - 1) * R + row) * C;
@@ -569,10 +577,7 @@ hipError_t launch_verify_tree(int* tokens, int* path, int* count, int* kv_len, c
     Draw* draw = reinterpret_cast<Draw*>(take((size_t)B * sizeof(Draw)));
     double* sums = reinterpret_cast<double*>(take((size_t)B * C * 8));
     const Verify a = {tokens, path, count, kv_len, logits, ldl, draft, parent, u, temp, q, ldq, ch, av, part, draw, sums, B, T, V, C, levels};
-    if (((uintptr_t)logits & 15) == 0 && ldl % 4 == 0)
-        hipLaunchKernelGGL(verify_stats_k<true>, dim3(C, R), dim3(256), 0, st, logits, ldl, parent, temp, T, V, ch);
-    else
-        hipLaunchKernelGGL(verify_stats_k<false>, dim3(C, R), dim3(256), 0, st, logits, ldl, parent, temp, T, V, ch);
+    hipLaunchKernelGGL(verify_stats_k, dim3(C, R), dim3(256), 0, st, logits, ldl, parent, temp, T, V, ch);
     for (int k = 1; k < levels; k++)
         hipLaunchKernelGGL(verify_mass_k, dim3(C, R), dim3(256), 0, st, logits, ldl, q, ldq, parent, temp, T, V, k, ch, av, part);
     if (q) hipLaunchKernelGGL(verify_residual_k, dim3(C, B), dim3(1024), 0, st, a);
