@@ -565,7 +565,7 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
 // The rows per workgroup and the units by a model of the time in us, fitted to sweeps of both over
 // 1 to 16 sequences of 1000 to 131001 keys and 1 to 64 nodes (off by 8% on average): a step of two
 // tiles takes 1.7, 2.1 or 2.9 (1 to 3 blocks) with one workgroup on a CU and 2.0, 3.05 or 4.2 with
-// two, all steps together at least the cache's bytes at 4.2 TB/s, the joining launch 3 and its states
+// two, all steps together at least the cache's bytes at 4.2 TB/s, the joining launch 4 and its states
 // (1 KB a row and unit, written and read) 0.3 a MB.  A unit's row groups stay on one XCD (an eighth
 // of the CUs), so the XCD with the most units decides.  (4 to 6 blocks fit too: 276 to 283 us where 3
 // take 283, 64 nodes over 131001 keys, and 43 against 37, 16 nodes over 32000.  A join in the same
@@ -588,7 +588,7 @@ TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_spli
             units = units < B ? B : kv_splits || units < (tiles + 1) / 2 ? units : (tiles + 1) / 2;
             const long wgs = (units * KVH + 7) / 8 * rg, steps = ((tiles + units - 1) / units + 1) / 2;
             const double run = steps * (wgs <= xcd ? one[nb - 1] : two[nb - 1] * fmax(1.0, wgs / (2.0 * xcd)));
-            const double cost = fmax(run, read) + (k == 0 ? 0 : 3 + 0.3e-3 * KVH * R * units);
+            const double cost = fmax(run, read) + (k == 0 ? 0 : 4 + 0.3e-3 * KVH * R * units);
             if (best == 0 || cost < best) best = cost, p = TreePlan{nb, rg, (int)units, kv_splits ? kv_splits : k == 0};
         }
     }
