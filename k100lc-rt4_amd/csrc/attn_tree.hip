@@ -101,8 +101,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const char* p, int bytes)
 
 // How the key tiles of the sequences (the cache's, then the draft tile) are shared out, lengths being
 // known here only.  A unit is a run of tiles of one sequence, for each KV head and row group a
-// workgroup: `fixed` units a sequence, or runs of equal length over all of them, such that there
-// are at most units + B of them, no sequence has more than kTreeMaxSplits and none is shorter than a
+// workgroup: `fixed` units a sequence, or runs of one length, the shortest by which there are at most
+// `units` of them (at least B), no sequence has more than kTreeMaxSplits and none is shorter than a
 // step.  So a batch's longest sequence takes no longer than its share.
 struct Run {
     int b, split, splits, first, tiles;  // sequence, which of its units, their number, the first's, its tiles
@@ -130,7 +130,15 @@ __device__ __forceinline__ Run run_of(const AttnTree& A, const TreePlan& P, int 
             total += wave_sum(t);
             most = max(most, wave_max(t));
         }
+        // between an even share of all tiles and one that allows for a shorter run at every sequence's end
         q = max(max(2, (total + P.units - 1) / P.units), (most + kTreeMaxSplits - 1) / kTreeMaxSplits);
+        int hi = P.units > A.B ? max(q, min(most, (total + P.units - A.B - 1) / (P.units - A.B))) : max(q, most);
+        if (A.B > 64) q = hi;
+        while (q < hi) {
+            const int mid = (q + hi) / 2;
+            if (wave_sum((held + mid - 1) / mid) <= P.units) hi = mid;
+            else q = mid + 1;
+        }
     }
     Run r = {-1, 0, 0, 0, 0};
     int before = 0;
@@ -562,20 +570,21 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
 
 }  // namespace
 
-// The rows per workgroup and the units by a model of the time in us, fitted to sweeps of both over
-// 1 to 16 sequences of 1000 to 131001 keys and 1 to 64 nodes (off by 8% on average): a step of two
-// tiles takes 1.7, 2.1 or 2.9 (1 to 3 blocks) with one workgroup on a CU and 2.0, 3.05 or 4.2 with
-// two, all steps together at least the cache's bytes at 4.2 TB/s, the joining launch 4 and its states
-// (1 KB a row and unit, written and read) 0.3 a MB.  A unit's row groups stay on one XCD (an eighth
-// of the CUs), so the XCD with the most units decides.  (4 to 6 blocks fit too: 276 to 283 us where 3
-// take 283, 64 nodes over 131001 keys, and 43 against 37, 16 nodes over 32000.  A join in the same
-// launch by the last workgroup of a row group took 14 us where both launches take 10: one node over
-// 1000 keys.)
+// The rows per workgroup and the units by a model of the time in us: a step of two tiles takes 1.3, 2.2
+// or 3.0 (1 to 3 blocks) with one workgroup on a CU and 1.6, 2.5 or 3.3 with two, the joining launch 4
+// and its states (1 KB a row and unit, written and read) 0.35 a MB, all sequences as long as the longest.
+// A unit's row groups stay on one XCD (an eighth of the CUs), so the XCD with the most units decides.
+// Over 241 sweeps of blocks and units, 1 to 16 sequences of 500 to 131000 keys and 1 to 64 nodes, the
+// choice by these figures takes 0.8% longer than the best on average and 12% at most where lengths are
+// alike (1.5% and 29% where they are drawn between 0 and the longest).
+// (4 to 6 blocks fit too: 276 to 283 us where 3 take 283, 64 nodes over 131001 keys, and 43 against 37,
+// 16 nodes over 32000.  A join in the same launch by the last workgroup of a row group took 14 us where
+// both launches take 10, one node over 1000 keys; 1024 threads a workgroup, four teams on a quarter of
+// the keys each that join in LDS, 16 at 500 keys where both launches take 11.)
 TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_splits, int cus) {
-    constexpr double one[] = {1.7, 2.1, 2.9}, two[] = {2.0, 3.05, 4.2};
+    constexpr double one[] = {1.3, 2.2, 3.0}, two[] = {1.6, 2.5, 3.3};
     const int R = T * ratio;
-    const long KVH = n_heads / ratio, tiles = (long)B * (kv_max / BNK + 2), xcd = cus > 8 ? cus / 8 : 1;
-    const double read = KVH * B * (double)kv_max * (HD + 24) / 4.2e6;
+    const long KVH = n_heads / ratio, tiles = (kv_max + BNK - 1) / BNK + 1, xcd = cus > 8 ? cus / 8 : 1;
     TreePlan p = {1, 1, 0, 0};
     double best = 0;
     for (int nb = 1; nb <= kTreeMaxBlocks; nb++) {
@@ -583,12 +592,11 @@ TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_spli
         if (nb > 1 && rg == (R + 16 * nb - 17) / (16 * nb - 16)) continue;      // no fewer groups than with fewer blocks
         for (int k = 0; k < 5; k++) {                          // a unit a sequence, or k / 2 workgroups a CU
             if (kv_splits && k != (kv_splits > 1)) continue;
-            // (of several sequences each may have a unit more than its share)
-            long units = kv_splits ? (long)B * kv_splits : k ? k * xcd / 2 / rg * 8 / KVH - (B > 1 ? B : 0) : B;
-            units = units < B ? B : kv_splits || units < (tiles + 1) / 2 ? units : (tiles + 1) / 2;
-            const long wgs = (units * KVH + 7) / 8 * rg, steps = ((tiles + units - 1) / units + 1) / 2;
+            long units = kv_splits ? (long)B * kv_splits : k ? k * xcd / 2 / rg * 8 / KVH : B;
+            units = units < B ? B : kv_splits || units < (tiles + 1) / 2 * B ? units : (tiles + 1) / 2 * B;
+            const long each = units / B, wgs = (units * KVH + 7) / 8 * rg, steps = ((tiles + each - 1) / each + 1) / 2;
             const double run = steps * (wgs <= xcd ? one[nb - 1] : two[nb - 1] * fmax(1.0, wgs / (2.0 * xcd)));
-            const double cost = fmax(run, read) + (k == 0 ? 0 : 4 + 0.3e-3 * KVH * R * units);
+            const double cost = run + (k == 0 ? 0 : 4 + 0.35e-3 * KVH * R * units);
             if (best == 0 || cost < best) best = cost, p = TreePlan{nb, rg, (int)units, kv_splits ? kv_splits : k == 0};
         }
     }
@@ -596,7 +604,7 @@ TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_spli
 }
 
 // Units that a launch may have.
-static size_t max_units(const AttnTree& a, const TreePlan& p) { return p.fixed ? (size_t)a.B * p.fixed : (size_t)p.units + a.B; }
+static size_t max_units(const AttnTree& a, const TreePlan& p) { return p.fixed ? (size_t)a.B * p.fixed : (size_t)p.units; }
 
 size_t tree_part_bytes(const AttnTree& a, const TreePlan& p) {
     if (p.fixed == 1) return 0;

@@ -163,7 +163,7 @@ struct AttnTree {
     int B, T, TP, n_heads, ratio, kv_cap;
 };
 // 16-row blocks per workgroup, workgroups per unit (a run of keys of a sequence) and KV head, units
-// of all sequences (at most that many and B more), or `fixed` units of each.
+// of all sequences (at most that many, at least one each), or `fixed` units of each.
 struct TreePlan {
     int blocks, groups, units, fixed;
 };
