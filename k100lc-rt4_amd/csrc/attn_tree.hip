@@ -28,8 +28,7 @@ __device__ __forceinline__ u64 tree_sees(const int* parent, int T) {
     const bool root = i == 0 && par == -1, node = i > 0 && par >= 0 && par < i;
     int up = node ? par : i;
     u64 anc = 1ull << i;
-#pragma unroll
-    for (int s = 0; s < 6; s++) {        // pointer doubling: 2^6 covers the deepest chain
+    for (int s = 1; s < T; s <<= 1) {    // pointer doubling: the deepest chain has T - 1 links
         anc |= __shfl(anc, up);
         up = __shfl(up, up);
     }
@@ -105,28 +104,33 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const char* p, int bytes)
 // `units` of them (at least B), no sequence has more than kTreeMaxSplits and none is shorter than a
 // step.  So a batch's longest sequence takes no longer than its share.
 struct Run {
-    int b, split, splits, first, tiles;  // sequence, which of its units, their number, the first's, its tiles
+    int b, split, splits, first, len, tiles;    // sequence, which of its units, their number, the first's, its cached keys and tiles
 };
-// Unit x (by_unit), b -1 past the last one, or sequence x.  By a whole wave; every lane gets it.
-template <bool BY_UNIT>
+__device__ __forceinline__ int tiles_of_len(int len) { return (len + BNK - 1) / BNK + 1; }
+// ceil(t / q) for t and q up to 2^19: the quotient of t + q - 1 + 1/2 is off by less than 2^-22 of
+// itself, which is below the 1 / 2q that lies between it and the next integers.
+__device__ __forceinline__ int ceil_div(int t, int q) {
+    return (int)(((float)(t + q - 1) + 0.5f) * __builtin_amdgcn_rcpf((float)q));
+}
+// Unit x, b -1 past the last one.  By a whole wave; every lane gets it.
 __device__ __forceinline__ Run run_of(const AttnTree& A, const TreePlan& P, int x) {
     const int lane = lane_id();
-    auto tiles_of = [&](int b) __attribute__((always_inline)) {
-        if (b >= A.B) return 0;
-        const int len = A.kv_len ? A.kv_len[b] : 0;
-        return ((len < 0 ? 0 : len > A.kv_cap ? A.kv_cap : len) + BNK - 1) / BNK + 1;
+    auto len_of = [&](int b) __attribute__((always_inline)) {
+        const int len = b < A.B && A.kv_len ? A.kv_len[b] : 0;
+        return len < 0 ? 0 : len > A.kv_cap ? A.kv_cap : len;
     };
+    auto tiles_of = [&](int b, int len) __attribute__((always_inline)) { return b < A.B ? tiles_of_len(len) : 0; };
     if (A.B == 1) {                                            // (the same without the reductions)
-        const int t = uniform(tiles_of(0)), q = max(max(2, (t + P.units - 1) / P.units), (t + kTreeMaxSplits - 1) / kTreeMaxSplits);
+        const int len = uniform(len_of(0)), t = tiles_of_len(len), q = max(max(2, (t + P.units - 1) / P.units), (t + kTreeMaxSplits - 1) / kTreeMaxSplits);
         const int n = P.fixed ? min(P.fixed, t) : (t + q - 1) / q;
-        return Run{!BY_UNIT || x < n ? 0 : -1, x, n, 0, t};
+        return Run{x < n ? 0 : -1, x, n, 0, len, t};
     }
-    const int held = tiles_of(lane);
+    const int held_len = len_of(lane), held = tiles_of(lane, held_len);
     int q = 0;
     if (!P.fixed) {
         int total = wave_sum(held), most = wave_max(held);
         for (int b0 = 64; b0 < A.B; b0 += 64) {
-            const int t = tiles_of(b0 + lane);
+            const int t = tiles_of(b0 + lane, len_of(b0 + lane));
             total += wave_sum(t);
             most = max(most, wave_max(t));
         }
@@ -136,22 +140,24 @@ __device__ __forceinline__ Run run_of(const AttnTree& A, const TreePlan& P, int 
         if (A.B > 64) q = hi;
         while (q < hi) {
             const int mid = (q + hi) / 2;
-            if (wave_sum((held + mid - 1) / mid) <= P.units) hi = mid;
+            if (wave_sum(ceil_div(held, mid)) <= P.units) hi = mid;
             else q = mid + 1;
         }
     }
-    Run r = {-1, 0, 0, 0, 0};
+    Run r = {-1, 0, 0, 0, 0, 0};
     int before = 0;
     for (int b0 = 0; b0 < A.B; b0 += 64) {
-        const int t = b0 ? tiles_of(b0 + lane) : held, n = P.fixed ? min(P.fixed, t) : (t + q - 1) / q;
+        const int len = b0 ? len_of(b0 + lane) : held_len, t = b0 ? tiles_of(b0 + lane, len) : held;
+        const int n = P.fixed ? min(P.fixed, t) : ceil_div(t, q);
         const int end = before + wave_scan(n);
-        const u64 hit = __ballot(BY_UNIT ? x >= end - n && x < end : b0 + lane == x);
+        const u64 hit = __ballot(x >= end - n && x < end);
         if (hit) {
             const int k = __ffsll((unsigned long long)hit) - 1;
             r.b = b0 + k;
             r.splits = __builtin_amdgcn_readlane(n, k);
             r.first = __builtin_amdgcn_readlane(end, k) - r.splits;
             r.split = x - r.first;
+            r.len = __builtin_amdgcn_readlane(len, k);
             r.tiles = __builtin_amdgcn_readlane(t, k);
             return r;
         }
@@ -159,6 +165,9 @@ __device__ __forceinline__ Run run_of(const AttnTree& A, const TreePlan& P, int 
     }
     return r;
 }
+
+// n / T for a row n of a KV head's (T at most 64, n below 2^26).
+__device__ __forceinline__ int by_nodes(int n, const AttnTree& A, const TreePlan& P) { return A.T == 1 ? n : (int)__umulhi((unsigned)n, P.inv_nodes); }
 
 constexpr float kPBits = 7.f;            // P is held times 2^7: at most 2^15 with the lazy maximum
 constexpr float kLazy = 8.f;             // the running maximum moves when a score exceeds it by 2^8
@@ -178,7 +187,7 @@ __device__ __forceinline__ v16f outer16(float x_of_lane, float y) {
 // step's P x V runs beside the next step's scores; two workgroups share a CU.
 template <int NB>
 __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const TreePlan P, float* __restrict__ opart,
-                                                      float2* __restrict__ mlpart) {
+                                                      float2* __restrict__ mlpart, int2* __restrict__ runs) {
     constexpr int RW = 16 * NB;
     constexpr bool QL = NB > 2;                                // Q operands in LDS instead of registers
     __shared__ __align__(16) v8h pf[NB][4][2][64];             // P: [32 keys][high, low part][lane]
@@ -191,14 +200,13 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
     const int rg = (int)(blockIdx.x / 8) % P.groups;
     const int unit = (int)(blockIdx.x / (8 * P.groups)) * 8 + (int)(blockIdx.x % 8);
     const int KVH = A.n_heads / A.ratio, R = A.T * A.ratio;
-    const Run run = run_of<true>(A, P, unit / KVH);
+    const Run run = run_of(A, P, unit / KVH);
     if (run.b < 0) return;
-    const int b = run.b, vh = unit % KVH;
+    const int b = uniform(run.b), vh = unit % KVH, len = uniform(run.len);
     const size_t seq = (size_t)b * KVH + vh;
-    int len = A.kv_len ? A.kv_len[b] : 0;
-    len = uniform(len < 0 ? 0 : len > A.kv_cap ? A.kv_cap : len);
-    const int nt = run.tiles - 1;                              // tile nt is the draft tile
-    const int t0 = (int)((long long)run.tiles * run.split / run.splits), t1 = (int)((long long)run.tiles * (run.split + 1) / run.splits);
+    const int tiles = run.tiles, nt = tiles - 1;       // tile nt is the draft tile
+    const int t0 = uniform(tiles * run.split / run.splits), t1 = uniform(tiles * (run.split + 1) / run.splits);     // (below 2^26)
+    if (P.fixed != 1 && run.split == 0 && vh == 0 && rg == 0 && tid == 0) runs[b] = make_int2(run.first, run.splits);
 
     const int hS = w & 1;                                      // half of the tile whose scores this wave makes
     v4u K[2][2], V[4];
@@ -259,7 +267,8 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
     // of group b / 2, block 2 pr + b % 2
     auto row_of = [&](int n) __attribute__((always_inline)) {      // of qq and out
         n = n < R ? n : 0;
-        return ((size_t)vh * A.ratio + n / A.T) * A.TP + (size_t)b * A.T + n % A.T;
+        const int head = by_nodes(n, A, P);
+        return ((size_t)vh * A.ratio + head) * A.TP + (size_t)b * A.T + (n - head * A.T);
     };
     v4i qop[QL ? 1 : NB][4];
     float qs[(NB + 1) / 2], m[NB], l[NB];
@@ -282,13 +291,13 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
 #pragma unroll
     for (int pr = 0; pr < (NB + 1) / 2; pr++) {
         const int nb = 2 * pr + (g & 1), n = rg * RW + (nb < NB ? nb : 0) * 16 + c;
-        const size_t head = (size_t)vh * A.ratio + (n < R ? n : 0) / A.T;
+        const size_t head = (size_t)vh * A.ratio + by_nodes(n < R ? n : 0, A, P);
         qs[pr] = A.qsc[row_of(n) + (head + (g >> 1)) * A.TP] * (L2E / 256.f);     // (both operands are 16 x code)
     }
     {
         const u64 sees = tree_sees(A.parent + (size_t)b * A.T, A.T);
-        const int n = rg * RW + tid;
-        const u64 x = __shfl(sees, (n < R ? n : 0) % A.T);
+        const int n = rg * RW + tid, in = n < R ? n : 0;
+        const u64 x = __shfl(sees, in - by_nodes(in, A, P) * A.T);
         if (tid < RW) {
             sees_l[tid] = n < R ? x : 0;
             row_l[tid] = row_of(n);
@@ -365,7 +374,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
             mt[nb] = max3(max2(mx[0][r], mx[1][r]), mx[2][r], mx[3][r]) - kPBits;
             any |= mt[nb] > kLazy;
         }
-        if (!__any(any)) return;
+        if (__builtin_expect(!__any(any), 1)) return;
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
             // (a row that sees nothing yet keeps its reference: -inf would not come back)
@@ -511,19 +520,18 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
 }
 
 // Sums the splits' states, W waves per row (all of a wave's loads in flight at once), four dims a lane:
-// four waves where a row has many splits, else one, which needs no exchange through LDS and leaves the
-// sequence's run to be found once for four rows (16 sequences of 8 nodes, 8 splits: 11.0 -> 7.9 us).
+// four waves where a row has many splits, else one, which needs no exchange through LDS.
 template <int W>
 __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const TreePlan P, const float* __restrict__ opart,
-                                                        const float2* __restrict__ mlpart) {
+                                                        const float2* __restrict__ mlpart, const int2* __restrict__ runs) {
     __shared__ __align__(16) v4f ol[W == 1 ? 1 : 4][64];
     const int KVH = A.n_heads / A.ratio, lane = lane_id(), w = uniform(threadIdx.x >> 6);
     const int n = W == 1 ? 4 * blockIdx.x + w : blockIdx.x, s0 = W == 1 ? 0 : w;
-    const int seq = blockIdx.y, b = seq / KVH, vh = seq % KVH, i = n % A.T;
+    const int seq = blockIdx.y, b = seq / KVH, vh = seq % KVH, in_head = by_nodes(n, A, P), i = n - in_head * A.T;
     if (n >= A.T * A.ratio) return;
-    const Run run = run_of<false>(A, P, b);
-    const size_t step = (size_t)KVH * P.groups * 16 * P.blocks, row = (size_t)run.first * step + (size_t)vh * P.groups * 16 * P.blocks + n;
-    const int splits = run.splits;
+    const int2 run = runs[b];                                  // the sequence's first unit and their number
+    const size_t step = (size_t)KVH * P.groups * 16 * P.blocks, row = (size_t)run.x * step + (size_t)vh * P.groups * 16 * P.blocks + n;
+    const int splits = uniform(run.y);
     // lane s has the states of splits s and s + 64
     float2 x[2];
 #pragma unroll
@@ -563,7 +571,7 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
 #pragma unroll
         for (int k = 1; k < 4; k++) o += ol[k][lane];
     }
-    const size_t head = (size_t)vh * A.ratio + n / A.T;
+    const size_t head = (size_t)vh * A.ratio + in_head;
     *reinterpret_cast<v4f*>(A.out + (head * A.TP + (size_t)b * A.T + i) * HD + 4 * lane) =
         live ? v4f{o[0] / ls, o[1] / ls, o[2] / ls, o[3] / ls} : v4f{0.f, 0.f, 0.f, 0.f};
 }
@@ -585,7 +593,8 @@ TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_spli
     constexpr double one[] = {1.3, 2.2, 3.0}, two[] = {1.6, 2.5, 3.3};
     const int R = T * ratio;
     const long KVH = n_heads / ratio, tiles = (kv_max + BNK - 1) / BNK + 1, xcd = cus > 8 ? cus / 8 : 1;
-    TreePlan p = {1, 1, 0, 0};
+    const unsigned inv = (unsigned)(((1ull << 32) + T - 1) / T);
+    TreePlan p = {1, 1, 0, 0, inv};
     double best = 0;
     for (int nb = 1; nb <= kTreeMaxBlocks; nb++) {
         const int rg = (R + 16 * nb - 1) / (16 * nb);
@@ -597,7 +606,7 @@ TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_spli
             const long each = units / B, wgs = (units * KVH + 7) / 8 * rg, steps = ((tiles + each - 1) / each + 1) / 2;
             const double run = steps * (wgs <= xcd ? one[nb - 1] : two[nb - 1] * fmax(1.0, wgs / (2.0 * xcd)));
             const double cost = run + (k == 0 ? 0 : 4 + 0.35e-3 * KVH * R * units);
-            if (best == 0 || cost < best) best = cost, p = TreePlan{nb, rg, (int)units, kv_splits ? kv_splits : k == 0};
+            if (best == 0 || cost < best) best = cost, p = TreePlan{nb, rg, (int)units, kv_splits ? kv_splits : k == 0, inv};
         }
     }
     return p;
@@ -609,7 +618,7 @@ static size_t max_units(const AttnTree& a, const TreePlan& p) { return p.fixed ?
 size_t tree_part_bytes(const AttnTree& a, const TreePlan& p) {
     if (p.fixed == 1) return 0;
     const size_t rows = max_units(a, p) * (a.n_heads / a.ratio) * p.groups * 16 * p.blocks;
-    return rows * (HD * sizeof(float) + sizeof(float2));
+    return rows * (HD * sizeof(float) + sizeof(float2)) + a.B * sizeof(int2);
 }
 
 hipError_t launch_attn_tree(const AttnTree& a, const TreePlan& p, void* ws, hipStream_t st) {
@@ -617,18 +626,19 @@ hipError_t launch_attn_tree(const AttnTree& a, const TreePlan& p, void* ws, hipS
     const size_t units = max_units(a, p) * KVH, rows = units * p.groups * 16 * p.blocks;
     float* opart = static_cast<float*>(ws);
     float2* mlpart = reinterpret_cast<float2*>(opart + rows * HD);
+    int2* runs = reinterpret_cast<int2*>(mlpart + rows);
     const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.groups));
     switch (p.blocks) {
-        case 1: hipLaunchKernelGGL(attn_tree_k<1>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
-        case 2: hipLaunchKernelGGL(attn_tree_k<2>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
-        default: hipLaunchKernelGGL(attn_tree_k<3>, grid, dim3(256), 0, st, a, p, opart, mlpart); break;
+        case 1: hipLaunchKernelGGL(attn_tree_k<1>, grid, dim3(256), 0, st, a, p, opart, mlpart, runs); break;
+        case 2: hipLaunchKernelGGL(attn_tree_k<2>, grid, dim3(256), 0, st, a, p, opart, mlpart, runs); break;
+        default: hipLaunchKernelGGL(attn_tree_k<3>, grid, dim3(256), 0, st, a, p, opart, mlpart, runs); break;
     }
     if (p.fixed != 1) {
         const int R = a.T * a.ratio;
         if ((p.fixed ? p.fixed : p.units / a.B) > 16)
-            hipLaunchKernelGGL(attn_tree_join_k<4>, dim3(R, a.B * KVH), dim3(256), 0, st, a, p, opart, mlpart);
+            hipLaunchKernelGGL(attn_tree_join_k<4>, dim3(R, a.B * KVH), dim3(256), 0, st, a, p, opart, mlpart, runs);
         else
-            hipLaunchKernelGGL(attn_tree_join_k<1>, dim3((R + 3) / 4, a.B * KVH), dim3(256), 0, st, a, p, opart, mlpart);
+            hipLaunchKernelGGL(attn_tree_join_k<1>, dim3((R + 3) / 4, a.B * KVH), dim3(256), 0, st, a, p, opart, mlpart, runs);
     }
     return hipGetLastError();
 }

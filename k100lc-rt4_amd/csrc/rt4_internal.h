@@ -166,6 +166,7 @@ struct AttnTree {
 // of all sequences (at most that many, at least one each), or `fixed` units of each.
 struct TreePlan {
     int blocks, groups, units, fixed;
+    unsigned inv_nodes;                  // ceil(2^32 / T)
 };
 constexpr int kTreeMaxBlocks = 3, kTreeMaxSplits = 128;
 TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_splits, int cus);
