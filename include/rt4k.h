@@ -9,8 +9,9 @@
  *
  * Library scratch: the drop-in linears' quantized activations, the split
  * workspaces of the GEMVs (W4A8 and W4A4 share one, partials plus counters that
- * every launch leaves at zero), of the GEMM and of the attention prefill, and the
- * prefill's staged K/V copy (24 KB per key tile and KV head) are one buffer per
+ * every launch leaves at zero), of the GEMM and of the attention prefill, the
+ * prefill's staged K/V copy (24 KB per key tile and KV head), the tree attention's
+ * split states and the verification's row statistics are one buffer per
  * device and kind, grown on demand like the reference's static
  * scratch (src/k_gemv.hip:16-23).  Calls that may run at the same time on one
  * device (different streams) therefore race on it; the caller orders them, as
@@ -21,8 +22,8 @@
  * Nothing is allocated while `stream` is being captured: a call that would
  * have to grow a scratch buffer then fails with RT4_E_CAPTURE, except that the
  * split GEMV falls back to its unsplit form, which needs no workspace, the attention
- * prefill (automatic split count) to the largest split count whose workspace is there,
- * down to one, and the prefill without room for its staged K/V copy stages the tiles in
+ * prefill and the tree attention (automatic split count) to the largest split count whose
+ * workspace is there, down to one, and the prefill without room for its staged K/V copy stages the tiles in
  * every workgroup (same results).
  *
  * Formats (docs/FORMAT.md:61-73 of the reference, unchanged here):
@@ -328,7 +329,9 @@ int rt4_kv_append_rows(uint32_t* kc, float* ksc, uint32_t* vc, float* vsc, float
  * padding nodes and of idle sequences are zeros; rows from B*T on are left as they were.
  * kv_len int32 [B] on the device, clamped to [0, kv_cap]; NULL: no cache (kc, ksc, vc, vsc
  * are not read).  kv_max: the longest length to plan for (a longer one is still right).
- * kv_splits: parts the keys are split into, 0 chooses (at most 128). */
+ * kv_splits: parts the keys are split into, 0 chooses (at most 128); the order of the fp32
+ * sums, and so the last bits, goes by it, by kv_max and by the lengths of the batch, but never
+ * from call to call.  out must not overlap an input.  The split states are library scratch. */
 int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const uint32_t* kc, const float* ksc,
                        const uint32_t* vc, const float* vsc, const int32_t* kv_len, const uint32_t* kd, const float* ksd,
                        const uint32_t* vd, const float* vsd, const int32_t* parent, int B, int T, int TP, int n_heads,
@@ -355,7 +358,8 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
  * Outputs: count[b] = n accepted nodes, the root included (0: idle); path int32 [B][T] their
  * numbers; tokens int32 [B][T] the n new tokens (n-1 accepted drafts, then the last token);
  * the rest of both is -1.  kv_len (optional): kv_len[b] += n, as rt4_kv_append_rows takes
- * it.  Decisions are made in 64 bits.  T <= 64, V <= 4194304, B*T <= 65535. */
+ * it.  Decisions are made in 64 bits.  T <= 64, V <= 4194304, B*T <= 65535; outputs must not
+ * overlap inputs or each other.  The rows' statistics are library scratch. */
 int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_len, const float* logits, int64_t ldl,
                     const int32_t* draft, const int32_t* parent, const float* u, const float* temp, const float* draft_p,
                     int64_t ldp, int B, int T, int V, int max_children, void* stream);

@@ -13,7 +13,9 @@ Reference interface mirrored (src/kernels.h of K100LC-RT4):
     k_attn_q_quant   -> attn_q_quant         (src/kernels.h:40)
     k_kv_append_k/v  -> kv_append_k / _v     (src/kernels.h:50, :53)
     k_attention      -> attention_prefill    (src/kernels.h:81, prefill branch)
-plus the pieces those wrappers launch internally (quant_act_a8, gemv_w4a8_q).
+plus the pieces those wrappers launch internally (quant_act_a8, gemv_w4a8_q), and
+the steps of speculative decoding over the int4-KV cache, which the reference does
+not have: kv_append_rows, attention_tree, verify_tree.
 """
 from __future__ import annotations
 
@@ -562,7 +564,7 @@ def verify_tree(logits, draft, parent, u, temp=None, draft_probs=None, max_child
     count int32 [B]): count accepted nodes (the root included), their numbers, and the new tokens; -1 behind them.
 
     logits f32 [B*T, V] (rows may be strided), draft and parent int32 [B, T], u f32 [B, T] uniforms in [0, 1), temp f32 [B]
-    (default 1; <= 0: greedy).  draft_probs f32 [B*T, V]: row n the distribution node n's children were drawn from, at
+    (default 1; <= 0 or NaN: greedy).  draft_probs f32 [B*T, V]: row n the distribution node n's children were drawn from, at
     most max_children of which are tested.  kv_len int32 [B] is advanced by count.  See rt4_verify_tree in include/rt4k.h."""
     torch = _torch()
     dev, f32, i32 = _dev(), torch.float32, torch.int32
