@@ -877,3 +877,42 @@ def test_verify_infinite_temperature(rt4, torch_gpu, probs):
                           max_children=2 if probs else None)
     for g, w in zip(got, want):
         assert np.array_equal(host(g), w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [2, 7, 63, 64, 65])
+def test_shares_of_ragged_lengths(rt4, torch_gpu, orc, B):
+    """Planned for any longest length, the keys of sequences of unlike lengths are all shared out."""
+    rng = np.random.default_rng(B)
+    T, H, ratio, cap = 2, 1, 2, 1024
+    qq, qs, kv, draft = attention_case(orc, rng, B, T, H, ratio, cap, 2)
+    lens = np.where(rng.random(B) < 0.3, rng.integers(0, 130, B), rng.integers(0, cap + 1, B))
+    lens[-1] = cap
+    parent = np.tile([[-1, 0]], (B, 1))
+    spoil_unseen(kv, draft, lens, T)
+    want, tol = tree_attention(qq, qs, kv, lens, draft, parent, ratio)
+    args = [dev(qq), dev(qs), *map(dev, kv), dev(lens), *map(dev, draft), dev(parent)]
+    for kv_max in (0, 64, 200, 256, 700, cap):
+        print(f"case ragged shares B={B} kv_max={kv_max}", flush=True)
+        check_attention(rt4.attention_tree(*args, ratio=ratio, kv_max=kv_max), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("probs,temp,scale", [(False, 1.0, 1.0), (False, 0.0, 1.0), (True, 1.0, 1.0), (False, 1.0, 0.05), (True, 1.0, 0.05)])
+def test_verify_star(rt4, torch_gpu, probs, temp, scale):
+    """63 children of one root, tokens named twice among them: long runs of rejections, and acceptances late in them."""
+    print(f"case star probs={probs} temp={temp} scale={scale}", flush=True)
+    rng = np.random.default_rng(31)
+    B, T, V = 12, 64, 200
+    logits = (rng.standard_normal((B * T, V)) * 2).astype(np.float32)
+    parent = np.tile(np.array([-1] + [0] * (T - 1)), (B, 1))
+    draft = rng.integers(0, V, (B, T))
+    draft[:, 40:] = draft[:, :24]
+    u = np.sqrt(rng.random((B, T))).astype(np.float32)
+    u[:4, 1:60] = 0.999
+    u[:, 1:] *= np.float32(scale)
+    q = None
+    if probs:
+        q = rng.random((B * T, V)).astype(np.float32) ** 4
+        q /= q.sum(1, keepdims=True)
+    check_verify(rt4, logits, draft, parent, u, [temp] * B, q, T - 1 if probs else None)
