@@ -30,10 +30,9 @@ constexpr float L2E = 1.4426950408889634f;
 typedef unsigned long long u64;
 
 // Nodes that node i of sequence b sees: itself and those above it, none where it hangs
-// under no root.  Lane i of the wave has node i.
-__device__ __forceinline__ u64 tree_sees(const int* parent, int T) {
+// under no root.  Lane i of the wave has node i, whose parent is par (-2 past the last node).
+__device__ __forceinline__ u64 tree_sees(int par, int T) {
     const int i = threadIdx.x & 63;
-    const int par = i < T ? parent[i] : -2;
     const bool root = i == 0 && par == -1, node = i > 0 && par >= 0 && par < i;
     int up = node ? par : i;
     u64 anc = 1ull << i;
@@ -264,14 +263,9 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
         const auto rs = rsrc(d ? vsd : vsc, (d ? 1 : A.kv_cap / BNK) * HD * 4);
         vs[x] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, wo, d ? 0 : t * (HD * 4), 0));
     };
-    if (t0 < t1) {                                             // (in flight while the rows are set up)
-        load_k(t0);
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            load_v(t0, x);
-            load_vs(t0, x);
-        }
-    }
+    // Loads in the order in which they are needed, since they come back in that order: the tree, K, Q, V
+    const int par = lane < A.T ? A.parent[(size_t)b * A.T + lane] : -2;
+    if (t0 < t1) load_k(t0);
     // Q operands (column c of block nb is row n) and this lane's column scales: lane 16 b + c has those
     // of group b / 2, block 2 pr + b % 2
     auto row_of = [&](int n) __attribute__((always_inline)) {      // of qq and out
@@ -279,32 +273,33 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
         const int head = by_nodes(n, A, P);
         return ((size_t)vh * A.ratio + head) * A.TP + (size_t)b * A.T + (n - head * A.T);
     };
-    v4i qop[QL ? 1 : NB][4];
+    v4u qd[QL ? 1 : NB][2];
     float qs[(NB + 1) / 2], m[NB], l[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
         m[nb] = 0.f;
         l[nb] = 0.f;
-        if (QL && (nb & 3) != w) continue;
+        if (QL && nb != w) continue;
         const uint32_t* qr = A.qq + row_of(rg * RW + nb * 16 + c) * KDW + 4 * g;
-        const v4u d0 = *reinterpret_cast<const v4u*>(qr), d1 = *reinterpret_cast<const v4u*>(qr + 16);
-        v4i (&q)[4] = qop[QL ? 0 : nb];
-        q[0] = bytes16(d0.x, d0.y);
-        q[1] = bytes16(d0.z, d0.w);
-        q[2] = bytes16(d1.x, d1.y);
-        q[3] = bytes16(d1.z, d1.w);
-        if (QL)
 #pragma unroll
-            for (int k = 0; k < 4; k++) qf[nb][k][lane] = q[k];
+        for (int k = 0; k < 2; k++) qd[QL ? 0 : nb][k] = *reinterpret_cast<const v4u*>(qr + 16 * k);
     }
 #pragma unroll
     for (int pr = 0; pr < (NB + 1) / 2; pr++) {
         const int nb = 2 * pr + (g & 1), n = rg * RW + (nb < NB ? nb : 0) * 16 + c;
         const size_t head = (size_t)vh * A.ratio + by_nodes(n < R ? n : 0, A, P);
-        qs[pr] = A.qsc[row_of(n) + (head + (g >> 1)) * A.TP] * (L2E / 256.f);     // (both operands are 16 x code)
+        qs[pr] = A.qsc[row_of(n) + (head + (g >> 1)) * A.TP];
     }
+    if (t0 < t1) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            load_v(t0, x);
+            load_vs(t0, x);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
     {
-        const u64 sees = tree_sees(A.parent + (size_t)b * A.T, A.T);
+        const u64 sees = tree_sees(par, A.T);
         const int n = rg * RW + tid, in = n < R ? n : 0;
         const u64 x = __shfl(sees, in - by_nodes(in, A, P) * A.T);
         if (tid < RW) {
@@ -312,6 +307,22 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
             row_l[tid] = row_of(n);
         }
     }
+    v4i qop[QL ? 1 : NB][4];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        if (QL && nb != w) continue;
+        const v4u (&d)[2] = qd[QL ? 0 : nb];
+        v4i (&q)[4] = qop[QL ? 0 : nb];
+        q[0] = bytes16(d[0].x, d[0].y);
+        q[1] = bytes16(d[0].z, d[0].w);
+        q[2] = bytes16(d[1].x, d[1].y);
+        q[3] = bytes16(d[1].z, d[1].w);
+        if (QL)
+#pragma unroll
+            for (int k = 0; k < 4; k++) qf[nb][k][lane] = q[k];
+    }
+#pragma unroll
+    for (int pr = 0; pr < (NB + 1) / 2; pr++) qs[pr] *= L2E / 256.f;     // (both operands are 16 x code)
     __syncthreads();
 
     v4f O[NB][4];
@@ -540,7 +551,7 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
     if (n >= A.T * A.ratio) return;
     const int2 run = runs[b];                                  // the sequence's first unit and their number
     const size_t step = (size_t)KVH * P.groups * 16 * P.blocks, row = (size_t)run.x * step + (size_t)vh * P.groups * 16 * P.blocks + n;
-    const int splits = uniform(run.y);
+    const int splits = uniform(run.y), par = lane < A.T ? A.parent[(size_t)b * A.T + lane] : -2;
     // lane s has the states of splits s and s + 64
     float2 x[2];
 #pragma unroll
@@ -548,7 +559,7 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
         x[k] = mlpart[row + min(lane + 64 * k, splits - 1) * step];
         if (lane + 64 * k >= splits) x[k] = make_float2(-1e30f, 0.f);
     }
-    const bool live = __shfl(tree_sees(A.parent + (size_t)b * A.T, A.T), i) != 0;
+    const bool live = __shfl(tree_sees(par, A.T), i) != 0;
     const float* src = opart + row * HD + 4 * lane;
     v4f v[16];
     auto read = [&](int h) __attribute__((always_inline)) {
