@@ -16,8 +16,8 @@
 // What bounds it (24 query heads over 4 KV heads):
 //   1 node over 1000 keys: 6.0 us and the join 4.5, the start of two launches; the loop is one step
 //   4 nodes over 32701 keys: 16.4 and 4.4 us, 36.7 MB at 1.8 TB/s, two steps after 3.5 us of start
-//   16 sequences of 8 nodes over up to 16384 keys: 60 us in all, 150 MB at 2.5 TB/s with 26 GFLOP beside it
-//   61 nodes over 131001 keys: 270 us in all, 196 GFLOP at 0.73 PFLOP/s; P's two parts make them 294,
+//   16 sequences of 8 nodes over up to 16384 keys: 58 us in all, 150 MB at 2.6 TB/s with 26 GFLOP beside it
+//   61 nodes over 131001 keys: 273 us in all, 196 GFLOP at 0.72 PFLOP/s; P's two parts make them 294,
 //   which take 222 us at the rates of large int8 and fp16 products, the softmax beside them
 #include "rt4_dev.h"
 #include "rt4_internal.h"
@@ -143,6 +143,7 @@ __device__ __forceinline__ Run run_of(const AttnTree& A, const TreePlan& P, int 
             most = max(most, wave_max(t));
         }
         // between an even share of all tiles and one that allows for a shorter run at every sequence's end
+        // (that one where there are more sequences than lanes)
         q = max(max(2, (total + P.units - 1) / P.units), (most + kTreeMaxSplits - 1) / kTreeMaxSplits);
         int hi = P.units > A.B ? max(q, min(most, (total + P.units - A.B - 1) / (P.units - A.B))) : max(q, most);
         if (A.B > 64) q = hi;

@@ -203,8 +203,9 @@ __global__ __launch_bounds__(256) void verify_mass_k(const float* __restrict__ l
                                                      double* __restrict__ av, double* __restrict__ part) {
     __shared__ double ss[4];
     const int row = blockIdx.y, b = row / T, c = blockIdx.x, C = gridDim.x, R = gridDim.y;
-    const int i = threadIdx.x & 63, n = row % T;               // (children of padding are counted too, to no harm)
-    if (__popcll(__ballot(i > n && i < T && parent[(size_t)b * T + i] == n)) <= level) return;
+    const int i = threadIdx.x & 63, n = row % T, par = i < T ? parent[(size_t)b * T + i] : -2;
+    if (__builtin_amdgcn_readlane(par, 0) != -1) return;       // idle
+    if (__popcll(__ballot(i > n && par == n)) <= level) return;     // (padding's children are counted too, to no harm)
     const double it = inv_temp(temp, b);
     if (!(it >= 0)) return;
     float l[PT], pq[PT];
