@@ -517,10 +517,18 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (rg * RW + nb * 16 + 4 * g + i < R)
-                    *reinterpret_cast<v4f*>(opart + (prow + nb * 16 + 4 * g + i) * HD + 64 * w + 4 * c) =
-                        v4f{O[nb][0][i], O[nb][1][i], O[nb][2][i], O[nb][3][i]};
+            for (int i = 0; i < 4; i++) {
+                if (rg * RW + nb * 16 + 4 * g + i >= R) continue;
+                v4f* to = reinterpret_cast<v4f*>(opart + (prow + nb * 16 + 4 * g + i) * HD + 64 * w + 4 * c);
+                const v4f o = {O[nb][0][i], O[nb][1][i], O[nb][2][i], O[nb][3][i]};
+                if (P.stream) {
+                    asm volatile("" ::: "memory");             // (or both stores become one, a plain one)
+                    __builtin_nontemporal_store(o, to);
+                    asm volatile("" ::: "memory");
+                } else {
+                    *to = o;
+                }
+            }
             if (w == 0 && g == 0) {
                 const int r = nb * 16 + c;
                 mlpart[prow + r] = make_float2(t0 < t1 ? m[nb] : -1e30f, mx[0][r] + mx[1][r] + mx[2][r] + mx[3][r]);
@@ -614,8 +622,7 @@ TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_spli
     constexpr double one[] = {1.3, 2.2, 3.0}, two[] = {1.6, 2.5, 3.3};
     const int R = T * ratio;
     const long KVH = n_heads / ratio, tiles = (kv_max + BNK - 1) / BNK + 1, xcd = cus > 8 ? cus / 8 : 1;
-    const unsigned inv = (unsigned)(((1ull << 32) + T - 1) / T);
-    TreePlan p = {1, 1, 0, 0, inv};
+    TreePlan p = {1, 1, 0, 0};
     double best = 0;
     for (int nb = 1; nb <= kTreeMaxBlocks; nb++) {
         const int rg = (R + 16 * nb - 1) / (16 * nb);
@@ -627,9 +634,16 @@ TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_spli
             const long each = units / B, wgs = (units * KVH + 7) / 8 * rg, steps = ((tiles + each - 1) / each + 1) / 2;
             const double run = steps * (wgs <= xcd ? one[nb - 1] : two[nb - 1] * fmax(1.0, wgs / (2.0 * xcd)));
             const double cost = run + (k == 0 ? 0 : 4 + 0.35e-3 * KVH * R * units);
-            if (best == 0 || cost < best) best = cost, p = TreePlan{nb, rg, (int)units, kv_splits ? kv_splits : k == 0, inv};
+            if (best == 0 || cost < best) best = cost, p = TreePlan{nb, rg, (int)units, kv_splits ? kv_splits : k == 0};
         }
     }
+    p.inv_nodes = (unsigned)(((1ull << 32) + T - 1) / T);
+    // States of more than 6 MB are written past the L2, which would write them back at the end of the
+    // launch (4 ragged sequences of 16 nodes, 25 MB: 28.6 -> 26.8 us; 4 of 8 nodes over 2000 keys, 8 MB:
+    // 18.9 -> 18.1), fewer through it (1.5 MB: 11.4 us, past it 12.1; 6 MB: 18.4, 19.2), and so where
+    // the caches are over 120 MB, which leaves them no place behind it (61 nodes over 131001 keys, 147
+    // MB: 282 us, past it 284; 16 sequences of 16 nodes over 8000, 143 MB: 101, 107).
+    p.stream = p.units * KVH * R > 6144 && KVH * B * (long)kv_max * (HD + 24) < 120000000;
     return p;
 }
 

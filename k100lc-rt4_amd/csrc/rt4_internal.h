@@ -167,6 +167,7 @@ struct AttnTree {
 struct TreePlan {
     int blocks, groups, units, fixed;
     unsigned inv_nodes;                  // ceil(2^32 / T)
+    int stream;                          // the states' stores pass the L2 by
 };
 constexpr int kTreeMaxBlocks = 3, kTreeMaxSplits = 128;
 TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_splits, int cus);
