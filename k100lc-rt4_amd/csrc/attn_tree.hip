@@ -568,7 +568,6 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
         x[k] = mlpart[row + min(lane + 64 * k, splits - 1) * step];
         if (lane + 64 * k >= splits) x[k] = make_float2(-1e30f, 0.f);
     }
-    const bool live = __shfl(tree_sees(par, A.T), i) != 0;
     const float* src = opart + row * HD + 4 * lane;
     v4f v[16];
     auto read = [&](int h) __attribute__((always_inline)) {
@@ -579,6 +578,8 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
         }
     };
     read(0);
+    __builtin_amdgcn_sched_barrier(0);
+    const bool live = __shfl(tree_sees(par, A.T), i) != 0;
     const float M = wave_max(fmaxf(x[0].x, x[1].x));
     const float f[2] = {__builtin_amdgcn_exp2f(x[0].x - M), __builtin_amdgcn_exp2f(x[1].x - M)};
     const float ls = wave_sum(x[0].y * f[0] + x[1].y * f[1]);
@@ -588,7 +589,7 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
 #pragma unroll
         for (int k = 0; k < 16; k++) {
             const int s = s0 + W * (16 * h + k);
-            const float fs = __shfl(s < 64 ? f[0] : f[1], s & 63);
+            const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s < 64 ? f[0] : f[1]), s & 63));
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] = fmaf(v[k][e], fs, o[e]);
         }
