@@ -69,8 +69,9 @@ __device__ __forceinline__ double weight(float l, float m, double it) {
     return l == m ? (m > -INFINITY ? 1.0 : 0.0) : x > -708.0 && l < m ? e : 0.0;
 }
 
-// The whole row's statistics from its chunks', by one wave, in a fixed order.
-__device__ __forceinline__ RowStat row_of_chunks(const RowStat* ch, int C, double it) {
+// The whole row's statistics from its chunks', by one wave, in a fixed order.  keep [64]: the first
+// chunks' masses.
+__device__ __forceinline__ RowStat row_of_chunks(const RowStat* ch, int C, double it, double* keep = nullptr) {
     const int lane = threadIdx.x & 63;
     RowStat first = {-INFINITY, INT_MAX, 0.0};
     if (lane < C) first = ch[lane];                          // (held: most rows have at most 64 chunks)
@@ -81,6 +82,7 @@ __device__ __forceinline__ RowStat row_of_chunks(const RowStat* ch, int C, doubl
     r.i = wave_min(r.m == m ? r.i : INT_MAX);
     r.m = m;
     r.s = first.s * weight(first.m, r.m, it);
+    if (keep) keep[lane] = r.s;
     for (int c = lane + 64; c < C; c += 64) r.s += ch[c].s * weight(ch[c].m, r.m, it);
     r.s = wave_sum(r.s);
     return r;
@@ -132,12 +134,13 @@ struct Verify {                          // the arguments of rt4_verify_tree and
     int B, T, V, C, levels;
 };
 
+struct __attribute__((packed, aligned(4))) Quad {    // (loads of 16 bytes need an alignment of 4 here)
+    float f[4];
+};
+
 // A thread's elements of chunk c of a row, element e of thread i at 1024 (e / 4) + 4 i + e % 4, `rest` past
-// the row's end.  Rows need not start at a multiple of 16 bytes (loads of 16 bytes need 4 here).
+// the row's end.
 __device__ __forceinline__ void load_chunk(float (&v)[PT], const float* row, int c, int V, float rest) {
-    struct __attribute__((packed, aligned(4))) Quad {
-        float f[4];
-    };
     const int at = c * CH + 4 * (int)threadIdx.x;
     if ((c + 1) * CH <= V) {
 #pragma unroll
@@ -346,45 +349,47 @@ __device__ void walk(const Verify& A, int b, double it, const Nodes& nd, const R
     }
 }
 
-// Residual weights of a thread's E tokens at, at + STEP, ..; their sum.
-template <int E, int STEP>
-__device__ __forceinline__ double residuals(double (&w)[E], const Verify& A, const Draw& d, double it, int at) {
-    const float* l = A.logits + (size_t)d.row * A.ldl;
-    const float* q = A.q ? A.q + (size_t)d.row * A.ldq : nullptr;
+// Residual weights of four tokens from `at` on; their sum.
+__device__ __forceinline__ double residuals(double (&w)[4], const Verify& A, const Draw& d, double it, int at) {
+    const float* l = A.logits + (size_t)d.row * A.ldl + at;
+    const float* q = A.q ? A.q + (size_t)d.row * A.ldq + at : nullptr;
     const double is = d.r.s > 0 ? 1.0 / d.r.s : 0.0;
-    float lv[E], qv[E];
+    Quad lv, qv = {};
+    if (at + 4 <= A.V) {
+        lv = *reinterpret_cast<const Quad*>(l);
+        if (q) qv = *reinterpret_cast<const Quad*>(q);
+    } else {
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int i = at + e * STEP;
-        lv[e] = i < A.V ? l[i] : -INFINITY;
-        qv[e] = q && i < A.V ? q[i] : 0.f;
+        for (int e = 0; e < 4; e++) {
+            lv.f[e] = at + e < A.V ? l[e] : -INFINITY;
+            if (q) qv.f[e] = at + e < A.V ? q[e] : 0.f;
+        }
     }
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        w[e] = weight(lv[e], d.r.m, it);
-        if (q) w[e] = fmax(w[e] * is - d.a * (double)qv[e], 0.0);
+    for (int e = 0; e < 4; e++) {
+        w[e] = weight(lv.f[e], d.r.m, it);
+        if (q) w[e] = fmax(w[e] * is - d.a * (double)qv.f[e], 0.0);
     }
     for (int k = 0; k < d.nrej; k++) {
         const int i = d.rej[k] - at;
 #pragma unroll
-        for (int e = 0; e < E; e++)
-            if (i == e * STEP) w[e] = 0.0;
+        for (int e = 0; e < 4; e++)
+            if (i == e) w[e] = 0.0;
     }
-    double s = 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) s += w[e];
-    return s;
+    return w[0] + w[1] + w[2] + w[3];
 }
 
 // Statistics of sequence b's rows into LDS, a wave per row, beside what the first wave reads of its
-// tree, and the walk.  mass [64]: the residual's sum that a later sibling is tested against.
-__device__ __forceinline__ void walk_sequence(const Verify& A, int b, double it, RowStat* rows, double* mass, bool write, Draw* d) {
+// tree, and the walk.  mass [64]: the residual's sum that a later sibling is tested against; keep: the
+// rows' first 64 chunks' masses.
+__device__ __forceinline__ void walk_sequence(const Verify& A, int b, double it, RowStat* rows, double* mass, double (*keep)[64],
+                                              bool write, Draw* d) {
     __shared__ u64 kids[64];
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), waves = blockDim.x >> 6;
     Nodes nd;
     if (w == 0) nd = read_nodes(A, b);
     for (int n = w; n < A.T; n += waves) {
-        const RowStat r = row_of_chunks(A.ch + ((size_t)b * A.T + n) * A.C, A.C, it);
+        const RowStat r = row_of_chunks(A.ch + ((size_t)b * A.T + n) * A.C, A.C, it, keep ? keep[n] : nullptr);
         if (lane == 0) rows[n] = r;
     }
     if (A.q && A.levels > 1 && it >= 0) {
@@ -406,20 +411,19 @@ __device__ __forceinline__ void walk_sequence(const Verify& A, int b, double it,
 }
 
 // With draft probabilities, the walk and the chunk sums of the residual: every workgroup of a
-// sequence walks for itself (a launch less), the first one writes.  grid (C, B), 512 threads.
+// sequence walks for itself (a launch less), the first one writes.  grid (C, B), 1024 threads.
 __global__ __launch_bounds__(1024) void verify_residual_k(const Verify A) {
-    constexpr int E = CH / 1024;
     __shared__ double ss[16];
     __shared__ RowStat rows[64];
     __shared__ double mass[64];
     __shared__ Draw d;
     const int b = blockIdx.y, c = blockIdx.x;
     const double it = inv_temp(A.temp, b);
-    walk_sequence(A, b, it, rows, mass, c == 0, &d);
+    walk_sequence(A, b, it, rows, mass, nullptr, c == 0, &d);
     if (c == 0 && threadIdx.x < sizeof(Draw) / 4) reinterpret_cast<int*>(A.draw + b)[threadIdx.x] = reinterpret_cast<const int*>(&d)[threadIdx.x];
     if (d.row < 0 || !(it >= 0)) return;
-    double w[E];
-    const double s = wave_sum(residuals<E, 1024>(w, A, d, it, c * CH + (int)threadIdx.x));
+    double w[4];
+    const double s = wave_sum(residuals(w, A, d, it, c * CH + 4 * (int)threadIdx.x));
     if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -478,17 +482,18 @@ __device__ __forceinline__ int thread_pick(const double (&x)[E], double& left) {
 }
 
 // The last token, after the walk where there are no draft probabilities.  grid B, kDrawThreads threads: a
-// thread has CE chunks in a row (V <= 2^22), then TE tokens of the chunk that is picked.
+// thread has CE chunks in a row (V <= 2^22), then four tokens of the chunk that is picked.
 //
 // Without draft probabilities a chunk's mass is the sum that verify_stats_k left, less the rejected
 // tokens'.  Where hardly anything is left that difference says little, and the chunks are summed anew; so
 // they are where the chunk that is picked turns out to hold rejected tokens alone.
 __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
-    constexpr int CE = kVerifyMaxV / CH / kDrawThreads, TE = CH / kDrawThreads;
+    constexpr int CE = kVerifyMaxV / CH / kDrawThreads;
+    static_assert(4 * kDrawThreads == CH, "a thread has four tokens of a chunk");
     __shared__ RowStat rows[64];
     __shared__ Draw d;
     __shared__ PickLds L;
-    __shared__ double s_sum[kDrawWaves], s_left;
+    __shared__ double s_sum[kDrawWaves], s_left, keep[64][64];
     __shared__ int s_chunk;
     const int b = blockIdx.x, tid = threadIdx.x;
     const double it = inv_temp(A.temp, b), u = (double)A.u[(size_t)b * A.T];
@@ -496,7 +501,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
 #pragma unroll
     for (int e = 0; e < CE; e++) mass[e] = A.q && CE * tid + e < A.C ? A.sums[(size_t)b * A.C + CE * tid + e] : 0.0;
     if (!A.q) {
-        walk_sequence(A, b, it, rows, nullptr, true, &d);
+        walk_sequence(A, b, it, rows, nullptr, keep, true, &d);
     } else {
         if (tid < (int)(sizeof(Draw) / 4)) reinterpret_cast<int*>(&d)[tid] = reinterpret_cast<const int*>(A.draw + b)[tid];
         __syncthreads();
@@ -514,7 +519,9 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
 #pragma unroll
         for (int e = 0; e < CE; e++) {
             const int c = CE * tid + e;
-            if (c < A.C) {
+            if (c < 64) {
+                mass[e] = keep[d.row - b * A.T][c];
+            } else if (c < A.C) {
                 const RowStat s = A.ch[(size_t)d.row * A.C + c];
                 mass[e] = s.s * weight(s.m, d.r.m, it);
             }
@@ -528,8 +535,8 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
     for (;; anew = true) {
         if (!A.q && anew) {
             for (int c = 0; c < A.C; c++) {
-                double x[TE];
-                const double s = wave_sum(residuals<TE, 1>(x, A, d, it, c * CH + tid * TE));
+                double x[4];
+                const double s = wave_sum(residuals(x, A, d, it, c * CH + 4 * tid));
                 if ((tid & 63) == 0) s_sum[tid >> 6] = s;
                 __syncthreads();
 #pragma unroll
@@ -554,9 +561,9 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
             s_left = fmax(r, 0.0);
         }
         __syncthreads();
-        const int at = s_chunk * CH + tid * TE;
-        double x[TE], left = s_left;
-        const int th = block_pick(residuals<TE, 1>(x, A, d, it, at), u, left, L);
+        const int at = s_chunk * CH + 4 * tid;
+        double x[4], left = s_left;
+        const int th = block_pick(residuals(x, A, d, it, at), u, left, L);
         if (th == tid) *out = at + thread_pick(x, left);
         if (th >= 0 || anew) return;                           // (else a chunk whose mass was rounding alone)
     }
