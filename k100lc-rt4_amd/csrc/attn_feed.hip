@@ -191,8 +191,8 @@ __global__ __launch_bounds__(256) void kv_append_v64_k(uint32_t* __restrict__ vc
 // and stage as kv_append_v64_k, bit for bit.  One launch: grid (vblocks + K workgroups, B), the
 // first vblocks = 4 H x tile slots workgroups a 64-key tile of 64 dims each, the others 8 K rows
 // of a head each.  A sequence whose keys would not lie in [0, kv_cap) is left as it is.
-// 4 rows of 4 heads into a draft tile take 4.3 us and 16 paths of up to 8 rows 6.9, the start of a
-// launch and dependent loads (count, length, rows, then the rows); 4 prompts of up to 1000 rows 9.2
+// 4 rows of 4 heads into a draft tile take 4.4 us and 16 paths of up to 8 rows 6.8, the start of a
+// launch and dependent loads (count, length, rows, then the rows); 4 prompts of up to 1000 rows 9.4
 // us, 20 MB at 2.1 TB/s.  (Loads under a condition: 17 us for those.)
 __global__ __launch_bounds__(256) void kv_append_rows_k(uint32_t* __restrict__ kc, float* __restrict__ ksc,
                                                         uint32_t* __restrict__ vc, float* __restrict__ vsc,

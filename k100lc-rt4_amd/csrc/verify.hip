@@ -18,9 +18,9 @@
 // one draw in about twenty.
 //
 // What bounds it: the read of the logits where they are many (8 sequences of 16 nodes, V = 248320:
-// verify_stats_k 28.4 us, 127 MB at 4.5 TB/s, then 9.4 for walk and draw), else a chain of short
-// launches, each the start of one and two or three trips to memory (one row of 32000: 5.6 + 7.2 us;
-// 4 rows of 248320 with draft probabilities 5.7 + 7.0 + 6.2; with siblings 6.3 more for each).
+// verify_stats_k 29 us, 127 MB at 4.4 TB/s, then 9.3 for walk and draw), else a chain of short
+// launches, each the start of one and two or three trips to memory (one row of 32000: 5.5 + 6.8 us;
+// 4 rows of 248320 with draft probabilities 5.7 + 6.6 + 5.1; with siblings 6.5 more for each).
 #include <climits>
 
 #include "rt4_dev.h"
