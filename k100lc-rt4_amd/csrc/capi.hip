@@ -873,7 +873,7 @@ int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_
     const int most = T > 1 ? T - 1 : 1, levels = !draft_p ? 1 : max_children < most ? max_children : most;
     hipStream_t st = as_stream(stream);
     void* ws = nullptr;
-    int rc = lib_scratch(kSlotVerify, rt4::verify_ws_bytes(B, T, V, levels), &ws, st);
+    int rc = lib_scratch(kSlotVerify, rt4::verify_ws_bytes(B, T, V, levels, draft_p != nullptr), &ws, st);
     if (rc) return rc;
     return hip_status(rt4::launch_verify_tree(tokens, path, count, kv_len, logits, (size_t)ldl, draft, parent, u, temp, draft_p,
                                               (size_t)ldp, B, T, V, levels, ws, st),

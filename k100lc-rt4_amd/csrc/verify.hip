@@ -18,9 +18,9 @@
 // one draw in about twenty.
 //
 // What bounds it: the read of the logits where they are many (8 sequences of 16 nodes, V = 248320:
-// verify_stats_k 29 us, 127 MB at 4.4 TB/s, then 9.3 for walk and draw), else a chain of short
-// launches, each the start of one and two or three trips to memory (one row of 32000: 5.5 + 6.8 us;
-// 4 rows of 248320 with draft probabilities 5.7 + 6.6 + 5.1; with siblings 6.5 more for each).
+// verify_stats_k 23 us, 127 MB at 5.5 TB/s, then 8.5 for walk and draw), else a chain of short
+// launches, each the start of one and two or three trips to memory (4 rows of 248320 with draft
+// probabilities 4.4 + 6.3 + 4.6 us; with siblings 5.2 more for each), or one launch (verify_small_k).
 #include <climits>
 
 #include "rt4_dev.h"
@@ -143,14 +143,14 @@ struct __attribute__((packed, aligned(4))) Quad {    // (loads of 16 bytes need 
     float f[4];
 };
 
-// A thread's elements of chunk c of a row, element e of thread i at 1024 (e / 4) + 4 i + e % 4, `rest` past
-// the row's end.
-__device__ __forceinline__ void load_chunk(float (&v)[PT], const float* row, int c, int V, float rest) {
-    const int at = c * CH + 4 * (int)threadIdx.x;
-    if ((c + 1) * CH <= V) {
+// 16 logits of a row, element e at `at` + STRIDE (e / 4) + e % 4; `rest` past the row's end, which is within
+// the span of the threads that load together unless `whole`.
+template <int STRIDE>
+__device__ __forceinline__ void load16(float (&v)[PT], const float* row, int at, bool whole, int V, float rest) {
+    if (whole) {
 #pragma unroll
         for (int e = 0; e < PT; e += 4) {
-            const Quad q = *reinterpret_cast<const Quad*>(row + at + 256 * e);
+            const Quad q = *reinterpret_cast<const Quad*>(row + at + STRIDE / 4 * e);
 #pragma unroll
             for (int k = 0; k < 4; k++) v[e + k] = q.f[k];
         }
@@ -158,12 +158,29 @@ __device__ __forceinline__ void load_chunk(float (&v)[PT], const float* row, int
     }
 #pragma unroll
     for (int e = 0; e < PT; e++) {                             // (unconditional loads: under a condition each waits)
-        const int i = at + 256 * (e & ~3) + (e & 3);
+        const int i = at + STRIDE * (e / 4) + e % 4;
         v[e] = row[i < V ? i : V - 1];
     }
 #pragma unroll
     for (int e = 0; e < PT; e++)
-        if (at + 256 * (e & ~3) + (e & 3) >= V) v[e] = rest;
+        if (at + STRIDE * (e / 4) + e % 4 >= V) v[e] = rest;
+}
+// Lowest index of a wave's largest logit m and its sum of weights.
+template <int STRIDE>
+__device__ __forceinline__ RowStat stat16(float (&v)[PT], int at, float m, double it) {
+    RowStat r = {m, INT_MAX, 0.0};
+#pragma unroll
+    for (int e = PT - 1; e >= 0; e--)
+        if (v[e] == m && m > -INFINITY) r.i = at + STRIDE * (e / 4) + e % 4;
+    if (it >= 0) {
+        float mf = m;
+        make_finite(v, mf);
+#pragma unroll
+        for (int e = 0; e < PT; e++) r.s += weight_finite(v[e], mf, it);
+    }
+    r.i = wave_min(r.i);
+    r.s = wave_sum(r.s);
+    return r;
 }
 
 // Statistics of a chunk of a row: one read of the logits, held in registers between the maximum and
@@ -178,7 +195,7 @@ __global__ __launch_bounds__(256) void verify_stats_k(const float* __restrict__ 
     const float* l = logits + (size_t)row * ldl;
     float v[PT], m = -INFINITY;
     const int at = c * CH + 4 * (int)threadIdx.x;
-    load_chunk(v, l, c, V, -INFINITY);
+    load16<1024>(v, l, at, (c + 1) * CH <= V, V, -INFINITY);
     const double it = inv_temp(temp, b);
 #pragma unroll
     for (int e = 0; e < PT; e++) m = fmaxf(m, v[e]);           // (drops NaN)
@@ -186,20 +203,8 @@ __global__ __launch_bounds__(256) void verify_stats_k(const float* __restrict__ 
     if ((threadIdx.x & 63) == 0) sm[w] = m;
     __syncthreads();
     m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    int mi = INT_MAX;
-#pragma unroll
-    for (int e = PT - 1; e >= 0; e--)
-        if (v[e] == m && m > -INFINITY) mi = at + 256 * (e & ~3) + (e & 3);
-    double s = 0;
-    if (it >= 0) {
-        float mf = m;
-        make_finite(v, mf);
-#pragma unroll
-        for (int e = 0; e < PT; e++) s += weight_finite(v[e], mf, it);
-    }
-    mi = wave_min(mi);
-    s = wave_sum(s);
-    if ((threadIdx.x & 63) == 0) si[w] = mi, ss[w] = s;
+    const RowStat part = stat16<1024>(v, at, m, it);
+    if ((threadIdx.x & 63) == 0) si[w] = part.i, ss[w] = part.s;
     __syncthreads();
     if (threadIdx.x == 0) {
         const int i01 = si[0] < si[1] ? si[0] : si[1], i23 = si[2] < si[3] ? si[2] : si[3];
@@ -221,8 +226,9 @@ __global__ __launch_bounds__(256) void verify_mass_k(const float* __restrict__ l
     const double it = inv_temp(temp, b);
     if (!(it >= 0)) return;
     float l[PT], pq[PT];
-    load_chunk(l, logits + (size_t)row * ldl, c, V, -INFINITY);
-    load_chunk(pq, q + (size_t)row * ldq, c, V, 0.f);
+    const int at = c * CH + 4 * (int)threadIdx.x;
+    load16<1024>(l, logits + (size_t)row * ldl, at, (c + 1) * CH <= V, V, -INFINITY);
+    load16<1024>(pq, q + (size_t)row * ldq, at, (c + 1) * CH <= V, V, 0.f);
     double a = 1.0;
     if (level > 1) {
         const double* prev = part + ((size_t)(level - 1) * R + row) * C;
@@ -582,11 +588,93 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
     }
 }
 
+// The whole verification in one launch, a workgroup a sequence, where its rows are few pieces of 1024 logits
+// (a wave each) and no residual levels are needed.  It saves the host's 3 us for a launch, and where one CU's
+// 64-bit rate does not bound it, time on the device: one row of 1000 logits 16.7 -> 13.6 us eagerly, 11.1 ->
+// 9.2 in a graph; of 24000 16.5 -> 13.2 and 11.8 -> 11.8; of 32000 16.6 -> 13.2 and 11.6 -> 13.6; 4 rows of
+// 4000 with draft probabilities 20.9 -> 14.6 and 15.2 -> 12.9.  Beyond: 32 rows of 1000 16.5 -> 17.4 and
+// 13.0 -> 18.2, a row of 32000 with draft probabilities 20.4 -> 20.7 and 15.2 -> 21.5.
+// grid B, 1024 threads; A.C: pieces in a row.
+constexpr int SP = 1024, kSmallPieces = 32;
+__global__ __launch_bounds__(1024) void verify_small_k(const Verify A) {
+    __shared__ RowStat ch[kSmallPieces], rows[64];
+    __shared__ double keep[kSmallPieces][64];
+    __shared__ u64 kids[64];
+    __shared__ Draw d;
+    __shared__ PickLds L;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6), C = A.C;
+    const double it = inv_temp(A.temp, b), u = (double)A.u[(size_t)b * A.T];
+    Nodes nd;
+    if (w == 0) nd = read_nodes(A, b);
+    for (int p = w; p < A.T * C; p += 16) {
+        const int n = p / C, c = p - n * C, at = c * SP + 4 * lane;
+        float v[PT], m = -INFINITY;
+        load16<256>(v, A.logits + ((size_t)b * A.T + n) * A.ldl, at, (c + 1) * SP <= A.V, A.V, -INFINITY);
+#pragma unroll
+        for (int e = 0; e < PT; e++) m = fmaxf(m, v[e]);       // (drops NaN)
+        const RowStat r = stat16<256>(v, at, wave_max(m), it);
+        if (lane == 0) ch[p] = r;
+    }
+    __syncthreads();
+    for (int n = w; n < A.T; n += 16) {
+        const RowStat r = row_of_chunks(ch + n * C, C, it, keep[n]);
+        if (lane == 0) rows[n] = r;
+    }
+    __syncthreads();
+    if (w == 0) walk(A, b, it, nd, rows, nullptr, kids, true, &d);
+    __syncthreads();
+    if (d.row < 0) return;
+    int* out = A.tokens + (size_t)b * A.T + d.n - 1;
+    const int best = d.r.i < A.V ? d.r.i : -1, row = d.row - b * A.T;
+    if (!(it >= 0) || best < 0) {                              // greedy, or a row with nothing in it
+        if (tid == 0) *out = best;
+        return;
+    }
+    double gone = 0;
+    for (int k = 0; k < d.nrej; k++) gone += d.rejw[k];
+    for (bool anew = A.q || d.r.s - gone < 1e-6 * d.r.s;; anew = true) {       // (see verify_draw_k)
+        if (anew) {
+            for (int c = w; c < C; c += 16) {
+                double s = 0, x[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) s += residuals(x, A, d, it, c * SP + 256 * k + 4 * lane);
+                s = wave_sum(s);
+                if (lane == 0) keep[row][c] = s;
+            }
+            __syncthreads();
+        }
+        double mine = tid < C ? keep[row][tid] : 0.0, r = -1.0;
+        if (!anew) {
+            for (int k = 0; k < d.nrej; k++)
+                if (d.rej[k] / SP == tid) mine -= d.rejw[k];
+            mine = fmax(mine, 0.0);
+        }
+        const int owner = block_pick(mine, u, r, L);
+        if (owner < 0) {                                       // nothing left: the largest
+            if (tid == 0) *out = best;
+            return;
+        }
+        __syncthreads();                                       // (every thread has its answer)
+        const int at = owner * SP + 4 * tid;
+        double x[4] = {}, left = fmax(r, 0.0);
+        const int th = block_pick(tid < SP / 4 ? residuals(x, A, d, it, at) : 0.0, u, left, L);
+        if (th == tid) *out = at + thread_pick(x, left);
+        if (th >= 0 || anew) return;
+    }
+}
+
 size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
 
 }  // namespace
 
-size_t verify_ws_bytes(int B, int T, int V, int levels) {
+// Whether verify_small_k takes it.
+static bool small(int T, int V, int levels, bool q) {
+    const int pieces = (V + SP - 1) / SP;
+    return levels == 1 && (q ? 3 : 2) * T * pieces + 2 * T <= 2 * kSmallPieces + 2;
+}
+
+size_t verify_ws_bytes(int B, int T, int V, int levels, bool q) {
+    if (small(T, V, levels, q)) return 0;
     const size_t R = (size_t)B * T, C = (V + CH - 1) / CH;
     return up16(R * C * sizeof(RowStat)) + up16(R * levels * 8) + up16(R * C * levels * 8) + up16(B * sizeof(Draw)) + up16(B * C * 8);
 }
@@ -603,6 +691,12 @@ hipError_t launch_verify_tree(int* tokens, int* path, int* count, int* kv_len, c
     Draw* draw = reinterpret_cast<Draw*>(take((size_t)B * sizeof(Draw)));
     double* sums = reinterpret_cast<double*>(take((size_t)B * C * 8));
     const Verify a = {tokens, path, count, kv_len, logits, ldl, draft, parent, u, temp, q, ldq, ch, av, part, draw, sums, B, T, V, C, levels};
+    if (small(T, V, levels, q != nullptr)) {
+        Verify one = a;
+        one.C = (V + SP - 1) / SP;
+        hipLaunchKernelGGL(verify_small_k, dim3(B), dim3(1024), 0, st, one);
+        return hipGetLastError();
+    }
     hipLaunchKernelGGL(verify_stats_k, dim3(C, R), dim3(256), 0, st, logits, ldl, parent, temp, T, V, ch);
     for (int k = 1; k < levels; k++)
         hipLaunchKernelGGL(verify_mass_k, dim3(C, R), dim3(256), 0, st, logits, ldl, q, ldq, parent, temp, T, V, k, ch, av, part);

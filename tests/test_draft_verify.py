@@ -916,3 +916,20 @@ def test_verify_star(rt4, torch_gpu, probs, temp, scale):
         q = rng.random((B * T, V)).astype(np.float32) ** 4
         q /= q.sum(1, keepdims=True)
     check_verify(rt4, logits, draft, parent, u, [temp] * B, q, T - 1 if probs else None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("B,T,V", [(1, 1, 1024), (3, 1, 1025), (2, 1, 32768), (2, 1, 32769), (20, 4, 2047), (5, 10, 1000), (2, 16, 1024), (2, 17, 1024),
+                                   (1, 33, 64)])
+def test_verify_few_logits(rt4, torch_gpu, B, T, V, probs):
+    """Sizes around those that are verified in one launch, chains and drafts that are drawn, greedy and not."""
+    print(f"case few logits B={B} T={T} V={V} probs={probs}", flush=True)
+    rng = np.random.default_rng(B * 1000 + T + V)
+    for kids in (1, 3):
+        logits, draft, parent, u, q = verify_case(rng, B, T, V, kids, probs)
+        logits[:, ::7] = -np.inf
+        if T > 2:
+            parent[-1, 0] = -3                          # an idle sequence
+        temp = [(1.0, 0.0, 0.3)[b % 3] for b in range(B)]
+        check_verify(rt4, logits, draft, parent, u, temp, q, 1 if probs else None, kv_len=list(range(B)), pad=1)
