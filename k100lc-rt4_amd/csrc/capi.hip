@@ -35,7 +35,7 @@ hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 // the retired buffers of a slot add up to at most twice its final size.  Not
 // safe for concurrent calls from several threads (the reference's scratch has
 // the same property, src/k_gemv.hip:47-51).
-enum Slot { kSlotActQ = 0, kSlotActS = 1, kSlotGemmA = 2, kSlotGemmPart = 3, kSlotAttnPart = 4, kSlotGemvPart = 5, kSlotGemvCnt = 6, kSlotAttnCnt = 7, kSlotAttnKV = 8, kSlotGemmCnt = 9, kSlotVerify = 10, kSlotTreePart = 11, kSlots = 12 };
+enum Slot { kSlotActQ = 0, kSlotActS = 1, kSlotGemmA = 2, kSlotGemmPart = 3, kSlotAttnPart = 4, kSlotGemvPart = 5, kSlotGemvCnt = 6, kSlotAttnCnt = 7, kSlotAttnKV = 8, kSlotGemmCnt = 9, kSlotVerify = 10, kSlotTreePart = 11, kSlotVerifyCnt = 12, kSlots = 13 };
 constexpr int kMaxDev = 64;
 struct Buf {
     void* p = nullptr;
@@ -872,11 +872,13 @@ int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_
         return fail(RT4_E_ARG, "rt4_verify_tree: misaligned pointer");
     const int most = T > 1 ? T - 1 : 1, levels = !draft_p ? 1 : max_children < most ? max_children : most;
     hipStream_t st = as_stream(stream);
-    void* ws = nullptr;
-    int rc = lib_scratch(kSlotVerify, rt4::verify_ws_bytes(B, T, V, levels, draft_p != nullptr), &ws, st);
-    if (rc) return rc;
+    void *ws = nullptr, *cnt = nullptr;
+    const size_t bytes = rt4::verify_ws_bytes(B, T, V, levels, draft_p != nullptr);
+    int rc = RT4_OK;
+    if (bytes && (rc = lib_scratch(kSlotVerify, bytes, &ws, st))) return rc;
+    if (bytes && draft_p && (rc = lib_scratch(kSlotVerifyCnt, (size_t)B * sizeof(int), &cnt, st, true))) return rc;
     return hip_status(rt4::launch_verify_tree(tokens, path, count, kv_len, logits, (size_t)ldl, draft, parent, u, temp, draft_p,
-                                              (size_t)ldp, B, T, V, levels, ws, st),
+                                              (size_t)ldp, B, T, V, levels, ws, static_cast<int*>(cnt), st),
                       "rt4_verify_tree launch");
 }
 

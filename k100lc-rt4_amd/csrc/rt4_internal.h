@@ -176,11 +176,12 @@ size_t tree_part_bytes(const AttnTree& a, const TreePlan& p);
 hipError_t launch_attn_tree(const AttnTree& a, const TreePlan& p, void* ws, hipStream_t st);
 
 // Draft verification; `levels`: children tested per node where draft probabilities q are
-// given (else 1); ws: verify_ws_bytes of scratch (0 where one launch does without).
+// given (else 1); ws: verify_ws_bytes of scratch (0 where one launch does without); cnt: B
+// counters that are 0 (with draft probabilities, unless ws needs nothing).
 constexpr int kVerifyChunk = 4096, kVerifyMaxV = 1 << 22;
 size_t verify_ws_bytes(int B, int T, int V, int levels, bool q);
 hipError_t launch_verify_tree(int* tokens, int* path, int* count, int* kv_len, const float* logits, size_t ldl, const int* draft,
                               const int* parent, const float* u, const float* temp, const float* q, size_t ldq, int B, int T, int V,
-                              int levels, void* ws, hipStream_t st);
+                              int levels, void* ws, int* cnt, hipStream_t st);
 
 }  // namespace rt4

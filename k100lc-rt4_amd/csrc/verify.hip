@@ -18,9 +18,9 @@
 // one draw in about twenty.
 //
 // What bounds it: the read of the logits where they are many (8 sequences of 16 nodes, V = 248320:
-// verify_stats_k 23 us, 127 MB at 5.5 TB/s, then 8.5 for walk and draw), else a chain of short
+// verify_stats_k 22.3 us, 127 MB at 5.7 TB/s, then 7.7 for walk and draw), else a chain of short
 // launches, each the start of one and two or three trips to memory (4 rows of 248320 with draft
-// probabilities 4.4 + 6.3 + 4.6 us; with siblings 5.2 more for each), or one launch (verify_small_k).
+// probabilities 4.1 + 9.6 us; with siblings 5.3 more for each), or one launch (verify_small_k).
 #include <climits>
 
 #include "rt4_dev.h"
@@ -134,8 +134,8 @@ struct Verify {                          // the arguments of rt4_verify_tree and
     size_t ldq;
     RowStat* ch;                         // [row][C] chunk statistics
     double *av, *part;                   // residual levels: a and chunk sums, [level][row], [level][row][C]
-    Draw* draw;
     double* sums;                        // [B][C] residual mass of the last token's row
+    int* cnt;                            // [B] workgroups that have written theirs, 0 between launches
     int B, T, V, C, levels;
 };
 
@@ -429,29 +429,6 @@ __device__ __forceinline__ void walk_sequence(const Verify& A, int b, double it,
     __syncthreads();
 }
 
-// With draft probabilities, the walk and the chunk sums of the residual: every workgroup of a
-// sequence walks for itself (a launch less), the first one writes.  grid (C, B), 1024 threads.
-__global__ __launch_bounds__(1024) void verify_residual_k(const Verify A) {
-    __shared__ double ss[16];
-    __shared__ RowStat rows[64];
-    __shared__ double mass[64];
-    __shared__ Draw d;
-    const int b = blockIdx.y, c = blockIdx.x;
-    const double it = inv_temp(A.temp, b);
-    walk_sequence(A, b, it, rows, mass, nullptr, c == 0, &d);
-    if (c == 0 && threadIdx.x < sizeof(Draw) / 4) reinterpret_cast<int*>(A.draw + b)[threadIdx.x] = reinterpret_cast<const int*>(&d)[threadIdx.x];
-    if (d.row < 0 || !(it >= 0)) return;
-    double w[4];
-    const double s = wave_sum(residuals(w, A, d, it, c * CH + 4 * (int)threadIdx.x));
-    if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double t = 0;
-        for (int k = 0; k < 16; k++) t += ss[k];
-        A.sums[(size_t)b * A.C + c] = t;
-    }
-}
-
 // The first thread at which the masses' running sum (in thread order) exceeds r, or u times their total
 // where r is negative; where rounding leaves none, the last one with any; -1 where there is no mass.
 // Every thread gets it; r becomes what of it is left there.  kDrawThreads threads.
@@ -500,31 +477,80 @@ __device__ __forceinline__ int thread_pick(const double (&x)[E], double& left) {
     return at;
 }
 
-// The last token, after the walk where there are no draft probabilities.  grid B, kDrawThreads threads: a
-// thread has CE chunks in a row (V <= 2^22), then four tokens of the chunk that is picked.
+// The last token, chunk tid having `mass`: by running sums over chunks, then over the tokens of one.  False
+// where that one has none (its mass was rounding alone).
+static_assert(kVerifyMaxV / CH == kDrawThreads && 4 * kDrawThreads == CH, "a thread has a chunk, and four tokens of one");
+__device__ __forceinline__ bool pick_token(double mass, const Verify& A, const Draw& d, double it, double u, PickLds& L, int best,
+                                           int* out) {
+    const int tid = threadIdx.x;
+    double r = -1.0;
+    const int chunk = block_pick(mass, u, r, L);
+    if (chunk < 0) {                                           // nothing left: the largest
+        if (tid == 0) *out = best;
+        return true;
+    }
+    __syncthreads();                                           // (every thread has its answer)
+    const int at = chunk * CH + 4 * tid;
+    double x[4], left = fmax(r, 0.0);
+    const int th = block_pick(residuals(x, A, d, it, at), u, left, L);
+    if (th == tid) *out = at + thread_pick(x, left);
+    return th >= 0;
+}
+
+// With draft probabilities, the walk, the chunk sums of the residual and the last token.  Every workgroup of a
+// sequence walks for itself (a launch less), the first one writes the path; the last to write its sum draws
+// (another launch less, 3 us of the host's).  Sums go through the L2 to where all XCDs see them (agent
+// scope), are there before the workgroup counts itself in, and are read from there; nobody waits.  grid (C, B),
+// kDrawThreads threads.
+__global__ __launch_bounds__(kDrawThreads) void verify_residual_k(const Verify A) {
+    __shared__ double ss[kDrawWaves];
+    __shared__ RowStat rows[64];
+    __shared__ double mass[64];
+    __shared__ Draw d;
+    __shared__ PickLds L;
+    __shared__ bool s_last;
+    const int b = blockIdx.y, c = blockIdx.x, tid = threadIdx.x;
+    const double it = inv_temp(A.temp, b), u = (double)A.u[(size_t)b * A.T];
+    walk_sequence(A, b, it, rows, mass, nullptr, c == 0, &d);
+    if (d.row < 0) return;
+    int* out = A.tokens + (size_t)b * A.T + d.n - 1;
+    const int best = d.r.i < A.V ? d.r.i : -1;
+    if (!(it >= 0) || best < 0) {                              // greedy, or a row with nothing in it
+        if (c == 0 && tid == 0) *out = best;
+        return;
+    }
+    double w[4];
+    const double s = wave_sum(residuals(w, A, d, it, c * CH + 4 * tid));
+    if ((tid & 63) == 0) ss[tid >> 6] = s;
+    __syncthreads();
+    u64* sums = reinterpret_cast<u64*>(A.sums + (size_t)b * A.C);
+    if (tid == 0) {
+        double t = 0;
+        for (int k = 0; k < kDrawWaves; k++) t += ss[k];
+        __hip_atomic_store(sums + c, __builtin_bit_cast(u64, t), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        s_last = __hip_atomic_fetch_add(A.cnt + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == A.C - 1;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    if (tid == 0) __hip_atomic_store(A.cnt + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const double m = tid < A.C ? __builtin_bit_cast(double, __hip_atomic_load(sums + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) : 0.0;
+    if (!pick_token(m, A, d, it, u, L, best, out) && tid == 0) *out = best;
+}
+
+// Without them, the walk and the last token, after verify_stats_k.  grid B, kDrawThreads threads.
 //
-// Without draft probabilities a chunk's mass is the sum that verify_stats_k left, less the rejected
-// tokens'.  Where hardly anything is left that difference says little, and the chunks are summed anew; so
-// they are where the chunk that is picked turns out to hold rejected tokens alone.
+// A chunk's mass is the sum that verify_stats_k left, less the rejected tokens'.  Where hardly anything is
+// left that difference says little, and the chunks are summed anew; so they are where the chunk that is
+// picked turns out to hold rejected tokens alone.
 __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
-    constexpr int CE = kVerifyMaxV / CH / kDrawThreads;
-    static_assert(4 * kDrawThreads == CH, "a thread has four tokens of a chunk");
     __shared__ RowStat rows[64];
     __shared__ Draw d;
     __shared__ PickLds L;
-    __shared__ double s_sum[kDrawWaves], s_left, keep[64][64];
-    __shared__ int s_chunk;
+    __shared__ double s_sum[kDrawWaves], keep[64][64];
     const int b = blockIdx.x, tid = threadIdx.x;
     const double it = inv_temp(A.temp, b), u = (double)A.u[(size_t)b * A.T];
-    double mass[CE];
-#pragma unroll
-    for (int e = 0; e < CE; e++) mass[e] = A.q && CE * tid + e < A.C ? A.sums[(size_t)b * A.C + CE * tid + e] : 0.0;
-    if (!A.q) {
-        walk_sequence(A, b, it, rows, nullptr, keep, true, &d);
-    } else {
-        if (tid < (int)(sizeof(Draw) / 4)) reinterpret_cast<int*>(&d)[tid] = reinterpret_cast<const int*>(A.draw + b)[tid];
-        __syncthreads();
-    }
+    walk_sequence(A, b, it, rows, nullptr, keep, true, &d);
     if (d.row < 0) return;
     int* out = A.tokens + (size_t)b * A.T + d.n - 1;
     const int best = d.r.i < A.V ? d.r.i : -1;
@@ -532,59 +558,36 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
         if (tid == 0) *out = best;
         return;
     }
-    bool anew = A.q;
-    if (!A.q) {
-        double gone = 0;
-#pragma unroll
-        for (int e = 0; e < CE; e++) {
-            const int c = CE * tid + e;
-            if (c < 64) {
-                mass[e] = keep[d.row - b * A.T][c];
-            } else if (c < A.C) {
-                const RowStat s = A.ch[(size_t)d.row * A.C + c];
-                mass[e] = s.s * weight(s.m, d.r.m, it);
-            }
-            for (int k = 0; k < d.nrej; k++)
-                if (d.rej[k] / CH == c) mass[e] -= d.rejw[k];
-            mass[e] = fmax(mass[e], 0.0);
-        }
-        for (int k = 0; k < d.nrej; k++) gone += d.rejw[k];
-        anew = d.r.s - gone < 1e-6 * d.r.s;
+    double mass = 0, gone = 0;
+    if (tid < 64) {
+        mass = keep[d.row - b * A.T][tid];
+    } else if (tid < A.C) {
+        const RowStat s = A.ch[(size_t)d.row * A.C + tid];
+        mass = s.s * weight(s.m, d.r.m, it);
     }
-    for (;; anew = true) {
-        if (!A.q && anew) {
+    for (int k = 0; k < d.nrej; k++) {
+        if (d.rej[k] / CH == tid) mass -= d.rejw[k];
+        gone += d.rejw[k];
+    }
+    mass = fmax(mass, 0.0);
+    for (bool anew = d.r.s - gone < 1e-6 * d.r.s;; anew = true) {
+        if (anew)
             for (int c = 0; c < A.C; c++) {
                 double x[4];
                 const double s = wave_sum(residuals(x, A, d, it, c * CH + 4 * tid));
                 if ((tid & 63) == 0) s_sum[tid >> 6] = s;
                 __syncthreads();
-#pragma unroll
-                for (int e = 0; e < CE; e++)
-                    if (CE * tid + e == c) {
-                        mass[e] = 0;
-                        for (int k = 0; k < kDrawWaves; k++) mass[e] += s_sum[k];
-                    }
+                if (tid == c) {
+                    mass = 0;
+                    for (int k = 0; k < kDrawWaves; k++) mass += s_sum[k];
+                }
                 __syncthreads();
             }
-        }
-        double mine = 0, r = -1.0;
-#pragma unroll
-        for (int e = 0; e < CE; e++) mine += mass[e];
-        const int owner = block_pick(mine, u, r, L);
-        if (owner < 0) {                                       // nothing left: the largest
+        if (pick_token(mass, A, d, it, u, L, best, out)) return;
+        if (anew) {
             if (tid == 0) *out = best;
             return;
         }
-        if (tid == owner) {
-            s_chunk = CE * tid + thread_pick(mass, r);
-            s_left = fmax(r, 0.0);
-        }
-        __syncthreads();
-        const int at = s_chunk * CH + 4 * tid;
-        double x[4], left = s_left;
-        const int th = block_pick(residuals(x, A, d, it, at), u, left, L);
-        if (th == tid) *out = at + thread_pick(x, left);
-        if (th >= 0 || anew) return;                           // (else a chunk whose mass was rounding alone)
     }
 }
 
@@ -659,7 +662,11 @@ __global__ __launch_bounds__(1024) void verify_small_k(const Verify A) {
         double x[4] = {}, left = fmax(r, 0.0);
         const int th = block_pick(tid < SP / 4 ? residuals(x, A, d, it, at) : 0.0, u, left, L);
         if (th == tid) *out = at + thread_pick(x, left);
-        if (th >= 0 || anew) return;
+        if (th >= 0) return;
+        if (anew) {
+            if (tid == 0) *out = best;
+            return;
+        }
     }
 }
 
@@ -676,21 +683,20 @@ static bool small(int T, int V, int levels, bool q) {
 size_t verify_ws_bytes(int B, int T, int V, int levels, bool q) {
     if (small(T, V, levels, q)) return 0;
     const size_t R = (size_t)B * T, C = (V + CH - 1) / CH;
-    return up16(R * C * sizeof(RowStat)) + up16(R * levels * 8) + up16(R * C * levels * 8) + up16(B * sizeof(Draw)) + up16(B * C * 8);
+    return up16(R * C * sizeof(RowStat)) + up16(R * levels * 8) + up16(R * C * levels * 8) + up16(B * C * 8);
 }
 
 hipError_t launch_verify_tree(int* tokens, int* path, int* count, int* kv_len, const float* logits, size_t ldl, const int* draft,
                               const int* parent, const float* u, const float* temp, const float* q, size_t ldq, int B, int T, int V,
-                              int levels, void* ws, hipStream_t st) {
+                              int levels, void* ws, int* cnt, hipStream_t st) {
     const int R = B * T, C = (V + CH - 1) / CH;
     unsigned char* p = static_cast<unsigned char*>(ws);
     auto take = [&](size_t n) { unsigned char* r = p; p += up16(n); return r; };
     RowStat* ch = reinterpret_cast<RowStat*>(take((size_t)R * C * sizeof(RowStat)));
     double* av = reinterpret_cast<double*>(take((size_t)R * levels * 8));
     double* part = reinterpret_cast<double*>(take((size_t)R * C * levels * 8));
-    Draw* draw = reinterpret_cast<Draw*>(take((size_t)B * sizeof(Draw)));
     double* sums = reinterpret_cast<double*>(take((size_t)B * C * 8));
-    const Verify a = {tokens, path, count, kv_len, logits, ldl, draft, parent, u, temp, q, ldq, ch, av, part, draw, sums, B, T, V, C, levels};
+    const Verify a = {tokens, path, count, kv_len, logits, ldl, draft, parent, u, temp, q, ldq, ch, av, part, sums, cnt, B, T, V, C, levels};
     if (small(T, V, levels, q != nullptr)) {
         Verify one = a;
         one.C = (V + SP - 1) / SP;
@@ -700,8 +706,10 @@ hipError_t launch_verify_tree(int* tokens, int* path, int* count, int* kv_len, c
     hipLaunchKernelGGL(verify_stats_k, dim3(C, R), dim3(256), 0, st, logits, ldl, parent, temp, T, V, ch);
     for (int k = 1; k < levels; k++)
         hipLaunchKernelGGL(verify_mass_k, dim3(C, R), dim3(256), 0, st, logits, ldl, q, ldq, parent, temp, T, V, k, ch, av, part);
-    if (q) hipLaunchKernelGGL(verify_residual_k, dim3(C, B), dim3(1024), 0, st, a);
-    hipLaunchKernelGGL(verify_draw_k, dim3(B), dim3(kDrawThreads), 0, st, a);
+    if (q)
+        hipLaunchKernelGGL(verify_residual_k, dim3(C, B), dim3(kDrawThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL(verify_draw_k, dim3(B), dim3(kDrawThreads), 0, st, a);
     return hipGetLastError();
 }
 

@@ -933,3 +933,28 @@ def test_verify_few_logits(rt4, torch_gpu, B, T, V, probs):
             parent[-1, 0] = -3                          # an idle sequence
         temp = [(1.0, 0.0, 0.3)[b % 3] for b in range(B)]
         check_verify(rt4, logits, draft, parent, u, temp, q, 1 if probs else None, kv_len=list(range(B)), pad=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,V", [(40, 3, 20000), (2, 4, 1 << 20), (300, 2, 9001)])
+def test_verify_repeats(rt4, torch_gpu, B, T, V):
+    """The workgroup that draws is whichever ends last: the same tokens every time, from calls right behind one another too."""
+    print(f"case repeats B={B} T={T} V={V}", flush=True)
+    torch = torch_gpu
+    g = torch.Generator(device="cuda").manual_seed(B)
+    logits = 2.5 * torch.randn((B * T, V), device="cuda", generator=g)
+    q = torch.softmax(logits + 0.5 * torch.randn((B * T, V), device="cuda", generator=g), -1)
+    draft = torch.randint(0, V, (B, T), dtype=torch.int32, device="cuda", generator=g)
+    draft[:, 1] = q.view(B, T, V)[:, 0].argmax(-1).int()
+    parent = torch.tensor([list(range(-1, T - 1))] * B, dtype=torch.int32, device="cuda")
+    u = torch.rand((B, T), device="cuda", generator=g)
+    outs = [[torch.full(s, -7, dtype=torch.int32, device="cuda") for s in ((B, T), (B, T), (B,))] for _ in range(12)]
+    for o in outs:
+        rt4.verify_tree(logits, draft, parent, u, draft_probs=q, max_children=1, tokens=o[0], path=o[1], count=o[2])
+    for o in outs:
+        assert all(torch.equal(a, b) for a, b in zip(o, outs[0]))
+    n = 8 if V < 100000 else 2                          # the first sequences against the walk in 64 bits
+    h = [host(x) for x in (logits[:n * T], draft[:n], parent[:n], u[:n], q[:n * T])]
+    want = verify(h[0], h[1], h[2], h[3], [1.0] * n, h[4], 1)
+    for a, b in zip(outs[0], want):
+        assert np.array_equal(host(a)[:n], b)
