@@ -11,7 +11,7 @@
  * workspaces of the GEMVs (W4A8 and W4A4 share one, partials plus counters that
  * every launch leaves at zero), of the GEMM and of the attention prefill, the
  * prefill's staged K/V copy (24 KB per key tile and KV head), the tree attention's
- * split states and the verification's row statistics are one buffer per
+ * split states and the verification's row statistics (and counters, left at zero) are one buffer per
  * device and kind, grown on demand like the reference's static
  * scratch (src/k_gemv.hip:16-23).  Calls that may run at the same time on one
  * device (different streams) therefore race on it; the caller orders them, as
