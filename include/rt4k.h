@@ -324,8 +324,9 @@ int rt4_kv_append_rows(uint32_t* kc, float* ksc, uint32_t* vc, float* vsc, float
 /* Attention of the trees' nodes, GQA (KV head = head / ratio): out f32 [n_heads][TP][256]
  * row b*T + i = softmax(Q K^T) V over the keys before kv_len[b] of sequence b's cache and
  * over node i and the nodes above it, whose K/V are keys 0..T-1 of the sequence's draft
- * tile (kd, ksd, vd, vsd: a cache of 64 keys).  Scores, P and sums in fp32 (Q codes and
- * scales as rt4_attn_q_quant writes them, qq u32 [n_heads][TP][32], TP >= B*T).  Rows of
+ * tile (kd, ksd, vd, vsd: a cache of 64 keys).  Scores and sums in fp32, P in two fp16 parts
+ * (off by at most 2^-22 of itself or 2^-38 of the row's largest; Q codes and scales as
+ * rt4_attn_q_quant writes them, qq u32 [n_heads][TP][32], TP >= B*T).  Rows of
  * padding nodes and of idle sequences are zeros; rows from B*T on are left as they were.
  * kv_len int32 [B] on the device, clamped to [0, kv_cap]; NULL: no cache (kc, ksc, vc, vsc
  * are not read).  kv_max: the longest length to plan for (a longer one is still right).

@@ -10,8 +10,9 @@
 //   it; out = softmax(S) V.  A node that hangs under no root sees nothing: zeros.
 // Scores are exact integers times two fp32 scales (the reference's decode attention has fp32
 // scores, P and sums too; the prefill's int4 P would cost a relative 1e-2 per row when there are
-// few keys).  P is two fp16 parts, high and low, which keep 22 bits of it, so that P V runs on the
-// fp16 matrix instructions with V's codes exact; states and sums are fp32.
+// few keys).  P is two fp16 parts, high and low, so that P V runs on the fp16 matrix instructions with
+// V's codes exact: off by at most 2^-22 of itself or 2^-38 of the row's largest so far; states and sums
+// are fp32.
 //
 // What bounds it (24 query heads over 4 KV heads):
 //   1 node over 1000 keys: 6.1 us and the join 3.7, the start of two launches; the loop is one step
@@ -178,8 +179,13 @@ __device__ __forceinline__ Run run_of(const AttnTree& A, const TreePlan& P, int 
 // n / T for a row n of a KV head's (T at most 64, n below 2^26).
 __device__ __forceinline__ int by_nodes(int n, const AttnTree& A, const TreePlan& P) { return A.T == 1 ? n : (int)__umulhi((unsigned)n, P.inv_nodes); }
 
-constexpr float kPBits = 7.f;            // P is held times 2^7: at most 2^15 with the lazy maximum
-constexpr float kLazy = 8.f;             // the running maximum moves when a score exceeds it by 2^8
+// P is held times 2^kPBits, and the running maximum moves when a score exceeds it by 2^kLazy, so that P is
+// at most 2^15 and fp16 holds it.  What is below 2^-(25 + kPBits) of the largest adds to the sum of P and
+// not to P V: over the n keys of a run at most n 2^-38 of the largest |V|, where the fp32 sums over the
+// n / 64 tiles may be off by n 2^-30.  (7 and 8: n 2^-32, 1e-4 of the output where one key is 22 nats above
+// 32768 others and its value small.  The lower floor moves the maximum more often: 1.9% on average over 45
+// sizes, 61 nodes over 131001 keys 282 -> 288 us.  The low part times 2^11, which needs no floor: 4.2%.)
+constexpr float kPBits = 13.f, kLazy = 2.f;
 
 // Products x[4g + r] * y[c] of four 16x16 tiles in their accumulator layout on the matrix core
 // (registers 4b + r: tile b, x from lane 16b + 4g + r, y from lane 16b + c), each rounded once.

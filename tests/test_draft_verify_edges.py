@@ -1,0 +1,48 @@
+"""Draft-and-verify decode steps where they can go wrong: outstanding keys, idle sequences, plans, capture, a cache's end.
+
+Expectations are those of test_draft_verify.py (64-bit softmax, a literal walk) or, for plans, the launches that a capture
+records.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from test_draft_verify import BG, D, G, dev, host
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- attention --
+@pytest.mark.parametrize("n", [4096, 32768, 131072, 1 << 20])
+def test_outstanding_key(rt4, torch_gpu, n):
+    """The cache's first key far above all the others, its value small: what the others weigh together counts.
+
+    Every head has its own distance, 10 to 33 nats.  The bound is relative to the output, whose terms are all positive, and
+    counts fp32 roundings as test_draft_verify.tree_attention does (8 S + 168, one a tile of a run, one a run in the join) and
+    2^-22 for P: no key may be lost for its small weight."""
+    torch = torch_gpu
+    print(f"case outstanding key n={n}", flush=True)
+    QH = 48
+    kv = [torch.zeros((1, 1, n, D // 8), dtype=torch.int32, device="cuda"), torch.ones((1, 1, 2, n), device="cuda"),
+          torch.full((1, 1, n // 8, D), 0x77777777, dtype=torch.int32, device="cuda"),
+          torch.full((1, 1, n // BG, D), np.float32(1 / 7), device="cuda")]
+    draft = [torch.zeros((1, 1, BG, D // 8), dtype=torch.int32, device="cuda"), torch.ones((1, 1, 2, BG), device="cuda"),
+             torch.full((1, 1, 8, D), 0x77777777, dtype=torch.int32, device="cuda"),
+             torch.full((1, 1, 1, D), np.float32(1 / 7), device="cuda")]
+    kv[0][0, 0, 0] = 0x11111111
+    kv[3][0, 0, 0] = float(np.float32(0.05 / 7))               # the first tile's values are all small
+    qq = torch.full((QH, 1, D // 8), 0x11111111, dtype=torch.int32, device="cuda")
+    qs = (np.linspace(10, 33, QH) / D).astype(np.float32)
+    parent = torch.full((1, 1), -1, dtype=torch.int32, device="cuda")
+    s = qs.astype(np.float64) * D                       # 256 products of 1 x 1
+    V, V0 = 7 * float(np.float32(1 / 7)), 7 * float(np.float32(0.05 / 7))
+    p = np.exp(-s)
+    want = (V0 + p * ((BG - 1) * V0 + (n - BG + 1) * V)) / (1 + n * p)
+    for splits in (1, 128, 0):
+        out = rt4.attention_tree(qq, dev(np.repeat(qs[:, None, None], 2, 1)), *kv, dev(np.array([n])), *draft, parent, ratio=QH,
+                                 kv_splits=splits)
+        tiles = n / BG / 128 + 128 if splits == 128 else n / BG
+        tol = (8 * s * 1.4427 + 168 + tiles) * 2.0**-24 + 2.0**-22
+        err = np.abs(host(out)[:, 0].astype(np.float64) / want[:, None] - 1)
+        assert (err <= tol[:, None]).all(), (splits, err.max(), (err / tol[:, None]).max())
