@@ -331,7 +331,7 @@ int rt4_kv_append_rows(uint32_t* kc, float* ksc, uint32_t* vc, float* vsc, float
  * kv_len int32 [B] on the device, clamped to [0, kv_cap]; NULL: no cache (kc, ksc, vc, vsc
  * are not read).  kv_max: the longest length to plan for (a longer one is still right).
  * kv_splits: parts the keys are split into, 0 chooses (at most 128); the order of the fp32
- * sums, and so the last bits, goes by it, by kv_max and by the lengths of the batch, but never
+ * sums, and so the last bits, goes by it, by kv_max and by the lengths of the live sequences, but never
  * from call to call.  out must not overlap an input.  The split states are library scratch. */
 int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const uint32_t* kc, const float* ksc,
                        const uint32_t* vc, const float* vsc, const int32_t* kv_len, const uint32_t* kd, const float* ksd,

@@ -111,7 +111,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const char* p, int bytes)
 // known here only.  A unit is a run of tiles of one sequence, for each KV head and row group a
 // workgroup: `fixed` units a sequence, or runs of one length, the shortest by which there are at most
 // `units` of them (at least B), no sequence has more than kTreeMaxSplits and none is shorter than a
-// step.  So a batch's longest sequence takes no longer than its share.
+// step.  So a batch's longest sequence takes no longer than its share.  An idle sequence has the draft
+// tile alone, whatever its length.
 struct Run {
     int b, split, splits, first, len, tiles;    // sequence, which of its units, their number, the first's, its cached keys and tiles
 };
@@ -125,8 +126,9 @@ __device__ __forceinline__ int ceil_div(int t, int q) {
 __device__ __forceinline__ Run run_of(const AttnTree& A, const TreePlan& P, int x) {
     const int lane = lane_id();
     auto len_of = [&](int b) __attribute__((always_inline)) {
-        const int len = b < A.B && A.kv_len ? A.kv_len[b] : 0;
-        return len < 0 ? 0 : len > A.kv_cap ? A.kv_cap : len;
+        if (b >= A.B || !A.kv_len) return 0;
+        const int len = A.kv_len[b];
+        return A.parent[(size_t)b * A.T] != -1 || len < 0 ? 0 : len > A.kv_cap ? A.kv_cap : len;
     };
     auto tiles_of = [&](int b, int len) __attribute__((always_inline)) { return b < A.B ? tiles_of_len(len) : 0; };
     if (A.B == 1) {                                            // (the same without the reductions)

@@ -8,7 +8,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from test_draft_verify import BG, D, G, dev, host
+from test_draft_verify import BG, D, G, attention_case, check_attention, dev, host, tree_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,26 @@ def test_outstanding_key(rt4, torch_gpu, n):
         tol = (8 * s * 1.4427 + 168 + tiles) * 2.0**-24 + 2.0**-22
         err = np.abs(host(out)[:, 0].astype(np.float64) / want[:, None] - 1)
         assert (err <= tol[:, None]).all(), (splits, err.max(), (err / tol[:, None]).max())
+
+
+@pytest.mark.parametrize("B,idle,cap", [(1, 1, 256), (3, 1, 32768), (4, 2, 16384), (70, 30, 2048)])
+def test_idle_sequences_take_no_share(rt4, torch_gpu, orc, B, idle, cap):
+    """Idle sequences' caches are not attended, however long: the others' bits do not depend on them, and their rows are zeros."""
+    print(f"case {idle} idle sequences of {B}", flush=True)
+    rng = np.random.default_rng(B)
+    T, H, ratio = 4, 1, 6
+    qq, qs, kv, draft = attention_case(orc, rng, B, T, H, ratio, cap, 2)
+    parent = np.tile([-1, 0, 1, 1], (B, 1))
+    parent[-idle:, 0] = -2
+    lens = np.array([cap - 3 * b % 200 for b in range(B)])
+    for x in (1, 3):
+        kv[x][-idle:], draft[x][-idle:] = np.nan, np.nan
+    args = [dev(qq), dev(qs), *map(dev, kv)], [*map(dev, draft), dev(parent)]
+    outs = []
+    for n in (cap, 0, 77):
+        lens[-idle:] = n
+        outs.append(rt4.attention_tree(*args[0], dev(lens), *args[1], ratio=ratio))
+    check_attention(outs[0], *tree_attention(qq, qs, kv, lens, draft, parent, ratio))
+    assert (host(outs[0])[:, (B - idle) * T:] == 0).all()
+    for o in outs[1:]:
+        assert np.array_equal(host(o).view(np.uint32), host(outs[0]).view(np.uint32))
