@@ -20,6 +20,8 @@
 //   16 sequences of 8 nodes over up to 16384 keys: 55 to 62 us in all, 150 MB at 2.6 TB/s with 26 GFLOP beside it
 //   61 nodes over 131001 keys: 270 to 283 us in all, 196 GFLOP at 0.7 PFLOP/s; P's two parts make them 294,
 //   which take 222 us at the rates of large int8 and fp16 products, the softmax beside them
+#include <algorithm>
+
 #include "rt4_dev.h"
 #include "rt4_internal.h"
 
@@ -619,7 +621,9 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
 // The rows per workgroup and the units by a model of the time in us: a step of two tiles takes 1.3, 2.2
 // or 3.0 (1 to 3 blocks) with one workgroup on a CU and 1.6, 2.5 or 3.3 with two, the joining launch 4
 // and its states (1 KB a row and unit, written and read) 0.35 a MB, all sequences as long as the longest.
-// A unit's row groups stay on one XCD (an eighth of the CUs), so the XCD with the most units decides.
+// A unit's row groups stay on one XCD (an eighth of the CUs), so the XCD with the most units decides; where
+// they are more workgroups than it takes at once, every XCD still has a unit, in whole rounds (64 nodes of
+// 64 heads over 1 KV head and 65536 keys 388 us; all on one XCD 3308, rounds counted in parts 433).
 // Over 241 sweeps of blocks and units, 1 to 16 sequences of 500 to 131000 keys and 1 to 64 nodes, the
 // choice by these figures takes 0.8% longer than the best on average and 12% at most where lengths are
 // alike (1.5% and 29% where they are drawn between 0 and the longest).
@@ -638,10 +642,12 @@ TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_spli
         if (nb > 1 && rg == (R + 16 * nb - 17) / (16 * nb - 16)) continue;      // no fewer groups than with fewer blocks
         for (int k = 0; k < 5; k++) {                          // a unit a sequence, or k / 2 workgroups a CU
             if (kv_splits && k != (kv_splits > 1)) continue;
-            long units = kv_splits ? (long)B * kv_splits : k ? k * xcd / 2 / rg * 8 / KVH : B;
+            // (one a XCD at least, where its row groups are more workgroups than the XCD takes at once)
+            long units = kv_splits ? (long)B * kv_splits : k ? std::max(1l, k * xcd / 2 / rg) * 8 / KVH : B;
             units = units < B ? B : kv_splits || units < (tiles + 1) / 2 * B ? units : (tiles + 1) / 2 * B;
             const long each = units / B, wgs = (units * KVH + 7) / 8 * rg, steps = ((tiles + each - 1) / each + 1) / 2;
-            const double run = steps * (wgs <= xcd ? one[nb - 1] : two[nb - 1] * fmax(1.0, wgs / (2.0 * xcd)));
+            const double rounds = fmax(1.0, wgs / (2.0 * xcd));
+            const double run = steps * (wgs <= xcd ? one[nb - 1] : two[nb - 1] * (k && !kv_splits ? ceil(rounds) : rounds));
             const double cost = run + (k == 0 ? 0 : 4 + 0.35e-3 * KVH * R * units);
             if (best == 0 || cost < best) best = cost, p = TreePlan{nb, rg, (int)units, kv_splits ? kv_splits : k == 0};
         }

@@ -5,12 +5,44 @@ records.
 """
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 
 from test_draft_verify import BG, D, G, attention_case, check_attention, dev, host, tree_attention
 
 pytestmark = pytest.mark.gpu
+
+
+class _KernelNode(ctypes.Structure):                    # hipKernelNodeParams
+    _fields_ = [("block", ctypes.c_uint32 * 3), ("extra", ctypes.c_void_p), ("func", ctypes.c_void_p), ("grid", ctypes.c_uint32 * 3),
+                ("params", ctypes.c_void_p), ("shared", ctypes.c_uint32)]
+
+
+def recorded(torch, fn):
+    """Grids (workgroups) of the launches that fn() makes, in order, from a capture that is not run."""
+    path = next(ln.split()[-1] for ln in open("/proc/self/maps") if "libamdhip64" in ln)
+    hip = ctypes.CDLL(path)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph, n = ctypes.c_void_p(), ctypes.c_size_t()
+    with torch.cuda.stream(stream):
+        assert hip.hipStreamBeginCapture(ctypes.c_void_p(stream.cuda_stream), 2) == 0
+        try:
+            fn()
+        finally:
+            assert hip.hipStreamEndCapture(ctypes.c_void_p(stream.cuda_stream), ctypes.byref(graph)) == 0
+    assert hip.hipGraphGetNodes(graph, None, ctypes.byref(n)) == 0
+    nodes = (ctypes.c_void_p * n.value)()
+    assert hip.hipGraphGetNodes(graph, nodes, ctypes.byref(n)) == 0
+    grids = []
+    for node in nodes:
+        p = _KernelNode()
+        assert hip.hipGraphKernelNodeGetParams(ctypes.c_void_p(node), ctypes.byref(p)) == 0
+        grids.append(tuple(p.grid))
+    assert hip.hipGraphDestroy(graph) == 0
+    return grids
 
 
 # ---------------------------------------------------------------- attention --
@@ -69,3 +101,35 @@ def test_idle_sequences_take_no_share(rt4, torch_gpu, orc, B, idle, cap):
     assert (host(outs[0])[:, (B - idle) * T:] == 0).all()
     for o in outs[1:]:
         assert np.array_equal(host(o).view(np.uint32), host(outs[0]).view(np.uint32))
+
+
+def blank_attention(torch, B, T, H, ratio, cap):
+    """Arguments of a call on zeros: (positional, keywords)."""
+    i = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    f = lambda *s: torch.zeros(s, device="cuda")  # noqa: E731
+    cache = lambda n: (i(B, H, n, D // 8), f(B, H, 2, n), i(B, H, n // 8, D), f(B, H, n // BG, D))  # noqa: E731
+    parent = i(B, T)
+    parent[:, 0] = -1
+    args = (i(H * ratio, B * T, D // 8), f(H * ratio, 2, B * T), *cache(cap), torch.full((B,), cap, dtype=torch.int32, device="cuda"),
+            *cache(BG), parent)
+    return args, dict(ratio=ratio, out=f(H * ratio, B * T, D))
+
+
+def test_more_row_groups_than_an_xcd_takes(rt4, torch_gpu):
+    """Many rows of one KV head are split over the XCDs too (the groups of one unit stay on one), and come out right."""
+    torch = torch_gpu
+    print("case 64 nodes of 64 heads over one KV head", flush=True)
+    B, T, H, ratio, cap = 1, 64, 1, 64, 8192
+    args, kw = blank_attention(torch, B, T, H, ratio, cap)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for x in (args[0], args[2], args[4], args[7], args[9]):
+        x.random_(-2**31, 2**31 - 1, generator=g)
+    for x in (args[1], args[3], args[5], args[8], args[10]):
+        x.uniform_(0.01, 0.02, generator=g)
+    out = rt4.attention_tree(*args, **kw).clone()
+    one = rt4.attention_tree(*args, **{**kw, "kv_splits": 1})
+    grids = recorded(torch, lambda: rt4.attention_tree(*args, **kw))
+    assert len(grids) == 2 and grids[0][0] >= 8 * T * ratio // 48, grids      # split, and joined by a second launch
+    # two orders of the same sums: S below 2 x 128 x 64 x 0.02^2 x 1.45 = 9.5, values below 8 x 0.02
+    tol = 2 * 8 * 0.02 * ((8 * 9.5 + 168 + cap / BG) * 2.0**-24 + 2.0**-22)
+    assert float((out - one).abs().max()) <= tol
