@@ -644,7 +644,8 @@ TreePlan tree_plan(int B, int T, int n_heads, int ratio, int kv_max, int kv_spli
             if (kv_splits && k != (kv_splits > 1)) continue;
             // (one a XCD at least, where its row groups are more workgroups than the XCD takes at once)
             long units = kv_splits ? (long)B * kv_splits : k ? std::max(1l, k * xcd / 2 / rg) * 8 / KVH : B;
-            units = units < B ? B : kv_splits || units < (tiles + 1) / 2 * B ? units : (tiles + 1) / 2 * B;
+            const long most = std::min((tiles + 1) / 2, (long)kTreeMaxSplits) * B;     // (run_of has no more)
+            units = units < B ? B : kv_splits || units < most ? units : most;
             const long each = units / B, wgs = (units * KVH + 7) / 8 * rg, steps = ((tiles + each - 1) / each + 1) / 2;
             const double rounds = fmax(1.0, wgs / (2.0 * xcd));
             const double run = steps * (wgs <= xcd ? one[nb - 1] : two[nb - 1] * (k && !kv_splits ? ceil(rounds) : rounds));

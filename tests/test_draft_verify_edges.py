@@ -133,3 +133,14 @@ def test_more_row_groups_than_an_xcd_takes(rt4, torch_gpu):
     # two orders of the same sums: S below 2 x 128 x 64 x 0.02^2 x 1.45 = 9.5, values below 8 x 0.02
     tol = 2 * 8 * 0.02 * ((8 * 9.5 + 168 + cap / BG) * 2.0**-24 + 2.0**-22)
     assert float((out - one).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("B,T,ratio", [(1, 1, 6), (1, 16, 8), (2, 1, 8)])
+def test_plan_has_no_more_units_than_there_are(rt4, torch_gpu, B, T, ratio):
+    """A sequence has at most 128 units, and no more are planned: few heads over a long cache launch nothing that ends at once."""
+    torch = torch_gpu
+    print(f"case one KV head, long cache, B={B} T={T}", flush=True)
+    args, kw = blank_attention(torch, B, T, 1, ratio, 131072)
+    rt4.attention_tree(*args, **kw)
+    grids = recorded(torch, lambda: rt4.attention_tree(*args, **kw))
+    assert len(grids) == 2 and grids[0][0] <= 128 * B * -(-T * ratio // 16), grids
