@@ -847,10 +847,16 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
     if (rc) return rc;
     hipStream_t st = as_stream(stream);
     rt4::TreePlan plan = rt4::tree_plan(B, T, n_heads, ratio, kv_len ? kv_max : 0, kv_splits, cus);
-    // under capture, as many units as the workspace that is there holds, at worst one a sequence
+    // under capture, as many units as the workspace that is there holds, at worst one a sequence, which needs none
     if (!kv_splits && plan.fixed != 1 && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan)) && capturing(st)) {
-        while (plan.units > B && !scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan))) plan.units = plan.units > 2 * B ? plan.units / 2 : B;
-        if (!scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan))) plan.fixed = 1;
+        int fit = B, most = plan.units;
+        while (fit < most) {
+            plan.units = fit + (most - fit + 1) / 2;
+            if (scratch_has(kSlotTreePart, rt4::tree_part_bytes(a, plan))) fit = plan.units;
+            else most = plan.units - 1;
+        }
+        plan.units = fit;
+        if (fit == B) plan.fixed = 1;
     }
     void* ws = nullptr;
     if (plan.fixed != 1 && (rc = lib_scratch(kSlotTreePart, rt4::tree_part_bytes(a, plan), &ws, st))) return rc;

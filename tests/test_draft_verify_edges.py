@@ -6,10 +6,13 @@ records.
 from __future__ import annotations
 
 import ctypes
+import subprocess
+import sys
 
 import numpy as np
 import pytest
 
+from conftest import PKG_DIR, ROOT
 from test_draft_verify import BG, D, G, attention_case, check_attention, dev, host, tree_attention
 
 pytestmark = pytest.mark.gpu
@@ -144,3 +147,37 @@ def test_plan_has_no_more_units_than_there_are(rt4, torch_gpu, B, T, ratio):
     rt4.attention_tree(*args, **kw)
     grids = recorded(torch, lambda: rt4.attention_tree(*args, **kw))
     assert len(grids) == 2 and grids[0][0] <= 128 * B * -(-T * ratio // 16), grids
+
+
+def in_a_fresh_process(script):
+    """Runs a script that prints OK where it succeeds, with this folder and the package at hand."""
+    head = f"import sys\nsys.path[:0] = [{str(ROOT)!r}, {str(PKG_DIR)!r}, {str(ROOT / 'tests')!r}]\n"
+    r = subprocess.run([sys.executable, "-u", "-c", head + script], capture_output=True, text=True, timeout=100)
+    print(r.stdout[-3000:], r.stderr[-3000:])
+    assert r.returncode == 0 and r.stdout.rstrip().endswith("OK")
+
+
+SPLITS_THAT_FIT = r"""
+import torch
+import rt4_amd
+from test_draft_verify_edges import blank_attention, recorded
+args, kw = blank_attention(torch, 1, 1, 1, 6, 131072)
+call = lambda **k: rt4_amd.attention_tree(*args, **kw, **k)
+assert len(recorded(torch, call)) == 1                    # no workspace: one unit
+for n in (3, 50, 100):
+    call(kv_splits=n)                                     # (scratch grows by a half at least: 3, 50 and 100 units)
+    grids = recorded(torch, call)
+    print(n, grids, flush=True)
+    assert len(grids) == 2 and grids[0][0] == (n + 7) // 8 * 8, grids
+call()
+full = recorded(torch, call)
+print(full, flush=True)
+assert grids[0][0] < full[0][0] <= 128
+print("OK", flush=True)
+"""
+
+
+def test_capture_takes_the_splits_that_fit(torch_gpu):
+    """Under capture the attention takes as many units as the workspace of earlier calls holds."""
+    print("case splits that fit", flush=True)
+    in_a_fresh_process(SPLITS_THAT_FIT)
