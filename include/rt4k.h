@@ -360,8 +360,9 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
  * numbers; tokens int32 [B][T] the n new tokens (n-1 accepted drafts, then the last token);
  * the rest of both is -1.  kv_len (optional): kv_len[b] += n, as rt4_kv_append_rows takes
  * it.  Decisions are made in 64 bits.  T <= 64, V <= 4194304, B*T <= 65535; outputs must not
- * overlap inputs or each other.  The rows' statistics are library scratch (none where a
- * sequence's rows are few logits). */
+ * overlap inputs or each other.  The rows' statistics are library scratch, which sequences
+ * whose rows are few logits do without (up to 32768 in one row): those verify in one launch, and
+ * a captured call of more than 20480 in two where the scratch is there; same results. */
 int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_len, const float* logits, int64_t ldl,
                     const int32_t* draft, const int32_t* parent, const float* u, const float* temp, const float* draft_p,
                     int64_t ldp, int B, int T, int V, int max_children, void* stream);

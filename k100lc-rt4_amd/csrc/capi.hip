@@ -879,10 +879,15 @@ int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_
     const int most = T > 1 ? T - 1 : 1, levels = !draft_p ? 1 : max_children < most ? max_children : most;
     hipStream_t st = as_stream(stream);
     void *ws = nullptr, *cnt = nullptr;
-    const size_t bytes = rt4::verify_ws_bytes(B, T, V, levels, draft_p != nullptr);
-    int rc = RT4_OK;
-    if (bytes && (rc = lib_scratch(kSlotVerify, bytes, &ws, st))) return rc;
-    if (bytes && draft_p && (rc = lib_scratch(kSlotVerifyCnt, (size_t)B * sizeof(int), &cnt, st, true))) return rc;
+    const rt4::OneLaunch one = rt4::verify_one_launch(T, V, levels, draft_p != nullptr);
+    const size_t bytes = rt4::verify_ws_bytes(B, T, V, levels), counters = draft_p ? (size_t)B * sizeof(int) : 0;
+    const bool eager = one == rt4::kEager && !capturing(st);
+    if (one == rt4::kNever || eager || (one == rt4::kEager && scratch_has(kSlotVerify, bytes) && scratch_has(kSlotVerifyCnt, counters))) {
+        int rc = lib_scratch(kSlotVerify, bytes, &ws, st);
+        if (!rc && counters) rc = lib_scratch(kSlotVerifyCnt, counters, &cnt, st, true);
+        if (rc) return rc;
+    }
+    if (eager) ws = nullptr;             // (it only sizes the scratch, for a capture of the same call)
     return hip_status(rt4::launch_verify_tree(tokens, path, count, kv_len, logits, (size_t)ldl, draft, parent, u, temp, draft_p,
                                               (size_t)ldp, B, T, V, levels, ws, static_cast<int*>(cnt), st),
                       "rt4_verify_tree launch");

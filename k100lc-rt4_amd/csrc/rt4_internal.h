@@ -176,10 +176,13 @@ size_t tree_part_bytes(const AttnTree& a, const TreePlan& p);
 hipError_t launch_attn_tree(const AttnTree& a, const TreePlan& p, void* ws, hipStream_t st);
 
 // Draft verification; `levels`: children tested per node where draft probabilities q are
-// given (else 1); ws: verify_ws_bytes of scratch (0 where one launch does without); cnt: B
-// counters that are 0 (with draft probabilities, unless ws needs nothing).
+// given (else 1); ws: verify_ws_bytes of scratch, null for the one-launch form, which does without
+// (verify_one_launch: where it is right and the faster one); cnt: B counters that are 0 (with draft
+// probabilities and ws).
 constexpr int kVerifyChunk = 4096, kVerifyMaxV = 1 << 22;
-size_t verify_ws_bytes(int B, int T, int V, int levels, bool q);
+enum OneLaunch { kNever, kEager, kAlways };     // kEager: in eager calls, in a captured one where ws is not there
+OneLaunch verify_one_launch(int T, int V, int levels, bool q);
+size_t verify_ws_bytes(int B, int T, int V, int levels);
 hipError_t launch_verify_tree(int* tokens, int* path, int* count, int* kv_len, const float* logits, size_t ldl, const int* draft,
                               const int* parent, const float* u, const float* temp, const float* q, size_t ldq, int B, int T, int V,
                               int levels, void* ws, int* cnt, hipStream_t st);

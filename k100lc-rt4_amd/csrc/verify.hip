@@ -592,11 +592,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_k(const Verify A) {
 }
 
 // The whole verification in one launch, a workgroup a sequence, where its rows are few pieces of 1024 logits
-// (a wave each) and no residual levels are needed.  It saves the host's 3 us for a launch, and where one CU's
-// 64-bit rate does not bound it, time on the device: one row of 1000 logits 16.7 -> 13.6 us eagerly, 11.1 ->
-// 9.2 in a graph; of 24000 16.5 -> 13.2 and 11.8 -> 11.8; of 32000 16.6 -> 13.2 and 11.6 -> 13.6; 4 rows of
-// 4000 with draft probabilities 20.9 -> 14.6 and 15.2 -> 12.9.  Beyond: 32 rows of 1000 16.5 -> 17.4 and
-// 13.0 -> 18.2, a row of 32000 with draft probabilities 20.4 -> 20.7 and 15.2 -> 21.5.
+// (a wave each) and no residual levels are needed; verify_one_launch says where.
 // grid B, 1024 threads; A.C: pieces in a row.
 constexpr int SP = 1024, kSmallPieces = 32;
 __global__ __launch_bounds__(1024) void verify_small_k(const Verify A) {
@@ -674,14 +670,21 @@ size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
 
 }  // namespace
 
-// Whether verify_small_k takes it.
-static bool small(int T, int V, int levels, bool q) {
+// Whether verify_small_k takes it, by the faster of the two in a call as it is made: eager calls are bound by
+// the host, whose 3 us for a launch it saves, captured ones by the device, where one CU's 64-bit rate counts.
+// Eagerly it gains as far as 32 pieces go: one row of 32768 logits 16.3 -> 13.0 us, 7 pieces for each of 4 rows
+// 16.1 -> 13.0, a row of 20480 with draft probabilities 16.9 -> 15.0 (32 rows of 1000 16.5 -> 17.4).
+// In a graph it gains up to about 20 pieces, or 24 with draft probabilities, whose residual counts as a row more:
+// one row of 19 pieces 10.4 -> 10.1 us, of 20 9.7 -> 10.0, of 24 9.8 -> 10.8, of 32 9.8 -> 12.5; 16 x 2 rows of
+// 10 11.1 -> 10.7, of 12 10.5 -> 11.3; 4 rows of 5 10.4 -> 10.5, of 6 10.8 -> 11.2; with draft probabilities one
+// row of 12 12.5 -> 11.9, of 13 12.6 -> 13.4, 2 rows of 8 12.1 -> 11.9, of 9 12.6 -> 13.2, 6 of 3 13.0 -> 12.0.
+OneLaunch verify_one_launch(int T, int V, int levels, bool q) {
     const int pieces = (V + SP - 1) / SP;
-    return levels == 1 && (q ? 3 : 2) * T * pieces + 2 * T <= 2 * kSmallPieces + 2;
+    if (levels != 1 || (q ? 3 : 2) * T * pieces + 2 * T > 2 * kSmallPieces + 2) return kNever;
+    return (q ? (T + 1) * pieces <= 24 : T * pieces <= 20) ? kAlways : kEager;
 }
 
-size_t verify_ws_bytes(int B, int T, int V, int levels, bool q) {
-    if (small(T, V, levels, q)) return 0;
+size_t verify_ws_bytes(int B, int T, int V, int levels) {
     const size_t R = (size_t)B * T, C = (V + CH - 1) / CH;
     return up16(R * C * sizeof(RowStat)) + up16(R * levels * 8) + up16(R * C * levels * 8) + up16(B * C * 8);
 }
@@ -697,7 +700,7 @@ hipError_t launch_verify_tree(int* tokens, int* path, int* count, int* kv_len, c
     double* part = reinterpret_cast<double*>(take((size_t)R * C * levels * 8));
     double* sums = reinterpret_cast<double*>(take((size_t)B * C * 8));
     const Verify a = {tokens, path, count, kv_len, logits, ldl, draft, parent, u, temp, q, ldq, ch, av, part, sums, cnt, B, T, V, C, levels};
-    if (small(T, V, levels, q != nullptr)) {
+    if (!ws) {
         Verify one = a;
         one.C = (V + SP - 1) / SP;
         hipLaunchKernelGGL(verify_small_k, dim3(B), dim3(1024), 0, st, one);

@@ -181,3 +181,57 @@ def test_capture_takes_the_splits_that_fit(torch_gpu):
     """Under capture the attention takes as many units as the workspace of earlier calls holds."""
     print("case splits that fit", flush=True)
     in_a_fresh_process(SPLITS_THAT_FIT)
+
+
+# ------------------------------------------------------------- verification --
+ONE_LAUNCH = r"""
+import torch
+import rt4_amd
+from test_draft_verify_edges import recorded
+g = torch.Generator(device="cuda").manual_seed(3)
+
+def case(B, T, V, probs):
+    i = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+    logits = 2.5 * torch.randn((B * T, V), device="cuda", generator=g)
+    q = torch.softmax(logits + 0.5 * torch.randn((B * T, V), device="cuda", generator=g), -1) if probs else None
+    draft = torch.zeros((B, T), dtype=torch.int32, device="cuda")
+    draft[:, 1:] = logits.view(B, T, V)[:, :-1].argmax(-1).int()
+    parent = torch.arange(-1, T - 1, dtype=torch.int32, device="cuda").repeat(B, 1)
+    u = torch.rand((B, T), device="cuda", generator=g)
+    outs = (i(B, T), i(B, T), i(B))
+    return outs, lambda: rt4_amd.verify_tree(logits, draft, parent, u, draft_probs=q, max_children=1 if probs else None,
+                                             tokens=outs[0], path=outs[1], count=outs[2])
+
+CASES = ((1, 1, 16000, 0, 1), (1, 1, 24000, 0, 2), (1, 1, 32768, 0, 2), (3, 4, 4096, 0, 1), (3, 4, 7000, 0, 2), (2, 1, 12000, 1, 1),
+         (2, 1, 16000, 1, 2), (2, 2, 10000, 1, 2), (2, 1, 40000, 0, 2), (2, 4, 8000, 1, 2))    # .., launches of a captured call
+made = [case(*c[:4]) for c in CASES]
+for c, (outs, call) in zip(CASES[:8], made):              # no scratch: one launch in any case
+    print(c, recorded(torch, call), flush=True)
+    assert len(recorded(torch, call)) == 1
+for c, (outs, call) in zip(CASES, made):
+    call()                                                # sizes the scratch, whichever form it takes itself
+    w = [x.clone() for x in outs]
+    n = len(recorded(torch, call))
+    print(c, n, flush=True)
+    assert n == c[4]
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        call()
+    for rep in range(3):
+        for x in outs:
+            x.fill_(9)
+        made[-1][1]()                                     # the program's own eager work between the replays
+        torch.cuda.synchronize()
+        for x in outs:
+            x.fill_(9)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, w))
+print("OK", flush=True)
+"""
+
+
+def test_verify_in_one_launch_where_it_is_faster(torch_gpu):
+    """A captured call takes the form that is faster on the device where its scratch is there, with equal tokens."""
+    print("case one launch or two", flush=True)
+    in_a_fresh_process(ONE_LAUNCH)
