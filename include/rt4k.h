@@ -353,8 +353,8 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
  * nothing is left, which only distributions that do not sum to 1 come to).  So the tokens
  * are distributed as the target's own.  temp NULL: 1; temp[b] <= 0 (or NaN): greedy, a child
  * is accepted iff it is the row's largest logit (lowest index among equals), and so is the
- * last token; temp[b] infinite: every logit that is not -inf weighs the same.
- * A NaN logit counts as -inf; a row of nothing but -inf ends the walk with token -1.
+ * last token; temp[b] infinite: every logit that is not -inf weighs the same (at any other
+ * temperature logits of +inf weigh the same and leave the rest nothing).  A NaN logit counts as -inf; a row of nothing but -inf ends the walk with token -1.
  * A draft token outside [0, V) is rejected.
  * Outputs: count[b] = n accepted nodes, the root included (0: idle); path int32 [B][T] their
  * numbers; tokens int32 [B][T] the n new tokens (n-1 accepted drafts, then the last token);

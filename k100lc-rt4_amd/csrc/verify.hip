@@ -61,16 +61,20 @@ __device__ __forceinline__ double weight_finite(float l, float m, double it) {
     q = fma(q, f, 0.69314718055994617);
     return __builtin_ldexp(fma(q, f, 1.0), __double2loint(t));
 }
-// The same for any m: where that is +inf, 1 for the logits that are.
+// Where m is +inf, the logits above this weigh the same and the rest nothing: those that are +inf, at an
+// infinite temperature all but -inf.
+__device__ __forceinline__ float weightless(double it) { return it == 0.0 ? -INFINITY : 3.402823466e38f; }
+// The same as weight_finite for any m.
 __device__ __forceinline__ double weight(float l, float m, double it) {
-    return m == INFINITY ? (l == m ? 1.0 : 0.0) : weight_finite(l, m, it);
+    return m == INFINITY ? (l > weightless(it) ? 1.0 : 0.0) : weight_finite(l, m, it);
 }
 // Logits of a row whose largest is m, made such that weight_finite(l, m) is right.
 template <int N>
-__device__ __forceinline__ void make_finite(float (&l)[N], float& m) {
+__device__ __forceinline__ void make_finite(float (&l)[N], float& m, double it) {
     if (m < INFINITY) return;
+    const float none = weightless(it);
 #pragma unroll
-    for (int e = 0; e < N; e++) l[e] = l[e] == m ? 0.f : -INFINITY;
+    for (int e = 0; e < N; e++) l[e] = l[e] > none ? 0.f : -INFINITY;
     m = 0.f;
 }
 
@@ -174,7 +178,7 @@ __device__ __forceinline__ RowStat stat16(float (&v)[PT], int at, float m, doubl
         if (v[e] == m && m > -INFINITY) r.i = at + STRIDE * (e / 4) + e % 4;
     if (it >= 0) {
         float mf = m;
-        make_finite(v, mf);
+        make_finite(v, mf, it);
 #pragma unroll
         for (int e = 0; e < PT; e++) r.s += weight_finite(v[e], mf, it);
     }
@@ -239,7 +243,7 @@ __global__ __launch_bounds__(256) void verify_mass_k(const float* __restrict__ l
     const RowStat r = row_of_chunks(ch + (size_t)row * C, C, it);
     const double is = r.s > 0 ? 1.0 / r.s : 0.0;
     float mf = r.m;
-    make_finite(l, mf);
+    make_finite(l, mf, it);
     double s = 0;
 #pragma unroll
     for (int e = 0; e < PT; e++) s += fmax(weight_finite(l[e], mf, it) * is - a * (double)pq[e], 0.0);
@@ -383,7 +387,7 @@ __device__ __forceinline__ double residuals(double (&w)[4], const Verify& A, con
         }
     }
     float mf = d.r.m;
-    make_finite(lv.f, mf);
+    make_finite(lv.f, mf, it);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         w[e] = weight_finite(lv.f[e], mf, it);

@@ -13,7 +13,7 @@ import numpy as np
 import pytest
 
 from conftest import PKG_DIR, ROOT
-from test_draft_verify import BG, D, G, attention_case, check_attention, dev, host, tree_attention
+from test_draft_verify import BG, D, G, attention_case, check_attention, check_verify, dev, host, tree_attention, verify, verify_case
 
 pytestmark = pytest.mark.gpu
 
@@ -235,3 +235,34 @@ def test_verify_in_one_launch_where_it_is_faster(torch_gpu):
     """A captured call takes the form that is faster on the device where its scratch is there, with equal tokens."""
     print("case one launch or two", flush=True)
     in_a_fresh_process(ONE_LAUNCH)
+
+
+@pytest.mark.parametrize("V", [3000, 70001])
+@pytest.mark.parametrize("probs", [False, True])
+def test_infinite_logits_at_an_infinite_temperature(rt4, torch_gpu, probs, V):
+    """Every logit that is not -inf or NaN weighs the same, +inf ones too."""
+    print(f"case infinite logits, infinite temperature, V={V} probs={probs}", flush=True)
+    rng = np.random.default_rng(13)
+    B, T = 8, 4
+    logits = rng.standard_normal((B * T, V)).astype(np.float32)
+    logits[:, ::3] = -np.inf
+    logits[:, 1::9] = np.nan
+    logits[::2, 200:240] = np.inf                       # (among finite ones)
+    parent = np.tile([-1, 0, 0, 1], (B, 1))
+    draft = rng.choice(np.flatnonzero(np.arange(V) % 9 == 2), (B, T))
+    left = np.count_nonzero(logits[0] > -np.inf)
+    # uniforms between the multiples of 1 / left, so that no sum's rounding decides
+    u = ((rng.integers(0, left - 2, (B, T)) + 0.5) / left).astype(np.float32)
+    u[::2, 1:] = 0.25 / left
+    q = None
+    if probs:
+        q = rng.random((B * T, V)).astype(np.float32)
+        q /= q.sum(1, keepdims=True)
+        q[np.arange(B) * T, draft[:, 1]] = 0.5
+    temp = np.full(B, np.inf, np.float32)
+    # (the walk in 64 bits divides by the temperature, so it takes the weights' logarithms at temperature 1)
+    want = verify(np.where(logits > -np.inf, np.float32(0), np.float32(-np.inf)), draft, parent, u, np.ones(B), q, 2 if probs else None)
+    got = rt4.verify_tree(dev(logits), dev(draft), dev(parent), dev(u), temp=dev(temp), draft_probs=None if q is None else dev(q),
+                          max_children=2 if probs else None)
+    for g, w in zip(got, want):
+        assert np.array_equal(host(g), w)
