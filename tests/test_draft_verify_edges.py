@@ -266,3 +266,120 @@ def test_infinite_logits_at_an_infinite_temperature(rt4, torch_gpu, probs, V):
                           max_children=2 if probs else None)
     for g, w in zip(got, want):
         assert np.array_equal(host(g), w)
+
+
+@pytest.mark.parametrize("temp", [1e-3, 1e-30, 1.0])
+def test_siblings_with_draft_probabilities_on_odd_rows(rt4, torch_gpu, temp):
+    """Equal mass on few tokens and what a cold temperature leaves of the others: three siblings tested against residuals."""
+    print(f"case odd rows, siblings, temp={temp}", flush=True)
+    rng = np.random.default_rng(17)
+    T, V = 6, 9000
+    parent = np.array([[-1, 0, 0, 0, 1, 2]] * 6)
+    B = len(parent)
+    logits = rng.standard_normal((B, T, V)).astype(np.float32)
+    draft = rng.integers(0, V, (B, T))
+    logits[0, :, 100:] = -np.inf                        # few tokens left
+    draft[0] = [0, 5, 200, 7, 3, 4]
+    logits[1, :, 7] = np.nan
+    logits[1, :, 8] = logits[1, :, 4500] = np.inf       # all the mass on two
+    draft[1] = [0, 7, 8, 4500, 8, 8]
+    logits[2, :, 3000:3010] = 50.0                      # ties of the largest
+    draft[2] = [0, 3001, 3000, 3002, 3000, 3000]
+    draft[3] = [0, 77, 77, 77, 1, 1]                    # the same token three times
+    logits[3, 0, 77] = 9.0
+    logits[4] = np.finfo(np.float32).min                # the type's lowest value, over a whole row and in part
+    logits[4, 0, 10:20] = 1.0
+    draft[4] = [0, 12, 13, 14, 12, 12]
+    logits[5, :, ::2] = -np.inf
+    flat = logits.reshape(B * T, V)
+    q = np.full((B * T, V), 1.0 / V, np.float32)
+    for rep in range(6):
+        check_verify(rt4, flat, draft, parent, rng.random((B, T)).astype(np.float32), [temp] * B, q, 3)
+
+
+@pytest.mark.parametrize("B,T,V,kids", [(1, 4, 300000, 3), (2, 5, 270001, 4), (1, 7, 1 << 19, 2)])
+def test_siblings_with_draft_probabilities_on_long_rows(rt4, torch_gpu, B, T, V, kids):
+    """Residual levels of rows of more chunks than a wave has lanes."""
+    print(f"case long rows, siblings, B={B} T={T} V={V}", flush=True)
+    rng = np.random.default_rng(V)
+    logits, draft, _, u, q = verify_case(rng, B, T, V, kids, True)
+    parent = np.array([[-1] + [0] * kids + [1] * (T - 1 - kids)] * B)
+    u[:, 1:] = 0.5 + u[:, 1:] / 2                       # (rejections are what residuals are for)
+    for temp in (1.0, 0.7):
+        check_verify(rt4, logits, draft, parent, u, [temp] * B, q, kids)
+
+
+CAPTURED_RESIDUALS = r"""
+import numpy as np
+import torch
+import rt4_amd
+from test_draft_verify import dev, verify, verify_case
+
+def case(seed, B, T, V, probs):
+    rng = np.random.default_rng(seed)
+    logits, draft, _, u, q = verify_case(rng, B, T, V, 2, True)
+    parent = np.array([[-1, 0, 0] + [1] * (T - 3)] * B)
+    q = q if probs else None
+    want = verify(logits, draft, parent, u, np.ones(B), q, 2 if probs else None)
+    ins = [dev(x) for x in (logits, draft, parent, u)]
+    qd = dev(q) if probs else None
+    outs = [torch.zeros(s, dtype=torch.int32, device="cuda") for s in ((B, T), (B, T), (B,))]
+    def call():
+        rt4_amd.verify_tree(*ins, draft_probs=qd, max_children=2 if probs else None, tokens=outs[0], path=outs[1], count=outs[2])
+    def check(what):
+        torch.cuda.synchronize()
+        for x, w in zip(outs, want):
+            assert np.array_equal(x.cpu().numpy(), w), what
+        for x in outs:
+            x.fill_(9)
+        torch.cuda.synchronize()
+    return call, check
+
+def capture(fn):
+    gr, err = torch.cuda.CUDAGraph(), None
+    with torch.cuda.graph(gr):
+        try:
+            fn()
+        except rt4_amd.RT4Error as e:
+            err = str(e)
+    return gr, err
+
+call, check = case(1, 3, 5, 20000, True)
+plain, check_plain = case(2, 8, 12, 20000, False)
+more, check_more = case(3, 20, 4, 9000, True)
+many, check_many = case(4, 200, 3, 9000, True)
+_, err = capture(call)
+assert err is not None and "captur" in err, err
+plain()                                                   # the statistics' scratch is there, the counters are not
+check_plain("first eager call")
+_, err = capture(call)
+print("without counters:", err, flush=True)
+assert err is not None and "captur" in err, err
+call()
+check("eager")
+gr, err = capture(call)
+assert err is None, err
+for rep in range(4):
+    gr.replay()
+    check(("replay", rep))
+    call()
+    check(("eager between", rep))
+    (more, many)[rep % 2]()                               # 20, then 200 counters: the graph keeps those that it was captured with
+    (check_more, check_many)[rep % 2](("more sequences", rep))
+    plain()
+    check_plain(("chosen tokens", rep))
+g2, err = capture(many)
+assert err is None, err
+for rep in range(3):
+    g2.replay()
+    gr.replay()
+    check_many(("replay", rep))
+    check(("both graphs", rep))
+print("OK", flush=True)
+"""
+
+
+def test_captured_residuals(torch_gpu):
+    """The workgroup that draws is the last to count itself in: its counters under capture, between eager calls and grown."""
+    print("case captured residuals", flush=True)
+    in_a_fresh_process(CAPTURED_RESIDUALS)
