@@ -306,6 +306,10 @@ int rt4_attention_launch_plan(int n_q, int n_heads, int ratio, int off, int n_ti
  * attends (rt4_attention_tree), verifies the logits (rt4_verify_tree, which also advances
  * the lengths) and appends the accepted rows (rt4_kv_append_rows).  Lengths, paths and
  * counts stay on the device, so a step has no host synchronisation and can be captured.
+ * A live sequence needs kv_len[b] + T <= kv_cap before its verification, which advances the
+ * length without knowing the cache: an append that would pass kv_cap is left out whole, and the
+ * next attention would take the kv_cap keys that are there, some never written.  One without that
+ * room is made idle (the parent of its node 0) until it has another cache.
  * No counterparts in the reference, which decodes one sequence, compares argmaxes on the
  * host and restores V tiles (src/model.cpp:1428-1460, :1838-1926). */
 

@@ -13,7 +13,8 @@ import numpy as np
 import pytest
 
 from conftest import PKG_DIR, ROOT
-from test_draft_verify import BG, D, G, attention_case, check_attention, check_verify, dev, host, tree_attention, verify, verify_case
+from test_draft_verify import (BG, D, append_expected, attention_case, check_attention, check_verify, dev, host, random_tree,
+                               tree_attention, verify, verify_case)
 
 pytestmark = pytest.mark.gpu
 
@@ -383,3 +384,52 @@ def test_captured_residuals(torch_gpu):
     """The workgroup that draws is the last to count itself in: its counters under capture, between eager calls and grown."""
     print("case captured residuals", flush=True)
     in_a_fresh_process(CAPTURED_RESIDUALS)
+
+
+# ------------------------------------------------------------ as one would use them --
+def test_sequences_retired_at_the_cache_end(rt4, torch_gpu, orc):
+    """A sequence without room for a whole path is made idle on the device: nothing is lost, nothing passes the cache's end."""
+    torch = torch_gpu
+    print("case cache end", flush=True)
+    rng = np.random.default_rng(19)
+    B, T, H, ratio, cap, V = 3, 6, 1, 2, 128, 500
+    kv = [torch.zeros((B, H, cap, D // 8), dtype=torch.int32, device="cuda"), torch.zeros((B, H, 2, cap), device="cuda"),
+          torch.zeros((B, H, cap // 8, D), dtype=torch.int32, device="cuda"), torch.zeros((B, H, cap // BG, D), device="cuda")]
+    want = [np.ascontiguousarray(host(x)).view(np.uint32) if x.dtype == torch.int32 else host(x).copy() for x in kv]
+    draft = [torch.zeros((B, H, BG, D // 8), dtype=torch.int32, device="cuda"), torch.zeros((B, H, 2, BG), device="cuda"),
+             torch.zeros((B, H, 8, D), dtype=torch.int32, device="cuda"), torch.zeros((B, H, 1, D), device="cuda")]
+    stage, wstage = torch.zeros((B, H, BG, D), device="cuda"), np.zeros((B, H, BG, D), np.float32)
+    length = np.array([100, 40, 126])
+    kv_len = dev(length)
+    kf, vf = (rng.standard_normal((B, cap, H, D)).astype(np.float32) for _ in range(2))
+    rt4.kv_append_rows(*kv, stage, dev(kf), dev(vf), kv_len=kv_len, count=kv_len)
+    append_expected(orc, want, wstage, kf, vf, np.zeros(B, int), np.tile(np.arange(cap), (B, 1)), length)
+    retired = np.zeros(B, int)
+    for step in range(60):
+        kf, vf = (rng.standard_normal((B, T, H, D)).astype(np.float32) for _ in range(2))
+        q = rng.standard_normal((B * T, H * ratio, D)).astype(np.float32) / 8
+        tree = np.array([random_tree(rng, T, 2) for _ in range(B)])
+        tok = rng.integers(0, 8, (B, T))
+        logits = rng.standard_normal((B * T, V)).astype(np.float32)
+        logits[:, :8] += 5
+        u = (rng.random((B, T)) * 0.3).astype(np.float32)
+        idle = length + T > cap
+        parent = dev(tree)
+        parent[:, 0] = torch.where(kv_len + T > cap, -2, parent[:, 0])
+        rt4.kv_append_rows(*draft, None, dev(kf), dev(vf))
+        qq, qs = rt4.attn_q_quant(dev(q), B * T)
+        out = host(rt4.attention_tree(qq, qs, *kv, kv_len, *draft, parent, ratio=ratio)).reshape(H * ratio, B, T, D)
+        tokens, path, count = (host(x) for x in rt4.verify_tree(dev(logits), dev(tok), parent, dev(u), kv_len=kv_len))
+        rt4.kv_append_rows(*kv, stage, dev(kf), dev(vf), kv_len=kv_len, rows=dev(path), count=dev(count))
+        assert (out[:, idle] == 0).all() and np.isfinite(out).all() and (np.abs(out[:, ~idle]).max(-1) > 0).all()
+        assert (count[idle] == 0).all() and (tokens[idle] == -1).all() and (count[~idle] > 0).all()
+        append_expected(orc, want, wstage, kf, vf, length, path, count)
+        length = length + count
+        retired = np.where(idle, retired, step + 1)
+        assert np.array_equal(host(kv_len), length) and (length <= cap).all()
+        if idle.all():
+            break
+    print("steps until retired", retired, "lengths", length, flush=True)
+    assert idle.all() and (length > cap - T).all() and retired[2] == 0 and retired[1] > retired[0] > 0
+    for name, g, w in zip(("kc", "ksc", "vc", "vsc", "stage"), (*kv, stage), (*want, wstage)):
+        assert np.array_equal(host(g).view(np.uint32), w.view(np.uint32)), name
