@@ -318,9 +318,12 @@ int rt4_attention_launch_plan(int n_q, int n_heads, int ratio, int off, int n_ti
  * count[b] clamped to [0, T] (NULL: T): kv_len holds the lengths once the rows are in.
  * Codes, scales and stage as rt4_kv_append_k and rt4_kv_append_v write them for those
  * rows, bit for bit.  kv_len NULL: every sequence starts at key 0, and stage may be NULL
- * (a draft tile: kv_cap = 64).  A row index outside [0, T) appends zeros; a sequence whose
- * keys would not lie in [0, kv_cap) is left as it is.  T <= kv_cap, kv_cap % 64 == 0 and at
- * most 16777152; kf and vf must not overlap what is written. */
+ * (a draft tile: kv_cap = 64).  A row index outside [0, T) appends zeros, which is how padding
+ * nodes go into a draft tile: V has one scale for each dim over a tile's rows, so what a node's
+ * own branch gives depends, by the rounding of the codes, on all rows appended, and one infinite
+ * value makes its dim NaN for every node.  A sequence whose keys would not lie in [0, kv_cap)
+ * is left as it is.  T <= kv_cap, kv_cap % 64 == 0 and at most 16777152; kf and vf must not
+ * overlap what is written. */
 int rt4_kv_append_rows(uint32_t* kc, float* ksc, uint32_t* vc, float* vsc, float* stage, const float* kf, const float* vf,
                        const int32_t* kv_len, const int32_t* rows, const int32_t* count, int B, int T, int H, int kv_cap,
                        void* stream);
@@ -355,7 +358,8 @@ int rt4_attention_tree(float* out, const uint32_t* qq, const float* qsc, const u
  * Where no child is accepted the last token is drawn from what is left: the smallest x
  * whose cumulated residual exceeds u[b][0] times its total (the row's largest logit where
  * nothing is left, which only distributions that do not sum to 1 come to).  So the tokens
- * are distributed as the target's own.  temp NULL: 1; temp[b] <= 0 (or NaN): greedy, a child
+ * are distributed as p, the logits' own distribution (which a draft tile ties to the other
+ * branches by the rounding of V, see rt4_kv_append_rows).  temp NULL: 1; temp[b] <= 0 (or NaN): greedy, a child
  * is accepted iff it is the row's largest logit (lowest index among equals), and so is the
  * last token; temp[b] infinite: every logit that is not -inf weighs the same (at any other
  * temperature logits of +inf weigh the same and leave the rest nothing).  A NaN logit counts as -inf; a row of nothing but -inf ends the walk with token -1.

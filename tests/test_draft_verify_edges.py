@@ -387,6 +387,30 @@ def test_captured_residuals(torch_gpu):
 
 
 # ------------------------------------------------------------ as one would use them --
+@pytest.mark.parametrize("bad", [np.inf, np.nan, 1e30])
+def test_padding_rows_are_appended_as_zeros(rt4, torch_gpu, orc, bad):
+    """Whatever a model gives for padding nodes, rows of -1 keep it out of the draft tile's scales."""
+    print(f"case padding rows of {bad}", flush=True)
+    rng = np.random.default_rng(23)
+    B, T, H, ratio = 3, 7, 2, 3
+    qq, qs, kv, draft = attention_case(orc, rng, B, T, H, ratio, 128, 2)
+    parent = np.array([[-1, 0, 0, 2, -1, 4, 9], [-1, 0, 1, 2, 3, 4, 5], [-2, 0, 0, 0, 0, 0, 0]])
+    real = np.array([[1, 1, 1, 1, 0, 0, 0], [1] * 7, [0] * 7], bool)
+    rows = np.where(real, np.arange(T), -1)
+    kf, vf = (rng.standard_normal((B, T, H, D)).astype(np.float32) for _ in range(2))
+    kf[~real] = vf[~real] = bad
+    got = [dev(x) for x in draft]
+    rt4.kv_append_rows(*got, None, dev(kf), dev(vf), rows=dev(rows))
+    append_expected(orc, draft, None, kf, vf, np.zeros(B, int), rows, np.full(B, T))
+    for name, g, w in zip(("kd", "ksd", "vd", "vsd"), got, draft):
+        assert np.array_equal(host(g).view(np.uint32), w.view(np.uint32)), name
+    lens = [100, 128, 64]
+    out = rt4.attention_tree(dev(qq), dev(qs), *map(dev, kv), dev(np.array(lens)), *got, dev(parent), ratio=ratio)
+    check_attention(out, *tree_attention(qq, qs, kv, lens, draft, parent, ratio))
+    o = host(out).reshape(H * ratio, B, T, D)
+    assert (o[:, ~real] == 0).all() and (o[:, real] != 0).any(-1).all()
+
+
 def test_sequences_retired_at_the_cache_end(rt4, torch_gpu, orc):
     """A sequence without room for a whole path is made idle on the device: nothing is lost, nothing passes the cache's end."""
     torch = torch_gpu
