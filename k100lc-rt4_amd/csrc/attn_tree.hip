@@ -30,21 +30,6 @@ namespace {
 
 constexpr int HD = 256, KDW = HD / 8, BNK = 64;
 constexpr float L2E = 1.4426950408889634f;
-typedef unsigned long long u64;
-
-// Nodes that node i of sequence b sees: itself and those above it, none where it hangs
-// under no root.  Lane i of the wave has node i, whose parent is par (-2 past the last node).
-__device__ __forceinline__ u64 tree_sees(int par, int T) {
-    const int i = threadIdx.x & 63;
-    const bool root = i == 0 && par == -1, node = i > 0 && par >= 0 && par < i;
-    int up = node ? par : i;
-    u64 anc = 1ull << i;
-    for (int s = 1; s < T; s <<= 1) {    // pointer doubling: the deepest chain has T - 1 links
-        anc |= __shfl(anc, up);
-        up = __shfl(up, up);
-    }
-    return (root || node) && __shfl((int)root, 0) && (anc & 1) ? anc : 0;
-}
 
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));

@@ -120,6 +120,23 @@ __device__ __forceinline__ T wave_scan(T v) {
     return scan_step<0x143, 0xC>(v);
 }
 
+typedef unsigned long long u64;
+
+// Nodes of a tree of new tokens that node i is or hangs under, as bits; none where its chain does not end
+// in a root (node 0, parent -1).  Lane i of the wave has node i, whose parent is par (-2 past the last node).
+__device__ __forceinline__ u64 tree_sees(int par, int T) {
+    const int i = threadIdx.x & 63;
+    const bool root = i == 0 && par == -1, node = i > 0 && par >= 0 && par < i;
+    int up = node ? par : i;
+    u64 anc = 1ull << i;
+    for (int s = 1; s < T; s <<= 1) {    // pointer doubling: the deepest chain has T - 1 links
+        anc |= __shfl(anc, up);
+        up = __shfl(up, up);
+    }
+    const bool rooted = __builtin_amdgcn_readlane((int)root, 0);     // (by all lanes, lane 0 among them)
+    return (root || node) && rooted && (anc & 1) ? anc : 0;
+}
+
 // int4 -> int8 unpack used by every MFMA kernel here.  An RT4 dword holds
 // codes k=8d..8d+7 as nibbles, low nibble first, two's complement.  Shifting a
 // nibble into the high half of a byte gives that byte the signed value 16*code

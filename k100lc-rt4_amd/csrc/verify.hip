@@ -32,8 +32,6 @@ namespace {
 constexpr int CH = kVerifyChunk;         // logits per workgroup: 256 threads x 16
 constexpr int PT = CH / 256;
 
-typedef unsigned long long u64;
-
 struct RowStat {                         // of a chunk or of a row: largest logit, its lowest index, sum of exp((l - m) / temp)
     float m;
     int i;
@@ -112,19 +110,9 @@ struct Tree {
     u64 anc;                             // the node and those above it; 0: not in the tree
 };
 __device__ __forceinline__ Tree tree_of(int par, int T) {      // (par: node i's parent, -2 past the last node)
-    const int i = threadIdx.x & 63;
     Tree t;
-    t.par = par;
-    const bool root = i == 0 && t.par == -1, node = i > 0 && t.par >= 0 && t.par < i;
-    int up = node ? t.par : i;
-    u64 anc = 1ull << i;
-    for (int s = 1; s < T; s <<= 1) {    // pointer doubling: the deepest chain has T - 1 links
-        anc |= __shfl(anc, up);
-        up = __shfl(up, up);
-    }
-    const bool rooted = __builtin_amdgcn_readlane((int)root, 0);
-    t.anc = (root || node) && rooted && (anc & 1) ? anc : 0;
-    if (!t.anc) t.par = -2;
+    t.anc = tree_sees(par, T);
+    t.par = t.anc ? par : -2;
     return t;
 }
 
