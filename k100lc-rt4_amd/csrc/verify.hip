@@ -17,10 +17,13 @@
 // bits: with V ~ 250k tokens of like weight a cumulated sum in 32 bits (2^-24) misplaces
 // one draw in about twenty.
 //
-// What bounds it: the read of the logits where they are many (8 sequences of 16 nodes, V = 248320:
-// verify_stats_k 22.3 us, 127 MB at 5.7 TB/s, then 7.7 for walk and draw), else a chain of short
-// launches, each the start of one and two or three trips to memory (4 rows of 248320 with draft
-// probabilities 4.1 + 9.6 us; with siblings 5.3 more for each), or one launch (verify_small_k).
+// What bounds it: where the logits are many their read and the arithmetic on them, which take the same
+// time and do not overlap wholly (8 chains of 16 nodes, V = 248320, every row read: verify_stats_k 33.8 us,
+// 127 MB at 3.8 TB/s, which a copy reads in 25.7, and vector instructions in 69% of the SIMDs' cycles, 30 a
+// logit; trees with an idle sequence and padding among them, 85 to 92 MB: 22.3 us; then 7.5 to 8 for walk and
+// draw), else a chain of short launches, each the start of one and two or three trips to memory (4 rows of
+// 248320 with draft probabilities 4.2 + 9.8 us; with siblings 5.3 more for each), or one launch
+// (verify_small_k).
 #include <climits>
 
 #include "rt4_dev.h"
@@ -41,8 +44,8 @@ struct RowStat {                         // of a chunk or of a row: largest logi
 // exp((l - m) / temp) for a finite m, it = log2(e) / temp: 1 at the maximum, 0 for -inf and NaN (and where m
 // is -inf).  2^y = 2^n 2^f, n the integer nearest y (its bits are the low ones of y + 1.5 * 2^52), |f| <= 1/2,
 // 2^f = 1 + f q(f), q of degree 9 interpolating (2^f - 1) / f at Chebyshev nodes: off by less than 6e-16.
-// What the 64-bit unit has to do for a logit decides the time of many rows: 19 instructions, 127 MB of logits
-// in 23 us (30 instructions of an exp to the base e with its special cases by selects: 29 us).
+// What the 64-bit unit has to do for a logit counts with many rows: 19 instructions, 88 MB of logits in 22
+// us (30 instructions of an exp to the base e with its special cases by selects: 29 us).
 __device__ __forceinline__ double weight_finite(float l, float m, double it) {
     constexpr double M = 6755399441055744.0;
     const double y = fmax(((double)l - (double)m) * it, -2000.0);
