@@ -62,9 +62,18 @@ __device__ __forceinline__ v4i bytes16(uint32_t a, uint32_t b) {
     return v4i{(int)even_x16(a), (int)odd_x16(a), (int)even_x16(b), (int)odd_x16(b)};
 }
 
-// The eight codes of a V dword as fp16, key pairs (0,4) (1,5) (2,6) (3,7): a nibble with its sign
-// bit flipped is u = code + 8, and under the exponent of 1024 it reads 1024 + u (1024 + 16 u one
-// nibble up), from which a packed add (or fma) takes the code exactly.
+// P is held times 2^kPBits, and the running maximum moves when a score exceeds it by 2^kLazy, so that P is
+// at most 2^15 and fp16 holds it.  What is below 2^-(25 + kPBits) of the largest adds to the sum of P and
+// not to P V: over the n keys of a run at most n 2^-38 of the largest |V|, where the fp32 sums over the
+// n / 64 tiles may be off by n 2^-30.  (7 and 8: n 2^-32, 1e-4 of the output where one key is 22 nats above
+// 32768 others and its value small.  The lower floor moves the maximum more often: 1.9% on average over 45
+// sizes, 61 nodes over 131001 keys 282 -> 288 us.  The low part times 2^11, which needs no floor: 4.2%.)
+constexpr float kPBits = 13.f, kLazy = 2.f, kPScale = 1.f / 8192;        // 2^-kPBits
+
+// The eight codes of a V dword times 2^-kPBits as fp16, key pairs (0,4) (1,5) (2,6) (3,7): a nibble with its
+// sign bit flipped is u = code + 8, and under the exponent of 1024 it reads 1024 + u (1024 + 16 u one nibble
+// up), from which a packed fma makes the scaled code exactly (its 2^-17 is subnormal, and exact).  So the sums
+// of P V are as large as the values that go into them, and overflow no sooner.
 __device__ __forceinline__ v8h codes_f16(uint32_t w) {
     const uint32_t y = w >> 8;
     const uint32_t t[4] = {(w & 0x000F000Fu) ^ 0x64086408u, (w & 0x00F000F0u) ^ 0x64806480u, (y & 0x000F000Fu) ^ 0x64086408u,
@@ -76,8 +85,8 @@ __device__ __forceinline__ v8h codes_f16(uint32_t w) {
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         const v2h a = __builtin_bit_cast(v2h, t[k]);
-        r.p[k] = (k & 1) ? a * v2h{(_Float16)0.0625f, (_Float16)0.0625f} + v2h{(_Float16)-72.f, (_Float16)-72.f}
-                         : a + v2h{(_Float16)-1032.f, (_Float16)-1032.f};
+        const _Float16 m = (_Float16)(k & 1 ? kPScale / 16 : kPScale), c = (_Float16)(k & 1 ? -72 * kPScale : -1032 * kPScale);
+        r.p[k] = a * v2h{m, m} + v2h{c, c};
     }
     return r.v;
 }
@@ -167,14 +176,6 @@ __device__ __forceinline__ Run run_of(const AttnTree& A, const TreePlan& P, int 
 
 // n / T for a row n of a KV head's (T at most 64, n below 2^26).
 __device__ __forceinline__ int by_nodes(int n, const AttnTree& A, const TreePlan& P) { return A.T == 1 ? n : (int)__umulhi((unsigned)n, P.inv_nodes); }
-
-// P is held times 2^kPBits, and the running maximum moves when a score exceeds it by 2^kLazy, so that P is
-// at most 2^15 and fp16 holds it.  What is below 2^-(25 + kPBits) of the largest adds to the sum of P and
-// not to P V: over the n keys of a run at most n 2^-38 of the largest |V|, where the fp32 sums over the
-// n / 64 tiles may be off by n 2^-30.  (7 and 8: n 2^-32, 1e-4 of the output where one key is 22 nats above
-// 32768 others and its value small.  The lower floor moves the maximum more often: 1.9% on average over 45
-// sizes, 61 nodes over 131001 keys 282 -> 288 us.  The low part times 2^11, which needs no floor: 4.2%.)
-constexpr float kPBits = 13.f, kLazy = 2.f;
 
 // Products x[4g + r] * y[c] of four 16x16 tiles in their accumulator layout on the matrix core
 // (registers 4b + r: tile b, x from lane 16b + 4g + r, y from lane 16b + c), each rounded once.
@@ -504,7 +505,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
     for (int nb = 0; nb < NB; nb++) {
         float t = l[nb] + __shfl_xor(l[nb], 16);
         t += __shfl_xor(t, 32);
-        if (g == 0) mx[w][nb * 16 + c] = t;
+        if (g == 0) mx[w][nb * 16 + c] = t * kPScale;
     }
     __syncthreads();
     const size_t prow = ((size_t)unit * P.groups + rg) * RW;

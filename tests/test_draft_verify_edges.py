@@ -84,6 +84,23 @@ def test_outstanding_key(rt4, torch_gpu, n):
         assert (err <= tol[:, None]).all(), (splits, err.max(), (err / tol[:, None]).max())
 
 
+@pytest.mark.parametrize("value", [2.0**110, 2.0**-110])
+def test_large_and_small_values(rt4, torch_gpu, value):
+    """A sum over 131072 equal keys is at most their number times their values: it neither overflows nor loses bits sooner."""
+    torch = torch_gpu
+    print(f"case values of {value}", flush=True)
+    n = 131072
+    args, kw = blank_attention(torch, 1, 2, 1, 3, n)
+    for x in (args[4], args[9]):
+        x.fill_(0x11111111)                             # code 1
+    for x in (args[5], args[10]):
+        x.fill_(value)
+    args[11][:, 1] = 0
+    for splits in (1, 0):
+        out = rt4.attention_tree(*args, **kw, kv_splits=splits)
+        assert float((out / value - 1).abs().max()) <= (168 + n / BG) * 2.0**-24 + 2.0**-22
+
+
 @pytest.mark.parametrize("B,idle,cap", [(1, 1, 256), (3, 1, 32768), (4, 2, 16384), (70, 30, 2048)])
 def test_idle_sequences_take_no_share(rt4, torch_gpu, orc, B, idle, cap):
     """Idle sequences' caches are not attended, however long: the others' bits do not depend on them, and their rows are zeros."""
