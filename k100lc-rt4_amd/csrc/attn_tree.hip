@@ -396,7 +396,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
         for (int nb = 0; nb < NB; nb++) {
             // (a row that sees nothing yet keeps its reference: -inf would not come back)
             if (NB > 2) __builtin_amdgcn_sched_barrier(0);
-            const float up = first ? (mt[nb] > -1e30f ? mt[nb] : 0.f) : fmaxf(mt[nb], 0.f);
+            const float up = first ? (mt[nb] > -INFINITY ? mt[nb] : 0.f) : fmaxf(mt[nb], 0.f);
             m[nb] += up;
 #pragma unroll
             for (int e = 0; e < 8; e++) s[nb][e] -= up;
@@ -527,7 +527,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_k(const AttnTree A, const Tr
             }
             if (w == 0 && g == 0) {
                 const int r = nb * 16 + c;
-                mlpart[prow + r] = make_float2(t0 < t1 ? m[nb] : -1e30f, mx[0][r] + mx[1][r] + mx[2][r] + mx[3][r]);
+                mlpart[prow + r] = make_float2(m[nb], mx[0][r] + mx[1][r] + mx[2][r] + mx[3][r]);
             }
         }
         return;
@@ -562,7 +562,7 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(const AttnTree A, const 
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         x[k] = mlpart[row + min(lane + 64 * k, splits - 1) * step];
-        if (lane + 64 * k >= splits) x[k] = make_float2(-1e30f, 0.f);
+        if (lane + 64 * k >= splits) x[k] = make_float2(-INFINITY, 0.f);
     }
     const float* src = opart + row * HD + 4 * lane;
     v4f v[16];

@@ -101,6 +101,33 @@ def test_large_and_small_values(rt4, torch_gpu, value):
         assert float((out / value - 1).abs().max()) <= (168 + n / BG) * 2.0**-24 + 2.0**-22
 
 
+@pytest.mark.parametrize("n", [0, 1, 300])
+def test_scores_far_below_zero(rt4, torch_gpu, n):
+    """Scores of -1e32 and less, as keys of 1e30 have them: the least of them takes all the weight."""
+    torch = torch_gpu
+    print(f"case scores far below zero, n={n}", flush=True)
+    args, kw = blank_attention(torch, 1, 2, 1, 3, 320)
+    args[0].fill_(-1)                                   # codes -1, scale 1
+    args[1].fill_(1.0)
+    for x in (args[2], args[7]):
+        x.fill_(0x11111111)                             # codes 1
+    args[3].copy_(1e30 * (2 + torch.arange(320, device="cuda") / 320))
+    args[8].fill_(1e30 if n == 0 else 4e30)
+    for x in (args[4], args[9]):
+        x.random_(-2**31, 2**31 - 1, generator=torch.Generator(device="cuda").manual_seed(n))
+    for x in (args[5], args[10]):
+        x.fill_(1.0)
+    args[6].fill_(n)
+    args[11][:, 1] = 0
+    first = args[4] if n else args[9]
+    want = ((first[0, 0, 0] << 28) >> 28).float()       # V of key 0, or of the root
+    if n == 0:
+        args[8][0, 0, :, 1] = 2e30                      # node 1 sees the root above its own key
+    for splits in (0, 1, 3):
+        out = rt4.attention_tree(*args, **kw, kv_splits=splits)
+        assert torch.equal(out, want.expand(3, 2, D)), splits
+
+
 @pytest.mark.parametrize("B,idle,cap", [(1, 1, 256), (3, 1, 32768), (4, 2, 16384), (70, 30, 2048)])
 def test_idle_sequences_take_no_share(rt4, torch_gpu, orc, B, idle, cap):
     """Idle sequences' caches are not attended, however long: the others' bits do not depend on them, and their rows are zeros."""
