@@ -15,10 +15,10 @@
 // are fp32.
 //
 // What bounds it (24 query heads over 4 KV heads):
-//   1 node over 1000 keys: 6.0 us and the join 3.6, the start of two launches; the loop is one step
-//   4 nodes over 32701 keys: 16.8 and 4.0 us, 36.7 MB at 1.8 TB/s, four steps after 2.7 us of start
+//   1 node over 1000 keys: 6.1 us and the join 3.8, the start of two launches; the loop is one step
+//   4 nodes over 32701 keys: 16.6 and 3.9 us, 36.7 MB at 1.8 TB/s, four steps after 2.7 us of start
 //   16 sequences of 8 nodes over up to 16384 keys: 55 to 62 us in all, 118 to 156 MB at 2.4 TB/s with 18 GFLOP beside it
-//   61 nodes over 131001 keys: 285 us in all, 196 GFLOP at 0.7 PFLOP/s; P's two parts make them 294,
+//   61 nodes over 131001 keys: 279 to 285 us in all, 196 GFLOP at 0.7 PFLOP/s; P's two parts make them 294,
 //   which take 222 us at the rates of large int8 and fp16 products, the softmax beside them
 #include <algorithm>
 
