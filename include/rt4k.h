@@ -375,6 +375,64 @@ int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_
                     const int32_t* draft, const int32_t* parent, const float* u, const float* temp, const float* draft_p,
                     int64_t ldp, int B, int T, int V, int max_children, void* stream);
 
+/* ------------------------------- 8-bit linears and norms between blocks ---- */
+/* The steps of a gated feed-forward block around the RT4 linears, and linears kept at 8 bits.
+ * No counterparts in the reference's kernel API as such (it runs RMSNorm, the residual sum, the
+ * activation and the quantizers as launches of their own, src/k_new.hip).  None of these uses
+ * library scratch: calls on different streams share nothing but their arguments.
+ * Element types: */
+#define RT4_F32 0
+#define RT4_BF16 1
+#define RT4_F16 2
+/* Activations of a gated half: x / (1 + exp(-x)), and 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))). */
+#define RT4_SILU 0
+#define RT4_GELU_TANH 1
+/* Forms of a norm's result, besides the element types: */
+#define RT4_TOKEN 3   /* int8 codes [M][K] in natural order, a scale [M] for each token (127 levels a side) */
+#define RT4_ACT 4     /* int8 codes [M][K] interleaved, scales [M][K/128]: as rt4_quant_act_a8 lays them out, for rt4_gemv_w4a8_q */
+#define RT4_ROWS 5    /* int8 codes [M][K] interleaved, scales [K/128][M], 119 levels: as rt4_quant_rows_i8, for rt4_gemm_w4a8_i8 */
+
+/* 8-bit product: c [M][N] (c_type, row stride ldc elements) = sx[m] sw[n] Σ_k xq[m][k] wq[n][k] with
+ * xq int8 [M][K] (row stride ldx bytes), a scale sx[m] for each token, wq int8 [N][K] (row stride ldw),
+ * a scale sw[n] for each channel; all in natural order.  Sums are exact int32: K % 16 == 0 and at most 131056.
+ * M >= 1, N >= 1; strides at least a row, ldx and ldw multiples of 16 below 2^24, xq and wq 16-byte aligned.
+ * Each output is the sum's fp32 value times sx times sw, rounded to c_type; a scale that is not finite makes its
+ * row or column so.  c must not overlap an input. */
+int rt4_gemm_w8a8(void* c, int64_t ldc, int c_type, const int8_t* wq, int64_t ldw, const float* sw, const int8_t* xq,
+                  int64_t ldx, const float* sx, int M, int N, int K, void* stream);
+
+/* First half of a gated feed-forward block on 8-bit weights: h [M][N] = act(g) * u with g and u the products of
+ * rt4_gemm_w8a8 with the gate weights wg, sg and the up weights wu, su, in fp32 until h's rounding.  Arguments as there. */
+int rt4_ffn_gate_w8a8(void* h, int64_t ldh, int h_type, const int8_t* wg, int64_t ldg, const float* sg, const int8_t* wu,
+                      int64_t ldu, const float* su, const int8_t* xq, int64_t ldx, const float* sx, int M, int N, int K,
+                      int act, void* stream);
+
+/* The same on RT4 weights for 1 to 4 rows: h f32 [rows][N] = act(g) * u with g and u what rt4_gemv_w4a8_q gives for the
+ * gate weights and for the up weights (up to the order of the fp32 sums over groups).  xq and sa from rt4_quant_act_a8
+ * or rt4_block_norm (RT4_ACT).  K % 128 == 0; h must not overlap an input. */
+int rt4_ffn_gate_w4a8(float* h, const uint32_t* wg, const uint16_t* sg, const uint32_t* wu, const uint16_t* su,
+                      const int8_t* xq, const float* sa, int rows, int N, int K, int act, void* stream);
+
+/* Between two blocks: y [M][K], the output of one, is normed (post_w given), multiplied by a gate, scaled and
+ * added to the residual h, and the sum is normed for the next:
+ *   y1 = post_w ? y * post_w / rms(y) : y
+ *   h_out = h + scale * gate * y1, rounded to fp32 and to h's type
+ *   n = h_out * (w + w_offset) / rms(h_out)         rms(x) = sqrt(mean(x^2) + eps)
+ * y NULL: h itself is normed and h_out is not written (it may be NULL).  w and n NULL: h_out alone.  h and h_out have
+ * h_type, y and gate y_type; gate (or NULL: 1) has row stride ldg, 0 for one row for all tokens.  Row strides in
+ * elements, at least K; w and post_w f32 [K].  h_out may be h with the same stride; otherwise outputs must not overlap
+ * inputs.  n_form: an element type, n [M][K] contiguous of that type, n_scale NULL; or RT4_TOKEN, RT4_ACT, RT4_ROWS
+ * with n_scale (the last two with K % 128 == 0).  A code is the nearest integer to levels * n / max|n| over its token
+ * or group (ties to even), decided in 64 bits; its scale max|n| / levels, 1 where all are zeros.  Where a value of a
+ * token or group is not finite its codes are 0 and its scale NaN.  1 <= K <= 65536. */
+int rt4_block_norm(void* h_out, int64_t ldho, const void* h, int64_t ldh, int h_type, const void* y, int64_t ldy, int y_type,
+                   const void* gate, int64_t ldg, const float* post_w, const float* w, double scale, double eps, double w_offset,
+                   void* n, float* n_scale, int n_form, int M, int K, void* stream);
+
+/* Quantizer with one scale a token, natural order: codes and scales as rt4_block_norm's RT4_TOKEN of x itself.
+ * x [M][K] of x_type, row stride ldx; xq int8 [M][K] contiguous, sx f32 [M].  1 <= K <= 65536. */
+int rt4_quant_token_a8(int8_t* xq, float* sx, const void* x, int64_t ldx, int x_type, int M, int K, void* stream);
+
 /* ----------------------------------------- W4A4 siblings (RT_ACT4 path) ---- */
 
 /* int4 activation quantizer.  Replaces k_quant_rows (src/kernels.h:36,

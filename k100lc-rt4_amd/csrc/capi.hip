@@ -893,4 +893,102 @@ int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_
                       "rt4_verify_tree launch");
 }
 
+// ---- 8-bit linears, gated halves, norms between blocks
+
+// Shapes and addresses of one operand pair of an 8-bit product: sums of K products of codes stay below 2^31, the
+// kernels address rows of one tile by 32-bit offsets and read 16 bytes at a time.
+constexpr int kMaxK8 = 131056;
+constexpr int64_t kMaxLd8 = 1 << 24;
+
+static int check_linear8(const char* who, const rt4::Linear8& a, int weights) {
+    if (!a.out || !a.x || !a.sx) return fail(RT4_E_ARG, "%s: null pointer", who);
+    for (int j = 0; j < weights; j++)
+        if (!a.w[j] || !a.sw[j]) return fail(RT4_E_ARG, "%s: null pointer", who);
+    if (a.type < RT4_F32 || a.type > RT4_F16) return fail(RT4_E_ARG, "%s: output type %d", who, a.type);
+    if (weights == 2 && (a.act < RT4_SILU || a.act > RT4_GELU_TANH)) return fail(RT4_E_ARG, "%s: activation %d", who, a.act);
+    if (a.M < 1 || a.N < 1 || a.M > (1 << 24) || a.N > (1 << 24))
+        return fail(RT4_E_SHAPE, "%s: M=%d N=%d (1 to 2^24)", who, a.M, a.N);
+    if (a.K < 16 || a.K % 16 || a.K > kMaxK8) return fail(RT4_E_SHAPE, "%s: K=%d is not a multiple of 16 from 16 to %d", who, a.K, kMaxK8);
+    if (a.ldo < a.N) return fail(RT4_E_SHAPE, "%s: output row stride %lld is below N=%d", who, (long long)a.ldo, a.N);
+    const long long ld[3] = {a.ldx, a.ldw[0], a.ldw[1]};
+    const void* at[3] = {a.x, a.w[0], a.w[1]};
+    for (int j = 0; j <= weights; j++) {
+        if (ld[j] < a.K || ld[j] % 16 || ld[j] >= kMaxLd8)
+            return fail(RT4_E_SHAPE, "%s: row stride %lld of codes (a multiple of 16, at least K=%d, below 2^24)", who, ld[j], a.K);
+        if (!aligned(at[j], 16)) return fail(RT4_E_ARG, "%s: misaligned pointer (codes need 16 bytes)", who);
+    }
+    if (!aligned(a.out, a.type == RT4_F32 ? 4 : 2) || !aligned(a.sx, 4) || !aligned(a.sw[0], 4) || !aligned(a.sw[1], 4))
+        return fail(RT4_E_ARG, "%s: misaligned pointer", who);
+    return RT4_OK;
+}
+
+int rt4_gemm_w8a8(void* c, int64_t ldc, int c_type, const int8_t* wq, int64_t ldw, const float* sw, const int8_t* xq,
+                  int64_t ldx, const float* sx, int M, int N, int K, void* stream) {
+    const rt4::Linear8 a{c, ldc, {wq, nullptr}, {ldw, 0}, {sw, nullptr}, xq, ldx, sx, M, N, K, c_type, -1};
+    int rc = check_linear8("rt4_gemm_w8a8", a, 1);
+    if (rc) return rc;
+    return hip_status(rt4::launch_linear8(a, as_stream(stream)), "rt4_gemm_w8a8 launch");
+}
+
+int rt4_ffn_gate_w8a8(void* h, int64_t ldh, int h_type, const int8_t* wg, int64_t ldg, const float* sg, const int8_t* wu,
+                      int64_t ldu, const float* su, const int8_t* xq, int64_t ldx, const float* sx, int M, int N, int K,
+                      int act, void* stream) {
+    const rt4::Linear8 a{h, ldh, {wg, wu}, {ldg, ldu}, {sg, su}, xq, ldx, sx, M, N, K, h_type, act};
+    int rc = check_linear8("rt4_ffn_gate_w8a8", a, 2);
+    if (rc) return rc;
+    return hip_status(rt4::launch_linear8(a, as_stream(stream)), "rt4_ffn_gate_w8a8 launch");
+}
+
+int rt4_ffn_gate_w4a8(float* h, const uint32_t* wg, const uint16_t* sg, const uint32_t* wu, const uint16_t* su,
+                      const int8_t* xq, const float* sa, int rows, int N, int K, int act, void* stream) {
+    if (!h || !wg || !sg || !wu || !su || !xq || !sa) return fail(RT4_E_ARG, "rt4_ffn_gate_w4a8: null pointer");
+    if (act < RT4_SILU || act > RT4_GELU_TANH) return fail(RT4_E_ARG, "rt4_ffn_gate_w4a8: activation %d", act);
+    int rc = check_gemv_shape("rt4_ffn_gate_w4a8", rows, N, K);
+    if (rc || (rc = check_gemv_align("rt4_ffn_gate_w4a8", h, wg, sg, xq, sa)) || (rc = check_gemv_align("rt4_ffn_gate_w4a8", h, wu, su, xq, sa)))
+        return rc;
+    const rt4::Gate4 a{h, {wg, wu}, {sg, su}, xq, sa, rows, N, K, act};
+    return hip_status(rt4::launch_gate4(a, as_stream(stream)), "rt4_ffn_gate_w4a8 launch");
+}
+
+// Bytes of an element of a type, and whether rows of them can be read 16 bytes at a time.
+static size_t type_bytes(int t) { return t == RT4_F32 ? 4 : 2; }
+static bool vec_rows(const void* p, long long ld, int type) { return aligned(p, 16) && ld * (long long)type_bytes(type) % 16 == 0; }
+
+static int run_norm(const char* who, rt4::BlockNorm& a, hipStream_t st) {
+    if (a.M < 1 || a.K < 1 || a.K > rt4::kNormMaxK) return fail(RT4_E_SHAPE, "%s: M=%d K=%d (1 to %d)", who, a.M, a.K, rt4::kNormMaxK);
+    if (a.h_type < RT4_F32 || a.h_type > RT4_F16 || (a.y && (a.y_type < RT4_F32 || a.y_type > RT4_F16)))
+        return fail(RT4_E_ARG, "%s: element types %d and %d", who, a.h_type, a.y_type);
+    if (a.ldh < a.K || (a.y && (a.ldy < a.K || a.ldho < a.K)) || (a.gate && a.ldg != 0 && a.ldg < a.K))
+        return fail(RT4_E_SHAPE, "%s: a row stride is below K=%d", who, a.K);
+    if (a.h == a.h_out && a.ldh != a.ldho) return fail(RT4_E_ARG, "%s: h_out in h's place needs h's row stride", who);
+    if (a.n && (a.form < RT4_F32 || a.form > RT4_ROWS)) return fail(RT4_E_ARG, "%s: form %d", who, a.form);
+    if (a.n && a.form > RT4_F16 && !a.n_scale) return fail(RT4_E_ARG, "%s: codes need n_scale", who);
+    if (a.n && a.form > RT4_TOKEN && a.K % 128) return fail(RT4_E_SHAPE, "%s: K=%d is not a multiple of 128", who, a.K);
+    const size_t hb = type_bytes(a.h_type), yb = type_bytes(a.y_type), nb = !a.n || a.form >= RT4_TOKEN ? 1 : type_bytes(a.form);
+    if (!aligned(a.h, hb) || !aligned(a.h_out, hb) || !aligned(a.y, yb) || !aligned(a.gate, yb) || !aligned(a.post_w, 4) ||
+        !aligned(a.w, 4) || !aligned(a.n, a.form > RT4_TOKEN ? 8 : nb) || !aligned(a.n_scale, 4))
+        return fail(RT4_E_ARG, "%s: misaligned pointer (codes of groups need 8 bytes)", who);
+    a.vec = vec_rows(a.h, a.ldh, a.h_type) && (!a.y || (vec_rows(a.y, a.ldy, a.y_type) && vec_rows(a.h_out, a.ldho, a.h_type))) &&
+            (!a.gate || vec_rows(a.gate, a.ldg, a.y_type));
+    a.wvec = aligned(a.w, 16) && aligned(a.post_w, 16);
+    a.nvec = aligned(a.n, 16) && (size_t)a.K * nb % (nb == 1 ? 8 : 16) == 0;
+    return hip_status(rt4::launch_block_norm(a, st), who);
+}
+
+int rt4_block_norm(void* h_out, int64_t ldho, const void* h, int64_t ldh, int h_type, const void* y, int64_t ldy, int y_type,
+                   const void* gate, int64_t ldg, const float* post_w, const float* w, double scale, double eps, double w_offset,
+                   void* n, float* n_scale, int n_form, int M, int K, void* stream) {
+    if (!h || (y && !h_out) || (!y && !n) || (!n != !w)) return fail(RT4_E_ARG, "rt4_block_norm: null pointer (h; h_out with y; n with w; n without y)");
+    if (!y && (gate || post_w)) return fail(RT4_E_ARG, "rt4_block_norm: a gate and a norm behind the block need y");
+    if (!(eps >= 0)) return fail(RT4_E_ARG, "rt4_block_norm: eps=%g", eps);
+    rt4::BlockNorm a{h_out, ldho, h, ldh, y, ldy, gate, ldg, post_w, w, n, n_scale, scale, eps, w_offset, M, K, h_type, y ? y_type : 0, n_form, false, false, false};
+    return run_norm("rt4_block_norm", a, as_stream(stream));
+}
+
+int rt4_quant_token_a8(int8_t* xq, float* sx, const void* x, int64_t ldx, int x_type, int M, int K, void* stream) {
+    if (!xq || !sx || !x) return fail(RT4_E_ARG, "rt4_quant_token_a8: null pointer");
+    rt4::BlockNorm a{nullptr, 0, x, ldx, nullptr, 0, nullptr, 0, nullptr, nullptr, xq, sx, 1.0, 0.0, 0.0, M, K, x_type, 0, RT4_TOKEN, false, false, false};
+    return run_norm("rt4_quant_token_a8", a, as_stream(stream));
+}
+
 }  // extern "C"

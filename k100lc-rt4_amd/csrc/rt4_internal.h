@@ -187,4 +187,51 @@ hipError_t launch_verify_tree(int* tokens, int* path, int* count, int* kv_len, c
                               const int* parent, const float* u, const float* temp, const float* q, size_t ldq, int B, int T, int V,
                               int levels, void* ws, int* cnt, hipStream_t st);
 
+// ---- 8-bit products, gated halves, norms between blocks (linear8.hip, gate4.hip, norm.hip)
+struct Linear8 {
+    void* out;
+    long long ldo;
+    const int8_t* w[2];                  // weights, or gate and up weights
+    long long ldw[2];
+    const float* sw[2];
+    const int8_t* x;
+    long long ldx;
+    const float* sx;
+    int M, N, K, type, act;              // act < 0: the product alone
+};
+hipError_t launch_linear8(const Linear8& a, hipStream_t st);
+
+struct Gate4 {
+    float* out;
+    const uint32_t* w[2];
+    const uint16_t* ws[2];
+    const int8_t* xq;
+    const float* sa;
+    int rows, N, K, act;
+};
+hipError_t launch_gate4(const Gate4& a, hipStream_t st);
+
+// Forms of the normed rows: floats by their type (0..2), int8 codes with a scale for each token, or for each
+// 128-group as the decode (kAct) and the prefill (kRows) quantizers lay them out.
+enum { kToken = 3, kAct = 4, kRows = 5 };
+constexpr int kNormMaxK = 65536;
+struct BlockNorm {
+    void* h_out;
+    long long ldho;
+    const void* h;
+    long long ldh;
+    const void* y;                       // null: h is normed as it is, h_out is not written
+    long long ldy;
+    const void* gate;
+    long long ldg;                       // 0: one row for all tokens
+    const float* post_w;
+    const float* w;                      // null (no y): the values as they are
+    void* n;                             // null: h_out alone
+    float* n_scale;
+    double scale, eps, w_offset;
+    int M, K, h_type, y_type, form;
+    bool vec, wvec, nvec;                // whether rows of h, y, gate and h_out, the weights, and n's rows are aligned for vector access
+};
+hipError_t launch_block_norm(const BlockNorm& a, hipStream_t st);
+
 }  // namespace rt4

@@ -15,7 +15,9 @@ Reference interface mirrored (src/kernels.h of K100LC-RT4):
     k_attention      -> attention_prefill    (src/kernels.h:81, prefill branch)
 plus the pieces those wrappers launch internally (quant_act_a8, gemv_w4a8_q), and
 the steps of speculative decoding over the int4-KV cache, which the reference does
-not have: kv_append_rows, attention_tree, verify_tree.
+not have: kv_append_rows, attention_tree, verify_tree.  Around the linears, where the
+reference runs launches of its own (RMSNorm, residual sum, activation): block_norm,
+ffn_gate_w4a8, and for layers kept at 8 bits gemm_w8a8, ffn_gate_w8a8, quant_token_a8.
 """
 from __future__ import annotations
 
@@ -39,6 +41,7 @@ C_EXPORTS = (
     "rt4_attn_q_quant", "rt4_kv_append_k", "rt4_kv_append_v", "rt4_attention_prefill",
     "rt4_attention_prefill_cfg", "rt4_attention_launch_plan",
     "rt4_kv_append_rows", "rt4_attention_tree", "rt4_verify_tree",
+    "rt4_gemm_w8a8", "rt4_ffn_gate_w8a8", "rt4_ffn_gate_w4a8", "rt4_block_norm", "rt4_quant_token_a8",
     "rt4_file_open", "rt4_file_close", "rt4_file_count", "rt4_file_find", "rt4_file_info", "rt4_file_data",
     "rt4_file_size", "rt4_file_upload", "rt4_file_upload_tensor",
 )
@@ -65,6 +68,7 @@ _lib = None
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
+_D = ctypes.c_double
 _SIGS = {
     "rt4_quant_act_a8": [_P, _P, _P, _P, _I, _I, _P],
     "rt4_quant_act_rowwise": [_P, _P, _P, _P, _I, _I, _I, _P],
@@ -96,6 +100,11 @@ _SIGS = {
     "rt4_attention_launch_plan": [_I, _I, _I, _I, _I, _I, _I, _P, _P, _P],
     "rt4_kv_append_rows": [_P] * 10 + [_I] * 4 + [_P],
     "rt4_attention_tree": [_P] * 13 + [_I] * 8 + [_P],
+    "rt4_gemm_w8a8": [_P, _L, _I, _P, _L, _P, _P, _L, _P, _I, _I, _I, _P],
+    "rt4_ffn_gate_w8a8": [_P, _L, _I, _P, _L, _P, _P, _L, _P, _P, _L, _P, _I, _I, _I, _I, _P],
+    "rt4_ffn_gate_w4a8": [_P] * 7 + [_I] * 4 + [_P],
+    "rt4_block_norm": [_P, _L, _P, _L, _I, _P, _L, _I, _P, _L, _P, _P, _D, _D, _D, _P, _P, _I, _I, _I, _P],
+    "rt4_quant_token_a8": [_P, _P, _P, _L, _I, _I, _I, _P],
     "rt4_verify_tree": [_P] * 5 + [_L] + [_P] * 5 + [_L] + [_I] * 4 + [_P],
 }
 
@@ -585,3 +594,163 @@ def verify_tree(logits, draft, parent, u, temp=None, draft_probs=None, max_child
         pp, _arg(u, f32, (B, T), dev, "u"), None if temp is None else _arg(temp, f32, (B,), dev, "temp"), qp, ldq, B, T, V,
         max_children or 0, _raw_stream(dev)))
     return tokens, path, count
+
+
+# ---------------------------------- 8-bit linears, norms between blocks ----
+ACTS = {"silu": 0, "gelu_tanh": 1}
+FORMS = {"f32": 0, "bf16": 1, "f16": 2, "token": 3, "act": 4, "rows": 5}
+_types = None
+
+
+def _type(dtype, name):
+    """The ABI's number of an element type."""
+    global _types
+    if _types is None:
+        torch = _torch()
+        _types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    t = _types.get(dtype)
+    if t is None:
+        raise RT4Error(f"{name}: expected float32, bfloat16 or float16, got {dtype}")
+    return t
+
+
+def _mat(t, rows, cols, dtype, dev, name):
+    """(data_ptr, row stride) of a matrix [rows, cols] whose rows are contiguous (dtype None: any of the element types)."""
+    if t.dim() == 2 and t.shape[0] == rows and t.shape[1] == cols and (dtype is None or t.dtype is dtype) and t.get_device() == dev:
+        r, c = t.stride()
+        if rows == 1:                            # (a single row's stride says nothing)
+            r = (cols + 15) // 16 * 16
+        if c == 1 or cols == 1:
+            return t.data_ptr(), r
+    raise RT4Error(f"{name}: expected {dtype or 'floating-point'} [{rows}, {cols}] with contiguous rows on device {dev}, got {t.dtype} "
+                   f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
+
+
+def _linear8(fn, weights, xq, sx, act, out, dtype):
+    torch = _torch()
+    dev, f32, i8 = _dev(), torch.float32, torch.int8
+    if xq.dim() != 2 or weights[0][1].dim() != 2:
+        raise RT4Error(f"xq {tuple(xq.shape)} [M, K] and {weights[0][0]} {tuple(weights[0][1].shape)} [N, K] are matrices")
+    M, K = xq.shape
+    N = weights[0][1].shape[0]
+    if out is None:
+        dtype = dtype or f32
+        t = _type(dtype, "dtype")
+        out = torch.empty_strided((M, N), (N, 1), dtype=dtype, device=dev)
+        op, ldo = out.data_ptr(), N
+    else:
+        if dtype is not None and out.dtype is not dtype:
+            raise RT4Error(f"out is {out.dtype}, dtype {dtype}")
+        t = _type(out.dtype, "out")
+        op, ldo = _mat(out, M, N, out.dtype, dev, "out")
+    xp, ldx = _mat(xq, M, K, i8, dev, "xq")
+    args = []
+    for name, w, sname, s in weights:
+        args += [*_mat(w, N, K, i8, dev, name), _arg(s, f32, (N,), dev, sname)]
+    _check(fn(op, ldo, t, *args, xp, ldx, _arg(sx, f32, (M,), dev, "sx"), M, N, K, *act, _raw_stream(dev)))
+    return out
+
+
+def gemm_w8a8(wq, sw, xq, sx, out=None, dtype=None):
+    """Product of int8 codes -> [M, N] of `dtype` (float32, bfloat16 or float16; default float32): xq int8 [M, K] with a scale
+    sx f32 [M] for each token (quant_token_a8, block_norm), wq int8 [N, K] with a scale sw f32 [N] for each channel.
+    K % 16 == 0 and at most 131056; rows may be strided by multiples of 16 bytes.  See rt4_gemm_w8a8 in include/rt4k.h."""
+    return _linear8(lib().rt4_gemm_w8a8, (("wq", wq, "sw", sw),), xq, sx, (), out, dtype)
+
+
+def _act_code(act):
+    a = ACTS.get(act)
+    if a is None:
+        raise RT4Error(f"act: expected one of {sorted(ACTS)}, got {act!r}")
+    return a
+
+
+def ffn_gate_w8a8(wg, sg, wu, su, xq, sx, act: str = "silu", out=None, dtype=None):
+    """First half of a gated feed-forward block -> act(x Wg^T) * (x Wu^T) [M, N]: weights and activations as gemm_w8a8's, act
+    "silu" or "gelu_tanh".  See rt4_ffn_gate_w8a8 in include/rt4k.h."""
+    return _linear8(lib().rt4_ffn_gate_w8a8, (("wg", wg, "sg", sg), ("wu", wu, "su", su)), xq, sx, (_act_code(act),), out, dtype)
+
+
+def ffn_gate_w4a8(wg, wsg, wu, wsu, xq, sa, act: str = "silu", out=None):
+    """The same on RT4 weights (wg, wu int32 [N, K/8], wsg, wsu int16/fp16 [N, K/128]) for 1 to 4 rows -> f32 [rows, N]; xq, sa as
+    gemv_w4a8_q's (quant_act_a8, or block_norm's "act" form).  See rt4_ffn_gate_w4a8 in include/rt4k.h."""
+    torch = _torch()
+    dev, f32, i32 = _dev(), torch.float32, torch.int32
+    if xq.dim() != 2 or wg.dim() != 2:
+        raise RT4Error(f"ffn_gate_w4a8: xq {tuple(xq.shape)} [rows, K] and wg {tuple(wg.shape)} [N, K/8] are matrices")
+    rows, K = xq.shape
+    N, G = wg.shape[0], K // GROUP
+    out, op = _out(out, f32, (rows, N), (N, 1), dev, "out")
+    half = torch.float16 if wsg.dtype is torch.float16 else torch.int16
+    _check(lib().rt4_ffn_gate_w4a8(
+        op, _arg(wg, i32, (N, K // 8), dev, "wg"), _arg(wsg, half, (N, G), dev, "wsg"), _arg(wu, i32, (N, K // 8), dev, "wu"),
+        _arg(wsu, half, (N, G), dev, "wsu"), _arg(xq, torch.int8, (rows, K), dev, "xq"), _arg(sa, f32, (rows, G), dev, "sa"),
+        rows, N, K, _act_code(act), _raw_stream(dev)))
+    return out
+
+
+def block_norm(h, y=None, weight=None, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-6,
+               weight_offset: float = 0.0, out: str = "f32", h_out=None):
+    """What stands between two blocks -> (h_out, n): the block's output y [M, K] normed (post_weight f32 [K]), multiplied by a gate
+    ([K] or [M, K], of y's type), scaled and added to the residual h [M, K]; the sum normed (weight f32 [K]) for the next block.
+
+    n: [M, K] of type "f32", "bf16" or "f16"; or (codes int8 [M, K], scales f32) with out "token" (scales [M], for gemm_w8a8 and
+    ffn_gate_w8a8), "act" (interleaved, scales [M, K/128], for gemv_w4a8_q and ffn_gate_w4a8) or "rows" (interleaved, scales
+    [K/128, M], for gemm_w4a8_i8); None without weight.  h_out: of h's type, h itself to update in place; without y it is h.
+    See rt4_block_norm in include/rt4k.h."""
+    torch = _torch()
+    dev, f32 = _dev(), torch.float32
+    form = FORMS.get(out)
+    if form is None:
+        raise RT4Error(f"out: expected one of {sorted(FORMS)}, got {out!r}")
+    if h.dim() != 2:
+        raise RT4Error(f"h {tuple(h.shape)} is a matrix [M, K]")
+    if y is None and (h_out is not None or weight is None):
+        raise RT4Error("block_norm: without y there is no new residual, and weight is needed")
+    M, K = h.shape
+    ht = _type(h.dtype, "h")
+    hp, ldh = _mat(h, M, K, h.dtype, dev, "h")
+    op, ldho, yp, ldy, yt, gp, ldg = None, 0, None, 0, 0, None, 0
+    if y is not None:
+        yt = _type(y.dtype, "y")
+        yp, ldy = _mat(y, M, K, y.dtype, dev, "y")
+        if h_out is None:
+            h_out = torch.empty_strided((M, K), (K, 1), dtype=h.dtype, device=dev)
+            op, ldho = h_out.data_ptr(), K
+        else:
+            op, ldho = _mat(h_out, M, K, h.dtype, dev, "h_out")
+        if gate is not None:
+            gp, ldg = (_arg(gate, y.dtype, (K,), dev, "gate"), 0) if gate.dim() == 1 else _mat(gate, M, K, y.dtype, dev, "gate")
+    else:
+        h_out = h
+        if gate is not None or post_weight is not None:
+            raise RT4Error("block_norm: a gate and post_weight need y")
+    n = s = np_ = sp = None
+    if weight is not None:
+        n = torch.empty_strided((M, K), (K, 1), dtype=(f32, torch.bfloat16, torch.float16)[form] if form < 3 else torch.int8, device=dev)
+        np_ = n.data_ptr()
+        if form >= 3:
+            shape = ((M,), (M, K // GROUP), (K // GROUP, M))[form - 3]
+            s = torch.empty_strided(shape, (1,) if form == 3 else (shape[1], 1), dtype=f32, device=dev)
+            sp = s.data_ptr()
+    _check(lib().rt4_block_norm(
+        op, ldho, hp, ldh, ht, yp, ldy, yt, gp, ldg, None if post_weight is None else _arg(post_weight, f32, (K,), dev, "post_weight"),
+        None if weight is None else _arg(weight, f32, (K,), dev, "weight"), scale, eps, weight_offset, np_, sp, form, M, K,
+        _raw_stream(dev)))
+    return h_out, (n if s is None else (n, s))
+
+
+def quant_token_a8(x, xq=None, sx=None):
+    """x [M, K] (float32, bfloat16 or float16, rows may be strided) -> (xq int8 [M, K] in natural order, sx f32 [M]): one scale a
+    token, for gemm_w8a8 and ffn_gate_w8a8.  See rt4_quant_token_a8 in include/rt4k.h."""
+    torch = _torch()
+    dev = _dev()
+    if x.dim() != 2:
+        raise RT4Error(f"x {tuple(x.shape)} is a matrix [M, K]")
+    M, K = x.shape
+    t = _type(x.dtype, "x")
+    xp, ldx = _mat(x, M, K, x.dtype, dev, "x")
+    xq, qp = _out(xq, torch.int8, (M, K), (K, 1), dev, "xq")
+    sx, sp = _out(sx, torch.float32, (M,), (1,), dev, "sx")
+    _check(lib().rt4_quant_token_a8(qp, sp, xp, ldx, t, M, K, _raw_stream(dev)))
+    return xq, sx
