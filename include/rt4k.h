@@ -397,15 +397,21 @@ int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_
  * a scale sw[n] for each channel; all in natural order.  Sums are exact int32: K % 16 == 0 and at most 131056.
  * M >= 1, N >= 1; strides at least a row, ldx and ldw multiples of 16 below 2^24, xq and wq 16-byte aligned.
  * Each output is the sum's fp32 value times sx times sw, rounded to c_type; a scale that is not finite makes its
- * row or column so.  c must not overlap an input. */
+ * row or column so.  c must not overlap an input.  work: rt4_w8a8_work_bytes of device memory; with less, or NULL, K is
+ * not split (the same result, slower). */
 int rt4_gemm_w8a8(void* c, int64_t ldc, int c_type, const int8_t* wq, int64_t ldw, const float* sw, const int8_t* xq,
-                  int64_t ldx, const float* sx, int M, int N, int K, void* stream);
+                  int64_t ldx, const float* sx, int M, int N, int K, void* work, int64_t work_bytes, void* stream);
+
+/* Bytes of `work` with which a product (weights 1) or a gated half (weights 2) of these sizes runs best on the current
+ * device, 0 where it needs none.  Products of few tiles split K; the runs' int32 sums meet there (16-byte aligned, not
+ * initialized, free again when the call's work on its stream is done; every call that may overlap has one of its own). */
+int rt4_w8a8_work_bytes(int M, int N, int K, int weights, int64_t* bytes);
 
 /* First half of a gated feed-forward block on 8-bit weights: h [M][N] = act(g) * u with g and u the products of
  * rt4_gemm_w8a8 with the gate weights wg, sg and the up weights wu, su, in fp32 until h's rounding.  Arguments as there. */
 int rt4_ffn_gate_w8a8(void* h, int64_t ldh, int h_type, const int8_t* wg, int64_t ldg, const float* sg, const int8_t* wu,
                       int64_t ldu, const float* su, const int8_t* xq, int64_t ldx, const float* sx, int M, int N, int K,
-                      int act, void* stream);
+                      int act, void* work, int64_t work_bytes, void* stream);
 
 /* The same on RT4 weights for 1 to 4 rows: h f32 [rows][N] = act(g) * u with g and u what rt4_gemv_w4a8_q gives for the
  * gate weights and for the up weights (up to the order of the fp32 sums over groups).  xq and sa from rt4_quant_act_a8

@@ -922,21 +922,37 @@ static int check_linear8(const char* who, const rt4::Linear8& a, int weights) {
     return RT4_OK;
 }
 
-int rt4_gemm_w8a8(void* c, int64_t ldc, int c_type, const int8_t* wq, int64_t ldw, const float* sw, const int8_t* xq,
-                  int64_t ldx, const float* sx, int M, int N, int K, void* stream) {
-    const rt4::Linear8 a{c, ldc, {wq, nullptr}, {ldw, 0}, {sw, nullptr}, xq, ldx, sx, M, N, K, c_type, -1};
-    int rc = check_linear8("rt4_gemm_w8a8", a, 1);
+// The plan of a product on this device; without room for its runs' sums, that of one run a tile.
+static int run_linear8(const char* who, const rt4::Linear8& a, int weights, void* work, int64_t work_bytes, hipStream_t st) {
+    int cus = 0, rc = check_linear8(who, a, weights);
+    if (rc || (rc = device_cus(&cus))) return rc;
+    rt4::Linear8Plan p = rt4::linear8_plan(a.M, a.N, a.K, weights, cus);
+    if (p.part_bytes && (!work || work_bytes < 0 || (uint64_t)work_bytes < p.part_bytes)) p.splits = 1, p.part_bytes = 0;
+    if (p.part_bytes && !aligned(work, 16)) return fail(RT4_E_ARG, "%s: misaligned workspace (16 bytes)", who);
+    return hip_status(rt4::launch_linear8(a, p, work, st), who);
+}
+
+int rt4_w8a8_work_bytes(int M, int N, int K, int weights, int64_t* bytes) {
+    if (!bytes) return fail(RT4_E_ARG, "rt4_w8a8_work_bytes: null pointer");
+    if (M < 1 || N < 1 || M > (1 << 24) || N > (1 << 24) || K < 16 || K % 16 || K > kMaxK8 || weights < 1 || weights > 2)
+        return fail(RT4_E_SHAPE, "rt4_w8a8_work_bytes: M=%d N=%d K=%d weights=%d", M, N, K, weights);
+    int cus = 0, rc = device_cus(&cus);
     if (rc) return rc;
-    return hip_status(rt4::launch_linear8(a, as_stream(stream)), "rt4_gemm_w8a8 launch");
+    *bytes = (int64_t)rt4::linear8_plan(M, N, K, weights, cus).part_bytes;
+    return RT4_OK;
+}
+
+int rt4_gemm_w8a8(void* c, int64_t ldc, int c_type, const int8_t* wq, int64_t ldw, const float* sw, const int8_t* xq,
+                  int64_t ldx, const float* sx, int M, int N, int K, void* work, int64_t work_bytes, void* stream) {
+    const rt4::Linear8 a{c, ldc, {wq, nullptr}, {ldw, 0}, {sw, nullptr}, xq, ldx, sx, M, N, K, c_type, -1};
+    return run_linear8("rt4_gemm_w8a8", a, 1, work, work_bytes, as_stream(stream));
 }
 
 int rt4_ffn_gate_w8a8(void* h, int64_t ldh, int h_type, const int8_t* wg, int64_t ldg, const float* sg, const int8_t* wu,
                       int64_t ldu, const float* su, const int8_t* xq, int64_t ldx, const float* sx, int M, int N, int K,
-                      int act, void* stream) {
+                      int act, void* work, int64_t work_bytes, void* stream) {
     const rt4::Linear8 a{h, ldh, {wg, wu}, {ldg, ldu}, {sg, su}, xq, ldx, sx, M, N, K, h_type, act};
-    int rc = check_linear8("rt4_ffn_gate_w8a8", a, 2);
-    if (rc) return rc;
-    return hip_status(rt4::launch_linear8(a, as_stream(stream)), "rt4_ffn_gate_w8a8 launch");
+    return run_linear8("rt4_ffn_gate_w8a8", a, 2, work, work_bytes, as_stream(stream));
 }
 
 int rt4_ffn_gate_w4a8(float* h, const uint32_t* wg, const uint16_t* sg, const uint32_t* wu, const uint16_t* su,

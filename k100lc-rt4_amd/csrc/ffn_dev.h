@@ -4,19 +4,18 @@
 
 namespace rt4 {
 
-// Element types as the ABI numbers them (RT4_F32, RT4_BF16, RT4_F16).
+// Element types and activations as the ABI numbers them (RT4_F32, RT4_BF16, RT4_F16; RT4_SILU, RT4_GELU_TANH).
 enum { kF32 = 0, kBF16 = 1, kF16 = 2 };
+enum { kSilu = 0, kGeluTanh = 1 };
 typedef __bf16 bf16;
 typedef _Float16 f16;
 
 // x / (1 + exp(-x)) or, by tanh's own definition, 0.5 x (1 + tanh z) = x / (1 + exp(-2 z)): one
 // exponential to the base 2 and one reciprocal (1 ulp each).  The exponent's rounding, 2^-24 of it,
 // is the largest error: 2^-24 |x| of the result, 5e-7 at |x| = 8.
-template <int ACT>
-__device__ __forceinline__ float activate(float x) {
-    float e;
-    if (ACT == 0) e = x * -1.44269504088896341f;
-    else e = x * fmaf(x * x, -2.0f * 1.44269504088896341f * 0.79788456080286536f * 0.044715f, -2.0f * 1.44269504088896341f * 0.79788456080286536f);
+__device__ __forceinline__ float activate(float x, int act) {
+    constexpr float log2e = 1.44269504088896341f, z = 2.0f * log2e * 0.79788456080286536f;
+    const float e = x * (act == kSilu ? -log2e : fmaf(x * x, -z * 0.044715f, -z));
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(e));
 }
 

@@ -9,7 +9,7 @@ namespace rt4 {
 namespace {
 
 // A wave owns one output column: lane l takes 16 bytes (a quarter of a 128-group) of both its weight rows.
-template <int M, int ACT>
+template <int M>
 __global__ __launch_bounds__(256) void gate4_k(Gate4 a) {
     const int lane = threadIdx.x & 63;
     const int n = uniform((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
@@ -42,15 +42,14 @@ __global__ __launch_bounds__(256) void gate4_k(Gate4 a) {
 #pragma unroll
     for (int m = 0; m < M; m++) {
         const float g = wave_sum(y[0][m]), u = wave_sum(y[1][m]);
-        if (lane == 0) a.out[(size_t)m * a.N + n] = activate<ACT>(g) * u;
+        if (lane == 0) a.out[(size_t)m * a.N + n] = activate(g, a.act) * u;
     }
 }
 
 template <int M>
 void launch_rows(const Gate4& a, hipStream_t st) {
     const dim3 grid((unsigned)((a.N + 3) / 4));
-    if (a.act == 0) hipLaunchKernelGGL((gate4_k<M, 0>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((gate4_k<M, 1>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((gate4_k<M>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace

@@ -199,7 +199,13 @@ struct Linear8 {
     const float* sx;
     int M, N, K, type, act;              // act < 0: the product alone
 };
-hipError_t launch_linear8(const Linear8& a, hipStream_t st);
+// How a product runs: the form of its tiles, how many runs their steps are split into, and the bytes of the runs' sums.
+struct Linear8Plan {
+    int form, tiles, splits;
+    size_t part_bytes;
+};
+Linear8Plan linear8_plan(int M, int N, int K, int weights, int cus);
+hipError_t launch_linear8(const Linear8& a, const Linear8Plan& p, void* part, hipStream_t st);
 
 struct Gate4 {
     float* out;

@@ -41,7 +41,7 @@ C_EXPORTS = (
     "rt4_attn_q_quant", "rt4_kv_append_k", "rt4_kv_append_v", "rt4_attention_prefill",
     "rt4_attention_prefill_cfg", "rt4_attention_launch_plan",
     "rt4_kv_append_rows", "rt4_attention_tree", "rt4_verify_tree",
-    "rt4_gemm_w8a8", "rt4_ffn_gate_w8a8", "rt4_ffn_gate_w4a8", "rt4_block_norm", "rt4_quant_token_a8",
+    "rt4_w8a8_work_bytes", "rt4_gemm_w8a8", "rt4_ffn_gate_w8a8", "rt4_ffn_gate_w4a8", "rt4_block_norm", "rt4_quant_token_a8",
     "rt4_file_open", "rt4_file_close", "rt4_file_count", "rt4_file_find", "rt4_file_info", "rt4_file_data",
     "rt4_file_size", "rt4_file_upload", "rt4_file_upload_tensor",
 )
@@ -100,8 +100,9 @@ _SIGS = {
     "rt4_attention_launch_plan": [_I, _I, _I, _I, _I, _I, _I, _P, _P, _P],
     "rt4_kv_append_rows": [_P] * 10 + [_I] * 4 + [_P],
     "rt4_attention_tree": [_P] * 13 + [_I] * 8 + [_P],
-    "rt4_gemm_w8a8": [_P, _L, _I, _P, _L, _P, _P, _L, _P, _I, _I, _I, _P],
-    "rt4_ffn_gate_w8a8": [_P, _L, _I, _P, _L, _P, _P, _L, _P, _P, _L, _P, _I, _I, _I, _I, _P],
+    "rt4_w8a8_work_bytes": [_I, _I, _I, _I, _P],
+    "rt4_gemm_w8a8": [_P, _L, _I, _P, _L, _P, _P, _L, _P, _I, _I, _I, _P, _L, _P],
+    "rt4_ffn_gate_w8a8": [_P, _L, _I, _P, _L, _P, _P, _L, _P, _P, _L, _P, _I, _I, _I, _I, _P, _L, _P],
     "rt4_ffn_gate_w4a8": [_P] * 7 + [_I] * 4 + [_P],
     "rt4_block_norm": [_P, _L, _P, _L, _I, _P, _L, _I, _P, _L, _P, _P, _D, _D, _D, _P, _P, _I, _I, _I, _P],
     "rt4_quant_token_a8": [_P, _P, _P, _L, _I, _I, _I, _P],
@@ -626,6 +627,9 @@ def _mat(t, rows, cols, dtype, dev, name):
                    f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
 
 
+_work_bytes = {}
+
+
 def _linear8(fn, weights, xq, sx, act, out, dtype):
     torch = _torch()
     dev, f32, i8 = _dev(), torch.float32, torch.int8
@@ -647,7 +651,18 @@ def _linear8(fn, weights, xq, sx, act, out, dtype):
     args = []
     for name, w, sname, s in weights:
         args += [*_mat(w, N, K, i8, dev, name), _arg(s, f32, (N,), dev, sname)]
-    _check(fn(op, ldo, t, *args, xp, ldx, _arg(sx, f32, (M,), dev, "sx"), M, N, K, *act, _raw_stream(dev)))
+    # The runs' sums of split products: memory of the caching allocator, which keeps it from others until the stream is past it.
+    key = (M, N, K, len(weights), dev)
+    nb = _work_bytes.get(key)
+    if nb is None:
+        b = ctypes.c_int64()
+        _check(lib().rt4_w8a8_work_bytes(M, N, K, len(weights), ctypes.byref(b)))
+        if len(_work_bytes) > 4096:              # (sizes alone; they are asked for again)
+            _work_bytes.clear()
+        nb = _work_bytes[key] = b.value
+    work = torch.empty_strided((nb,), (1,), dtype=torch.uint8, device=dev) if nb else None
+    _check(fn(op, ldo, t, *args, xp, ldx, _arg(sx, f32, (M,), dev, "sx"), M, N, K, *act, None if work is None else work.data_ptr(), nb,
+              _raw_stream(dev)))
     return out
 
 

@@ -72,7 +72,8 @@ def gate_flushed(g, u):
 
 SHAPES = [(1, 1, 16), (1, 33, 48), (2, 64, 112), (3, 100, 256), (4, 129, 144), (5, 31, 2064), (16, 160, 320), (17, 257, 1040), (31, 65, 528),
           (33, 500, 64), (64, 300, 400), (65, 640, 208), (100, 1000, 1120), (128, 128, 128), (129, 385, 656), (200, 77, 5120), (257, 513, 272),
-          (300, 1100, 1024), (513, 260, 784), (1030, 520, 192)]
+          (300, 1100, 1024), (513, 260, 784), (1030, 520, 192), (6, 66, 4112), (7, 10, 16), (8, 1023, 2064), (9, 20, 20000),
+          (40, 130, 8208), (130, 70, 16400), (300, 140, 12304), (1024, 2500, 160), (2, 6, 5120)]
 
 
 @pytest.mark.gpu
@@ -489,7 +490,7 @@ def test_product_refusals(rt4):
     L = rt4.lib()
 
     def call(c=DUMMY, ldc=64, t=0, w=DUMMY, ldw=256, sw=DUMMY, x=DUMMY, ldx=256, sx=DUMMY, M=4, N=64, K=256):
-        return L.rt4_gemm_w8a8(c, ldc, t, w, ldw, sw, x, ldx, sx, M, N, K, None)
+        return L.rt4_gemm_w8a8(c, ldc, t, w, ldw, sw, x, ldx, sx, M, N, K, None, 0, None)
 
     for name in ("c", "w", "sw", "x", "sx"):
         assert call(**{name: None}) == 2
@@ -505,7 +506,7 @@ def test_gated_refusals(rt4):
     L = rt4.lib()
 
     def call(h=DUMMY, ldh=64, t=1, wg=DUMMY, ldg=256, sg=DUMMY, wu=DUMMY, ldu=256, su=DUMMY, x=DUMMY, ldx=256, sx=DUMMY, M=4, N=64, K=256, act=0):
-        return L.rt4_ffn_gate_w8a8(h, ldh, t, wg, ldg, sg, wu, ldu, su, x, ldx, sx, M, N, K, act, None)
+        return L.rt4_ffn_gate_w8a8(h, ldh, t, wg, ldg, sg, wu, ldu, su, x, ldx, sx, M, N, K, act, None, 0, None)
 
     for name in ("h", "wg", "sg", "wu", "su", "x", "sx"):
         assert call(**{name: None}) == 2
