@@ -415,7 +415,7 @@ int rt4_ffn_gate_w8a8(void* h, int64_t ldh, int h_type, const int8_t* wg, int64_
 
 /* The same on RT4 weights for 1 to 4 rows: h f32 [rows][N] = act(g) * u with g and u what rt4_gemv_w4a8_q gives for the
  * gate weights and for the up weights (up to the order of the fp32 sums over groups).  xq and sa from rt4_quant_act_a8
- * or rt4_block_norm (RT4_ACT).  K % 128 == 0; h must not overlap an input. */
+ * or rt4_block_norm (RT4_ACT).  K % 128 == 0 and at most 38912; h must not overlap an input. */
 int rt4_ffn_gate_w4a8(float* h, const uint32_t* wg, const uint16_t* sg, const uint32_t* wu, const uint16_t* su,
                       const int8_t* xq, const float* sa, int rows, int N, int K, int act, void* stream);
 

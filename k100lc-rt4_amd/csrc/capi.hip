@@ -962,8 +962,11 @@ int rt4_ffn_gate_w4a8(float* h, const uint32_t* wg, const uint16_t* sg, const ui
     int rc = check_gemv_shape("rt4_ffn_gate_w4a8", rows, N, K);
     if (rc || (rc = check_gemv_align("rt4_ffn_gate_w4a8", h, wg, sg, xq, sa)) || (rc = check_gemv_align("rt4_ffn_gate_w4a8", h, wu, su, xq, sa)))
         return rc;
+    if (K > rt4::kGate4MaxK) return fail(RT4_E_SHAPE, "rt4_ffn_gate_w4a8: K=%d is above %d", K, rt4::kGate4MaxK);
+    int cus = 0;
+    if ((rc = device_cus(&cus))) return rc;
     const rt4::Gate4 a{h, {wg, wu}, {sg, su}, xq, sa, rows, N, K, act};
-    return hip_status(rt4::launch_gate4(a, as_stream(stream)), "rt4_ffn_gate_w4a8 launch");
+    return hip_status(rt4::launch_gate4(a, cus, as_stream(stream)), "rt4_ffn_gate_w4a8 launch");
 }
 
 // Bytes of an element of a type, and whether rows of them can be read 16 bytes at a time.
@@ -984,10 +987,9 @@ static int run_norm(const char* who, rt4::BlockNorm& a, hipStream_t st) {
     if (!aligned(a.h, hb) || !aligned(a.h_out, hb) || !aligned(a.y, yb) || !aligned(a.gate, yb) || !aligned(a.post_w, 4) ||
         !aligned(a.w, 4) || !aligned(a.n, a.form > RT4_TOKEN ? 8 : nb) || !aligned(a.n_scale, 4))
         return fail(RT4_E_ARG, "%s: misaligned pointer (codes of groups need 8 bytes)", who);
-    a.vec = vec_rows(a.h, a.ldh, a.h_type) && (!a.y || (vec_rows(a.y, a.ldy, a.y_type) && vec_rows(a.h_out, a.ldho, a.h_type))) &&
-            (!a.gate || vec_rows(a.gate, a.ldg, a.y_type));
-    a.wvec = aligned(a.w, 16) && aligned(a.post_w, 16);
-    a.nvec = aligned(a.n, 16) && (size_t)a.K * nb % (nb == 1 ? 8 : 16) == 0;
+    a.vec = a.K % 8 == 0 && vec_rows(a.h, a.ldh, a.h_type) && (!a.y || (vec_rows(a.y, a.ldy, a.y_type) && vec_rows(a.h_out, a.ldho, a.h_type))) &&
+            (!a.gate || vec_rows(a.gate, a.ldg, a.y_type)) && aligned(a.w, 16) && aligned(a.post_w, 16) && aligned(a.n, 16);
+    a.inv_k = 1.0 / a.K;
     return hip_status(rt4::launch_block_norm(a, st), who);
 }
 
@@ -997,13 +999,13 @@ int rt4_block_norm(void* h_out, int64_t ldho, const void* h, int64_t ldh, int h_
     if (!h || (y && !h_out) || (!y && !n) || (!n != !w)) return fail(RT4_E_ARG, "rt4_block_norm: null pointer (h; h_out with y; n with w; n without y)");
     if (!y && (gate || post_w)) return fail(RT4_E_ARG, "rt4_block_norm: a gate and a norm behind the block need y");
     if (!(eps >= 0)) return fail(RT4_E_ARG, "rt4_block_norm: eps=%g", eps);
-    rt4::BlockNorm a{h_out, ldho, h, ldh, y, ldy, gate, ldg, post_w, w, n, n_scale, scale, eps, w_offset, M, K, h_type, y ? y_type : 0, n_form, false, false, false};
+    rt4::BlockNorm a{h_out, ldho, h, ldh, y, ldy, gate, ldg, post_w, w, n, n_scale, scale, eps, w_offset, 0, M, K, h_type, y ? y_type : 0, n_form, false};
     return run_norm("rt4_block_norm", a, as_stream(stream));
 }
 
 int rt4_quant_token_a8(int8_t* xq, float* sx, const void* x, int64_t ldx, int x_type, int M, int K, void* stream) {
     if (!xq || !sx || !x) return fail(RT4_E_ARG, "rt4_quant_token_a8: null pointer");
-    rt4::BlockNorm a{nullptr, 0, x, ldx, nullptr, 0, nullptr, 0, nullptr, nullptr, xq, sx, 1.0, 0.0, 0.0, M, K, x_type, 0, RT4_TOKEN, false, false, false};
+    rt4::BlockNorm a{nullptr, 0, x, ldx, nullptr, 0, nullptr, 0, nullptr, nullptr, xq, sx, 1.0, 0.0, 0.0, 0, M, K, x_type, 0, RT4_TOKEN, false};
     return run_norm("rt4_quant_token_a8", a, as_stream(stream));
 }
 

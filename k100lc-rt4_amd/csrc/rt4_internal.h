@@ -215,7 +215,8 @@ struct Gate4 {
     const float* sa;
     int rows, N, K, act;
 };
-hipError_t launch_gate4(const Gate4& a, hipStream_t st);
+constexpr int kGate4MaxK = 38912;     // four rows of codes and scales in a workgroup's LDS
+hipError_t launch_gate4(const Gate4& a, int cus, hipStream_t st);
 
 // Forms of the normed rows: floats by their type (0..2), int8 codes with a scale for each token, or for each
 // 128-group as the decode (kAct) and the prefill (kRows) quantizers lay them out.
@@ -234,9 +235,9 @@ struct BlockNorm {
     const float* w;                      // null (no y): the values as they are
     void* n;                             // null: h_out alone
     float* n_scale;
-    double scale, eps, w_offset;
+    double scale, eps, w_offset, inv_k;
     int M, K, h_type, y_type, form;
-    bool vec, wvec, nvec;                // whether rows of h, y, gate and h_out, the weights, and n's rows are aligned for vector access
+    bool vec;                            // whether all rows are whole chunks of 8, aligned for vector access
 };
 hipError_t launch_block_norm(const BlockNorm& a, hipStream_t st);
 
