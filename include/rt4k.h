@@ -395,7 +395,7 @@ int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_
 /* 8-bit product: c [M][N] (c_type, row stride ldc elements) = sx[m] sw[n] Σ_k xq[m][k] wq[n][k] with
  * xq int8 [M][K] (row stride ldx bytes), a scale sx[m] for each token, wq int8 [N][K] (row stride ldw),
  * a scale sw[n] for each channel; all in natural order.  Sums are exact int32: K % 16 == 0 and at most 131056.
- * M >= 1, N >= 1; strides at least a row, ldx and ldw multiples of 16 below 2^24, xq and wq 16-byte aligned.
+ * 1 <= M, N <= 2^24 and at most 2^31 tiles of 64 x 32 outputs; strides at least a row, ldx and ldw multiples of 16 below 2^24, xq and wq 16-byte aligned.
  * Each output is the sum's fp32 value times sx times sw, rounded to c_type; a scale that is not finite makes its
  * row or column so.  c must not overlap an input.  work: rt4_w8a8_work_bytes of device memory; with less, or NULL, K is
  * not split (the same result, slower). */

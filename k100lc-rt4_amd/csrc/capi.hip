@@ -906,8 +906,8 @@ static int check_linear8(const char* who, const rt4::Linear8& a, int weights) {
         if (!a.w[j] || !a.sw[j]) return fail(RT4_E_ARG, "%s: null pointer", who);
     if (a.type < RT4_F32 || a.type > RT4_F16) return fail(RT4_E_ARG, "%s: output type %d", who, a.type);
     if (weights == 2 && (a.act < RT4_SILU || a.act > RT4_GELU_TANH)) return fail(RT4_E_ARG, "%s: activation %d", who, a.act);
-    if (a.M < 1 || a.N < 1 || a.M > (1 << 24) || a.N > (1 << 24))
-        return fail(RT4_E_SHAPE, "%s: M=%d N=%d (1 to 2^24)", who, a.M, a.N);
+    if (a.M < 1 || a.N < 1 || a.M > (1 << 24) || a.N > (1 << 24) || (long long)((a.M + 63) / 64) * ((a.N + 31) / 32) > INT32_MAX)
+        return fail(RT4_E_SHAPE, "%s: M=%d N=%d (1 to 2^24, at most 2^31 tiles of 64 x 32)", who, a.M, a.N);
     if (a.K < 16 || a.K % 16 || a.K > kMaxK8) return fail(RT4_E_SHAPE, "%s: K=%d is not a multiple of 16 from 16 to %d", who, a.K, kMaxK8);
     if (a.ldo < a.N) return fail(RT4_E_SHAPE, "%s: output row stride %lld is below N=%d", who, (long long)a.ldo, a.N);
     const long long ld[3] = {a.ldx, a.ldw[0], a.ldw[1]};
@@ -934,7 +934,7 @@ static int run_linear8(const char* who, const rt4::Linear8& a, int weights, void
 
 int rt4_w8a8_work_bytes(int M, int N, int K, int weights, int64_t* bytes) {
     if (!bytes) return fail(RT4_E_ARG, "rt4_w8a8_work_bytes: null pointer");
-    if (M < 1 || N < 1 || M > (1 << 24) || N > (1 << 24) || K < 16 || K % 16 || K > kMaxK8 || weights < 1 || weights > 2)
+    if (M < 1 || N < 1 || M > (1 << 24) || N > (1 << 24) || (long long)((M + 63) / 64) * ((N + 31) / 32) > INT32_MAX || K < 16 || K % 16 || K > kMaxK8 || weights < 1 || weights > 2)
         return fail(RT4_E_SHAPE, "rt4_w8a8_work_bytes: M=%d N=%d K=%d weights=%d", M, N, K, weights);
     int cus = 0, rc = device_cus(&cus);
     if (rc) return rc;

@@ -23,20 +23,22 @@ __device__ __forceinline__ float finish(int i0, int i1, float sx, float s0, floa
 
 // ---- Tiles on the matrix cores.  A workgroup of WM x WN waves owns BM tokens and BN weight rows, a wave 32 TM x 32 TN of
 // them as fragments of v_mfma_i32_32x32x32_i8 with the weights as A: a lane then holds one token (lane & 31) and runs of 4
-// channels (8 (i >> 2) + 4 (lane >> 5) + (i & 3)).  With two weight matrices (NW) the first half of a wave's fragments are
-// gate rows and the second half the up rows of the same channels, so both factors of an output meet in one lane.
+// channels (8 (i >> 2) + 4 (lane >> 5) + (i & 3)).  With two weight matrices (NW) a fragment is 16 gate rows and the up rows
+// of the same 16 channels, so both factors of an output meet in one lane, as registers i and i + 8.
 //
 // Steps are 128 codes deep: whole cache lines of a row.  Operands arrive by DMA (8 rows x 128 bytes an instruction) in a
 // ring of ST stages; in a stage, chunk c (16 bytes) of row r lies at slot c ^ (r >> 1 & 7), which puts the 16 rows that one
 // cycle of a read serves into 16 different bank groups.  One barrier a step, before its last quarter: by then every wave
 // has read the stage for the last time, and the DMA of the step ST further on goes into it from there on.
-template <int TM_, int TN_, int WM_, int WN_, int ST_>
+template <int TM_, int TN_, int WM_, int WN_, int ST_, int PER_CU_>
 struct Tile {
-    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, ST = ST_, W = WM * WN;
-    static constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128, LDS = ST * STAGE;
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, ST = ST_, W = WM * WN, PER_CU = PER_CU_;
+    static constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128;
+    static constexpr int SLAB = 32 * (TN * 32 * 4 + 16) + TN * 128;       // a wave's share of LDS for fp32 outputs and scales
+    static constexpr int LDS = ST * STAGE > W * SLAB ? ST * STAGE : W * SLAB;
     static constexpr int PA = BM / 8 / W, PB = BN / 8 / W, P = PA + PB;   // DMA instructions of a wave a step
-    static_assert(BM % (8 * W) == 0 && BN % (8 * W) == 0 && TN % 2 == 0 && WM <= 2, "");
-    static_assert(LDS <= 160 * 1024 && 32 * (TN * 32 * 4 + 16) * W <= LDS, "a slab of fp32 outputs fits a wave's share");
+    static_assert(BM % (8 * W) == 0 && BN % (8 * W) == 0 && (ST - 2) * P < 64, "");
+    static_assert(LDS * PER_CU <= 160 * 1024, "");
 };
 
 struct Where {                           // a workgroup's tile and steps
@@ -56,51 +58,42 @@ __device__ __forceinline__ Where where(const Linear8& a, int splits, int b, int 
     w.m0 = (first + in % rows) * C::BM;
     w.n0 = in / rows * (C::BN / NW);
     const int steps = (a.K + 127) >> 7;
-    w.s0 = (int)((long long)steps * w.part / splits);
-    w.s1 = (int)((long long)steps * (w.part + 1) / splits);
-    return w;
+    w.s0 = steps * w.part / splits;
+    w.s1 = steps * (w.part + 1) / splits;
+    // The divisions above are done on the vector ALU.  Everything that goes by them is made scalar here, once: a base address
+    // that v_readfirstlane writes needs five wait states before a load reads it, and before those in inline assembly the
+    // compiler puts none.
+    return Where{uniform(w.tile), uniform(w.part), uniform(w.m0), uniform(w.n0), uniform(w.s0), uniform(w.s1)};
 }
 
-// The scales of a lane's channels: runs of 4 from n0 + 8 q + 4 (lane >> 5).
-template <int NC>
-__device__ __forceinline__ void load_scales(float (&s)[NC * 16], const float* sw, int n0, int N) {
-    const int hi = (threadIdx.x & 63) >> 5;
-#pragma unroll
-    for (int q = 0; q < NC * 4; q++) {
-        const int n = n0 + 8 * q + 4 * hi;
-        if (n + 4 <= N) __builtin_memcpy(&s[4 * q], sw + n, 16);
-        else
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[4 * q + e] = sw[min(n + e, N - 1)];
-    }
-}
-
-// 32 tokens x 32 NC channels of a wave from its sums: through the wave's own LDS, out in 16-byte pieces of rows.
-template <int NW, class T, int NC>
-__device__ __forceinline__ void write_slab(const Linear8& a, const v16i* i0, const v16i* i1, const float* s0, const float* s1, int m0, int n0,
-                                           unsigned char* lds) {
-    constexpr int PITCH = NC * 32 * (int)sizeof(T) + 16, PER = 16 / (int)sizeof(T), LPR = NC * 32 / PER;
+// 32 tokens of a wave's TN fragments from their sums: through the wave's own LDS, out in 16-byte pieces of rows.
+template <int NW, class T, int TN>
+__device__ __forceinline__ void write_slab(const Linear8& a, const v16i* acc, const float* scales, int m0, int n0, unsigned char* lds) {
+    constexpr int COLS = TN * 32 / NW, PITCH = COLS * (int)sizeof(T) + 16, PER = 16 / (int)sizeof(T), LPR = COLS / PER;
     const int lane = threadIdx.x & 63, ml = lane & 31, hi = lane >> 5;
     const float sx = a.sx[min(m0 + ml, a.M - 1)];
 #pragma unroll
-    for (int c = 0; c < NC; c++)
+    for (int q = 0; q < COLS / 8; q++) {         // 8 channels: registers 4 (q % per) .. of fragment q / per
+        constexpr int per = 4 / NW;
+        const v16i& f = acc[q / per];
+        float s[NW][4];
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            T t[4];
+        for (int j = 0; j < NW; j++) __builtin_memcpy(s[j], scales + j * COLS + 8 * q + 4 * hi, 16);
+        T t[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int k = 16 * c + 4 * q + e;
-                t[e] = (T)finish<NW>(i0[c][4 * q + e], NW == 1 ? 0 : i1[c][4 * q + e], sx, s0[k], NW == 1 ? 0.f : s1[k], a.act);
-            }
-            __builtin_memcpy(lds + ml * PITCH + (32 * c + 8 * q + 4 * hi) * sizeof(T), t, sizeof(t));
+        for (int e = 0; e < 4; e++) {
+            const int r = 4 * (q % per) + e;
+            t[e] = (T)finish<NW>(f[r], NW == 1 ? 0 : f[r + 8], sx, s[0][e], s[NW - 1][e], a.act);
         }
+        __builtin_memcpy(lds + ml * PITCH + (8 * q + 4 * hi) * sizeof(T), t, sizeof(t));
+    }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     const bool vec = ((uintptr_t)a.out & 15) == 0 && a.ldo * (int)sizeof(T) % 16 == 0;
-    const int col = lane % LPR * PER, n = n0 + col;
+    static_assert(32 * LPR % 64 == 0, "");
 #pragma unroll
     for (int k = 0; k < 32 * LPR / 64; k++) {
-        const int r = lane / LPR + k * (64 / LPR), m = m0 + r;
+        const int id = lane + 64 * k, r = id / LPR, col = id % LPR * PER, m = m0 + r, n = n0 + col;
         const uint4 d = *reinterpret_cast<const uint4*>(lds + r * PITCH + col * sizeof(T));
         if (m < a.M && n < a.N) {
             T* o = static_cast<T*>(a.out) + (size_t)m * a.ldo + n;
@@ -119,17 +112,17 @@ __device__ __forceinline__ void write_slab(const Linear8& a, const v16i* i0, con
     __builtin_amdgcn_wave_barrier();
 }
 
-// All outputs of a wave.
+// All outputs of a wave, whose share of LDS holds its channels' scales behind the slab.
 template <class C, int NW, int ROWS>
 __device__ __forceinline__ void write_wave(const Linear8& a, const v16i (&acc)[ROWS][C::TN], int m0, int n0, unsigned char* lds) {
-    constexpr int NC = C::TN / NW;
-    float s0[NC * 16], s1[NC * 16];
-    load_scales<NC>(s0, a.sw[0], n0, a.N);
-    if (NW == 2) load_scales<NC>(s1, a.sw[1], n0, a.N);
+    constexpr int COLS = C::TN * 32 / NW;
+    float* scales = reinterpret_cast<float*>(lds + C::SLAB - C::TN * 128);
+    for (int i = threadIdx.x & 63; i < C::TN * 32; i += 64) scales[i] = a.sw[NW == 1 ? 0 : i / COLS][min(n0 + i % COLS, a.N - 1)];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     const auto all = [&](auto t) {
 #pragma unroll
-        for (int i = 0; i < ROWS; i++)
-            write_slab<NW, decltype(t), NC>(a, acc[i], acc[i] + (NW == 2 ? NC : 0), s0, s1, m0 + 32 * i, n0, lds);
+        for (int i = 0; i < ROWS; i++) write_slab<NW, decltype(t), C::TN>(a, acc[i], scales, m0 + 32 * i, n0, lds);
     };
     if (a.type == kF32) all(float{});
     else if (a.type == kBF16) all(bf16{});
@@ -141,10 +134,18 @@ __device__ __forceinline__ void wait_dma_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// A DMA in two parts: where its rows go (M0, which the compiler leaves alone; one wait state until its use), and the load, whose immediate offset is added
+// to both addresses.
+__device__ __forceinline__ void set_m0(uint32_t l) { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" ::"s"((uint32_t)__builtin_amdgcn_readfirstlane((int)l)) : "memory"); }
+template <int IMM>
+__device__ __forceinline__ void dma16_m0(uint32_t voff, const void* gbase) {
+    asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2" ::"v"(voff), "s"(sptr(gbase)), "n"(IMM) : "memory");
+}
+
 // part null: whole tiles; else this workgroup's sums (of one of `splits` runs of steps), a fragment's registers as they are.
 template <class C, int NW>
 __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int splits, int4* part) {
-    constexpr int TM = C::TM, TN = C::TN, ST = C::ST, PA = C::PA, P = C::P, FR = TM + TN, MF = TM * TN;
+    constexpr int TM = C::TM, TN = C::TN, ST = C::ST, PA = C::PA, P = C::P, FR = TM + TN, MF = TM * TN, HALF = P / 2;
     extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 63, w = uniform((int)(threadIdx.x >> 6)), wm = w / C::WN, wn = w % C::WN;
     const Where at = where<C, NW>(a, splits, blockIdx.x, gridDim.x);
@@ -157,23 +158,24 @@ __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int sp
     const int even = (lane & 7) ^ (lane >> 4);    // chunk that a lane brings of even pieces; of odd ones it is even ^ 4
     const int pa0 = w * PA, pb0 = w * C::PB;     // first pieces
     const auto chunk = [&](int t) { return even ^ ((t < PA ? pa0 + t : pb0 + t - PA) & 1) * 4; };
-    const auto mat = [&](int t) { return NW == 1 ? 0 : C::WM == 2 ? w & 1 : t - PA >= 2 * TN; };   // whose rows a weight piece is
+    const auto mat = [&](int t) { return NW == 1 ? 0 : (pb0 + t - PA) >> 1 & 1; };    // whose rows a weight piece is: see above
 #pragma unroll
     for (int t = 0; t < P; t++) {
         const int c = chunk(t);
         if (t < PA) {
-            voff[t] = (uint32_t)min((pa0 + t) * 8 + (lane >> 3), a.M - 1 - at.m0) * (uint32_t)a.ldx + c * 16;
+            voff[t] = (uint32_t)min((pa0 + t) * 8 + (lane >> 3), a.M - 1 - at.m0) * (uint32_t)a.ldx + c * 16 + (3 - t % 4) * 1024;
         } else {
-            int r = (pb0 + t - PA) * 8 + (lane >> 3);                                  // channel in the tile
-            if (NW == 2) r = (C::WM == 2 ? w >> 1 : w) * 16 * TN + (C::WM == 2 ? t - PA : (t - PA) % (2 * TN)) * 8 + (lane >> 3);
-            voff[t] = (uint32_t)min(r, a.N - 1 - at.n0) * (uint32_t)(mat(t) ? a.ldw[1] : a.ldw[0]) + c * 16;
+            const int b = pb0 + t - PA, r = (NW == 1 ? b : (b >> 2) * 2 + (b & 1)) * 8 + (lane >> 3);   // channel in the tile
+            voff[t] = (uint32_t)min(r, a.N - 1 - at.n0) * (uint32_t)(mat(t) ? a.ldw[1] : a.ldw[0]) + c * 16 + (3 - (t - PA) % 4) * 1024;
         }
     }
     const size_t k0 = (size_t)at.s0 * 128;
-    const int8_t* ga = a.x + (size_t)at.m0 * a.ldx + k0;
+    // An instruction's immediate offset counts for both addresses: pieces 1 KB apart in LDS need M0 set for every fourth
+    // alone.  In memory it is taken out again: voff holds 3072 less it, the bases 3072 less.
+    const int8_t* ga = a.x + (size_t)at.m0 * a.ldx + k0 - 3072;
     const int8_t* gb[NW];
 #pragma unroll
-    for (int j = 0; j < NW; j++) gb[j] = a.w[j] + (size_t)at.n0 * a.ldw[j] + k0;
+    for (int j = 0; j < NW; j++) gb[j] = a.w[j] + (size_t)at.n0 * a.ldw[j] + k0 - 3072;
     const uint32_t lds0 = lds_addr(smem);
     const uint32_t la = lds0 + (uint32_t)pa0 * 1024, lb = lds0 + C::BM * 128 + (uint32_t)pb0 * 1024;
     int issue = at.s0;                           // next step to bring
@@ -189,8 +191,15 @@ __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int sp
         }
     };
     const auto dma_piece = [&](int t) {          // (t is a constant wherever loops are unrolled)
-        if (t < PA) dma16<0>(voff[t], ga, la + in + t * 1024);
-        else dma16<0>(voff[t], gb[NW == 1 ? 0 : mat(t)], lb + in + (t - PA) * 1024);
+        const int u = t < PA ? t : t - PA;
+        if (u % 4 == 0 || t == HALF) set_m0((t < PA ? la : lb) + in + u / 4 * 4096);
+        const int8_t* g = t < PA ? ga : gb[NW == 1 ? 0 : mat(t)];
+        switch (u % 4) {
+            case 0: dma16_m0<0>(voff[t], g); break;
+            case 1: dma16_m0<1024>(voff[t], g); break;
+            case 2: dma16_m0<2048>(voff[t], g); break;
+            default: dma16_m0<3072>(voff[t], g);
+        }
     };
     const auto issued = [&]() {
         issue++;
@@ -199,9 +208,6 @@ __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int sp
         for (int j = 0; j < NW; j++) gb[j] += 128;
         in = next(in);
     };
-    // Pieces of a step that are brought behind the barrier, and in the first quarter of the step that follows.
-    constexpr int P3 = P / 2;
-
     v16i acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; i++)
@@ -239,11 +245,12 @@ __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int sp
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // M1: step s + ST - 1 is still being brought; M2: there is a step s + ST.
+    // Pieces of step s + ST are brought behind the barrier of step s and in the first quarter of the next.
+    // M1: there is a step s + ST - 1; M2: there is a step s + ST.
     const auto step = [&](int s, auto m1, auto m2) {
         constexpr bool M1 = decltype(m1)::value, M2 = decltype(m2)::value;
 #define RT4_C(x) std::integral_constant<int, (x)>{}
-        quarter(RT4_C(0), RT4_C(P3), RT4_C(M1 ? P : P3), true);
+        quarter(RT4_C(0), RT4_C(HALF), RT4_C(M1 ? P : HALF), true);
         if (M1) issued();
         quarter(RT4_C(1), RT4_C(0), RT4_C(0), true);
         quarter(RT4_C(2), RT4_C(0), RT4_C(0), true);
@@ -252,8 +259,7 @@ __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int sp
         else wait_dma_barrier<0>();
         if (whole && s + 2 == steps && s + 1 < at.s1) clear_tail();
         if (M2) begin_issue();
-        if (M1) quarter(RT4_C(3), RT4_C(0), RT4_C(M2 ? P3 : 0), true);
-        else quarter(RT4_C(3), RT4_C(0), RT4_C(0), s + 1 < at.s1);
+        quarter(RT4_C(3), RT4_C(0), RT4_C(M2 ? HALF : 0), M1 || s + 1 < at.s1);
 #undef RT4_C
     };
     typedef std::true_type yes;
@@ -266,7 +272,7 @@ __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int sp
             for (int t = 0; t < P; t++) dma_piece(t);
             issued();
         }
-    if (at.s1 - at.s0 >= ST) wait_dma_barrier<(ST - 2) * P>();
+    if (at.s1 - at.s0 >= ST - 1) wait_dma_barrier<(ST - 2) * P>();
     else wait_dma_barrier<0>();
     if (whole && at.s0 == steps - 1) clear_tail();
 #pragma unroll
@@ -274,7 +280,7 @@ __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int sp
     if (issue < at.s1) {
         begin_issue();
 #pragma unroll
-        for (int t = 0; t < P3; t++) dma_piece(t);
+        for (int t = 0; t < HALF; t++) dma_piece(t);
     }
     int s = at.s0;
     for (; s < at.s1 - ST; s++) step(s, yes{}, yes{});
@@ -293,21 +299,21 @@ __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int sp
         return;
     }
     __syncthreads();                             // the stages are free for the outputs
-    write_wave<C, NW, TM>(a, acc, at.m0 + wm * TM * 32, at.n0 + wn * (TN / NW) * 32, smem + (size_t)w * (C::LDS / C::W));
+    write_wave<C, NW, TM>(a, acc, at.m0 + wm * TM * 32, at.n0 + wn * (TN * 32 / NW), smem + (size_t)w * C::SLAB);
 }
 
 // Sums the runs of split tiles: a wave takes 32 tokens of a tile's wave.
 template <class C, int NW>
 __global__ __launch_bounds__(256) void linear8_join_k(Linear8 a, int splits, const int4* part, int waves) {
-    constexpr int TM = C::TM, TN = C::TN, SLAB = 32 * (TN / NW * 32 * 4 + 16);
-    __shared__ __align__(16) unsigned char smem[4 * SLAB];
+    constexpr int TM = C::TM, TN = C::TN;
+    extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 63, id = uniform((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
     if (id >= waves) return;                     // whole waves; no barrier follows
     const int i = id % TM, w = id / TM % C::W, tile = id / (TM * C::W);
     const int nm = (a.M + C::BM - 1) / C::BM, nn = (a.N + C::BN / NW - 1) / (C::BN / NW);
     constexpr int GM = 4;
     const int first = tile / (GM * nn) * GM, rows = min(GM, nm - first), in = tile - first * nn;
-    const int m0 = (first + in % rows) * C::BM + (w / C::WN * TM + i) * 32, n0 = in / rows * (C::BN / NW) + w % C::WN * (TN / NW) * 32;
+    const int m0 = (first + in % rows) * C::BM + (w / C::WN * TM + i) * 32, n0 = in / rows * (C::BN / NW) + w % C::WN * (TN * 32 / NW);
     if (m0 >= a.M || n0 >= a.N) return;
     v16i acc[1][TN];
 #pragma unroll
@@ -323,25 +329,25 @@ __global__ __launch_bounds__(256) void linear8_join_k(Linear8 a, int splits, con
                 const int4 v = p[(j * 4 + q) * 64];
                 acc[0][j][4 * q] += v.x, acc[0][j][4 * q + 1] += v.y, acc[0][j][4 * q + 2] += v.z, acc[0][j][4 * q + 3] += v.w;
             }
-    write_wave<C, NW, 1>(a, acc, m0, n0, smem + (threadIdx.x >> 6) * SLAB);
+    write_wave<C, NW, 1>(a, acc, m0, n0, smem + (threadIdx.x >> 6) * C::SLAB);
 }
 
-typedef Tile<4, 4, 2, 2, 2> T256x256;
-typedef Tile<2, 4, 2, 2, 3> T128x256;
-typedef Tile<2, 2, 2, 2, 2> T128x128;
-typedef Tile<1, 2, 2, 2, 3> T64x128;
-typedef Tile<1, 2, 1, 4, 2> T32x256;
-
+// Forms, by number: tiles whose counts fill rounds of workgroups for as many sizes as possible.
+#define RT4_TILES(F)                                                                                                              \
+    F(0, 4, 4, 2, 2, 2, 1) F(1, 2, 7, 4, 1, 2, 1) F(2, 2, 5, 4, 1, 3, 1) F(3, 2, 4, 2, 2, 3, 1) F(4, 1, 7, 4, 1, 3, 1)            \
+    F(5, 1, 5, 4, 1, 4, 1) F(6, 2, 2, 2, 2, 2, 2) F(7, 1, 2, 2, 2, 3, 2) F(8, 1, 1, 2, 2, 4, 2)
 template <class C, int NW>
 hipError_t launch_tile(const Linear8& a, const Linear8Plan& p, void* part, hipStream_t st) {
     auto k = linear8_tile_k<C, NW>;
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(k, dim3((unsigned)(p.tiles * p.splits)), dim3(64 * C::W), C::LDS, st, a, p.splits, p.splits > 1 ? static_cast<int4*>(part) : nullptr);
-    if (p.splits > 1) {
-        const int waves = p.tiles * C::W * C::TM;
-        hipLaunchKernelGGL((linear8_join_k<C, NW>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a, p.splits, static_cast<const int4*>(part), waves);
-    }
+    if (p.splits == 1) return hipGetLastError();
+    auto j = linear8_join_k<C, NW>;
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(j), hipFuncAttributeMaxDynamicSharedMemorySize, 4 * C::SLAB);
+    if (e != hipSuccess) return e;
+    const int waves = p.tiles * C::W * C::TM;
+    hipLaunchKernelGGL(j, dim3((unsigned)((waves + 3) / 4)), dim3(256), 4 * C::SLAB, st, a, p.splits, static_cast<const int4*>(part), waves);
     return hipGetLastError();
 }
 
@@ -421,46 +427,50 @@ hipError_t launch_dot(const Linear8& a, hipStream_t st) {
     return hipGetLastError();
 }
 
-// Forms: the tiles' sizes, workgroups a CU holds, and what a step and a tile's beginning and end take (us).
+constexpr int kDotMaxM = 8;
+// A form's tile, workgroups a CU holds, and its measured cost (us): a step where few workgroups run, what is added to that
+// where all do (power, the L2's rate), and a tile's beginning and end.  Fitted to 1045 times of 54 sizes (M 16..4000, N
+// 1000..17408, K 1024..17408, one and two weight matrices, every form, 1 to 4 splits); the choice made by them takes 2% longer
+// than the best one of each size.
 struct Shape {
     int bm, bn, per_cu;
-    double step, ends;
+    double step, full, ends;
 };
-constexpr int kDotForm = 5, kDotMaxM = 8;
-constexpr Shape kShapes[kDotForm] = {{256, 256, 1, 0.85, 8}, {128, 256, 1, 0.5, 5}, {128, 128, 2, 0.35, 4}, {64, 128, 2, 0.25, 3}, {32, 256, 2, 0.3, 3}};
+constexpr double kCost[][3] = {{1.284, 0.579, 4.234}, {0.826, 0.522, 19.111}, {0.495, 0.459, 12.053}, {0.692, 0.251, 3.318}, {0.475, 0.122, 15.473}, {0.469, 0.145, 8.014}, {0.733, 0.548, 0}, {0.359, 0.633, 0}, {0.184, 0.256, 1.108}};
+#define RT4_SHAPE(f, tm, tn, wm, wn, st, pc) {32 * tm * wm, 32 * tn * wn, pc, kCost[f][0], kCost[f][1], kCost[f][2]},
+constexpr Shape kShapes[] = {RT4_TILES(RT4_SHAPE)};
+constexpr int kDotForm = sizeof(kShapes) / sizeof(kShapes[0]);
+static_assert(kDotForm == sizeof(kCost) / sizeof(kCost[0]), "");
 
 }  // namespace
 
 Linear8Plan linear8_plan(int M, int N, int K, int weights, int cus) {
     Linear8Plan p{kDotForm, 0, 1, 0};
     if (M <= kDotMaxM) return p;
-    // An estimate of each form's time (us) with each number of splits.
+    // The form and number of splits of the lowest estimate.
     double best = 1e30;
     const int steps = (K + 127) / 128;
     for (int f = 0; f < kDotForm; f++) {
         const Shape& s = kShapes[f];
-        const int tiles = ((M + s.bm - 1) / s.bm) * ((N + s.bn / weights - 1) / (s.bn / weights));
-        for (int sp = 1; sp <= 16 && sp <= steps; sp++) {
-            const int groups = tiles * sp, slots = cus * s.per_cu;
-            const double rounds = (groups + slots - 1) / slots, share = groups < slots ? (double)groups / cus : s.per_cu;
-            const double step = fmax(s.step * fmax(1., share), 0.) ;
-            const double bytes = (double)tiles * sp * s.bm * s.bn * 4;
-            const double t = rounds * ((double)((steps + sp - 1) / sp) * step + s.ends) + (sp > 1 ? 3 + 2 * bytes / 4e6 : 0);
-            if (t < best) best = t, p = Linear8Plan{f, tiles, sp, sp > 1 ? (size_t)bytes : 0};
+        const long long tiles = (long long)((M + s.bm - 1) / s.bm) * ((N + s.bn / weights - 1) / (s.bn / weights)), slots = (long long)cus * s.per_cu;
+        for (int sp = 1; sp <= 8 && sp <= steps; sp++) {
+            const long long groups = tiles * sp;
+            if (sp > 1 && groups > 2 * slots) break;
+            const int n = (steps + sp - 1) / sp;
+            const double bytes = 4.0 * groups * s.bm * s.bn, part = (double)(groups % slots) / slots;
+            double t = groups / slots * (n * (s.step + s.full) + s.ends);
+            if (part > 0) t += n * (s.step + s.full * part) + s.ends;
+            if (sp > 1) t += 7.4 + 0.276e-6 * bytes;        // the runs' sums, out and in again, and the launch that joins them
+            if (t < best) best = t, p = Linear8Plan{f, (int)tiles, sp, sp > 1 ? (size_t)bytes : 0};
         }
     }
     return p;
 }
 
 hipError_t launch_linear8(const Linear8& a, const Linear8Plan& p, void* part, hipStream_t st) {
-    const bool one = a.act < 0;
-    switch (p.form) {
-        case 0: return one ? launch_tile<T256x256, 1>(a, p, part, st) : launch_tile<T256x256, 2>(a, p, part, st);
-        case 1: return one ? launch_tile<T128x256, 1>(a, p, part, st) : launch_tile<T128x256, 2>(a, p, part, st);
-        case 2: return one ? launch_tile<T128x128, 1>(a, p, part, st) : launch_tile<T128x128, 2>(a, p, part, st);
-        case 3: return one ? launch_tile<T64x128, 1>(a, p, part, st) : launch_tile<T64x128, 2>(a, p, part, st);
-        case 4: return one ? launch_tile<T32x256, 1>(a, p, part, st) : launch_tile<T32x256, 2>(a, p, part, st);
-    }
+#define RT4_LAUNCH(f, ...) \
+    if (p.form == f) return a.act < 0 ? launch_tile<Tile<__VA_ARGS__>, 1>(a, p, part, st) : launch_tile<Tile<__VA_ARGS__>, 2>(a, p, part, st);
+    RT4_TILES(RT4_LAUNCH)
     switch (a.M) {
         case 1: return launch_dot<1>(a, st);
         case 2: return launch_dot<2>(a, st);

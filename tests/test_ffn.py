@@ -495,7 +495,8 @@ def test_product_refusals(rt4):
     for name in ("c", "w", "sw", "x", "sx"):
         assert call(**{name: None}) == 2
     for kw in ({"M": 0}, {"N": 0}, {"M": -1}, {"K": 0}, {"K": 8}, {"K": 250}, {"K": 131072, "ldx": 131072, "ldw": 131072}, {"ldc": 63}, {"ldx": 240},
-               {"ldx": 264}, {"ldw": 255}, {"ldw": 1 << 24}, {"M": (1 << 24) + 1}, {"N": (1 << 24) + 1}):
+               {"ldx": 264}, {"ldw": 255}, {"ldw": 1 << 24}, {"M": (1 << 24) + 1}, {"N": (1 << 24) + 1},
+               {"M": 1 << 24, "N": 1 << 24, "ldc": 1 << 24}):
         assert call(**kw) == 1, kw
         assert "rt4_gemm_w8a8" in L.rt4_last_error().decode()
     for kw in ({"t": 3}, {"t": -1}, {"w": ODD}, {"x": ODD}, {"c": ctypes.c_void_p(0x1002)}, {"sx": ctypes.c_void_p(0x1002)}):
