@@ -113,8 +113,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gate4_k(Gate4 a) {
 template <int M>
 hipError_t launch_rows(const Gate4& a, int waves, hipStream_t st) {
     const size_t lds = (size_t)M * a.K + (size_t)M * (a.K >> 7) * 4;
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(gate4_k<M>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
+    if (lds > 65536) {                           // (what a launch is granted without asking)
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(gate4_k<M>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
     hipLaunchKernelGGL((gate4_k<M>), dim3((unsigned)((a.N + 2 * waves - 1) / (2 * waves))), dim3(64 * waves), lds, st, a);
     return hipGetLastError();
 }

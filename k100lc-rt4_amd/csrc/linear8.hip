@@ -146,7 +146,7 @@ __device__ __forceinline__ void dma16_m0(uint32_t voff, const void* gbase) {
 template <class C, int NW>
 __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int splits, int4* part) {
     constexpr int TM = C::TM, TN = C::TN, ST = C::ST, PA = C::PA, P = C::P, FR = TM + TN, MF = TM * TN, HALF = P / 2;
-    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ __align__(16) unsigned char smem[C::LDS];
     const int lane = threadIdx.x & 63, w = uniform((int)(threadIdx.x >> 6)), wm = w / C::WN, wn = w % C::WN;
     const Where at = where<C, NW>(a, splits, blockIdx.x, gridDim.x);
 
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int sp
 template <class C, int NW>
 __global__ __launch_bounds__(256) void linear8_join_k(Linear8 a, int splits, const int4* part, int waves) {
     constexpr int TM = C::TM, TN = C::TN;
-    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ __align__(16) unsigned char smem[4 * C::SLAB];
     const int lane = threadIdx.x & 63, id = uniform((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
     if (id >= waves) return;                     // whole waves; no barrier follows
     const int i = id % TM, w = id / TM % C::W, tile = id / (TM * C::W);
@@ -339,15 +339,11 @@ __global__ __launch_bounds__(256) void linear8_join_k(Linear8 a, int splits, con
 template <class C, int NW>
 hipError_t launch_tile(const Linear8& a, const Linear8Plan& p, void* part, hipStream_t st) {
     auto k = linear8_tile_k<C, NW>;
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k, dim3((unsigned)(p.tiles * p.splits)), dim3(64 * C::W), C::LDS, st, a, p.splits, p.splits > 1 ? static_cast<int4*>(part) : nullptr);
+    hipLaunchKernelGGL(k, dim3((unsigned)(p.tiles * p.splits)), dim3(64 * C::W), 0, st, a, p.splits, p.splits > 1 ? static_cast<int4*>(part) : nullptr);
     if (p.splits == 1) return hipGetLastError();
     auto j = linear8_join_k<C, NW>;
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(j), hipFuncAttributeMaxDynamicSharedMemorySize, 4 * C::SLAB);
-    if (e != hipSuccess) return e;
     const int waves = p.tiles * C::W * C::TM;
-    hipLaunchKernelGGL(j, dim3((unsigned)((waves + 3) / 4)), dim3(256), 4 * C::SLAB, st, a, p.splits, static_cast<const int4*>(part), waves);
+    hipLaunchKernelGGL(j, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a, p.splits, static_cast<const int4*>(part), waves);
     return hipGetLastError();
 }
 

@@ -598,79 +598,102 @@ def verify_tree(logits, draft, parent, u, temp=None, draft_probs=None, max_child
 
 
 # ---------------------------------- 8-bit linears, norms between blocks ----
+# These calls launch a few microseconds of GPU work, so what they need of torch and of the library is looked up once, and the
+# arguments of a good call are checked in one expression; `_refuse` finds out what is wrong with a bad one.
 ACTS = {"silu": 0, "gelu_tanh": 1}
 FORMS = {"f32": 0, "bf16": 1, "f16": 2, "token": 3, "act": 4, "rows": 5}
-_types = None
 
 
-def _type(dtype, name):
-    """The ABI's number of an element type."""
-    global _types
-    if _types is None:
+class _Env:
+    def __init__(self):
         torch = _torch()
-        _types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    t = _types.get(dtype)
-    if t is None:
-        raise RT4Error(f"{name}: expected float32, bfloat16 or float16, got {dtype}")
-    return t
+        torch.cuda.current_device()              # (initialises CUDA, or says why it cannot)
+        L = lib()
+        self.f32, self.i8, self.i32, self.i16, self.f16, self.u8 = (torch.float32, torch.int8, torch.int32, torch.int16, torch.float16,
+                                                                    torch.uint8)
+        self.types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+        self.out_types = (torch.float32, torch.bfloat16, torch.float16, torch.int8, torch.int8, torch.int8)
+        self.empty, self.dev = torch.empty_strided, torch._C._cuda_getDevice
+        self.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+        self.gemm, self.gate8, self.gate4, self.norm, self.quant = (L.rt4_gemm_w8a8, L.rt4_ffn_gate_w8a8, L.rt4_ffn_gate_w4a8, L.rt4_block_norm,
+                                                                    L.rt4_quant_token_a8)
 
 
-def _mat(t, rows, cols, dtype, dev, name):
-    """(data_ptr, row stride) of a matrix [rows, cols] whose rows are contiguous (dtype None: any of the element types)."""
-    if t.dim() == 2 and t.shape[0] == rows and t.shape[1] == cols and (dtype is None or t.dtype is dtype) and t.get_device() == dev:
-        r, c = t.stride()
-        if rows == 1:                            # (a single row's stride says nothing)
-            r = (cols + 15) // 16 * 16
-        if c == 1 or cols == 1:
-            return t.data_ptr(), r
-    raise RT4Error(f"{name}: expected {dtype or 'floating-point'} [{rows}, {cols}] with contiguous rows on device {dev}, got {t.dtype} "
-                   f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
-
-
+_e = None
 _work_bytes = {}
 
 
-def _linear8(fn, weights, xq, sx, act, out, dtype):
-    torch = _torch()
-    dev, f32, i8 = _dev(), torch.float32, torch.int8
-    if xq.dim() != 2 or weights[0][1].dim() != 2:
-        raise RT4Error(f"xq {tuple(xq.shape)} [M, K] and {weights[0][0]} {tuple(weights[0][1].shape)} [N, K] are matrices")
-    M, K = xq.shape
-    N = weights[0][1].shape[0]
+def _env():
+    global _e
+    _e = _Env()
+    return _e
+
+
+def _refuse(dev, *args):
+    """Raises for the first of (name, tensor, shape, dtypes, contiguous) that is not as asked: on device `dev`, of one of the types,
+    all contiguous or with contiguous rows."""
+    for name, t, shape, dtypes, whole in args:
+        if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or t.get_device() != dev or not (
+                t.is_contiguous() if whole else t.dim() == 2 and t.stride(1) == 1):
+            raise RT4Error(f"{name}: expected {' or '.join(map(str, dtypes))} {tuple(shape)}, {'' if whole else 'rows '}contiguous, on device {dev}, "
+                           f"got {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
+    raise RT4Error("arguments do not fit each other")
+
+
+def _rows_of(t):
+    """Row stride of a matrix; of a single row, whose stride says nothing, its length up to a multiple of 16."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+
+def _output(e, out, dtype, M, N, dev):
+    """(tensor, data_ptr, row stride, type) of an output [M, N]."""
     if out is None:
-        dtype = dtype or f32
-        t = _type(dtype, "dtype")
-        out = torch.empty_strided((M, N), (N, 1), dtype=dtype, device=dev)
-        op, ldo = out.data_ptr(), N
-    else:
-        if dtype is not None and out.dtype is not dtype:
-            raise RT4Error(f"out is {out.dtype}, dtype {dtype}")
-        t = _type(out.dtype, "out")
-        op, ldo = _mat(out, M, N, out.dtype, dev, "out")
-    xp, ldx = _mat(xq, M, K, i8, dev, "xq")
-    args = []
-    for name, w, sname, s in weights:
-        args += [*_mat(w, N, K, i8, dev, name), _arg(s, f32, (N,), dev, sname)]
-    # The runs' sums of split products: memory of the caching allocator, which keeps it from others until the stream is past it.
-    key = (M, N, K, len(weights), dev)
-    nb = _work_bytes.get(key)
-    if nb is None:
+        dtype = dtype or e.f32
+        t = e.types.get(dtype)
+        if t is None:
+            raise RT4Error(f"dtype: expected float32, bfloat16 or float16, got {dtype}")
+        out = e.empty((M, N), (N, 1), dtype=dtype, device=dev)
+        return out, out.data_ptr(), N, t
+    t = e.types.get(out.dtype)
+    if t is None or (dtype is not None and out.dtype is not dtype) or out.shape != (M, N) or out.get_device() != dev or out.stride(1) != 1:
+        _refuse(dev, ("out", out, (M, N), (dtype,) if dtype else tuple(e.types), False))
+    return out, out.data_ptr(), _rows_of(out), t
+
+
+def _work(e, M, N, K, weights, dev):
+    """(memory, its size) for the runs' sums of a split product: of the caching allocator, which keeps it from others until the
+    stream is past the call.  How much goes by the sizes alone, asked for once."""
+    key = (M, N, K, weights, dev)
+    n = _work_bytes.get(key)
+    if n is None:
         b = ctypes.c_int64()
-        _check(lib().rt4_w8a8_work_bytes(M, N, K, len(weights), ctypes.byref(b)))
-        if len(_work_bytes) > 4096:              # (sizes alone; they are asked for again)
+        _check(lib().rt4_w8a8_work_bytes(M, N, K, weights, ctypes.byref(b)))
+        if len(_work_bytes) > 4096:
             _work_bytes.clear()
-        nb = _work_bytes[key] = b.value
-    work = torch.empty_strided((nb,), (1,), dtype=torch.uint8, device=dev) if nb else None
-    _check(fn(op, ldo, t, *args, xp, ldx, _arg(sx, f32, (M,), dev, "sx"), M, N, K, *act, None if work is None else work.data_ptr(), nb,
-              _raw_stream(dev)))
-    return out
+        n = _work_bytes[key] = b.value
+    return (e.empty((n,), (1,), dtype=e.u8, device=dev), n) if n else (None, 0)
 
 
 def gemm_w8a8(wq, sw, xq, sx, out=None, dtype=None):
     """Product of int8 codes -> [M, N] of `dtype` (float32, bfloat16 or float16; default float32): xq int8 [M, K] with a scale
     sx f32 [M] for each token (quant_token_a8, block_norm), wq int8 [N, K] with a scale sw f32 [N] for each channel.
     K % 16 == 0 and at most 131056; rows may be strided by multiples of 16 bytes.  See rt4_gemm_w8a8 in include/rt4k.h."""
-    return _linear8(lib().rt4_gemm_w8a8, (("wq", wq, "sw", sw),), xq, sx, (), out, dtype)
+    e = _e or _env()
+    dev, i8, f32 = e.dev(), e.i8, e.f32
+    if xq.dim() != 2 or wq.dim() != 2:
+        raise RT4Error(f"xq {tuple(xq.shape)} [M, K] and wq {tuple(wq.shape)} [N, K] are matrices")
+    M, K = xq.shape
+    N, k = wq.shape
+    if not (k == K and xq.dtype is i8 and wq.dtype is i8 and xq.get_device() == dev and wq.get_device() == dev and xq.stride(1) == 1 and
+            wq.stride(1) == 1 and sx.shape == (M,) and sw.shape == (N,) and sx.dtype is f32 and sw.dtype is f32 and sx.is_contiguous() and
+            sw.is_contiguous() and sx.get_device() == dev and sw.get_device() == dev):
+        _refuse(dev, ("xq", xq, (M, K), (i8,), False), ("wq", wq, (N, K), (i8,), False), ("sx", sx, (M,), (f32,), True), ("sw", sw, (N,), (f32,), True))
+    out, op, ldo, t = _output(e, out, dtype, M, N, dev)
+    work, n = _work(e, M, N, K, 1, dev)
+    if e.gemm(op, ldo, t, wq.data_ptr(), _rows_of(wq), sw.data_ptr(), xq.data_ptr(), _rows_of(xq), sx.data_ptr(), M, N, K,
+              work.data_ptr() if n else None, n, e.stream(dev)):
+        _check(1)
+    return out
 
 
 def _act_code(act):
@@ -683,24 +706,57 @@ def _act_code(act):
 def ffn_gate_w8a8(wg, sg, wu, su, xq, sx, act: str = "silu", out=None, dtype=None):
     """First half of a gated feed-forward block -> act(x Wg^T) * (x Wu^T) [M, N]: weights and activations as gemm_w8a8's, act
     "silu" or "gelu_tanh".  See rt4_ffn_gate_w8a8 in include/rt4k.h."""
-    return _linear8(lib().rt4_ffn_gate_w8a8, (("wg", wg, "sg", sg), ("wu", wu, "su", su)), xq, sx, (_act_code(act),), out, dtype)
+    e = _e or _env()
+    dev, i8, f32 = e.dev(), e.i8, e.f32
+    if xq.dim() != 2 or wg.dim() != 2 or wu.dim() != 2:
+        raise RT4Error(f"xq {tuple(xq.shape)} [M, K], wg {tuple(wg.shape)} and wu {tuple(wu.shape)} [N, K] are matrices")
+    M, K = xq.shape
+    N, k = wg.shape
+    if not (k == K and wu.shape == (N, K) and xq.dtype is i8 and wg.dtype is i8 and wu.dtype is i8 and xq.get_device() == dev and
+            wg.get_device() == dev and wu.get_device() == dev and xq.stride(1) == 1 and wg.stride(1) == 1 and wu.stride(1) == 1 and
+            sx.shape == (M,) and sg.shape == (N,) and su.shape == (N,) and sx.dtype is f32 and sg.dtype is f32 and su.dtype is f32 and
+            sx.is_contiguous() and sg.is_contiguous() and su.is_contiguous() and sx.get_device() == dev and sg.get_device() == dev and
+            su.get_device() == dev):
+        _refuse(dev, ("xq", xq, (M, K), (i8,), False), ("wg", wg, (N, K), (i8,), False), ("wu", wu, (N, K), (i8,), False),
+                ("sx", sx, (M,), (f32,), True), ("sg", sg, (N,), (f32,), True), ("su", su, (N,), (f32,), True))
+    a = _act_code(act)
+    out, op, ldo, t = _output(e, out, dtype, M, N, dev)
+    work, n = _work(e, M, N, K, 2, dev)
+    if e.gate8(op, ldo, t, wg.data_ptr(), _rows_of(wg), sg.data_ptr(), wu.data_ptr(), _rows_of(wu), su.data_ptr(), xq.data_ptr(), _rows_of(xq),
+               sx.data_ptr(), M, N, K, a, work.data_ptr() if n else None, n, e.stream(dev)):
+        _check(1)
+    return out
 
 
 def ffn_gate_w4a8(wg, wsg, wu, wsu, xq, sa, act: str = "silu", out=None):
     """The same on RT4 weights (wg, wu int32 [N, K/8], wsg, wsu int16/fp16 [N, K/128]) for 1 to 4 rows -> f32 [rows, N]; xq, sa as
     gemv_w4a8_q's (quant_act_a8, or block_norm's "act" form).  See rt4_ffn_gate_w4a8 in include/rt4k.h."""
-    torch = _torch()
-    dev, f32, i32 = _dev(), torch.float32, torch.int32
+    e = _e or _env()
+    dev, f32 = e.dev(), e.f32
     if xq.dim() != 2 or wg.dim() != 2:
         raise RT4Error(f"ffn_gate_w4a8: xq {tuple(xq.shape)} [rows, K] and wg {tuple(wg.shape)} [N, K/8] are matrices")
     rows, K = xq.shape
-    N, G = wg.shape[0], K // GROUP
+    N, D = wg.shape
+    G = K // GROUP
+    st = wsg.dtype
+    if not (D * 8 == K and wu.shape == (N, D) and wsg.shape == (N, G) and wsu.shape == (N, G) and sa.shape == (rows, G) and xq.dtype is e.i8 and
+            wg.dtype is e.i32 and wu.dtype is e.i32 and (st is e.i16 or st is e.f16) and wsu.dtype is st and sa.dtype is f32 and
+            xq.is_contiguous() and wg.is_contiguous() and wu.is_contiguous() and wsg.is_contiguous() and wsu.is_contiguous() and
+            sa.is_contiguous() and xq.get_device() == dev and wg.get_device() == dev and wu.get_device() == dev and wsg.get_device() == dev and
+            wsu.get_device() == dev and sa.get_device() == dev):
+        words = (e.i32, getattr(_torch(), "uint32", e.i32))
+        if not (wg.dtype in words and wu.dtype in words):
+            words = (e.i32,)
+        half = (e.i16, e.f16)
+        bad = [a for a in (("xq", xq, (rows, K), (e.i8,), True), ("wg", wg, (N, K // 8), words, True), ("wu", wu, (N, K // 8), words, True),
+                           ("wsg", wsg, (N, G), half, True), ("wsu", wsu, (N, G), half, True), ("sa", sa, (rows, G), (f32,), True))
+               if tuple(a[1].shape) != a[2] or a[1].dtype not in a[3] or a[1].get_device() != dev or not a[1].is_contiguous()]
+        if bad or D * 8 != K:
+            _refuse(dev, *bad)
+    a = _act_code(act)
     out, op = _out(out, f32, (rows, N), (N, 1), dev, "out")
-    half = torch.float16 if wsg.dtype is torch.float16 else torch.int16
-    _check(lib().rt4_ffn_gate_w4a8(
-        op, _arg(wg, i32, (N, K // 8), dev, "wg"), _arg(wsg, half, (N, G), dev, "wsg"), _arg(wu, i32, (N, K // 8), dev, "wu"),
-        _arg(wsu, half, (N, G), dev, "wsu"), _arg(xq, torch.int8, (rows, K), dev, "xq"), _arg(sa, f32, (rows, G), dev, "sa"),
-        rows, N, K, _act_code(act), _raw_stream(dev)))
+    if e.gate4(op, wg.data_ptr(), wsg.data_ptr(), wu.data_ptr(), wsu.data_ptr(), xq.data_ptr(), sa.data_ptr(), rows, N, K, a, e.stream(dev)):
+        _check(1)
     return out
 
 
@@ -713,59 +769,74 @@ def block_norm(h, y=None, weight=None, post_weight=None, gate=None, scale: float
     ffn_gate_w8a8), "act" (interleaved, scales [M, K/128], for gemv_w4a8_q and ffn_gate_w4a8) or "rows" (interleaved, scales
     [K/128, M], for gemm_w4a8_i8); None without weight.  h_out: of h's type, h itself to update in place; without y it is h.
     See rt4_block_norm in include/rt4k.h."""
-    torch = _torch()
-    dev, f32 = _dev(), torch.float32
+    e = _e or _env()
+    dev, f32, types = e.dev(), e.f32, e.types
     form = FORMS.get(out)
     if form is None:
         raise RT4Error(f"out: expected one of {sorted(FORMS)}, got {out!r}")
     if h.dim() != 2:
         raise RT4Error(f"h {tuple(h.shape)} is a matrix [M, K]")
-    if y is None and (h_out is not None or weight is None):
-        raise RT4Error("block_norm: without y there is no new residual, and weight is needed")
     M, K = h.shape
-    ht = _type(h.dtype, "h")
-    hp, ldh = _mat(h, M, K, h.dtype, dev, "h")
-    op, ldho, yp, ldy, yt, gp, ldg = None, 0, None, 0, 0, None, 0
+    ht = types.get(h.dtype)
+    if ht is None or h.get_device() != dev or h.stride(1) != 1:
+        _refuse(dev, ("h", h, (M, K), tuple(types), False))
+    op = yp = gp = wp = pp = np_ = sp = n = s = None
+    ldho = ldy = yt = ldg = 0
     if y is not None:
-        yt = _type(y.dtype, "y")
-        yp, ldy = _mat(y, M, K, y.dtype, dev, "y")
+        yt = types.get(y.dtype)
+        if yt is None or y.shape != (M, K) or y.get_device() != dev or y.stride(1) != 1:
+            _refuse(dev, ("y", y, (M, K), tuple(types), False))
+        yp, ldy = y.data_ptr(), _rows_of(y)
         if h_out is None:
-            h_out = torch.empty_strided((M, K), (K, 1), dtype=h.dtype, device=dev)
+            h_out = e.empty((M, K), (K, 1), dtype=h.dtype, device=dev)
             op, ldho = h_out.data_ptr(), K
         else:
-            op, ldho = _mat(h_out, M, K, h.dtype, dev, "h_out")
+            if h_out.shape != (M, K) or h_out.dtype is not h.dtype or h_out.get_device() != dev or h_out.stride(1) != 1:
+                _refuse(dev, ("h_out", h_out, (M, K), (h.dtype,), False))
+            op, ldho = h_out.data_ptr(), _rows_of(h_out)
         if gate is not None:
-            gp, ldg = (_arg(gate, y.dtype, (K,), dev, "gate"), 0) if gate.dim() == 1 else _mat(gate, M, K, y.dtype, dev, "gate")
+            rows = gate.dim() == 2
+            if gate.shape != ((M, K) if rows else (K,)) or gate.dtype is not y.dtype or gate.get_device() != dev or gate.stride(-1) != 1:
+                _refuse(dev, ("gate", gate, (M, K) if rows else (K,), (y.dtype,), not rows))
+            gp, ldg = gate.data_ptr(), _rows_of(gate) if rows else 0
+        if post_weight is not None:
+            pp = _arg(post_weight, f32, (K,), dev, "post_weight")
     else:
+        if h_out is not None or weight is None or gate is not None or post_weight is not None:
+            raise RT4Error("block_norm: without y there is no new residual, a gate and post_weight have nothing to act on, and weight is needed")
         h_out = h
-        if gate is not None or post_weight is not None:
-            raise RT4Error("block_norm: a gate and post_weight need y")
-    n = s = np_ = sp = None
     if weight is not None:
-        n = torch.empty_strided((M, K), (K, 1), dtype=(f32, torch.bfloat16, torch.float16)[form] if form < 3 else torch.int8, device=dev)
+        wp = _arg(weight, f32, (K,), dev, "weight")
+        n = e.empty((M, K), (K, 1), dtype=e.out_types[form], device=dev)
         np_ = n.data_ptr()
         if form >= 3:
-            shape = ((M,), (M, K // GROUP), (K // GROUP, M))[form - 3]
-            s = torch.empty_strided(shape, (1,) if form == 3 else (shape[1], 1), dtype=f32, device=dev)
+            s = e.empty((M,), (1,), dtype=f32, device=dev) if form == 3 else e.empty((M, K // GROUP), (K // GROUP, 1), dtype=f32, device=dev) \
+                if form == 4 else e.empty((K // GROUP, M), (M, 1), dtype=f32, device=dev)
             sp = s.data_ptr()
-    _check(lib().rt4_block_norm(
-        op, ldho, hp, ldh, ht, yp, ldy, yt, gp, ldg, None if post_weight is None else _arg(post_weight, f32, (K,), dev, "post_weight"),
-        None if weight is None else _arg(weight, f32, (K,), dev, "weight"), scale, eps, weight_offset, np_, sp, form, M, K,
-        _raw_stream(dev)))
+    if e.norm(op, ldho, h.data_ptr(), _rows_of(h), ht, yp, ldy, yt, gp, ldg, pp, wp, scale, eps, weight_offset, np_, sp, form, M, K, e.stream(dev)):
+        _check(1)
     return h_out, (n if s is None else (n, s))
 
 
 def quant_token_a8(x, xq=None, sx=None):
     """x [M, K] (float32, bfloat16 or float16, rows may be strided) -> (xq int8 [M, K] in natural order, sx f32 [M]): one scale a
     token, for gemm_w8a8 and ffn_gate_w8a8.  See rt4_quant_token_a8 in include/rt4k.h."""
-    torch = _torch()
-    dev = _dev()
+    e = _e or _env()
+    dev = e.dev()
     if x.dim() != 2:
         raise RT4Error(f"x {tuple(x.shape)} is a matrix [M, K]")
     M, K = x.shape
-    t = _type(x.dtype, "x")
-    xp, ldx = _mat(x, M, K, x.dtype, dev, "x")
-    xq, qp = _out(xq, torch.int8, (M, K), (K, 1), dev, "xq")
-    sx, sp = _out(sx, torch.float32, (M,), (1,), dev, "sx")
-    _check(lib().rt4_quant_token_a8(qp, sp, xp, ldx, t, M, K, _raw_stream(dev)))
+    t = e.types.get(x.dtype)
+    if t is None or x.get_device() != dev or x.stride(1) != 1:
+        _refuse(dev, ("x", x, (M, K), tuple(e.types), False))
+    if xq is None:
+        xq = e.empty((M, K), (K, 1), dtype=e.i8, device=dev)
+    elif xq.shape != (M, K) or xq.dtype is not e.i8 or xq.get_device() != dev or not xq.is_contiguous():
+        _refuse(dev, ("xq", xq, (M, K), (e.i8,), True))
+    if sx is None:
+        sx = e.empty((M,), (1,), dtype=e.f32, device=dev)
+    elif sx.shape != (M,) or sx.dtype is not e.f32 or sx.get_device() != dev or not sx.is_contiguous():
+        _refuse(dev, ("sx", sx, (M,), (e.f32,), True))
+    if e.quant(xq.data_ptr(), sx.data_ptr(), x.data_ptr(), _rows_of(x), t, M, K, e.stream(dev)):
+        _check(1)
     return xq, sx
