@@ -182,7 +182,8 @@ def rt4_case(torch, M, N, K, seed):
 @pytest.mark.gpu
 @pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 128), (1, 37, 256), (2, 100, 640), (3, 17, 1152), (4, 33, 5120), (4, 515, 384), (1, 700, 5120),
-                                   (2, 48, 17408), (1, 5, 17408), (3, 1200, 512), (4, 4100, 1024)])
+                                   (2, 48, 17408), (1, 5, 17408), (3, 1200, 512), (4, 4100, 1024),
+                                   (3, 9, 2048), (4, 7, 1152), (2, 3, 896), (1, 2, 3328), (4, 3, 38912)])
 def test_gated_half_of_rt4_weights(rt4, torch_gpu, M, N, K, act):
     """Group sums are exact and folded in fp32: each of the K/128 terms carries 3 u and passes through at most K/128 + 8 sums."""
     torch = torch_gpu
