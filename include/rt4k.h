@@ -407,6 +407,13 @@ int rt4_gemm_w8a8(void* c, int64_t ldc, int c_type, const int8_t* wq, int64_t ld
  * initialized, free again when the call's work on its stream is done; every call that may overlap has one of its own). */
 int rt4_w8a8_work_bytes(int M, int N, int K, int weights, int64_t* bytes);
 
+/* How a product or gated half of these sizes runs with that workspace on a device of `cus` CUs (0: the current device, the
+ * only case that touches one): one launch or two (channels[1] is 0 or those of the second), each by a form (0 to 8: tiles
+ * of tile_m tokens and tile_n weight rows; 9: dot products, tile sizes 0) with K split into that many runs.  For tests and
+ * reports; all outputs int[2]. */
+int rt4_w8a8_launch_plan(int M, int N, int K, int weights, int cus, int* form, int* channels, int* splits, int* tile_m,
+                         int* tile_n);
+
 /* First half of a gated feed-forward block on 8-bit weights: h [M][N] = act(g) * u with g and u the products of
  * rt4_gemm_w8a8 with the gate weights wg, sg and the up weights wu, su, in fp32 until h's rounding.  Arguments as there. */
 int rt4_ffn_gate_w8a8(void* h, int64_t ldh, int h_type, const int8_t* wg, int64_t ldg, const float* sg, const int8_t* wu,

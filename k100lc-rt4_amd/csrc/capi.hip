@@ -927,18 +927,41 @@ static int run_linear8(const char* who, const rt4::Linear8& a, int weights, void
     int cus = 0, rc = check_linear8(who, a, weights);
     if (rc || (rc = device_cus(&cus))) return rc;
     rt4::Linear8Plan p = rt4::linear8_plan(a.M, a.N, a.K, weights, cus);
-    if (p.part_bytes && (!work || work_bytes < 0 || (uint64_t)work_bytes < p.part_bytes)) p.splits = 1, p.part_bytes = 0;
+    if (p.part_bytes && (!work || work_bytes < 0 || (uint64_t)work_bytes < p.part_bytes)) p.part[0].splits = p.part[1].splits = 1, p.part_bytes = 0;
     if (p.part_bytes && !aligned(work, 16)) return fail(RT4_E_ARG, "%s: misaligned workspace (16 bytes)", who);
     return hip_status(rt4::launch_linear8(a, p, work, st), who);
 }
 
+static int check_w8a8_size(const char* who, int M, int N, int K, int weights) {
+    if (M < 1 || N < 1 || M > (1 << 24) || N > (1 << 24) || (long long)((M + 63) / 64) * ((N + 31) / 32) > INT32_MAX || K < 16 || K % 16 ||
+        K > kMaxK8 || weights < 1 || weights > 2)
+        return fail(RT4_E_SHAPE, "%s: M=%d N=%d K=%d weights=%d", who, M, N, K, weights);
+    return RT4_OK;
+}
+
 int rt4_w8a8_work_bytes(int M, int N, int K, int weights, int64_t* bytes) {
     if (!bytes) return fail(RT4_E_ARG, "rt4_w8a8_work_bytes: null pointer");
-    if (M < 1 || N < 1 || M > (1 << 24) || N > (1 << 24) || (long long)((M + 63) / 64) * ((N + 31) / 32) > INT32_MAX || K < 16 || K % 16 || K > kMaxK8 || weights < 1 || weights > 2)
-        return fail(RT4_E_SHAPE, "rt4_w8a8_work_bytes: M=%d N=%d K=%d weights=%d", M, N, K, weights);
-    int cus = 0, rc = device_cus(&cus);
-    if (rc) return rc;
+    int cus = 0, rc = check_w8a8_size("rt4_w8a8_work_bytes", M, N, K, weights);
+    if (rc || (rc = device_cus(&cus))) return rc;
     *bytes = (int64_t)rt4::linear8_plan(M, N, K, weights, cus).part_bytes;
+    return RT4_OK;
+}
+
+int rt4_w8a8_launch_plan(int M, int N, int K, int weights, int cus, int* form, int* channels, int* splits, int* tile_m, int* tile_n) {
+    if (!form || !channels || !splits || !tile_m || !tile_n) return fail(RT4_E_ARG, "rt4_w8a8_launch_plan: null pointer");
+    int rc = check_w8a8_size("rt4_w8a8_launch_plan", M, N, K, weights);
+    if (rc) return rc;
+    if (cus < 0) return fail(RT4_E_SHAPE, "rt4_w8a8_launch_plan: cus=%d", cus);
+    if (cus == 0 && (rc = device_cus(&cus))) return rc;
+    const rt4::Linear8Plan p = rt4::linear8_plan(M, N, K, weights, cus);
+    for (int i = 0; i < 2; i++) {
+        const bool on = i < p.parts;
+        form[i] = on ? p.part[i].form : 0;
+        channels[i] = on ? p.part[i].N : 0;
+        splits[i] = on ? p.part[i].splits : 0;
+        tile_m[i] = tile_n[i] = 0;
+        if (on) rt4::linear8_tile(p.part[i].form, &tile_m[i], &tile_n[i]);
+    }
     return RT4_OK;
 }
 

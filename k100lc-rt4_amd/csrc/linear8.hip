@@ -337,7 +337,7 @@ __global__ __launch_bounds__(256) void linear8_join_k(Linear8 a, int splits, con
     F(0, 4, 4, 2, 2, 2, 1) F(1, 2, 7, 4, 1, 2, 1) F(2, 2, 5, 4, 1, 3, 1) F(3, 2, 4, 2, 2, 3, 1) F(4, 1, 7, 4, 1, 3, 1)            \
     F(5, 1, 5, 4, 1, 4, 1) F(6, 2, 2, 2, 2, 2, 2) F(7, 1, 2, 2, 2, 3, 2) F(8, 1, 1, 2, 2, 4, 2)
 template <class C, int NW>
-hipError_t launch_tile(const Linear8& a, const Linear8Plan& p, void* part, hipStream_t st) {
+hipError_t launch_tile(const Linear8& a, const Linear8Part& p, void* part, hipStream_t st) {
     auto k = linear8_tile_k<C, NW>;
     hipLaunchKernelGGL(k, dim3((unsigned)(p.tiles * p.splits)), dim3(64 * C::W), 0, st, a, p.splits, p.splits > 1 ? static_cast<int4*>(part) : nullptr);
     if (p.splits == 1) return hipGetLastError();
@@ -425,45 +425,86 @@ hipError_t launch_dot(const Linear8& a, hipStream_t st) {
 
 constexpr int kDotMaxM = 8;
 // A form's tile, workgroups a CU holds, and its measured cost (us): a step where few workgroups run, what is added to that
-// where all do (power, the L2's rate), and a tile's beginning and end.  Fitted to 1045 times of 54 sizes (M 16..4000, N
-// 1000..17408, K 1024..17408, one and two weight matrices, every form, 1 to 4 splits); the choice made by them takes 2% longer
-// than the best one of each size.
+// where all do (power, the L2's rate), a tile's beginning and end; and the rate at which it streams weights (TB/s), which bounds
+// few tokens.  Fitted to 1045 times of 54 sizes (M 16..4000, N 1000..17408, K 1024..17408, one and two weight matrices, every
+// form, 1 to 4 splits); the form they choose takes 2% longer than the best one of each size.
 struct Shape {
     int bm, bn, per_cu;
-    double step, full, ends;
+    double step, full, ends, rate;
 };
-constexpr double kCost[][3] = {{1.284, 0.579, 4.234}, {0.826, 0.522, 19.111}, {0.495, 0.459, 12.053}, {0.692, 0.251, 3.318}, {0.475, 0.122, 15.473}, {0.469, 0.145, 8.014}, {0.733, 0.548, 0}, {0.359, 0.633, 0}, {0.184, 0.256, 1.108}};
-#define RT4_SHAPE(f, tm, tn, wm, wn, st, pc) {32 * tm * wm, 32 * tn * wn, pc, kCost[f][0], kCost[f][1], kCost[f][2]},
+constexpr double kCost[][4] = {{1.294, 0.406, 4.932, 4.5}, {0.875, 0.456, 19.139, 4.5}, {0.505, 0.46, 12.229, 4.5}, {0.688, 0.211, 3.819, 4}, {0.58, 0.134, 15.555, 4.3}, {0.577, 0.115, 8.16, 5.1}, {0.766, 0.454, 0, 3.6}, {0.359, 0.47, 0.199, 3.95}, {0.208, 0.227, 1.427, 4.3}};
+#define RT4_SHAPE(f, tm, tn, wm, wn, st, pc) {32 * tm * wm, 32 * tn * wn, pc, kCost[f][0], kCost[f][1], kCost[f][2], kCost[f][3]},
 constexpr Shape kShapes[] = {RT4_TILES(RT4_SHAPE)};
 constexpr int kDotForm = sizeof(kShapes) / sizeof(kShapes[0]);
 static_assert(kDotForm == sizeof(kCost) / sizeof(kCost[0]), "");
 
 }  // namespace
 
-Linear8Plan linear8_plan(int M, int N, int K, int weights, int cus) {
-    Linear8Plan p{kDotForm, 0, 1, 0};
-    if (M <= kDotMaxM) return p;
-    // The form and number of splits of the lowest estimate.
+namespace {
+
+// Form f over M x N with K split into sp runs: the estimated time, and the number of tiles.
+double estimate(int f, int M, int N, int K, int weights, int cus, int sp, long long* tiles_out) {
+    const Shape& s = kShapes[f];
+    const long long tiles = (long long)((M + s.bm - 1) / s.bm) * ((N + s.bn / weights - 1) / (s.bn / weights)), slots = (long long)cus * s.per_cu;
+    const long long groups = tiles * sp;
+    const int n = ((K + 127) / 128 + sp - 1) / sp;
+    const double part = (double)(groups % slots) / slots;
+    double t = groups / slots * (n * (s.step + s.full) + s.ends);
+    if (part > 0) t += n * (s.step + s.full * part) + s.ends;
+    if (sp > 1) t += 7.8 + 0.274e-6 * 4 * groups * s.bm * s.bn;      // the runs' sums, out and in again, and the launch that joins them
+    *tiles_out = tiles;
+    return 2 + std::max(t, (double)N * K * weights / s.rate * 1e-6);
+}
+
+// The form and number of splits of the lowest estimate.
+double choose(int M, int N, int K, int weights, int cus, Linear8Part* p) {
     double best = 1e30;
-    const int steps = (K + 127) / 128;
+    for (int f = 0; f < kDotForm; f++)
+        for (int sp = 1; sp <= 8 && sp <= (K + 127) / 128; sp++) {
+            long long tiles;
+            const double t = estimate(f, M, N, K, weights, cus, sp, &tiles);
+            if (sp > 1 && tiles * sp > 2ll * cus * kShapes[f].per_cu) break;
+            if (t < best) best = t, *p = Linear8Part{f, N, (int)tiles, sp};
+        }
+    return best;
+}
+
+}  // namespace
+
+Linear8Plan linear8_plan(int M, int N, int K, int weights, int cus) {
+    Linear8Plan p{{{kDotForm, N, 0, 1}, {}}, 1, 0};
+    if (M <= kDotMaxM) return p;
+    double best = choose(M, N, K, weights, cus, &p.part[0]);
+    // Or whole rounds of a form's tiles over the first channels, and what is left of a last round with few tiles by the form
+    // that is best for it, in a launch of its own.
     for (int f = 0; f < kDotForm; f++) {
         const Shape& s = kShapes[f];
-        const long long tiles = (long long)((M + s.bm - 1) / s.bm) * ((N + s.bn / weights - 1) / (s.bn / weights)), slots = (long long)cus * s.per_cu;
-        for (int sp = 1; sp <= 8 && sp <= steps; sp++) {
-            const long long groups = tiles * sp;
-            if (sp > 1 && groups > 2 * slots) break;
-            const int n = (steps + sp - 1) / sp;
-            const double bytes = 4.0 * groups * s.bm * s.bn, part = (double)(groups % slots) / slots;
-            double t = groups / slots * (n * (s.step + s.full) + s.ends);
-            if (part > 0) t += n * (s.step + s.full * part) + s.ends;
-            if (sp > 1) t += 7.4 + 0.276e-6 * bytes;        // the runs' sums, out and in again, and the launch that joins them
-            if (t < best) best = t, p = Linear8Plan{f, (int)tiles, sp, sp > 1 ? (size_t)bytes : 0};
-        }
+        const int nm = (M + s.bm - 1) / s.bm, bn = s.bn / weights;
+        const long long slots = (long long)cus * s.per_cu, rounds = (long long)nm * ((N + bn - 1) / bn) / slots;
+        const long long first = rounds * slots / nm * bn;
+        if (rounds < 1 || first >= N) continue;
+        long long tiles;
+        Linear8Part rest;
+        const double t = estimate(f, M, (int)first, K, weights, cus, 1, &tiles) + choose(M, N - (int)first, K, weights, cus, &rest);
+        if (t < best) best = t, p = Linear8Plan{{{f, (int)first, (int)tiles, 1}, rest}, 2, 0};
+    }
+    for (int i = 0; i < p.parts; i++) {
+        const Linear8Part& q = p.part[i];
+        const size_t bytes = q.splits > 1 ? (size_t)4 * q.tiles * q.splits * kShapes[q.form].bm * kShapes[q.form].bn : 0;
+        p.part_bytes = bytes > p.part_bytes ? bytes : p.part_bytes;
     }
     return p;
 }
 
-hipError_t launch_linear8(const Linear8& a, const Linear8Plan& p, void* part, hipStream_t st) {
+void linear8_tile(int form, int* bm, int* bn) {
+    const bool tile = form < kDotForm;
+    *bm = tile ? kShapes[form].bm : 0;
+    *bn = tile ? kShapes[form].bn : 0;
+}
+
+namespace {
+
+hipError_t launch_part(const Linear8& a, const Linear8Part& p, void* part, hipStream_t st) {
 #define RT4_LAUNCH(f, ...) \
     if (p.form == f) return a.act < 0 ? launch_tile<Tile<__VA_ARGS__>, 1>(a, p, part, st) : launch_tile<Tile<__VA_ARGS__>, 2>(a, p, part, st);
     RT4_TILES(RT4_LAUNCH)
@@ -477,6 +518,22 @@ hipError_t launch_linear8(const Linear8& a, const Linear8Plan& p, void* part, hi
         case 7: return launch_dot<7>(a, st);
         default: return launch_dot<8>(a, st);
     }
+}
+
+}  // namespace
+
+hipError_t launch_linear8(const Linear8& a, const Linear8Plan& p, void* part, hipStream_t st) {
+    int n = 0;
+    for (int i = 0; i < p.parts; i++) {
+        Linear8 b = a;
+        b.N = p.part[i].N;
+        b.out = static_cast<char*>(a.out) + (size_t)n * (a.type == kF32 ? 4 : 2);
+        for (int j = 0; j < (a.act < 0 ? 1 : 2); j++) b.w[j] = a.w[j] + (size_t)n * a.ldw[j], b.sw[j] = a.sw[j] + n;
+        const hipError_t e = launch_part(b, p.part[i], part, st);
+        if (e != hipSuccess) return e;
+        n += p.part[i].N;
+    }
+    return hipSuccess;
 }
 
 }  // namespace rt4

@@ -199,12 +199,18 @@ struct Linear8 {
     const float* sx;
     int M, N, K, type, act;              // act < 0: the product alone
 };
-// How a product runs: the form of its tiles, how many runs their steps are split into, and the bytes of the runs' sums.
+// How a product runs: one or two launches, each of N of the channels by tiles of one form, their steps split into runs; the
+// bytes of the runs' sums.
+struct Linear8Part {
+    int form, N, tiles, splits;
+};
 struct Linear8Plan {
-    int form, tiles, splits;
+    Linear8Part part[2];
+    int parts;
     size_t part_bytes;
 };
 Linear8Plan linear8_plan(int M, int N, int K, int weights, int cus);
+void linear8_tile(int form, int* bm, int* bn);       // (0 for the dot products)
 hipError_t launch_linear8(const Linear8& a, const Linear8Plan& p, void* part, hipStream_t st);
 
 struct Gate4 {

@@ -41,7 +41,7 @@ C_EXPORTS = (
     "rt4_attn_q_quant", "rt4_kv_append_k", "rt4_kv_append_v", "rt4_attention_prefill",
     "rt4_attention_prefill_cfg", "rt4_attention_launch_plan",
     "rt4_kv_append_rows", "rt4_attention_tree", "rt4_verify_tree",
-    "rt4_w8a8_work_bytes", "rt4_gemm_w8a8", "rt4_ffn_gate_w8a8", "rt4_ffn_gate_w4a8", "rt4_block_norm", "rt4_quant_token_a8",
+    "rt4_w8a8_work_bytes", "rt4_w8a8_launch_plan", "rt4_gemm_w8a8", "rt4_ffn_gate_w8a8", "rt4_ffn_gate_w4a8", "rt4_block_norm", "rt4_quant_token_a8",
     "rt4_file_open", "rt4_file_close", "rt4_file_count", "rt4_file_find", "rt4_file_info", "rt4_file_data",
     "rt4_file_size", "rt4_file_upload", "rt4_file_upload_tensor",
 )
@@ -101,6 +101,7 @@ _SIGS = {
     "rt4_kv_append_rows": [_P] * 10 + [_I] * 4 + [_P],
     "rt4_attention_tree": [_P] * 13 + [_I] * 8 + [_P],
     "rt4_w8a8_work_bytes": [_I, _I, _I, _I, _P],
+    "rt4_w8a8_launch_plan": [_I] * 5 + [_P] * 5,
     "rt4_gemm_w8a8": [_P, _L, _I, _P, _L, _P, _P, _L, _P, _I, _I, _I, _P, _L, _P],
     "rt4_ffn_gate_w8a8": [_P, _L, _I, _P, _L, _P, _P, _L, _P, _P, _L, _P, _I, _I, _I, _I, _P, _L, _P],
     "rt4_ffn_gate_w4a8": [_P] * 7 + [_I] * 4 + [_P],
@@ -672,6 +673,14 @@ def _work(e, M, N, K, weights, dev):
             _work_bytes.clear()
         n = _work_bytes[key] = b.value
     return (e.empty((n,), (1,), dtype=e.u8, device=dev), n) if n else (None, 0)
+
+
+def w8a8_launch_plan(M: int, N: int, K: int, weights: int = 1, cus: int = 0) -> list:
+    """How gemm_w8a8 (weights 1) or ffn_gate_w8a8 (2) of these sizes runs on a device of `cus` CUs (0: the current device): its
+    one or two launches, each with its form, channels, splits of K and tile (see rt4_w8a8_launch_plan in include/rt4k.h)."""
+    a = [(ctypes.c_int * 2)() for _ in range(5)]
+    _check(lib().rt4_w8a8_launch_plan(M, N, K, weights, cus, *a))
+    return [dict(zip(("form", "channels", "splits", "tile_m", "tile_n"), v)) for v in zip(*a) if v[1]]
 
 
 def gemm_w8a8(wq, sw, xq, sx, out=None, dtype=None):

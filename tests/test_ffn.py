@@ -103,6 +103,64 @@ def test_gated_half(rt4, torch_gpu, M, N, K, act):
         near(torch, got, act64(torch, g, act) * u, gate_bound(torch, g, act), dtype, gate_flushed(g, u))
 
 
+# Sizes that take each tile form, whole and with K split, with one and with two weight matrices, and two launches for one call:
+# (M, N, K, weights, the (form, whether K is split) of each launch on 256 CUs).
+FORM_SIZES = [(3000, 3500, 1040, 1, [(0, 0)]), (400, 12000, 1040, 2, [(0, 0)]), (3391, 735, 18672, 2, [(0, 1)]), (392, 11815, 6496, 2, [(1, 0)]),
+              (1703, 6875, 5744, 1, [(1, 0)]), (6730, 324, 16640, 2, [(1, 1)]), (2000, 5000, 2064, 1, [(2, 0)]), (145, 6349, 14912, 2, [(2, 1)]),
+              (513, 9000, 2064, 1, [(3, 0)]), (66, 5295, 22944, 1, [(3, 1)]), (10, 25881, 2736, 2, [(4, 0)]), (11, 8056, 18464, 2, [(4, 1)]),
+              (9, 31099, 4384, 1, [(5, 0)]), (10, 8631, 17040, 2, [(5, 1)]), (1000, 3500, 112, 1, [(6, 0)]), (79, 3896, 11936, 2, [(6, 1)]),
+              (9, 30, 112, 2, [(7, 0)]), (10, 16, 5824, 1, [(7, 1)]), (9, 30, 1040, 1, [(8, 0)]), (9, 16, 12320, 2, [(8, 1)]),
+              (700, 12000, 1040, 1, [(6, 0), (8, 0)]), (700, 12000, 1040, 2, [(0, 0), (8, 0)]), (13, 21740, 7680, 2, [(5, 0), (8, 1)]),
+              (347, 27804, 9808, 1, [(3, 0), (3, 1)])]
+
+
+@pytest.mark.parametrize("M,N,K,weights,forms", FORM_SIZES)
+def test_forms_are_reached(rt4, M, N, K, weights, forms):
+    plan = rt4.w8a8_launch_plan(M, N, K, weights, cus=256)
+    assert [(p["form"], int(p["splits"] > 1)) for p in plan] == forms
+    assert sum(p["channels"] for p in plan) == N
+    assert all(p["tile_m"] % 32 == 0 and p["tile_n"] % 32 == 0 and p["tile_m"] > 0 for p in plan)
+    assert [p["form"] for p in rt4.w8a8_launch_plan(8, N, K, weights, cus=256)] == [9]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,weights,forms", FORM_SIZES)
+def test_forms(rt4, torch_gpu, M, N, K, weights, forms):
+    """Against 64-bit products on the device (sums of K products of codes are exact in them)."""
+    torch = torch_gpu
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    code = lambda r: torch.randint(-128, 128, (r, K), generator=g, dtype=torch.int8, device="cuda")  # noqa: E731
+    scale = lambda r: torch.rand((r,), generator=g, device="cuda") * 0.01 / math.sqrt(K) + 1e-6  # noqa: E731
+    x, sx = code(M), scale(M)
+    w = [(code(N), scale(N)) for _ in range(weights)]
+    ref = [torch.mm(x.double(), c.double().t().contiguous()) * sx.double()[:, None] * s.double() for c, s in w]
+    if weights == 1:
+        near(torch, rt4.gemm_w8a8(*w[0], x, sx), ref[0], 3 * U, torch.float32)
+        near(torch, rt4.gemm_w8a8(*w[0], x, sx, dtype=torch.bfloat16), ref[0], 3 * U, torch.bfloat16)
+    else:
+        got = rt4.ffn_gate_w8a8(*w[0], *w[1], x, sx)
+        near(torch, got, act64(torch, ref[0], "silu") * ref[1], gate_bound(torch, ref[0], "silu"), torch.float32, gate_flushed(*ref))
+
+
+@pytest.mark.gpu
+def test_product_without_workspace(rt4, torch_gpu):
+    """The C entry without memory for split sums runs unsplit, with the same result; too little is as none."""
+    torch = torch_gpu
+    M, N, K = 40, 130, 8208
+    x, sx = (t.cuda() for t in codes8(torch, M, K, 21))
+    w, sw = (t.cuda() for t in codes8(torch, N, K, 22))
+    want = rt4.gemm_w8a8(w, sw, x, sx)
+    n = ctypes.c_int64()
+    L = rt4.lib()
+    assert L.rt4_w8a8_work_bytes(M, N, K, 1, ctypes.byref(n)) == 0 and n.value > 0
+    work = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    for ptr, size in ((None, 0), (work.data_ptr(), n.value - 1), (work.data_ptr(), n.value)):
+        out = torch.zeros(M, N, device="cuda")
+        assert L.rt4_gemm_w8a8(out.data_ptr(), N, 0, w.data_ptr(), K, sw.data_ptr(), x.data_ptr(), K, sx.data_ptr(), M, N, K, ptr, size,
+                               torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out, want)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("M", [1, 3, 40, 300])
 def test_product_of_extreme_codes(rt4, torch_gpu, M):
@@ -502,6 +560,16 @@ def test_product_refusals(rt4):
         assert "rt4_gemm_w8a8" in L.rt4_last_error().decode()
     for kw in ({"t": 3}, {"t": -1}, {"w": ODD}, {"x": ODD}, {"c": ctypes.c_void_p(0x1002)}, {"sx": ctypes.c_void_p(0x1002)}):
         assert call(**kw) == 2, kw
+
+
+def test_plan_refusals(rt4):
+    for args in ((0, 64, 256, 1), (4, 0, 256, 1), (4, 64, 24, 1), (4, 64, 131072, 1), (4, 64, 256, 0), (4, 64, 256, 3)):
+        with pytest.raises(rt4.RT4Error):
+            rt4.w8a8_launch_plan(*args, cus=256)
+    with pytest.raises(rt4.RT4Error):
+        rt4.w8a8_launch_plan(4, 64, 256, 1, cus=-1)
+    assert rt4.lib().rt4_w8a8_work_bytes(4, 64, 24, 1, ctypes.byref(ctypes.c_int64())) == 1
+    assert rt4.lib().rt4_w8a8_work_bytes(4, 64, 256, 1, None) == 2
 
 
 def test_gated_refusals(rt4):
