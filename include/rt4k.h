@@ -395,7 +395,8 @@ int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_
 /* 8-bit product: c [M][N] (c_type, row stride ldc elements) = sx[m] sw[n] Σ_k xq[m][k] wq[n][k] with
  * xq int8 [M][K] (row stride ldx bytes), a scale sx[m] for each token, wq int8 [N][K] (row stride ldw),
  * a scale sw[n] for each channel; all in natural order.  Sums are exact int32: K % 16 == 0 and at most 131056.
- * 1 <= M, N <= 2^24 and at most 2^31 tiles of 64 x 32 outputs; strides at least a row, ldx and ldw multiples of 16 below 2^24, xq and wq 16-byte aligned.
+ * 1 <= M, N <= 2^24, M * N <= 2^37; strides at least a row, ldx and ldw multiples of 16 below 2^24, xq and wq 16-byte
+ * aligned.
  * Each output is the sum's fp32 value times sx times sw, rounded to c_type; a scale that is not finite makes its
  * row or column so.  c must not overlap an input.  work: rt4_w8a8_work_bytes of device memory; with less, or NULL, K is
  * not split (the same result, slower). */
@@ -437,13 +438,13 @@ int rt4_ffn_gate_w4a8(float* h, const uint32_t* wg, const uint16_t* sg, const ui
  * inputs.  n_form: an element type, n [M][K] contiguous of that type, n_scale NULL; or RT4_TOKEN, RT4_ACT, RT4_ROWS
  * with n_scale (the last two with K % 128 == 0).  A code is the nearest integer to levels * n / max|n| over its token
  * or group (ties to even), decided in 64 bits; its scale max|n| / levels, 1 where all are zeros.  Where a value of a
- * token or group is not finite its codes are 0 and its scale NaN.  1 <= K <= 65536. */
+ * token or group is not finite its codes are 0 and its scale NaN.  1 <= M < 2^22, 1 <= K <= 65536. */
 int rt4_block_norm(void* h_out, int64_t ldho, const void* h, int64_t ldh, int h_type, const void* y, int64_t ldy, int y_type,
                    const void* gate, int64_t ldg, const float* post_w, const float* w, double scale, double eps, double w_offset,
                    void* n, float* n_scale, int n_form, int M, int K, void* stream);
 
 /* Quantizer with one scale a token, natural order: codes and scales as rt4_block_norm's RT4_TOKEN of x itself.
- * x [M][K] of x_type, row stride ldx; xq int8 [M][K] contiguous, sx f32 [M].  1 <= K <= 65536. */
+ * x [M][K] of x_type, row stride ldx; xq int8 [M][K] contiguous, sx f32 [M].  1 <= M < 2^22, 1 <= K <= 65536. */
 int rt4_quant_token_a8(int8_t* xq, float* sx, const void* x, int64_t ldx, int x_type, int M, int K, void* stream);
 
 /* ----------------------------------------- W4A4 siblings (RT_ACT4 path) ---- */

@@ -900,15 +900,22 @@ int rt4_verify_tree(int32_t* tokens, int32_t* path, int32_t* count, int32_t* kv_
 constexpr int kMaxK8 = 131056;
 constexpr int64_t kMaxLd8 = 1 << 24;
 
+static int check_w8a8_size(const char* who, int M, int N, int K, int weights) {
+    if (M < 1 || N < 1 || M > (1 << 24) || N > (1 << 24) || (long long)M * N > (1ll << 37))
+        return fail(RT4_E_SHAPE, "%s: M=%d N=%d (1 to 2^24, M * N at most 2^37)", who, M, N);
+    if (K < 16 || K % 16 || K > kMaxK8) return fail(RT4_E_SHAPE, "%s: K=%d is not a multiple of 16 from 16 to %d", who, K, kMaxK8);
+    if (weights < 1 || weights > 2) return fail(RT4_E_SHAPE, "%s: weights=%d (1 or 2)", who, weights);
+    return RT4_OK;
+}
+
 static int check_linear8(const char* who, const rt4::Linear8& a, int weights) {
     if (!a.out || !a.x || !a.sx) return fail(RT4_E_ARG, "%s: null pointer", who);
     for (int j = 0; j < weights; j++)
         if (!a.w[j] || !a.sw[j]) return fail(RT4_E_ARG, "%s: null pointer", who);
     if (a.type < RT4_F32 || a.type > RT4_F16) return fail(RT4_E_ARG, "%s: output type %d", who, a.type);
     if (weights == 2 && (a.act < RT4_SILU || a.act > RT4_GELU_TANH)) return fail(RT4_E_ARG, "%s: activation %d", who, a.act);
-    if (a.M < 1 || a.N < 1 || a.M > (1 << 24) || a.N > (1 << 24) || (long long)((a.M + 63) / 64) * ((a.N + 31) / 32) > INT32_MAX)
-        return fail(RT4_E_SHAPE, "%s: M=%d N=%d (1 to 2^24, at most 2^31 tiles of 64 x 32)", who, a.M, a.N);
-    if (a.K < 16 || a.K % 16 || a.K > kMaxK8) return fail(RT4_E_SHAPE, "%s: K=%d is not a multiple of 16 from 16 to %d", who, a.K, kMaxK8);
+    const int rc = check_w8a8_size(who, a.M, a.N, a.K, weights);
+    if (rc) return rc;
     if (a.ldo < a.N) return fail(RT4_E_SHAPE, "%s: output row stride %lld is below N=%d", who, (long long)a.ldo, a.N);
     const long long ld[3] = {a.ldx, a.ldw[0], a.ldw[1]};
     const void* at[3] = {a.x, a.w[0], a.w[1]};
@@ -930,13 +937,6 @@ static int run_linear8(const char* who, const rt4::Linear8& a, int weights, void
     if (p.part_bytes && (!work || work_bytes < 0 || (uint64_t)work_bytes < p.part_bytes)) p.part[0].splits = p.part[1].splits = 1, p.part_bytes = 0;
     if (p.part_bytes && !aligned(work, 16)) return fail(RT4_E_ARG, "%s: misaligned workspace (16 bytes)", who);
     return hip_status(rt4::launch_linear8(a, p, work, st), who);
-}
-
-static int check_w8a8_size(const char* who, int M, int N, int K, int weights) {
-    if (M < 1 || N < 1 || M > (1 << 24) || N > (1 << 24) || (long long)((M + 63) / 64) * ((N + 31) / 32) > INT32_MAX || K < 16 || K % 16 ||
-        K > kMaxK8 || weights < 1 || weights > 2)
-        return fail(RT4_E_SHAPE, "%s: M=%d N=%d K=%d weights=%d", who, M, N, K, weights);
-    return RT4_OK;
 }
 
 int rt4_w8a8_work_bytes(int M, int N, int K, int weights, int64_t* bytes) {
@@ -997,7 +997,8 @@ static size_t type_bytes(int t) { return t == RT4_F32 ? 4 : 2; }
 static bool vec_rows(const void* p, long long ld, int type) { return aligned(p, 16) && ld * (long long)type_bytes(type) % 16 == 0; }
 
 static int run_norm(const char* who, rt4::BlockNorm& a, hipStream_t st) {
-    if (a.M < 1 || a.K < 1 || a.K > rt4::kNormMaxK) return fail(RT4_E_SHAPE, "%s: M=%d K=%d (1 to %d)", who, a.M, a.K, rt4::kNormMaxK);
+    if (a.M < 1 || a.M > rt4::kNormMaxM || a.K < 1 || a.K > rt4::kNormMaxK)
+        return fail(RT4_E_SHAPE, "%s: M=%d (1 to %d) K=%d (1 to %d)", who, a.M, rt4::kNormMaxM, a.K, rt4::kNormMaxK);
     if (a.h_type < RT4_F32 || a.h_type > RT4_F16 || (a.y && (a.y_type < RT4_F32 || a.y_type > RT4_F16)))
         return fail(RT4_E_ARG, "%s: element types %d and %d", who, a.h_type, a.y_type);
     if (a.ldh < a.K || (a.y && (a.ldy < a.K || a.ldho < a.K)) || (a.gate && a.ldg != 0 && a.ldg < a.K))

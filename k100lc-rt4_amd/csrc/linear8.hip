@@ -38,7 +38,7 @@ struct Tile {
     static constexpr int LDS = ST * STAGE > W * SLAB ? ST * STAGE : W * SLAB;
     static constexpr int PA = BM / 8 / W, PB = BN / 8 / W, P = PA + PB;   // DMA instructions of a wave a step
     static_assert(BM % (8 * W) == 0 && BN % (8 * W) == 0 && (ST - 2) * P < 64, "");
-    static_assert(LDS * PER_CU <= 160 * 1024, "");
+    static_assert(LDS * PER_CU <= 160 * 1024 && W == 4, "");
 };
 
 struct Where {                           // a workgroup's tile and steps
@@ -171,11 +171,11 @@ __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int sp
     }
     const size_t k0 = (size_t)at.s0 * 128;
     // An instruction's immediate offset counts for both addresses: pieces 1 KB apart in LDS need M0 set for every fourth
-    // alone.  In memory it is taken out again: voff holds 3072 less it, the bases 3072 less.
-    const int8_t* ga = a.x + (size_t)at.m0 * a.ldx + k0 - 3072;
+    // alone.  In memory it is taken out again: voff holds 3 KB less it, the bases 3 KB less.
+    const int8_t* ga = a.x + (size_t)at.m0 * a.ldx + k0 - 3 * 1024;
     const int8_t* gb[NW];
 #pragma unroll
-    for (int j = 0; j < NW; j++) gb[j] = a.w[j] + (size_t)at.n0 * a.ldw[j] + k0 - 3072;
+    for (int j = 0; j < NW; j++) gb[j] = a.w[j] + (size_t)at.n0 * a.ldw[j] + k0 - 3 * 1024;
     const uint32_t lds0 = lds_addr(smem);
     const uint32_t la = lds0 + (uint32_t)pa0 * 1024, lb = lds0 + C::BM * 128 + (uint32_t)pb0 * 1024;
     int issue = at.s0;                           // next step to bring
@@ -196,9 +196,9 @@ __global__ __launch_bounds__(64 * C::W, 1) void linear8_tile_k(Linear8 a, int sp
         const int8_t* g = t < PA ? ga : gb[NW == 1 ? 0 : mat(t)];
         switch (u % 4) {
             case 0: dma16_m0<0>(voff[t], g); break;
-            case 1: dma16_m0<1024>(voff[t], g); break;
-            case 2: dma16_m0<2048>(voff[t], g); break;
-            default: dma16_m0<3072>(voff[t], g);
+            case 1: dma16_m0<1 * 1024>(voff[t], g); break;
+            case 2: dma16_m0<2 * 1024>(voff[t], g); break;
+            default: dma16_m0<3 * 1024>(voff[t], g);
         }
     };
     const auto issued = [&]() {
@@ -424,6 +424,7 @@ hipError_t launch_dot(const Linear8& a, hipStream_t st) {
 }
 
 constexpr int kDotMaxM = 8;
+constexpr long long kMaxGroups = 1 << 24;        // workgroups of 256 threads in a grid
 // A form's tile, workgroups a CU holds, and its measured cost (us): a step where few workgroups run, what is added to that
 // where all do (power, the L2's rate), a tile's beginning and end; and the rate at which it streams weights (TB/s), which bounds
 // few tokens.  Fitted to 1045 times of 54 sizes (M 16..4000, N 1000..17408, K 1024..17408, one and two weight matrices, every
@@ -456,14 +457,15 @@ double estimate(int f, int M, int N, int K, int weights, int cus, int sp, long l
     return 2 + std::max(t, (double)N * K * weights / s.rate * 1e-6);
 }
 
-// The form and number of splits of the lowest estimate.
+// The form and number of splits of the lowest estimate.  (A grid counts its threads in 32 bits: large tiles alone for the
+// largest products.)
 double choose(int M, int N, int K, int weights, int cus, Linear8Part* p) {
     double best = 1e30;
     for (int f = 0; f < kDotForm; f++)
         for (int sp = 1; sp <= 8 && sp <= (K + 127) / 128; sp++) {
             long long tiles;
             const double t = estimate(f, M, N, K, weights, cus, sp, &tiles);
-            if (sp > 1 && tiles * sp > 2ll * cus * kShapes[f].per_cu) break;
+            if ((sp > 1 && tiles * sp > 2ll * cus * kShapes[f].per_cu) || tiles * sp >= kMaxGroups) break;
             if (t < best) best = t, *p = Linear8Part{f, N, (int)tiles, sp};
         }
     return best;
@@ -486,7 +488,7 @@ Linear8Plan linear8_plan(int M, int N, int K, int weights, int cus) {
         long long tiles;
         Linear8Part rest;
         const double t = estimate(f, M, (int)first, K, weights, cus, 1, &tiles) + choose(M, N - (int)first, K, weights, cus, &rest);
-        if (t < best) best = t, p = Linear8Plan{{{f, (int)first, (int)tiles, 1}, rest}, 2, 0};
+        if (t < best && tiles < kMaxGroups) best = t, p = Linear8Plan{{{f, (int)first, (int)tiles, 1}, rest}, 2, 0};
     }
     for (int i = 0; i < p.parts; i++) {
         const Linear8Part& q = p.part[i];

@@ -147,9 +147,9 @@ __device__ __forceinline__ int code_of(double p, double f, double a, double most
     if (fabs(q - r) > 0.5 - 0x1p-40) r = rint(p * most / a);
     return (int)r;
 }
-// Codes of 8 values p = v * w (w the weight with its offset) from fp32 products: six roundings (w's sum, the product, the
-// maximum's, the factor's 2, the quotient's) of at most 2^-24 each leave the quotient, below 128, off by 2^-14.4 at most.
-// Where it lies within 2^-14 of a half, 64 bits decide.
+// Codes of 8 values p = v * w (w the weight with its offset, an fp32 value) from fp32 products: six roundings (w's sum, the
+// product, the maximum's, the factor's 2, the quotient's) of at most 2^-24 each leave the quotient, below 128, off by 2^-14.4
+// at most.  Where it lies within 2^-14 of a half, 64 bits decide.
 // The sum of the quotient and 3 * 2^22 is rounded to an integer (ties to even), which its low byte holds.
 template <class P>
 __device__ __forceinline__ uint2 codes_of(const float (&hi)[8], P exact, float f32, double a, double most, bool interleaved) {
@@ -172,8 +172,8 @@ __device__ __forceinline__ uint2 codes_of(const float (&hi)[8], P exact, float f
     };
     return interleaved ? make_uint2(four(0, 2, 4, 6), four(1, 3, 5, 7)) : make_uint2(four(0, 1, 2, 3), four(4, 5, 6, 7));
 }
-// h + t for a 16-bit residual, t formed in fp32 with at most 6 roundings: where both ends of the error's range round to
-// the same bits, those; otherwise `open` is set, and 64 bits decide.
+// h + t for a 16-bit residual, t formed in fp32 with at most 6 roundings, each of at most 2^-24 (see `least`): where both ends
+// of the error's range round to the same bits, those; otherwise `open` is set, and 64 bits decide.
 template <class T>
 __device__ __forceinline__ T sum_of(float h, float t, bool& open) {
     typedef T two __attribute__((ext_vector_type(2)));
@@ -184,6 +184,13 @@ __device__ __forceinline__ T sum_of(float h, float t, bool& open) {
     const uint32_t b = __builtin_bit_cast(uint32_t, r);
     open |= (b & 0xFFFFu) != b >> 16;
     return r[1];
+}
+// The lesser of m and the magnitudes of eight products, NaN where one of them is.  At 2^-100 and above all of them were rounded to
+// 24 bits; a NaN may come of an overflow on the way.
+__device__ __forceinline__ float least(float m, const float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) m = __builtin_elementwise_minimum(__builtin_elementwise_minimum(m, fabsf(v[e])), fabsf(v[e + 1]));
+    return m;
 }
 // The scale that belongs to maximum a: 1 for zeros (as the other quantizers), NaN where a value was not finite.
 __device__ __forceinline__ float scale_of(double a, double r, double most) {
@@ -245,6 +252,7 @@ __global__ __launch_bounds__(MOST) void norm_k(BlockNorm a) {
                 for (int i = 0; i < 2; i++) asm volatile("" : "+v"(yr[c].d[i].x), "+v"(yr[c].d[i].y), "+v"(yr[c].d[i].z), "+v"(yr[c].d[i].w));
         }
         const float k32 = (float)k;
+        const bool k_fine = fabsf(k32) >= 0x1p-126f && fabsf(k32) < __builtin_inff();
         TH* orow = static_cast<TH*>(a.h_out) + m * a.ldho;
 #pragma unroll
         for (int c = 0; c < C; c++) {
@@ -270,19 +278,23 @@ __global__ __launch_bounds__(MOST) void norm_k(BlockNorm a) {
                 widen(yr[c], a.y_type, y);
 #pragma unroll
                 for (int e = 0; e < 8; e++) y[e] *= k32;
+                float small = least(0x1p0f, y);
                 if (a.gate) {
                     float g[8];
                     widen(gr, a.y_type, g);
 #pragma unroll
                     for (int e = 0; e < 8; e++) y[e] *= g[e];
+                    small = least(small, y);
                 }
-                if (a.post_w)
+                if (a.post_w) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) y[e] *= elem(pw, e);
-                bool open = false;
+                    small = least(small, y);
+                }
+                bool open = !(k_fine && small >= 0x1p-100f);
 #pragma unroll
                 for (int e = 0; e < 8; e++) t[e] = sum_of<TH>(elem(hr[c], e), y[e], open);
-                if (open) exact(t);
+                if (open && i < K) exact(t);
             }
             store8<VEC>(orow, i, K, t);
             if (!VEC)                            // (what lies behind the row: 0 times an infinite k is NaN)
@@ -297,6 +309,7 @@ __global__ __launch_bounds__(MOST) void norm_k(BlockNorm a) {
     if (!a.n) return;
     next_pass();
     const float off32 = (float)a.w_offset;
+    const bool off_fine = off32 == a.w_offset;   // else a weight may cancel all of it but its rounding: 64 bits throughout
     const auto weights = [&](int c) {
         Raw<float> w = {};
         if (NORM) w = load_raw<VEC>(a.w + zero, place(c), K);
@@ -353,9 +366,9 @@ __global__ __launch_bounds__(MOST) void norm_k(BlockNorm a) {
             __builtin_amdgcn_sched_barrier(0);
         }
     } else if (a.form == kToken) {
-        // The exact maximum: of the values whose fp32 product is within its error of the largest.  Where fp32's range does not
-        // hold the products, of all values, and all codes in 64 bits.
-        const bool range = most > 0x1p-100 && most < __builtin_inf();
+        // The exact maximum: of the values whose fp32 product is within its error of the largest.  Where fp32 does not hold the
+        // products, of all values, and all codes in 64 bits.
+        const bool range = off_fine && most > 0x1p-100 && most < __builtin_inf();
         if constexpr (NORM) {                    // (without a norm the products are the values themselves)
             if (!range || most32 >= (float)most * (1 - 0x1p-21f)) {
                 double mine = 0;
@@ -411,7 +424,7 @@ __global__ __launch_bounds__(MOST) void norm_k(BlockNorm a) {
             g = max2(g, pair_of<2>(g));
             g = max2(g, pair_of<3>(g));
             const bool fine = g > 0 && g < __builtin_inf();
-            const float f32 = g > 0x1p-100 && g < 0x1p100 ? (float)levels / (float)g : __builtin_nanf("");
+            const float f32 = off_fine && g > 0x1p-100 && g < 0x1p100 ? (float)levels / (float)g : __builtin_nanf("");
             uint2 q = make_uint2(0, 0);
             float hi[8];
 #pragma unroll

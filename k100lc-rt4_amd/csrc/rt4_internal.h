@@ -228,6 +228,7 @@ hipError_t launch_gate4(const Gate4& a, int cus, hipStream_t st);
 // 128-group as the decode (kAct) and the prefill (kRows) quantizers lay them out.
 enum { kToken = 3, kAct = 4, kRows = 5 };
 constexpr int kNormMaxK = 65536;
+constexpr int kNormMaxM = (1 << 22) - 1;   // a workgroup of up to 1024 threads a row, in a grid that counts threads in 32 bits
 struct BlockNorm {
     void* h_out;
     long long ldho;

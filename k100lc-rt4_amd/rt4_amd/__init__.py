@@ -641,6 +641,9 @@ def _refuse(dev, *args):
     raise RT4Error("arguments do not fit each other")
 
 
+_MOST = 2 ** 31 - 1       # sizes that the C ABI's ints hold; what it takes of them it checks itself
+
+
 def _rows_of(t):
     """Row stride of a matrix; of a single row, whose stride says nothing, its length up to a multiple of 16."""
     return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
@@ -693,6 +696,8 @@ def gemm_w8a8(wq, sw, xq, sx, out=None, dtype=None):
         raise RT4Error(f"xq {tuple(xq.shape)} [M, K] and wq {tuple(wq.shape)} [N, K] are matrices")
     M, K = xq.shape
     N, k = wq.shape
+    if M > _MOST or N > _MOST or K > _MOST:
+        raise RT4Error(f"xq {tuple(xq.shape)}, wq {tuple(wq.shape)}: too large")
     if not (k == K and xq.dtype is i8 and wq.dtype is i8 and xq.get_device() == dev and wq.get_device() == dev and xq.stride(1) == 1 and
             wq.stride(1) == 1 and sx.shape == (M,) and sw.shape == (N,) and sx.dtype is f32 and sw.dtype is f32 and sx.is_contiguous() and
             sw.is_contiguous() and sx.get_device() == dev and sw.get_device() == dev):
@@ -721,6 +726,8 @@ def ffn_gate_w8a8(wg, sg, wu, su, xq, sx, act: str = "silu", out=None, dtype=Non
         raise RT4Error(f"xq {tuple(xq.shape)} [M, K], wg {tuple(wg.shape)} and wu {tuple(wu.shape)} [N, K] are matrices")
     M, K = xq.shape
     N, k = wg.shape
+    if M > _MOST or N > _MOST or K > _MOST:
+        raise RT4Error(f"xq {tuple(xq.shape)}, wg {tuple(wg.shape)}: too large")
     if not (k == K and wu.shape == (N, K) and xq.dtype is i8 and wg.dtype is i8 and wu.dtype is i8 and xq.get_device() == dev and
             wg.get_device() == dev and wu.get_device() == dev and xq.stride(1) == 1 and wg.stride(1) == 1 and wu.stride(1) == 1 and
             sx.shape == (M,) and sg.shape == (N,) and su.shape == (N,) and sx.dtype is f32 and sg.dtype is f32 and su.dtype is f32 and
@@ -746,6 +753,8 @@ def ffn_gate_w4a8(wg, wsg, wu, wsu, xq, sa, act: str = "silu", out=None):
         raise RT4Error(f"ffn_gate_w4a8: xq {tuple(xq.shape)} [rows, K] and wg {tuple(wg.shape)} [N, K/8] are matrices")
     rows, K = xq.shape
     N, D = wg.shape
+    if rows > 4 or N > _MOST or K > _MOST:
+        raise RT4Error(f"ffn_gate_w4a8: xq {tuple(xq.shape)} (1 to 4 rows), wg {tuple(wg.shape)}: too large")
     G = K // GROUP
     st = wsg.dtype
     if not (D * 8 == K and wu.shape == (N, D) and wsg.shape == (N, G) and wsu.shape == (N, G) and sa.shape == (rows, G) and xq.dtype is e.i8 and
@@ -786,6 +795,8 @@ def block_norm(h, y=None, weight=None, post_weight=None, gate=None, scale: float
     if h.dim() != 2:
         raise RT4Error(f"h {tuple(h.shape)} is a matrix [M, K]")
     M, K = h.shape
+    if M > _MOST or K > _MOST:
+        raise RT4Error(f"h {tuple(h.shape)}: too large")
     ht = types.get(h.dtype)
     if ht is None or h.get_device() != dev or h.stride(1) != 1:
         _refuse(dev, ("h", h, (M, K), tuple(types), False))
@@ -835,6 +846,8 @@ def quant_token_a8(x, xq=None, sx=None):
     if x.dim() != 2:
         raise RT4Error(f"x {tuple(x.shape)} is a matrix [M, K]")
     M, K = x.shape
+    if M > _MOST or K > _MOST:
+        raise RT4Error(f"x {tuple(x.shape)}: too large")
     t = e.types.get(x.dtype)
     if t is None or x.get_device() != dev or x.stride(1) != 1:
         _refuse(dev, ("x", x, (M, K), tuple(e.types), False))

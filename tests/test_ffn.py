@@ -309,7 +309,8 @@ def expect_form(torch, rt4, out, n, h, w, eps, offset):
             scale, a = scale.T, a.T
     assert np.array_equal(got, codes), int((got != codes).sum())
     scale = np.where(a > 0, scale, 1.0)
-    np.testing.assert_allclose(s.cpu().numpy(), scale, rtol=2.0 ** -24 * 1.001, atol=0)
+    # (atol: half of fp32's smallest subnormal, what the rounding of a scale below its normal numbers is off by at most)
+    np.testing.assert_allclose(s.cpu().numpy(), scale, rtol=2.0 ** -24 * 1.001, atol=2.0 ** -150)
 
 
 TYPES = ["float32", "bfloat16", "float16"]
@@ -435,6 +436,96 @@ def test_values_that_are_not_finite(rt4, torch_gpu, bad):
 
 
 # ------------------------------------------------------- the block, whole --
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("K", [256, 99])
+def test_residual_whose_factors_leave_fp32(rt4, torch_gpu, dtype, K):
+    """scale * gate * y is formed in fp32 where that decides a 16-bit residual: not where a product on the way underflows, loses
+    digits or overflows though the whole does not."""
+    torch = torch_gpu
+    t = getattr(torch, dtype)
+    for scale, yv, gv, hv in ((1e-20, 1e-30, 1e35, 0.0), (1e-20, 1e-30, 1e35, 2e-15), (1e-42, 1e30, 1e12, 0.0), (1e-60, 1e30, 1e30, 1.0), (1e20, 1e30, 1e-37, 5.0),
+                              (1e20, 1e30, 0.0, 5.0), (1e40, 0.0, 1.0, 3.0), (1e40, 1e-38, 1.0, 3.0), (1.0, 1e-38, 1.0, 0.0), (0.0, 1e30, 1.0, 2.0)):
+        g = torch.Generator().manual_seed(K)
+        some = lambda v: (v * (1 + torch.rand((2, K), generator=g)))  # noqa: E731
+        h, y, gate = some(hv).to(t), some(yv).float(), some(gv).float()
+        got, _ = rt4.block_norm(h.cuda(), y.cuda(), gate=gate.cuda(), scale=scale)
+        ref = h.double() + scale * gate.double() * y.double()
+        want = ref.float().to(t)
+        # ref is off by 2^-51: within that of two neighbours' border, either
+        low, high = (ref * (1 - 2.0 ** -50)).float().to(t), (ref * (1 + 2.0 ** -50)).float().to(t)
+        ok = (got.cpu() == want) | (got.cpu() == low) | (got.cpu() == high)
+        assert bool(ok.all()), (scale, yv, gv, hv, got.cpu()[~ok][:4], want[~ok][:4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", ["token", "act", "rows"])
+@pytest.mark.parametrize("offset", [0.1, 1.0 / 3.0, 1e-40, 0.5])
+def test_codes_whose_weights_nearly_cancel(rt4, torch_gpu, out, offset):
+    """weight + offset in 64 bits also where the offset is no fp32 value and the sum is next to nothing."""
+    torch = torch_gpu
+    M, K = 3, 512
+    g = torch.Generator().manual_seed(7)
+    h = torch.randn((M, K), generator=g)
+    w = (-torch.full((K,), offset, dtype=torch.float64) * (1 + torch.randint(-2, 3, (K,), generator=g) * U)).float()
+    got, n = rt4.block_norm(h.cuda(), weight=w.cuda(), weight_offset=offset, out=out)
+    expect_form(torch, rt4, out, n, h, w, 1e-6, offset)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("weights", [1, 2])
+@pytest.mark.parametrize("M", [2, 8, 40, 300])
+def test_rows_far_apart(rt4, torch_gpu, M, weights):
+    """The largest row strides of codes (offsets within a tile pass 31 bits, rows 32), and outputs whose rows lie as far apart."""
+    torch = torch_gpu
+    N, K, ld = 300, 272, 2 ** 24 - 16
+    x, sx = codes8(torch, M, K, 31)
+    w, sw = codes8(torch, N, K, 32)
+    far = torch.empty(299 * ld + K, dtype=torch.int8, device="cuda")
+    xf, wf = far.as_strided((M, K), (ld, 1), 0), far.as_strided((N, K), (ld, 1), 0)
+    o = torch.empty(299 * 2 ** 23 + N, dtype=torch.bfloat16, device="cuda").as_strided((M, N), (2 ** 23, 1), 0)
+    xf.copy_(x)
+    args = (w.cuda(), sw.cuda(), sx.cuda())
+    if weights == 1:
+        want = rt4.gemm_w8a8(args[0], args[1], x.cuda(), args[2], dtype=torch.bfloat16)
+        assert torch.equal(rt4.gemm_w8a8(args[0], args[1], xf, args[2], out=o), want)
+        wf.copy_(w)
+        assert torch.equal(rt4.gemm_w8a8(wf, args[1], x.cuda(), args[2], out=o), want)
+    else:
+        want = rt4.ffn_gate_w8a8(args[0], args[1], args[0], args[1], x.cuda(), args[2], dtype=torch.bfloat16)
+        assert torch.equal(rt4.ffn_gate_w8a8(args[0], args[1], args[0], args[1], xf, args[2], out=o), want)
+        wf.copy_(w)
+        assert torch.equal(rt4.ffn_gate_w8a8(args[0], args[1], wf, args[1], x.cuda(), args[2], out=o), want)
+
+
+@pytest.mark.gpu
+def test_wide_decode_half_captured(rt4, torch_gpu):
+    """Four rows whose codes need more LDS than a launch is granted without asking, captured and replayed."""
+    torch = torch_gpu
+    rows, N, K = 4, 70, 20480
+    g = torch.Generator().manual_seed(3)
+    w = [torch.randint(-2 ** 31, 2 ** 31, (N, K // 8), generator=g, dtype=torch.int64).to(torch.int32).cuda() for _ in range(2)]
+    s = [(torch.rand((N, K // 128), generator=g) * 0.01).to(torch.float16).cuda() for _ in range(2)]
+    x = torch.randn((rows, K), generator=g).cuda()
+
+    def run():
+        return rt4.ffn_gate_w4a8(w[0], s[0], w[1], s[1], *rt4.block_norm(x, weight=torch.ones(K, device="cuda"), out="act")[1])
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for i in range(3):
+        x.copy_(torch.randn((rows, K), generator=g))
+        want = run()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), i
+
+
 def ffn_block(rt4, h, y, p):
     """One feed-forward block at 8 bits: norm and quantize, gated half, quantize, down, and the residual normed for the next block."""
     h1, (xq, sx) = rt4.block_norm(h, y, weight=p["w1"], post_weight=p["pw"], scale=0.5, out="token")
@@ -562,6 +653,20 @@ def test_product_refusals(rt4):
         assert call(**kw) == 2, kw
 
 
+def test_sizes_beyond_a_launch(rt4):
+    """What a grid of workgroups cannot count is refused."""
+    L = rt4.lib()
+    assert L.rt4_gemm_w8a8(DUMMY, 2 ** 14, 1, DUMMY, 16, DUMMY, DUMMY, 16, DUMMY, 2 ** 24, 2 ** 14, 16, None, 0, None) == 1
+    assert L.rt4_w8a8_work_bytes(2 ** 24, 2 ** 14, 16, 1, ctypes.byref(ctypes.c_int64())) == 1
+    for M, N in ((2 ** 24, 2 ** 13), (2 ** 13, 2 ** 24), (2 ** 24, 33), (9, 2 ** 24)):
+        for weights in (1, 2):
+            for p in rt4.w8a8_launch_plan(M, N, 16, weights, cus=256):
+                tiles = -(-M // p["tile_m"]) * -(-p["channels"] // (p["tile_n"] // weights))
+                assert tiles * p["splits"] * 256 < 2 ** 32
+    assert L.rt4_quant_token_a8(DUMMY, DUMMY, DUMMY, 1, 1, 2 ** 22, 1, None) == 1
+    assert L.rt4_block_norm(None, 0, DUMMY, 16, 1, None, 0, 0, None, 0, None, DUMMY, 1.0, 1e-6, 0.0, DUMMY, None, 1, 2 ** 22, 16, None) == 1
+
+
 def test_plan_refusals(rt4):
     for args in ((0, 64, 256, 1), (4, 0, 256, 1), (4, 64, 24, 1), (4, 64, 131072, 1), (4, 64, 256, 0), (4, 64, 256, 3)):
         with pytest.raises(rt4.RT4Error):
@@ -640,3 +745,14 @@ def test_wrapper_refusals(rt4, torch_gpu):
                lambda: rt4.quant_token_a8(h, xq=torch.empty(4, 255, dtype=torch.int8).cuda())):
         with pytest.raises(rt4.RT4Error):
             fn()
+
+
+@pytest.mark.gpu
+def test_rows_beyond_32_bits_are_refused(rt4, torch_gpu):
+    """More rows than the C ABI's ints hold: refused, not cut."""
+    torch = torch_gpu
+    x = torch.empty((2 ** 32 + 1, 1), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(rt4.RT4Error):
+        rt4.quant_token_a8(x)
+    with pytest.raises(rt4.RT4Error):
+        rt4.block_norm(x, weight=torch.ones(1, device="cuda"))
