@@ -3,6 +3,15 @@
 //
 //   c[m][n] = sx[m] sw[n] Σ_k xq[m][k] wq[n][k]                     (exact int32 sums, K < 2^17)
 //   h[m][n] = act(sx[m] sg[n] Σ_k xq[m][k] wg[n][k]) * (sx[m] su[n] Σ_k xq[m][k] wu[n][k])
+//
+// What bounds it, and where it stands:
+//   up to 8 tokens   the weights' stream; 2 x 17408 x 5120 of one token 30.4 us, 5.9 TB/s; 5120 x 5120 5.4 us, most of it the
+//                    launch and the first loads' latency
+//   tens of tokens   the stream, and the split of K that fills the CUs: 37 tokens of 4999 x 7056 16.4 us, 2.2 TB/s,
+//                    of which the launch that joins the runs is a third
+//   many tokens      the matrix cores, at the clock that power leaves them (1.7 to 1.9 GHz under these kernels): 4096 tokens of
+//                    17408 x 5120 329 to 350 us by card, 2.1 to 2.2 Pop/s; 1000 of 2 x 17408 x 5120 178 to 190 us, 1.9 to 2.0;
+//                    1024 of 5120 x 17408 95 us, 1.9 (a library's int8 product of 8192^3: 2.07)
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -134,8 +143,8 @@ __device__ __forceinline__ void wait_dma_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// A DMA in two parts: where its rows go (M0, which the compiler leaves alone; one wait state until its use), and the load, whose immediate offset is added
-// to both addresses.
+// A DMA in two parts: where its rows go (M0, which the compiler leaves alone; one wait state until its use), and the load,
+// whose immediate offset is added to both addresses.
 __device__ __forceinline__ void set_m0(uint32_t l) { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" ::"s"((uint32_t)__builtin_amdgcn_readfirstlane((int)l)) : "memory"); }
 template <int IMM>
 __device__ __forceinline__ void dma16_m0(uint32_t voff, const void* gbase) {
@@ -478,7 +487,8 @@ Linear8Plan linear8_plan(int M, int N, int K, int weights, int cus) {
     if (M <= kDotMaxM) return p;
     double best = choose(M, N, K, weights, cus, &p.part[0]);
     // Or whole rounds of a form's tiles over the first channels, and what is left of a last round with few tiles by the form
-    // that is best for it, in a launch of its own.
+    // that is best for it, in a launch of its own (4096 tokens of 17408 x 5120: 1088 tiles of 256 x 256, 4.25 rounds, in one launch
+    // 354 us, four rounds and the rest apart 329; 1000 tokens of 2 x 17408 x 5120 190 and 178).
     for (int f = 0; f < kDotForm; f++) {
         const Shape& s = kShapes[f];
         const int nm = (M + s.bm - 1) / s.bm, bn = s.bn / weights;

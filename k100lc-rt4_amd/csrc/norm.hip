@@ -10,8 +10,12 @@
 // Results are those of 64-bit arithmetic (p is exact in it, sums and quotients are off by 2^-51), so each has one right
 // value; but a 64-bit conversion costs four fp32 operations, so what fp32 decides is left to it: a quotient, or a residual
 // of 16 bits, is formed in fp32 with a bound of its error, and in 64 bits by the lanes whose rounding that leaves open
-// (one of 8000 codes, of 4000 residuals).  4096 tokens of 5120 (bf16, post norm, gate, token codes): 48 us, with 64 bits
-// throughout 71; their 147 MB take 31 us at the rate of a large copy, the vector ALU's ~45 operations an element the rest.
+// (one of 8000 codes, of 4000 residuals).  4096 tokens of 5120 (bf16, post norm, gate, token codes): 54 us, with 64 bits
+// throughout 71; their 147 MB take 31 us at the rate of a large copy, the vector ALU's ~50 operations an element the rest, at
+// the 4 waves a SIMD that 123 registers leave (93 and 5 waves without the check of products' range, `least`: 48 us; held to 96
+// registers, which spills, 75; two chunks a thread, 60).  4 rows of 5120: 5.5 us, 1000 rows of 17408 to codes alone: 16 us for 52 MB.
+#include <type_traits>
+
 #include "ffn_dev.h"
 #include "rt4_internal.h"
 
@@ -21,7 +25,9 @@ namespace {
 
 constexpr int kMaxWaves = 16;
 
-// Eight elements as they are in memory.  VEC: rows are whole chunks of 8, aligned for vector access.
+// Eight elements as they are in memory.  VEC: rows are whole chunks of 8, aligned for vector access.  Others: whole chunks by
+// the same loads and stores, which global memory takes at any alignment (1000 rows of 17401 bf16 to codes: 20 us, element by
+// element 34), the row's last by elements.
 template <class T>
 struct Raw {
     uint4 d[sizeof(T) / 2];
@@ -33,7 +39,9 @@ __device__ __forceinline__ Raw<T> load_raw(const T* row, int i, int K) {
         if (i < K)
 #pragma unroll
             for (int k = 0; k < (int)sizeof(T) / 2; k++) r.d[k] = reinterpret_cast<const uint4*>(row + i)[k];
-    } else {
+    } else if (i + 8 <= K) {
+        __builtin_memcpy(&r, row + i, sizeof(r));
+    } else if (i < K) {
         T t[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) t[e] = i + e < K ? row[i + e] : (T)0.f;
@@ -86,6 +94,8 @@ __device__ __forceinline__ void store8(T* row, int i, int K, const T (&t)[8]) {
         if (i < K)
 #pragma unroll
             for (int k = 0; k < (int)sizeof(T) / 2; k++) reinterpret_cast<uint4*>(row + i)[k] = d[k];
+    } else if (i + 8 <= K) {
+        __builtin_memcpy(row + i, t, sizeof(t));
     } else {
 #pragma unroll
         for (int e = 0; e < 8; e++)
@@ -399,6 +409,8 @@ __global__ __launch_bounds__(MOST) void norm_k(BlockNorm a) {
                 q = codes_of(hi, [&](int e) { return NORM ? (double)elem(hr[c], e) * ((double)elem(w, e) + a.w_offset) : (double)hi[e]; }, f32, most, 127., false);
             if (VEC) {
                 if (i < K) *reinterpret_cast<uint2*>(qrow + i) = q;
+            } else if (i + 8 <= K) {
+                __builtin_memcpy(qrow + i, &q, sizeof(q));
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; e++)
@@ -445,25 +457,25 @@ template <class TH, bool HASY, bool NORM>
 void launch_chunks(const BlockNorm& a, hipStream_t st) {
     // Few rows: many waves a row, a chunk or two a thread.  Many: few waves a row, whose reductions cost little; 3 chunks a
     // thread (5 without y) leave registers for as many rows a CU as hide each other's latencies (4096 tokens of 5120, bf16: 3
-    // chunks 48 us, 2 50, 5 49, 10 61).  Waves enough to fill the CUs either way.
+    // chunks 54 us, 2 60).  Waves enough to fill the CUs either way.
     const int lanes = (a.K + 7) / 8, most = HASY ? 3 : 5;
     const auto go = [&](auto k, int C) {
         hipLaunchKernelGGL(k, dim3((unsigned)a.M), dim3((unsigned)(((lanes + C - 1) / C + 63) / 64 * 64)), 0, st, a);
     };
-    if (!a.vec) {
-        if (lanes <= 1024) go(norm_k<1, 1024, false, TH, HASY, NORM>, 1);
-        else go(norm_k<8, 1024, false, TH, HASY, NORM>, 8);
-        return;
-    }
     const int all = (lanes + 63) / 64, least = (all + most - 1) / most, want = a.M < 2048 ? 2048 / a.M : 1;
     int waves = want < least ? least : want;
     if (waves > 16) waves = 16;
     const int C = (all + waves - 1) / waves;
-    if (C <= 1) go(norm_k<1, 1024, true, TH, HASY, NORM>, 1);
-    else if (C <= 2 && lanes <= 2 * 512) go(norm_k<2, 512, true, TH, HASY, NORM>, 2);
-    else if (C <= 3 && lanes <= 3 * 512) go(norm_k<3, 512, true, TH, HASY, NORM>, 3);
-    else if (C <= 5 && lanes <= 5 * 512) go(norm_k<5, 512, true, TH, HASY, NORM>, 5);
-    else go(norm_k<8, 1024, true, TH, HASY, NORM>, 8);
+    const auto pick = [&](auto vec) {
+        constexpr bool V = decltype(vec)::value;
+        if (C <= 1) go(norm_k<1, 1024, V, TH, HASY, NORM>, 1);
+        else if (C <= 2 && lanes <= 2 * 512) go(norm_k<2, 512, V, TH, HASY, NORM>, 2);
+        else if (C <= 3 && lanes <= 3 * 512) go(norm_k<3, 512, V, TH, HASY, NORM>, 3);
+        else if (C <= 5 && lanes <= 5 * 512) go(norm_k<5, 512, V, TH, HASY, NORM>, 5);
+        else go(norm_k<8, 1024, V, TH, HASY, NORM>, 8);
+    };
+    if (a.vec) pick(std::true_type{});
+    else pick(std::false_type{});
 }
 template <class TH>
 void launch_y(const BlockNorm& a, hipStream_t st) {
