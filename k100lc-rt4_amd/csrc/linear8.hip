@@ -98,7 +98,6 @@ __device__ __forceinline__ void write_slab(const Linear8& a, const v16i* acc, co
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const bool vec = ((uintptr_t)a.out & 15) == 0 && a.ldo * (int)sizeof(T) % 16 == 0;
     static_assert(32 * LPR % 64 == 0, "");
 #pragma unroll
     for (int k = 0; k < 32 * LPR / 64; k++) {
@@ -106,8 +105,8 @@ __device__ __forceinline__ void write_slab(const Linear8& a, const v16i* acc, co
         const uint4 d = *reinterpret_cast<const uint4*>(lds + r * PITCH + col * sizeof(T));
         if (m < a.M && n < a.N) {
             T* o = static_cast<T*>(a.out) + (size_t)m * a.ldo + n;
-            if (vec && n + PER <= a.N) {
-                *reinterpret_cast<uint4*>(o) = d;
+            if (n + PER <= a.N) {                // (global memory takes 16 bytes at any alignment)
+                __builtin_memcpy(o, &d, 16);
             } else {
                 T t[PER];
                 __builtin_memcpy(t, &d, 16);
