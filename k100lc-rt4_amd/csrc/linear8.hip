@@ -7,10 +7,10 @@
 // What bounds it, and where it stands:
 //   up to 8 tokens   the weights' stream; 2 x 17408 x 5120 of one token 30.4 us, 5.9 TB/s; 5120 x 5120 5.4 us, most of it the
 //                    launch and the first loads' latency
-//   tens of tokens   the stream, and the split of K that fills the CUs: 37 tokens of 4999 x 7056 16.4 us, 2.2 TB/s,
-//                    of which the launch that joins the runs is a third
+//   tens of tokens   latency: a workgroup's steps, of 0.25 us, one after the other; 37 tokens of 4999 x 7056 15.9 us, 79
+//                    workgroups of 56 steps (a launch that joins runs of split K costs 7.8)
 //   many tokens      the matrix cores, at the clock that power leaves them (1.7 to 1.9 GHz under these kernels): 4096 tokens of
-//                    17408 x 5120 329 to 350 us by card, 2.1 to 2.2 Pop/s; 1000 of 2 x 17408 x 5120 178 to 190 us, 1.9 to 2.0;
+//                    17408 x 5120 329 to 352 us by card, 2.1 to 2.2 Pop/s; 1000 of 2 x 17408 x 5120 178 to 193 us, 1.85 to 2.0;
 //                    1024 of 5120 x 17408 95 us, 1.9 (a library's int8 product of 8192^3: 2.07)
 #include <algorithm>
 #include <cmath>
