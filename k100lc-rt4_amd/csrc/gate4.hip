@@ -9,6 +9,7 @@
 // bytes of codes to int8 (times 16), and 8 v_dot4 and 3 for the fold a token.
 // A wave goes on to further pairs without a pause, so that loads and arithmetic overlap throughout.
 // The quarter sums are exact and folded as rt4_gemv_w4a8_q folds group sums, fp32(16 I) * (f16(ws) / 16 * sa).
+#include <atomic>
 #include <type_traits>
 
 #include "ffn_dev.h"
@@ -145,11 +146,29 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gate4_k(Gate4 a) {
     }
 }
 
+constexpr size_t lds_bytes(int rows, int K) { return (size_t)rows * K + (size_t)rows * (K >> 7) * 4; }
+
+// The limit of a launch's LDS is the kernel's on a device, shared by all threads that call it: it is raised once, to what the
+// largest K needs, and never lowered under another thread's launch.
+template <int M>
+hipError_t raise_lds_limit() {
+    constexpr int kMaxDev = 64;
+    static std::atomic<bool> raised[kMaxDev];
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const bool known = dev >= 0 && dev < kMaxDev;
+    if (known && raised[dev].load(std::memory_order_acquire)) return hipSuccess;
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(gate4_k<M>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes(M, kGate4MaxK));
+    if (e == hipSuccess && known) raised[dev].store(true, std::memory_order_release);
+    return e;
+}
+
 template <int M>
 hipError_t launch_rows(const Gate4& a, int cus, hipStream_t st) {
-    const size_t lds = (size_t)M * a.K + (size_t)M * (a.K >> 7) * 4;
+    const size_t lds = lds_bytes(M, a.K);
     if (lds > 65536) {                           // (what a launch is granted without asking)
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(gate4_k<M>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        const hipError_t e = raise_lds_limit<M>();
         if (e != hipSuccess) return e;
     }
     // Two workgroups a CU (one where LDS holds no more), of as many waves as leave every CU one at least (4 rows of 5120 x 17408:
