@@ -267,13 +267,13 @@ __device__ __forceinline__ const void* sptr(const void* p) {
 // address additions, and a carry lost there is an address 4 GiB off.
 template <int IMM>
 __device__ __forceinline__ void dma16(uint32_t voff, const void* gbase, uint32_t lbase) {
-    asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sptr(gbase)),
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sptr(gbase)),
                  "s"((uint32_t)__builtin_amdgcn_readfirstlane((int)lbase)), "n"(IMM)
                  : "memory", "scc");
 }
 template <int IMM>
 __device__ __forceinline__ void dma4(uint32_t voff, const void* gbase, uint32_t lbase) {
-    asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sptr(gbase)),
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sptr(gbase)),
                  "s"((uint32_t)__builtin_amdgcn_readfirstlane((int)lbase)), "n"(IMM)
                  : "memory", "scc");
 }
