@@ -202,10 +202,11 @@ __device__ __forceinline__ float least(float m, const float (&v)[8]) {
     for (int e = 0; e < 8; e += 2) m = __builtin_elementwise_minimum(__builtin_elementwise_minimum(m, fabsf(v[e])), fabsf(v[e + 1]));
     return m;
 }
-// The scale that belongs to maximum a: 1 for zeros (as the other quantizers), NaN where a value was not finite.
+// The scale that belongs to maximum a: 1 for zeros (as the other quantizers), so where r = 1 / rms is 0 for an infinite value in
+// another group; NaN where a value was not finite.
 __device__ __forceinline__ float scale_of(double a, double r, double most) {
-    const double s = a * r / most;
-    return a > 0 ? (a < __builtin_inf() ? (float)s : __builtin_nanf("")) : r == r ? 1.f : __builtin_nanf("");
+    if (!(a < __builtin_inf()) || r != r) return __builtin_nanf("");
+    return a > 0 && r > 0 ? (float)(a * r / most) : 1.f;
 }
 
 // One workgroup a row; a thread holds C chunks of 8 elements, chunk c at (c * threads + thread) * 8.  What lies behind the
@@ -435,7 +436,7 @@ __global__ __launch_bounds__(MOST) void norm_k(BlockNorm a) {
             g = max2(g, pair_of<1>(g));
             g = max2(g, pair_of<2>(g));
             g = max2(g, pair_of<3>(g));
-            const bool fine = g > 0 && g < __builtin_inf();
+            const bool fine = g > 0 && g < __builtin_inf() && r > 0;
             const float f32 = off_fine && g > 0x1p-100 && g < 0x1p100 ? (float)levels / (float)g : __builtin_nanf("");
             uint2 q = make_uint2(0, 0);
             float hi[8];
