@@ -1023,6 +1023,7 @@ int rt4_block_norm(void* h_out, int64_t ldho, const void* h, int64_t ldh, int h_
     if (!h || (y && !h_out) || (!y && !n) || (!n != !w)) return fail(RT4_E_ARG, "rt4_block_norm: null pointer (h; h_out with y; n with w; n without y)");
     if (!y && (gate || post_w)) return fail(RT4_E_ARG, "rt4_block_norm: a gate and a norm behind the block need y");
     if (!(eps >= 0)) return fail(RT4_E_ARG, "rt4_block_norm: eps=%g", eps);
+    if (!y) h_out = nullptr, ldho = 0;           // not written: its place and stride say nothing
     rt4::BlockNorm a{h_out, ldho, h, ldh, y, ldy, gate, ldg, post_w, w, n, n_scale, scale, eps, w_offset, 0, M, K, h_type, y ? y_type : 0, n_form, false};
     return run_norm("rt4_block_norm", a, as_stream(stream));
 }

@@ -73,10 +73,24 @@ void gate4_lds() {
     check(gate4(1, 38912) == RT4_OK && g_lds <= 65536, "one row needs no limit");
 }
 
+int norm(void* h_out, int64_t ldho, const void* y) {
+    return rt4_block_norm(h_out, ldho, kAt, 256, RT4_F32, y, 256, RT4_F32, nullptr, 0, nullptr, (const float*)kAt, 1.0, 1e-6, 0.0, (void*)0x9000, nullptr,
+                          RT4_F32, 4, 256, nullptr);
+}
+
+// Without y nothing is written to h_out, so nothing is asked of it.
+void norm_without_y() {
+    check(norm(nullptr, 0, nullptr) == RT4_OK, "no h_out");
+    check(norm(kAt, 0, nullptr) == RT4_OK, "h_out as h, any stride");
+    check(norm((char*)kAt + 1, 3, nullptr) == RT4_OK, "h_out not aligned");
+    check(norm(kAt, 300, kAt) == RT4_E_ARG && norm((char*)kAt + 1, 256, kAt) == RT4_E_ARG && norm(kAt, 256, kAt) == RT4_OK, "with y they count");
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
     if (argc == 2 && !std::strcmp(argv[1], "gate4_lds")) gate4_lds();
+    else if (argc == 2 && !std::strcmp(argv[1], "norm_without_y")) norm_without_y();
     else return 2;
     std::printf("launches %d\n", g_launches);
     return 0;

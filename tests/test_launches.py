@@ -19,7 +19,7 @@ def recorder(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("case", ["gate4_lds"])
+@pytest.mark.parametrize("case", ["gate4_lds", "norm_without_y"])
 def test_launches(rt4, recorder, case):
     r = subprocess.run([str(recorder), case], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stderr
