@@ -635,7 +635,7 @@ def _refuse(dev, *args):
     all contiguous or with contiguous rows."""
     for name, t, shape, dtypes, whole in args:
         if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or t.get_device() != dev or not (
-                t.is_contiguous() if whole else t.dim() == 2 and t.stride(1) == 1):
+                t.is_contiguous() if whole else t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1)):
             raise RT4Error(f"{name}: expected {' or '.join(map(str, dtypes))} {tuple(shape)}, {'' if whole else 'rows '}contiguous, on device {dev}, "
                            f"got {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
     raise RT4Error("arguments do not fit each other")
@@ -644,6 +644,7 @@ def _refuse(dev, *args):
 _MOST = 2 ** 31 - 1       # sizes that the C ABI's ints hold; what it takes of them it checks itself
 
 
+# (In the checks below `t.stride(1) != 1 != K` asks for contiguous rows; of rows of one element the stride says nothing.)
 def _rows_of(t):
     """Row stride of a matrix; of a single row, whose stride says nothing, its length up to a multiple of 16."""
     return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
@@ -659,7 +660,7 @@ def _output(e, out, dtype, M, N, dev):
         out = e.empty((M, N), (N, 1), dtype=dtype, device=dev)
         return out, out.data_ptr(), N, t
     t = e.types.get(out.dtype)
-    if t is None or (dtype is not None and out.dtype is not dtype) or out.shape != (M, N) or out.get_device() != dev or out.stride(1) != 1:
+    if t is None or (dtype is not None and out.dtype is not dtype) or out.shape != (M, N) or out.get_device() != dev or out.stride(1) != 1 != N:
         _refuse(dev, ("out", out, (M, N), (dtype,) if dtype else tuple(e.types), False))
     return out, out.data_ptr(), _rows_of(out), t
 
@@ -798,25 +799,25 @@ def block_norm(h, y=None, weight=None, post_weight=None, gate=None, scale: float
     if M > _MOST or K > _MOST:
         raise RT4Error(f"h {tuple(h.shape)}: too large")
     ht = types.get(h.dtype)
-    if ht is None or h.get_device() != dev or h.stride(1) != 1:
+    if ht is None or h.get_device() != dev or h.stride(1) != 1 != K:
         _refuse(dev, ("h", h, (M, K), tuple(types), False))
     op = yp = gp = wp = pp = np_ = sp = n = s = None
     ldho = ldy = yt = ldg = 0
     if y is not None:
         yt = types.get(y.dtype)
-        if yt is None or y.shape != (M, K) or y.get_device() != dev or y.stride(1) != 1:
+        if yt is None or y.shape != (M, K) or y.get_device() != dev or y.stride(1) != 1 != K:
             _refuse(dev, ("y", y, (M, K), tuple(types), False))
         yp, ldy = y.data_ptr(), _rows_of(y)
         if h_out is None:
             h_out = e.empty((M, K), (K, 1), dtype=h.dtype, device=dev)
             op, ldho = h_out.data_ptr(), K
         else:
-            if h_out.shape != (M, K) or h_out.dtype is not h.dtype or h_out.get_device() != dev or h_out.stride(1) != 1:
+            if h_out.shape != (M, K) or h_out.dtype is not h.dtype or h_out.get_device() != dev or h_out.stride(1) != 1 != K:
                 _refuse(dev, ("h_out", h_out, (M, K), (h.dtype,), False))
             op, ldho = h_out.data_ptr(), _rows_of(h_out)
         if gate is not None:
             rows = gate.dim() == 2
-            if gate.shape != ((M, K) if rows else (K,)) or gate.dtype is not y.dtype or gate.get_device() != dev or gate.stride(-1) != 1:
+            if gate.shape != ((M, K) if rows else (K,)) or gate.dtype is not y.dtype or gate.get_device() != dev or gate.stride(-1) != 1 != K:
                 _refuse(dev, ("gate", gate, (M, K) if rows else (K,), (y.dtype,), not rows))
             gp, ldg = gate.data_ptr(), _rows_of(gate) if rows else 0
         if post_weight is not None:
@@ -849,7 +850,7 @@ def quant_token_a8(x, xq=None, sx=None):
     if M > _MOST or K > _MOST:
         raise RT4Error(f"x {tuple(x.shape)}: too large")
     t = e.types.get(x.dtype)
-    if t is None or x.get_device() != dev or x.stride(1) != 1:
+    if t is None or x.get_device() != dev or x.stride(1) != 1 != K:
         _refuse(dev, ("x", x, (M, K), tuple(e.types), False))
     if xq is None:
         xq = e.empty((M, K), (K, 1), dtype=e.i8, device=dev)
