@@ -416,7 +416,8 @@ int rt4_w8a8_launch_plan(int M, int N, int K, int weights, int cus, int* form, i
                          int* tile_n);
 
 /* First half of a gated feed-forward block on 8-bit weights: h [M][N] = act(g) * u with g and u the products of
- * rt4_gemm_w8a8 with the gate weights wg, sg and the up weights wu, su, in fp32 until h's rounding.  Arguments as there. */
+ * rt4_gemm_w8a8 with the gate weights wg, sg and the up weights wu, su, in fp32 until h's rounding (an act(g) that is
+ * below 2^-126 |g| counts as 0).  Arguments as there. */
 int rt4_ffn_gate_w8a8(void* h, int64_t ldh, int h_type, const int8_t* wg, int64_t ldg, const float* sg, const int8_t* wu,
                       int64_t ldu, const float* su, const int8_t* xq, int64_t ldx, const float* sx, int M, int N, int K,
                       int act, void* work, int64_t work_bytes, void* stream);
@@ -437,8 +438,9 @@ int rt4_ffn_gate_w4a8(float* h, const uint32_t* wg, const uint16_t* sg, const ui
  * elements, at least K; w and post_w f32 [K].  h_out may be h with the same stride; otherwise outputs must not overlap
  * inputs.  n_form: an element type, n [M][K] contiguous of that type, n_scale NULL; or RT4_TOKEN, RT4_ACT, RT4_ROWS
  * with n_scale (the last two with K % 128 == 0).  A code is the nearest integer to levels * n / max|n| over its token
- * or group (ties to even), decided in 64 bits; its scale max|n| / levels, 1 where all are zeros.  Where a value of a
- * token or group is not finite its codes are 0 and its scale NaN.  1 <= M < 2^22, 1 <= K <= 65536. */
+ * or group (ties to even), decided in 64 bits; its scale max|n| / levels, 1 where all are zeros (also where rms(h_out)
+ * is 0, with eps 0).  Where a value n of a token or group is not finite its codes are 0 and its scale NaN; beside an
+ * infinite h_out the other groups' n are zeros, beside a NaN they are NaN.  1 <= M < 2^22, 1 <= K <= 65536. */
 int rt4_block_norm(void* h_out, int64_t ldho, const void* h, int64_t ldh, int h_type, const void* y, int64_t ldy, int y_type,
                    const void* gate, int64_t ldg, const float* post_w, const float* w, double scale, double eps, double w_offset,
                    void* n, float* n_scale, int n_form, int M, int K, void* stream);

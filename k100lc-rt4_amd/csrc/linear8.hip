@@ -5,13 +5,15 @@
 //   h[m][n] = act(sx[m] sg[n] Σ_k xq[m][k] wg[n][k]) * (sx[m] su[n] Σ_k xq[m][k] wu[n][k])
 //
 // What bounds it, and where it stands:
-//   up to 8 tokens   the weights' stream; 2 x 17408 x 5120 of one token 30.4 us, 5.9 TB/s; 5120 x 5120 5.4 us, most of it the
-//                    launch and the first loads' latency
-//   tens of tokens   latency: a workgroup's steps, of 0.25 us, one after the other; 37 tokens of 4999 x 7056 15.9 us, 79
-//                    workgroups of 56 steps (a launch that joins runs of split K costs 7.8)
-//   many tokens      the matrix cores, at the clock that power leaves them (1.7 to 1.9 GHz under these kernels): 4096 tokens of
-//                    17408 x 5120 329 to 352 us by card, 2.1 to 2.2 Pop/s; 1000 of 2 x 17408 x 5120 178 to 193 us, 1.85 to 2.0;
-//                    1024 of 5120 x 17408 95 us, 1.9 (a library's int8 product of 8192^3: 2.07)
+//   up to 8 tokens   the weights' stream; 2 x 17408 x 5120 of one token 30.4 us, 5.9 TB/s; 5120 x 5120 7.6 us for a stream of 5.5:
+//                    the launch, the first loads' latency, and a second round, since 266 registers leave one wave a SIMD and
+//                    1280 waves do not fit the 1024 SIMDs
+//   9 to 400 tokens  latency: a workgroup's steps, of 0.25 us, one after the other, where tiles are fewer than the CUs; 37 tokens
+//                    of 4999 x 7056, 79 workgroups of 56 steps, 15.9 us with the weights in the last-level cache and 24 from
+//                    memory, for a floor of 7.5; 100 tokens of 5120 x 17408 35 us for 19 (a launch that joins runs of split K: 7.8)
+//   many tokens      the matrix cores, at the clock that power leaves them (1.7 to 1.8 GHz, busy 57 to 62% of the cycles): 4096
+//                    tokens of 17408 x 5120 329 to 352 us by card, 2.1 to 2.2 Pop/s; 1000 of 2 x 17408 x 5120 178 to 193 us,
+//                    1.85 to 2.0; 1024 of 5120 x 17408 95 us, 1.9 (a library's int8 product of 8192^3: 2.07)
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -57,7 +59,9 @@ struct Where {                           // a workgroup's tile and steps
 template <class C, int NW>
 __device__ __forceinline__ Where where(const Linear8& a, int splits, int b, int blocks) {
     const int nm = (a.M + C::BM - 1) / C::BM, nn = (a.N + C::BN / NW - 1) / (C::BN / NW);
-    // Workgroups go round the XCDs: each takes a run of the list, in which tiles that share operands are neighbours.
+    // Workgroups go round the XCDs: each takes a run of the list, in which tiles that share operands are neighbours: columns of GM
+    // tiles, one beside the other (4096 tokens of 17408 x 5120: GM 4 340 to 345 us, 1 355 to 359, 2 349, 8 343; 2000 tokens 180,
+    // 188 to 194, 184, 183).
     const int x = b & 7, per = blocks >> 3, rem = blocks & 7, t = x * per + min(x, rem) + (b >> 3);
     Where w;
     w.part = t % splits;
@@ -359,6 +363,8 @@ hipError_t launch_tile(const Linear8& a, const Linear8Part& p, void* part, hipSt
 // and up rows of 2) and goes through them 1 KB of each at a time, a lane 16 codes of each row, with the codes of every token
 // beside them: each token's 16 bytes serve 4 rows.  The next loads are under way while 4 M v_dot4 an operand are done.  A
 // workgroup is one wave, so that they spread evenly over the CUs.
+// U, the KB of each row at a time (1 token of 5120 x 5120, of 17408 x 5120, 4 tokens of the latter, 8 tokens, from memory): as it is
+// 7.7, 17.6, 19.6, 25.2 us; 2 for one token 6.3, 15.5; 1 everywhere 6.4, 15.3, 18.4, 25.4; 2 for 5 to 8 tokens 33.6.
 template <int M, int NW>
 __global__ __launch_bounds__(64) void linear8_dot_k(Linear8 a) {
     constexpr int RN = 4 / NW, U = M == 1 ? 4 : M <= 4 ? 2 : 1;      // channels of a wave; KB of each row at a time
@@ -431,12 +437,16 @@ hipError_t launch_dot(const Linear8& a, hipStream_t st) {
     return hipGetLastError();
 }
 
+// 8 tokens by dot products and by tiles: 5120 x 5120 10.3 and 12.6 us, 17408 x 5120 25.2 and 25.3, 5120 x 17408 24.3 and 25.0, 2 x
+// 2500 x 2560 8.1 and 9.2; but 2 x 17408 x 5120 42.6 and 38.5 (6 tokens 37.3 and 38.1).
 constexpr int kDotMaxM = 8;
 constexpr long long kMaxGroups = 1 << 24;        // workgroups of 256 threads in a grid
 // A form's tile, workgroups a CU holds, and its measured cost (us): a step where few workgroups run, what is added to that
 // where all do (power, the L2's rate), a tile's beginning and end; and the rate at which it streams weights (TB/s), which bounds
 // few tokens.  Fitted to 1045 times of 54 sizes (M 16..4000, N 1000..17408, K 1024..17408, one and two weight matrices, every
-// form, 1 to 4 splits); the form they choose takes 2% longer than the best one of each size.
+// form, 1 to 4 splits); the form they choose takes 2% longer than the best one of each of these sizes.  On 24 sizes that the fit
+// has not seen (M 14..2475, N 532..16714, K 1360..15776) it takes 8.5% longer on average, over 10% at 8 of them and 45% at worst
+// (170 tokens of 2 x 4543 x 12912: 79 us, the best form 55).
 struct Shape {
     int bm, bn, per_cu;
     double step, full, ends, rate;
@@ -466,7 +476,8 @@ double estimate(int f, int M, int N, int K, int weights, int cus, int sp, long l
 }
 
 // The form and number of splits of the lowest estimate.  (A grid counts its threads in 32 bits: large tiles alone for the
-// largest products.)
+// largest products.)  Up to 8 splits: 100 tokens of 1024 x 131056 57 us, with up to 4 95, up to 16 66; 16 of 1000 x 17408 13.2,
+// 15.1, 14.7; 9 of 512 x 65536 24.6, 36.4, 20.4.
 double choose(int M, int N, int K, int weights, int cus, Linear8Part* p) {
     double best = 1e30;
     for (int f = 0; f < kDotForm; f++)

@@ -7,13 +7,19 @@
 // n goes out as floats or as int8 codes, one scale a token or one a 128-group.  A code is the nearest integer
 // to most * n / max|n|, and 1 / rms cancels in that quotient, so codes go by p = h' (w + w_offset) alone.
 //
-// Results are those of 64-bit arithmetic (p is exact in it, sums and quotients are off by 2^-51), so each has one right
-// value; but a 64-bit conversion costs four fp32 operations, so what fp32 decides is left to it: a quotient, or a residual
+// Results are those of 64-bit arithmetic.  p is exact in it and a quotient off by 2^-51, so a code has one right value.  A sum of
+// squares passes through n roundings, 34 for 5120 elements and 86 for 65536, and is off by n 2^-53 of itself, 1 / rms by half of
+// that: 2^-47.6 at most, which can move a residual behind a norm, or a float result, over a border that it lies next to.
+// A 64-bit conversion costs four fp32 operations, so what fp32 decides is left to it: a quotient, or a residual
 // of 16 bits, is formed in fp32 with a bound of its error, and in 64 bits by the lanes whose rounding that leaves open
-// (one of 8000 codes, of 4000 residuals).  4096 tokens of 5120 (bf16, post norm, gate, token codes): 54 us, with 64 bits
-// throughout 71; their 147 MB take 31 us at the rate of a large copy, the vector ALU's ~50 operations an element the rest, at
-// the 4 waves a SIMD that 123 registers leave (93 and 5 waves without the check of products' range, `least`: 48 us; held to 96
-// registers, which spills, 75; two chunks a thread, 60).  4 rows of 5120: 5.5 us, 1000 rows of 17408 to codes alone: 16 us for 52 MB.
+// (one of 8000 codes, of 4000 residuals).
+//
+// 4096 tokens of 5120 (bf16, post norm, gate, token codes): 62 us from memory (58 where the last-level cache holds a part); their
+// 147 MB take 31 at the rate of a large copy, and the vector ALU works for 40 of them (74 instructions an element, active 71% of
+// the cycles), at the 4 waves a SIMD that 123 registers leave.  Without the check of products' range, `least`, 93 registers and
+// 57 us; held to 96 registers, which spills, 82; two chunks a thread, 81.  A tenth of y zero, which that check leaves to 64 bits:
+// 67; every other row zero: 63.  Without post norm and gate: token codes 55, group codes 53, bf16 47; without y 31, 30, 26.
+// 4 rows of 5120: 5.4 us.  1000 rows of 17408 to codes alone: 19 us for 52 MB (16 to 17 from the cache).
 #include <type_traits>
 
 #include "ffn_dev.h"
@@ -456,9 +462,13 @@ __global__ __launch_bounds__(MOST) void norm_k(BlockNorm a) {
 
 template <class TH, bool HASY, bool NORM>
 void launch_chunks(const BlockNorm& a, hipStream_t st) {
-    // Few rows: many waves a row, a chunk or two a thread.  Many: few waves a row, whose reductions cost little; 3 chunks a
-    // thread (5 without y) leave registers for as many rows a CU as hide each other's latencies (4096 tokens of 5120, bf16: 3
-    // chunks 54 us, 2 60).  Waves enough to fill the CUs either way.
+    // Few rows: many waves a row.  Many: few waves a row, whose reductions cost little; 3 chunks a thread (5 without y) leave
+    // registers for as many rows a CU as hide each other's latencies (4096 tokens of 5120, bf16, post norm and gate: 3 chunks 62
+    // us, 2 81).  Waves enough to fill the CUs either way.
+    // Forms of 2 to 5 chunks hold 512 threads.  So rows above 12288 elements take 5 chunks, with y at 149 to 188 registers and 2
+    // or 3 waves a SIMD, and rows above 20480 take 8 at 1024 threads, whose 128 registers do not hold them with a norm: 40 to 344
+    // bytes of a lane go to scratch without y, 556 to 788 with it (1000 rows with a post norm: of 12288 elements 34 us, of 17408
+    // 68, of 20480 70, of 24576 184; without y 27, 26, 29, 79).
     const int lanes = (a.K + 7) / 8, most = HASY ? 3 : 5;
     const auto go = [&](auto k, int C) {
         hipLaunchKernelGGL(k, dim3((unsigned)a.M), dim3((unsigned)(((lanes + C - 1) / C + 63) / 64 * 64)), 0, st, a);
