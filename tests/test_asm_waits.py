@@ -43,15 +43,24 @@ def states(op, args):
     return int(args.split()[0], 0) + 1 if op == "s_nop" else 1
 
 
+def scalars(text):
+    """Scalar registers that a text names."""
+    regs = set()
+    for m in re.finditer(r"\bs\[(\d+):(\d+)\]|\bs(\d+)\b|\bvcc(_lo|_hi)?\b", text):
+        if m[0].startswith("vcc"):
+            regs |= {"": {106, 107}, "_lo": {106}, "_hi": {107}}[m[4] or ""]
+        else:
+            regs |= set(range(int(m[1] or m[3]), int(m[2] or m[3]) + 1))
+    return regs
+
+
 def written_by_vector(op, args):
     """Scalar registers that a vector instruction writes."""
     if not op.startswith("v_"):
         return set()
     regs = set()
     for a in args.split(", ")[:2 if "_co_" in op or "div_scale" in op or "mad_u64" in op or "mad_i64" in op else 1]:
-        m = re.fullmatch(r"s(?:(\d+)|\[(\d+):(\d+)\])", a.strip())
-        if m:
-            regs |= set(range(int(m[1] or m[2]), int(m[1] or m[3]) + 1))
+        regs |= scalars(a.strip())
     return regs
 
 
@@ -71,9 +80,7 @@ def faults(code):
     for i, (op, args, _) in enumerate(code):
         if not (op.startswith("global_load_lds") or (op.startswith("buffer_load") and re.search(r"\blds\b", args))):
             continue
-        base = set()
-        for m in re.finditer(r"\bs\[(\d+):(\d+)\]|\bs(\d+)\b", args):
-            base |= set(range(int(m[1] or m[3]), int(m[2] or m[3]) + 1))
+        base = scalars(args)
         ways = [(p, 0) for p in before(i)]       # (instruction, wait states between it and the load)
         while ways:
             p, n = ways.pop()
@@ -104,6 +111,7 @@ def test_the_checker_sees_faults():
     assert not faults(code("v_readfirstlane_b32 s5, v2", "s_mov_b32 m0, s3", "s_nop 3", load))
     assert not faults(code("v_readfirstlane_b32 s6, v2", "s_nop 0", load))
     assert len(faults(code("v_cmp_gt_f32_e64 s[4:5], v2, v3", "s_nop 1", load))) == 1
+    assert len(faults(code("v_cmp_gt_f32_e32 vcc, v2, v3", "global_load_lds_dword v1, vcc offset:16"))) == 1
     # by way of a branch
     assert len(faults(code("v_readfirstlane_b32 s4, v2", ("s_cbranch_scc0 3", 16), "s_nop 7", "s_nop 7", load))) == 1
     assert not faults(code("v_readfirstlane_b32 s4, v2", ("s_branch 1", 12), load, "s_endpgm"))
